@@ -15,7 +15,7 @@ NVFLAGS := $(ARCH) -O3 -lineinfo -std=c++17 -Xcompiler -fPIC -Xcompiler -Wall \
 LDFLAGS := -cudart static -lpthread -ldl -lrt
 
 LIB_CC  := $(wildcard csrc/common/*.cc csrc/control/*.cc csrc/runtime/*.cc)
-LIB_CU  := $(wildcard csrc/runtime/*.cu csrc/fused/*.cu)
+LIB_CU  := $(wildcard csrc/runtime/*.cu csrc/fused/*.cu csrc/model/*.cu)
 LIB_OBJ := $(patsubst csrc/%,$(OBJ)/%.o,$(LIB_CC) $(LIB_CU))
 HDRS    := $(wildcard include/*.h csrc/*/*.h csrc/*/*.cuh)
 

@@ -1,0 +1,96 @@
+// SPDX-License-Identifier: Apache-2.0
+// Shared by the model operators: 8-element vectors of 16-bit types, checks
+// of tensor descriptions, launch results.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common/log.h"
+#include "common/trace.h"
+#include "vccl_model.h"
+
+namespace vccl {
+namespace model {
+
+// What a kernel needs of a vcclHeads_t.
+struct Heads {
+  void* data;
+  long long tok;
+  long long head;
+  int heads;
+};
+
+inline Heads headsOf(const vcclHeads_t* h) {
+  if (h == nullptr) return {nullptr, 0, 0, 0};
+  return {h->data, h->tokenStride, h->headStride, h->heads};
+}
+
+// 16-byte vectors: base and strides in whole vectors of 8 elements.
+inline bool headsOk(const vcclHeads_t* h, int elemBytes) {
+  if (h == nullptr || h->data == nullptr || h->heads <= 0) return false;
+  const long long vec = 16 / elemBytes;
+  return (reinterpret_cast<uintptr_t>(h->data) & 15u) == 0 && h->tokenStride % vec == 0 && h->headStride % vec == 0;
+}
+
+inline vcclResult_t launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return vcclSuccess;
+  VERR("%s: %s", what, cudaGetErrorString(e));
+  return vcclSystemError;
+}
+
+// T is __nv_bfloat16 or __half.
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]);
+
+template <>
+__device__ __forceinline__ void unpack8<__nv_bfloat16>(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+
+template <>
+__device__ __forceinline__ void unpack8<__half>(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]);
+
+template <>
+__device__ __forceinline__ uint4 pack8<__nv_bfloat16>(const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <>
+__device__ __forceinline__ uint4 pack8<__half>(const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+}  // namespace model
+}  // namespace vccl

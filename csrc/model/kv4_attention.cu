@@ -1,0 +1,735 @@
+// SPDX-License-Identifier: Apache-2.0
+// Attention of ragged query rows over the 4-bit paged cache.
+//
+// Mathematics.  With value = mid + scale (code - 7.5) for each token and group
+// of 64 channels,
+//   q . k_t = sum_g [ scale_tg (q_g . c_tg) + (mid_tg - 7.5 scale_tg) sum(q_g) ]
+//   sum_t p_t v_t = sum_t (p_t scale_tg) (c_tg - 7.5) + sum_t p_t mid_tg
+// so the tensor cores multiply the codes themselves, and scale and midpoint
+// act on accumulators and on the softmax weights.  A code c read as an f16
+// bit pattern is the subnormal c * 2^-24 (its neighbour in bits 4-7 is
+// 16 c * 2^-24), exact in the tensor cores' products; one AND makes a pair
+// of operands.  Query rows are scaled by a power of two and held in f16,
+// which is exact for bf16 and f16 inputs but for channels below 2^-26 of the
+// row's largest.  The weights p_t scale_tg are rounded to f16 (11 bits)
+// relative to a power of two above the scales seen so far; the sum of the
+// rounded ones, which the 7.5 multiplies, is a product with ones on the
+// tensor cores.  Everything else is f32.
+//
+// Shape.  S^T = K Q^T: rows of the m16n8k16 products are 16 tokens, columns 8
+// query rows (a query row is one head of one token; the heads that share a key
+// head stand together), so a group of 8 heads fills the tile.  O^T = V^T P^T
+// the same way; movmatrix turns the accumulator of S^T into the operand P^T.
+//
+// Work.  A unit is a request, a key head and R = 8 * NT query rows; its
+// length is the request's tokens in tiles of 32.  The tiles of all units in a
+// row are cut into equal ranges, one for each warp of the grid, whatever the
+// lengths are; a warp that gets a whole unit writes the result, the others
+// write partial sums (unnormalised output, maximum, sum) that a second kernel
+// joins in order.
+#include <cfloat>
+#include <climits>
+
+#include "kernels/kv4.cuh"
+#include "model/common.cuh"
+
+namespace vccl {
+namespace model {
+namespace {
+
+constexpr int kWarps = 4;          // per block
+constexpr int kTile = 32;          // tokens in a unit of work
+constexpr int kMaxBatch = 4096;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kNone = -1e30f;    // a maximum over nothing
+
+struct AttnArgs {
+  const void* q;
+  long long qTok, qHead;
+  const uint8_t* cache;
+  const int* table;
+  const int* kvLens;
+  const int* qStarts;
+  void* out;
+  long long oTok, oHead;
+  float* lse;
+  long long* prefix;  // [batch + 1] tiles before each request (written by block 0)
+  float2* stats;      // [2 * workers][R] maximum (log2), sum
+  float* partial;     // [2 * workers][R][D]
+  int width, batch, tokens, qHeads, kvHeads, group, pages, blocksPerPage;
+  int workers, half16, zeroTail;
+  float scaleLog2;
+};
+
+// What a request brings: its first row, its rows, its tokens.
+struct Request {
+  int start, rows, kv;
+};
+
+__device__ __forceinline__ Request requestOf(const AttnArgs& p, int b) {
+  const int s = min(max(p.qStarts[b], 0), p.tokens), e = min(max(p.qStarts[b + 1], s), p.tokens);
+  const long long most = static_cast<long long>(p.width) * p.blocksPerPage * kv4::kBlockTokens;
+  return {s, e - s, static_cast<int>(min(static_cast<long long>(max(p.kvLens[b], 0)), most))};
+}
+
+__device__ __forceinline__ int unitsOf(const AttnArgs& p, const Request& r, int R) {
+  const long long rows = static_cast<long long>(r.rows) * p.group;
+  return static_cast<int>((rows + R - 1) / R);
+}
+
+__device__ __forceinline__ int tilesOf(const Request& r) { return (r.kv + kTile - 1) / kTile; }
+
+__device__ __forceinline__ long long rangeStart(long long w, long long total, int workers) { return w * total / workers; }
+__device__ __forceinline__ int workerOf(long long tile, long long total, int workers) {
+  return static_cast<int>(((tile + 1) * workers - 1) / total);
+}
+
+// Every warp that takes part has at least one tile.
+__device__ __forceinline__ int workersFor(const AttnArgs& p, long long total) {
+  return static_cast<int>(min(static_cast<long long>(p.workers), total));
+}
+
+// prefix[b] = tiles of the requests before b (all heads and row tiles).
+template <int THREADS>
+__device__ void scanTiles(const AttnArgs& p, int R, long long* prefix) {
+  __shared__ long long warpSums[THREADS / 32];
+  __shared__ long long carry;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    carry = 0;
+    prefix[0] = 0;
+  }
+  __syncthreads();
+  for (int base = 0; base < p.batch; base += THREADS) {
+    const int b = base + threadIdx.x;
+    long long v = 0;
+    if (b < p.batch) {
+      const Request r = requestOf(p, b);
+      v = static_cast<long long>(unitsOf(p, r, R)) * p.kvHeads * tilesOf(r);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(~0u, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) warpSums[warp] = v;
+    __syncthreads();
+    long long before = carry;
+    for (int i = 0; i < warp; i++) before += warpSums[i];
+    if (b < p.batch) prefix[b + 1] = before + v;
+    __syncthreads();
+    if (threadIdx.x == THREADS - 1) carry = before + v;
+    __syncthreads();
+  }
+}
+
+__device__ __forceinline__ int findRequest(const long long* prefix, int batch, long long tile) {
+  int lo = 0, hi = batch - 1;  // the last b with prefix[b] <= tile whose tiles are not all before
+  while (lo < hi) {
+    const int m = (lo + hi) >> 1;
+    if (prefix[m + 1] > tile) hi = m;
+    else lo = m + 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t packHalf(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float exp2Fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The codes and parameters of one block of 16 tokens, as one lane reads them.
+template <int G>
+struct BlockRegs {
+  uint32_t k[2][2 * G];  // tokens g, g + 8: words (group, half)
+  uint32_t v[4][G];      // tokens 2q, 2q + 1, 8 + 2q, 9 + 2q: word of each group
+  uint32_t kp[2][G], vp[2][G];
+};
+
+template <int WORDS>
+__device__ __forceinline__ void loadWords(const uint8_t* p, uint32_t* w) {
+  if constexpr (WORDS == 4) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
+  } else if constexpr (WORDS == 2) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
+}
+
+template <int G>
+__device__ __forceinline__ void loadBlock(BlockRegs<G>& r, const uint8_t* block, int lane) {
+  constexpr int D = 64 * G;
+  const int g = lane >> 2, q = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    loadWords<2 * G>(block + (g + 8 * i) * (D / 2) + q * (8 * G), r.k[i]);
+    loadWords<G>(block + 16 * D + (g + 8 * i) * (4 * G), r.kp[i]);
+    loadWords<G>(block + 17 * D + (g + 8 * i) * (4 * G), r.vp[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) loadWords<G>(block + 8 * D + (4 * i + q) * (D / 2) + g * (4 * G), r.v[i]);
+}
+
+// A warp's state for one unit.
+template <int G, int NT>
+struct Unit {
+  uint32_t qb[NT][G][4][2];  // Q^T operands: word half h, code pair u -> [2h + u]
+  float qs[NT][2];           // log2(e) * scale * 2^24 / (power of two of the row), rows 2q and 2q + 1
+  float sq[NT][G][2];        // log2(e) * scale * sum of the row's group
+  int limit[NT][2];          // tokens that the row sees
+  int most, least;           // of all rows of the unit
+  float m[NT][2], l[NT][2];
+  float o[NT][G][4][4];      // 2^24 (16 for odd u) * 2^-r * sum p' c
+  float ones[NT][G][4];      // 2^-r * sum p'
+  float mid[NT][G][2];       // sum p mid
+  float inv[G], lim[G];      // 2^-r, and the scale above which r grows
+};
+
+template <int G, int NT>
+__device__ __forceinline__ void loadQuery(Unit<G, NT>& u, const AttnArgs& p, const Request& r, int head, int row0,
+                                          int lane) {
+  const int g = lane >> 2, q = lane & 3;
+  int most = 0, least = INT_MAX;
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    const long long row = static_cast<long long>(row0) + 8 * n + g;
+    const bool live = row < static_cast<long long>(r.rows) * p.group;
+    const int i = live ? static_cast<int>(row / p.group) : 0, h = head * p.group + (live ? static_cast<int>(row % p.group) : 0);
+    float x[G][16];
+    float amax = 0.0f;
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) {
+      uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+      if (live) {
+        const uint16_t* src = static_cast<const uint16_t*>(p.q) + (r.start + i) * p.qTok + h * p.qHead + 64 * gr + 16 * q;
+        v[0] = *reinterpret_cast<const uint4*>(src);
+        v[1] = *reinterpret_cast<const uint4*>(src + 8);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        float y[8];
+        if (p.half16) unpack8<__half>(v[j], y);
+        else unpack8<__nv_bfloat16>(v[j], y);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          x[gr][8 * j + e] = y[e];
+          amax = fmaxf(amax, fabsf(y[e]));
+        }
+      }
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+    // f = 2^(12 - exponent of the largest); kept in f32's range.
+    const int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+    const bool plain = amax == 0.0f || e > 120 || e < -100;
+    const float f = plain ? 1.0f : __uint_as_float(static_cast<uint32_t>(127 + 12 - e) << 23);
+    const float back = plain ? 1.0f : __uint_as_float(static_cast<uint32_t>(127 - 12 + e) << 23);
+    float qs = back * p.scaleLog2 * 16777216.0f;
+    float sq[G];
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) {
+      float s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; j++) s += x[gr][j];
+      s += __shfl_xor_sync(~0u, s, 1);
+      s += __shfl_xor_sync(~0u, s, 2);
+      sq[gr] = s * p.scaleLog2;
+#pragma unroll
+      for (int w = 0; w < 4; w++) {  // word half w / 2, code pair w % 2: channels 4w .. 4w + 3 of the lane's 16
+        const float* y = &x[gr][4 * w];
+        u.qb[n][gr][w][0] = packHalf(y[0] * f, y[1] * f);
+        u.qb[n][gr][w][1] = packHalf(y[2] * f * 0.0625f, y[3] * f * 0.0625f);
+      }
+    }
+    // A row behind the last one is computed like the last one, and not stored.
+    const int lim = live ? max(r.kv - r.rows + i + 1, 0) : r.kv;
+    // Columns 2q and 2q + 1 of the accumulators belong to the rows of lanes 8q and 8q + 4.
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      const int src = 4 * (2 * q + c);
+      u.qs[n][c] = __shfl_sync(~0u, qs, src);
+      u.limit[n][c] = min(__shfl_sync(~0u, lim, src), r.kv);
+#pragma unroll
+      for (int gr = 0; gr < G; gr++) u.sq[n][gr][c] = __shfl_sync(~0u, sq[gr], src);
+      u.m[n][c] = kNone;
+      u.l[n][c] = 0.0f;
+      most = max(most, u.limit[n][c]);
+      least = min(least, u.limit[n][c]);
+#pragma unroll
+      for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] = 0.0f;
+    }
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        u.ones[n][gr][j] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) u.o[n][gr][j][k] = 0.0f;
+      }
+    }
+  }
+#pragma unroll
+  for (int gr = 0; gr < G; gr++) {
+    u.inv[gr] = 1.0f;
+    u.lim[gr] = 0.0f;
+  }
+  most = max(most, __shfl_xor_sync(~0u, most, 1));
+  u.most = max(most, __shfl_xor_sync(~0u, most, 2));
+  least = min(least, __shfl_xor_sync(~0u, least, 1));
+  u.least = min(least, __shfl_xor_sync(~0u, least, 2));
+}
+
+// One block of 16 tokens that starts at token t0 of the request.
+template <int G, int NT>
+__device__ __forceinline__ void blockStep(Unit<G, NT>& u, const BlockRegs<G>& r, int t0, int lane) {
+  const int g = lane >> 2;
+  float x[NT][4];
+  // S^T, group by group: the scale of a token and group acts on the group's sum.
+#pragma unroll
+  for (int gr = 0; gr < G; gr++) {
+    float acc[NT][4] = {};
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint32_t w0 = r.k[0][2 * gr + h], w1 = r.k[1][2 * gr + h];
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+        mma(acc[n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, u.qb[n][gr][2 * h][0],
+            u.qb[n][gr][2 * h][1]);
+      const uint32_t s0 = w0 >> 8, s1 = w1 >> 8;
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+        mma(acc[n], s0 & 0x000F000Fu, s1 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x00F000F0u, u.qb[n][gr][2 * h + 1][0],
+            u.qb[n][gr][2 * h + 1][1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {  // tokens g, g + 8
+      const float s = kv4::bf16Lo(r.kp[i][gr]), off = fmaf(-7.5f, s, kv4::bf16Hi(r.kp[i][gr]));
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          const float y = fmaf(acc[n][2 * i + c] * s, u.qs[n][c], off * u.sq[n][gr][c]);
+          x[n][2 * i + c] = gr == 0 ? y : x[n][2 * i + c] + y;
+        }
+    }
+  }
+  float s[2][G], mid[2][G];
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) {
+      s[i][gr] = kv4::bf16Lo(r.vp[i][gr]);
+      mid[i][gr] = kv4::bf16Hi(r.vp[i][gr]);
+    }
+  // Tokens behind some row's last one: their scores are none, and the
+  // parameters of those that no row sees may be anything.
+  const bool edge = t0 + kv4::kBlockTokens > u.least;
+  if (edge) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int t = t0 + g + 8 * i;
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+          if (t >= u.limit[n][c]) x[n][2 * i + c] = -INFINITY;
+      if (t >= u.most) {
+#pragma unroll
+        for (int gr = 0; gr < G; gr++) s[i][gr] = mid[i][gr] = 0.0f;
+      }
+    }
+  }
+  // The maximum is followed loosely: it moves when a score passes it by 8
+  // (weights reach 2^8), and the power of two of the scales when one passes
+  // it by 4, so most blocks take neither a reduction nor a rescaling.
+  bool grow = false;
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int c = 0; c < 2; c++) grow = grow || fmaxf(x[n][c], x[n][2 + c]) > u.m[n][c] + 8.0f;
+#pragma unroll
+  for (int gr = 0; gr < G; gr++) grow = grow || fmaxf(s[0][gr], s[1][gr]) > u.lim[gr];
+  if (__any_sync(~0u, grow)) {
+    float alpha[NT][2], beta[G];
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) {
+      float top = fmaxf(s[0][gr], s[1][gr]);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+      beta[gr] = 1.0f;
+      if (top > u.lim[gr]) {
+        // 2^r with top in [2^r, 2^(r+1)); subnormal scales share the smallest r.
+        const int e = max(static_cast<int>(__float_as_uint(top) >> 23), 1);
+        const float inv = __uint_as_float(static_cast<uint32_t>(min(254 - e, 253)) << 23);
+        beta[gr] = u.lim[gr] > 0.0f ? inv / u.inv[gr] : 1.0f;  // a quotient of powers of two
+        u.inv[gr] = inv;
+        u.lim[gr] = e < 252 ? __uint_as_float(static_cast<uint32_t>(e + 2) << 23) : INFINITY;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        float top = fmaxf(x[n][c], x[n][2 + c]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        const float m = fmaxf(u.m[n][c], top);
+        alpha[n][c] = exp2Fast(u.m[n][c] - m);
+        u.m[n][c] = m;
+        u.l[n][c] *= alpha[n][c];
+#pragma unroll
+        for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] *= alpha[n][c];
+      }
+#pragma unroll
+      for (int gr = 0; gr < G; gr++) {
+        const float f[2] = {alpha[n][0] * beta[gr], alpha[n][1] * beta[gr]};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          u.ones[n][gr][k] *= f[k & 1];
+#pragma unroll
+          for (int j = 0; j < 4; j++) u.o[n][gr][j][k] *= f[k & 1];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const float w = exp2Fast(x[n][2 * i + c] - u.m[n][c]);
+        x[n][2 * i + c] = w;
+        u.l[n][c] += w;
+#pragma unroll
+        for (int gr = 0; gr < G; gr++) {
+          // at the edge a row must not meet a NaN of a token that it does not see
+          const float add = edge && w == 0.0f ? 0.0f : mid[i][gr];
+          u.mid[n][gr][c] = fmaf(w, add, u.mid[n][gr][c]);
+        }
+      }
+  // O^T: rows are channels 8g + 2j (from the low halves) and 8g + 2j + 1.
+#pragma unroll
+  for (int gr = 0; gr < G; gr++) {
+    const float f0 = s[0][gr] * u.inv[gr], f1 = s[1][gr] * u.inv[gr];
+    uint32_t b0[NT], b1[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      float w[4] = {x[n][0] * f0, x[n][1] * f0, x[n][2] * f1, x[n][3] * f1};
+      if (edge) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = x[n][k] == 0.0f ? 0.0f : w[k];
+      }
+      b0[n] = transpose8x8(packHalf(w[0], w[1]));
+      b1[n] = transpose8x8(packHalf(w[2], w[3]));
+      mma(u.ones[n][gr], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, b0[n], b1[n]);
+    }
+    const uint32_t x0 = __byte_perm(r.v[0][gr], r.v[1][gr], 0x5410), y0 = __byte_perm(r.v[0][gr], r.v[1][gr], 0x7632);
+    const uint32_t x1 = __byte_perm(r.v[2][gr], r.v[3][gr], 0x5410), y1 = __byte_perm(r.v[2][gr], r.v[3][gr], 0x7632);
+    const uint32_t xs0 = x0 >> 8, ys0 = y0 >> 8, xs1 = x1 >> 8, ys1 = y1 >> 8;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      mma(u.o[n][gr][0], x0 & 0x000F000Fu, y0 & 0x000F000Fu, x1 & 0x000F000Fu, y1 & 0x000F000Fu, b0[n], b1[n]);
+      mma(u.o[n][gr][1], x0 & 0x00F000F0u, y0 & 0x00F000F0u, x1 & 0x00F000F0u, y1 & 0x00F000F0u, b0[n], b1[n]);
+      mma(u.o[n][gr][2], xs0 & 0x000F000Fu, ys0 & 0x000F000Fu, xs1 & 0x000F000Fu, ys1 & 0x000F000Fu, b0[n], b1[n]);
+      mma(u.o[n][gr][3], xs0 & 0x00F000F0u, ys0 & 0x00F000F0u, xs1 & 0x00F000F0u, ys1 & 0x00F000F0u, b0[n], b1[n]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void storeOut(void* out, long long at, const float (&y)[8]) {
+  *reinterpret_cast<uint4*>(static_cast<T*>(out) + at) = pack8<T>(y);
+}
+
+// slot < 0: the unit is whole, write the result; else the partial sums.
+template <int G, int NT>
+__device__ __forceinline__ void finish(Unit<G, NT>& u, const AttnArgs& p, const Request& r, int head, int row0, int lane,
+                                       int slot) {
+  constexpr int D = 64 * G, R = 8 * NT;
+  const int g = lane >> 2, q = lane & 3;
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      float l = u.l[n][c], mid[G];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(~0u, l, o);
+#pragma unroll
+      for (int gr = 0; gr < G; gr++) {
+        mid[gr] = u.mid[n][gr][c];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mid[gr] += __shfl_xor_sync(~0u, mid[gr], o);
+      }
+      const int local = 8 * n + 2 * q + c;
+      const long long row = static_cast<long long>(row0) + local;
+      if (row >= static_cast<long long>(r.rows) * p.group) continue;
+      const int i = static_cast<int>(row / p.group), h = head * p.group + static_cast<int>(row % p.group);
+      const bool none = l == 0.0f;
+      const float norm = slot < 0 ? (none ? 0.0f : 1.0f / l) : 1.0f;
+#pragma unroll
+      for (int gr = 0; gr < G; gr++) {
+        const float back = 1.0f / u.inv[gr];
+        const float base = fmaf(-7.5f * u.ones[n][gr][c], back, mid[gr]);
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float f = (j & 1) ? 1048576.0f : 16777216.0f;
+          y[2 * j] = fmaf(u.o[n][gr][j][c] * f, back, base) * norm;
+          y[2 * j + 1] = fmaf(u.o[n][gr][j][2 + c] * f, back, base) * norm;
+        }
+        if (slot < 0) {
+          const long long at = (r.start + i) * p.oTok + h * p.oHead + 64 * gr + 8 * g;
+          if (p.half16) storeOut<__half>(p.out, at, y);
+          else storeOut<__nv_bfloat16>(p.out, at, y);
+        } else {
+          float* dst = p.partial + (static_cast<long long>(slot) * R + local) * D + 64 * gr + 8 * g;
+          *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<float4*>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
+        }
+      }
+      if (g == 0) {
+        if (slot >= 0) p.stats[static_cast<long long>(slot) * R + local] = make_float2(u.m[n][c], l);
+        else if (p.lse != nullptr)
+          p.lse[static_cast<long long>(r.start + i) * p.qHeads + h] = none ? -INFINITY : (u.m[n][c] + log2f(l)) * kLn2;
+      }
+    }
+}
+
+template <int G, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) attnKernel(AttnArgs p) {
+  extern __shared__ long long prefix[];
+  constexpr int R = 8 * NT;
+  scanTiles<kWarps * 32>(p, R, prefix);
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b <= p.batch; b += kWarps * 32) p.prefix[b] = prefix[b];
+  const long long total = prefix[p.batch];
+  if (total == 0) return;
+  const int lane = threadIdx.x & 31;
+  // Neighbouring ranges go to different blocks, so that few tiles spread over the SMs.
+  const int w = (threadIdx.x >> 5) * gridDim.x + blockIdx.x, workers = workersFor(p, total);
+  if (w >= workers) return;
+  const long long first = rangeStart(w, total, workers), last = rangeStart(w + 1, total, workers);
+  long long tile = first;
+  while (tile < last) {
+    const int b = findRequest(prefix, p.batch, tile);
+    const Request r = requestOf(p, b);
+    const int nt = tilesOf(r), units = unitsOf(p, r, R);
+    const long long off = tile - prefix[b];
+    const int unit = static_cast<int>(off / nt), from = static_cast<int>(off % nt);
+    const int head = unit / units, row0 = (unit % units) * R;
+    const int upto = static_cast<int>(min(static_cast<long long>(nt), from + (last - tile)));
+
+    Unit<G, NT> u;
+    loadQuery<G, NT>(u, p, r, head, row0, lane);
+    // Blocks of this range that some row sees; page numbers come 32 blocks at a time.
+    const int end = min(upto * (kTile / kv4::kBlockTokens), (u.most + kv4::kBlockTokens - 1) / kv4::kBlockTokens);
+    for (int base = from * (kTile / kv4::kBlockTokens); base < end; base += 32) {
+      const int mine = base + lane;
+      int page = -1;
+      if (mine < end) page = p.table[static_cast<long long>(b) * p.width + mine / p.blocksPerPage];
+      const int count = min(32, end - base);
+      BlockRegs<G> regs[2];
+      auto fetch = [&](BlockRegs<G>& to, int k) {
+        const int pg = __shfl_sync(~0u, page, k);
+        const bool ok = pg >= 0 && pg < p.pages;
+        if (ok)
+          loadBlock<G>(to,
+                       p.cache + ((static_cast<long long>(pg) * p.kvHeads + head) * p.blocksPerPage +
+                                  (base + k) % p.blocksPerPage) * kv4::blockBytes(64 * G),
+                       lane);
+        return ok;
+      };
+      bool ok0 = fetch(regs[0], 0), ok1 = false;
+      for (int k = 0; k < count; k += 2) {
+        if (k + 1 < count) ok1 = fetch(regs[1], k + 1);
+        if (ok0) blockStep<G, NT>(u, regs[0], (base + k) * kv4::kBlockTokens, lane);
+        if (k + 2 < count) ok0 = fetch(regs[0], k + 2);
+        if (k + 1 < count && ok1) blockStep<G, NT>(u, regs[1], (base + k + 1) * kv4::kBlockTokens, lane);
+      }
+    }
+    const bool whole = from == 0 && upto == nt;
+    // A range has at most two partial units: the one it starts in, and the one it ends in.
+    finish<G, NT>(u, p, r, head, row0, lane, whole ? -1 : tile == first ? 2 * w : 2 * w + 1);
+    tile += upto - from;
+  }
+}
+
+// Joins the partial sums of every row whose unit was cut, and clears the rows
+// that see nothing or stand behind the last request.  A warp takes one row.
+template <int G>
+__global__ void __launch_bounds__(128) joinKernel(AttnArgs p, int R) {
+  constexpr int D = 64 * G;
+  const int lane = threadIdx.x & 31;
+  const long long id = blockIdx.x * 4LL + (threadIdx.x >> 5);
+  if (id >= static_cast<long long>(p.tokens) * p.qHeads) return;
+  const int t = static_cast<int>(id / p.qHeads), h = static_cast<int>(id % p.qHeads);
+  int lo = 0, hi = p.batch;  // the first request that ends behind t
+  while (lo < hi) {
+    const int m = (lo + hi) >> 1;
+    if (p.qStarts[m + 1] > t) hi = m;
+    else lo = m + 1;
+  }
+  float y[2 * G] = {};
+  float m = kNone, l = 0.0f;
+  const Request r = lo < p.batch ? requestOf(p, lo) : Request{0, 0, 0};
+  if (t < r.start || t >= r.start + r.rows) {
+    if (!p.zeroTail) return;
+  } else {
+    const int nt = tilesOf(r);
+    if (nt > 0) {
+      const int row = (t - r.start) * p.group + h % p.group, units = unitsOf(p, r, R);
+      const long long total = p.prefix[p.batch];
+      const long long a = p.prefix[lo] + (static_cast<long long>(h / p.group) * units + row / R) * nt;
+      const int workers = workersFor(p, total);
+      const int w0 = workerOf(a, total, workers), w1 = workerOf(a + nt - 1, total, workers);
+      if (w0 == w1) return;  // written by its warp
+      for (int w = w0; w <= w1; w++) {
+        const long long slot = 2LL * w + (rangeStart(w, total, workers) < a ? 1 : 0);
+        const float2 st = p.stats[slot * R + row % R];
+        const float top = fmaxf(m, st.x);
+        const float old = exp2Fast(m - top), add = exp2Fast(st.x - top);
+        m = top;
+        l = l * old + st.y * add;
+        const float2* src = reinterpret_cast<const float2*>(p.partial + (slot * R + row % R) * D) + lane;
+#pragma unroll
+        for (int gr = 0; gr < G; gr++) {
+          const float2 v = src[32 * gr];
+          y[2 * gr] = y[2 * gr] * old + v.x * add;
+          y[2 * gr + 1] = y[2 * gr + 1] * old + v.y * add;
+        }
+      }
+    }
+  }
+  const bool none = l == 0.0f;
+  const float norm = none ? 0.0f : 1.0f / l;
+  const long long at = t * p.oTok + h * p.oHead + 2 * lane;
+#pragma unroll
+  for (int gr = 0; gr < G; gr++) {
+    if (p.half16) *reinterpret_cast<__half2*>(static_cast<__half*>(p.out) + at + 64 * gr) = __floats2half2_rn(y[2 * gr] * norm, y[2 * gr + 1] * norm);
+    else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) + at + 64 * gr) = __floats2bfloat162_rn(y[2 * gr] * norm, y[2 * gr + 1] * norm);
+  }
+  if (lane == 0 && p.lse != nullptr) p.lse[static_cast<long long>(t) * p.qHeads + h] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+int smsOfDevice() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
+}
+
+// Two tiles of 8 query rows where a request brings more than 8 rows of a key
+// head on average (a warp then reads the cache once for 16 rows).
+int rowTiles(int batch, int tokens, int group) {
+  return group > 8 || static_cast<long long>(tokens) * group > 8LL * batch ? 2 : 1;
+}
+
+size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+}  // namespace
+}  // namespace model
+}  // namespace vccl
+
+using namespace vccl;
+using namespace vccl::model;
+
+extern "C" {
+
+size_t vcclKv4AttentionWorkspace(int batch, int tokens, int qHeads, int kvHeads, int D) {
+  if (batch <= 0 || kvHeads <= 0 || qHeads <= 0 || D <= 0) return 0;
+  const int nt = rowTiles(batch, tokens, qHeads / kvHeads);
+  const size_t slots = static_cast<size_t>(smsOfDevice()) * (nt == 1 ? 3 : 2) * kWarps * 2;
+  return align256((batch + 1) * sizeof(long long)) + align256(slots * 8 * nt * sizeof(float2)) +
+         slots * 8 * nt * D * sizeof(float);
+}
+
+vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, const int* table, int width,
+                              const int* kvLens, const int* qStarts, int batch, int tokens, float scale,
+                              const vcclHeads_t* out, float* lse, int zeroTail, void* workspace,
+                              vcclDataType_t datatype, vcclStream_t stream) {
+  if (cache == nullptr || cache->data == nullptr || (reinterpret_cast<uintptr_t>(cache->data) & 15u) != 0 ||
+      cache->pages <= 0 || cache->pageSize <= 0 || cache->pageSize % kv4::kBlockTokens != 0 || cache->kvHeads <= 0 ||
+      (cache->D != 64 && cache->D != 128) || tokens < 0 || batch <= 0 || batch > kMaxBatch || width <= 0 ||
+      static_cast<long long>(width) * cache->pageSize > INT_MAX ||
+      (datatype != vcclBfloat16 && datatype != vcclFloat16))
+    return vcclInvalidArgument;
+  if (tokens == 0) return vcclSuccess;
+  if (!headsOk(q, 2) || !headsOk(out, 2) || q->heads != out->heads || q->heads % cache->kvHeads != 0 || !table ||
+      !kvLens || !qStarts || !workspace || static_cast<long long>(tokens) * q->heads > INT_MAX)
+    return vcclInvalidArgument;
+  TraceRange trace("vccl Kv4Attention");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int group = q->heads / cache->kvHeads, nt = rowTiles(batch, tokens, group), R = 8 * nt;
+  const int grid = smsOfDevice() * (nt == 1 ? 3 : 2);
+  AttnArgs p{};
+  p.q = q->data;
+  p.qTok = q->tokenStride;
+  p.qHead = q->headStride;
+  p.cache = static_cast<const uint8_t*>(cache->data);
+  p.table = table;
+  p.kvLens = kvLens;
+  p.qStarts = qStarts;
+  p.out = out->data;
+  p.oTok = out->tokenStride;
+  p.oHead = out->headStride;
+  p.lse = lse;
+  p.width = width;
+  p.batch = batch;
+  p.tokens = tokens;
+  p.qHeads = q->heads;
+  p.kvHeads = cache->kvHeads;
+  p.group = group;
+  p.pages = cache->pages;
+  p.blocksPerPage = cache->pageSize / kv4::kBlockTokens;
+  p.workers = grid * kWarps;
+  p.half16 = datatype == vcclFloat16;
+  p.zeroTail = zeroTail;
+  p.scaleLog2 = scale * 1.44269504088896340736f;
+  char* ws = static_cast<char*>(workspace);
+  p.prefix = reinterpret_cast<long long*>(ws);
+  ws += align256((batch + 1) * sizeof(long long));
+  p.stats = reinterpret_cast<float2*>(ws);
+  ws += align256(static_cast<size_t>(p.workers) * 2 * R * sizeof(float2));
+  p.partial = reinterpret_cast<float*>(ws);
+  const size_t smem = static_cast<size_t>(batch + 1) * sizeof(long long);
+  if (cache->D == 128) {
+    if (nt == 1) attnKernel<2, 1><<<grid, kWarps * 32, smem, st>>>(p);
+    else attnKernel<2, 2><<<grid, kWarps * 32, smem, st>>>(p);
+  } else {
+    if (nt == 1) attnKernel<1, 1><<<grid, kWarps * 32, smem, st>>>(p);
+    else attnKernel<1, 2><<<grid, kWarps * 32, smem, st>>>(p);
+  }
+  const int rows = static_cast<int>((static_cast<long long>(tokens) * q->heads + 3) / 4);
+  if (cache->D == 128) joinKernel<2><<<rows, 128, 0, st>>>(p, R);
+  else joinKernel<1><<<rows, 128, 0, st>>>(p, R);
+  return launched("vcclKv4Attention");
+}
+
+}  // extern "C"

@@ -135,7 +135,7 @@ def _declare(h: ctypes.CDLL) -> None:
 
 
 def _declare_extensions(h: ctypes.CDLL) -> None:
-    """Fused tensor-parallel entry points (vccl_tp.h), when built."""
+    """Fused tensor-parallel and model entry points (vccl_tp.h, vccl_model.h), when built."""
     c = ctypes
     P, I, Z, F = c.c_void_p, c.c_int, c.c_size_t, c.c_float
     ext = {
@@ -152,9 +152,22 @@ def _declare_extensions(h: ctypes.CDLL) -> None:
         "vcclAllGatherGemm": [P, P, P, I, I, I, I, P, P],
         "vcclMoeDispatchFp8": [P, P, P, P, P, P, P, I, I, I, I, I, P, P],
         "vcclMoeCombine": [P, P, P, P, P, I, I, I, I, P, P],
+        # vccl_model.h
+        "vcclPagePlan": [P, P, P, P, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P],
+        "vcclQkNormRope": [P, P, P, P, P, I, I, I, P],
+        "vcclQkNormRopeBackward": [P, P, P, P, P, P, P, P, P, P, I, I, I, P],
+        "vcclKv4Append": [P, P, P, P, P, P, P, I, I, P],
+        "vcclKv4Read": [P, P, P, P, I, I, P],
+        "vcclKv4Attention": [P, P, P, I, P, P, I, I, F, P, P, I, P, I, P],
     }
     for name, args in ext.items():
         fn = getattr(h, name, None)
         if fn is not None:
             fn.argtypes = args
             fn.restype = c.c_int
+    sizes = {"vcclQkNormRopeBackwardWorkspace": [I], "vcclKv4AttentionWorkspace": [I, I, I, I, I]}
+    for name, args in sizes.items():
+        fn = getattr(h, name, None)
+        if fn is not None:
+            fn.argtypes = args
+            fn.restype = Z

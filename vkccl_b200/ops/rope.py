@@ -1,0 +1,96 @@
+# SPDX-License-Identifier: Apache-2.0
+"""RMS norm of query and key heads and the position rotation, in one pass.
+
+qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None)
+    x / sqrt(mean(x^2) + eps) * weight for every head where a weight is given,
+    then the first 2 * len(inv_freq) channels rotate by position * inv_freq.
+qk_norm_rope_backward(dq, dk, q, k, positions, inv_freq, ...)
+    its gradients, with those of the weights.
+
+Tensors are [tokens, heads, head dim] in bf16 or fp16, with any token and head
+strides that are multiples of 8 elements: slices of one projection's output
+need no copy.  The angle is taken in 64 bits, so far positions keep it.
+"""
+
+from __future__ import annotations
+
+from ctypes import byref
+from typing import Optional, Tuple
+
+import torch
+
+from vkccl_b200._lib import lib
+from vkccl_b200.comm import _check
+from vkccl_b200.ops._args import DTYPES, float16s, heads, on_device, rope_of, stream
+
+
+def _dim(q: torch.Tensor) -> int:
+    float16s(q, "q")
+    dim = q.shape[2]
+    if dim % 8 or not 16 <= dim <= 256:
+        raise ValueError(f"the head dimension must be a multiple of 8 from 16 to 256, got {dim}")
+    return dim
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
+                 k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Norm and rotation of q [T, q heads, D] and k [T, k heads, D].
+
+    positions [T] int32, inv_freq f32 [rotated / 2] (a multiple of 8), weights
+    [D] in q's type or None (no norm).  interleaved: channels (2j, 2j + 1) turn
+    together, else (j, j + rotated / 2).  An output may be its input; it must
+    not overlap it in another way.
+    """
+    dim = _dim(q)
+    dev, dtype, t = q.device, q.dtype, q.shape[0]
+    hq, hk = heads(q, "q", dtype, dev, t, dim), heads(k, "k", dtype, dev, t, dim)
+    rope = rope_of(positions, inv_freq, q_weight, k_weight, eps, interleaved, dtype, dev, t, dim)
+    if q_out is None:
+        q_out = torch.empty((t, hq.heads, dim), dtype=dtype, device=dev)
+    if k_out is None:
+        k_out = torch.empty((t, hk.heads, dim), dtype=dtype, device=dev)
+    oq = heads(q_out, "q_out", dtype, dev, t, dim, hq.heads, written=True)
+    ok = heads(k_out, "k_out", dtype, dev, t, dim, hk.heads, written=True)
+    with on_device(dev):
+        _check(lib().vcclQkNormRope(byref(hq), byref(hk), byref(rope), byref(oq), byref(ok), t, dim, DTYPES[dtype],
+                                    stream(dev)), "vcclQkNormRope")
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
+                          inv_freq: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                          k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                          dq_in: Optional[torch.Tensor] = None, dk_in: Optional[torch.Tensor] = None
+                          ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """Gradients of ``qk_norm_rope`` from dq, dk (of its outputs) and q, k (its inputs).
+
+    Returns (dq_in, dk_in, dq_weight, dk_weight); a weight's gradient is None
+    where there is no weight.  The sums over tokens and heads are f32 (their
+    join f64) in a fixed order: the same bits on every run.  dq_in may be dq,
+    dk_in may be dk.
+    """
+    dim = _dim(q)
+    dev, dtype, t = q.device, q.dtype, q.shape[0]
+    hq, hk = heads(q, "q", dtype, dev, t, dim), heads(k, "k", dtype, dev, t, dim)
+    gq, gk = heads(dq, "dq", dtype, dev, t, dim, hq.heads), heads(dk, "dk", dtype, dev, t, dim, hk.heads)
+    rope = rope_of(positions, inv_freq, q_weight, k_weight, eps, interleaved, dtype, dev, t, dim)
+    if dq_in is None:
+        dq_in = torch.empty((t, hq.heads, dim), dtype=dtype, device=dev)
+    if dk_in is None:
+        dk_in = torch.empty((t, hk.heads, dim), dtype=dtype, device=dev)
+    oq = heads(dq_in, "dq_in", dtype, dev, t, dim, hq.heads, written=True)
+    ok = heads(dk_in, "dk_in", dtype, dev, t, dim, hk.heads, written=True)
+    dwq = None if q_weight is None else torch.empty(dim, dtype=dtype, device=dev)
+    dwk = None if k_weight is None else torch.empty(dim, dtype=dtype, device=dev)
+    ws = None
+    if q_weight is not None or k_weight is not None:
+        ws = torch.empty(lib().vcclQkNormRopeBackwardWorkspace(dim), dtype=torch.uint8, device=dev)
+    with on_device(dev):
+        _check(lib().vcclQkNormRopeBackward(byref(gq), byref(gk), byref(hq), byref(hk), byref(rope), byref(oq), byref(ok),
+                                            None if dwq is None else dwq.data_ptr(),
+                                            None if dwk is None else dwk.data_ptr(),
+                                            None if ws is None else ws.data_ptr(), t, dim, DTYPES[dtype], stream(dev)),
+               "vcclQkNormRopeBackward")
+    return dq_in, dk_in, dwq, dwk
