@@ -42,12 +42,15 @@ __device__ __forceinline__ uint8_t* cacheBlock(const Cache& c, int slot, int hea
                       kv4::blockBytes(c.D);
 }
 
-// cos and sin of position * f: k turns of 2 pi are taken off in 64 bits.
+// cos and sin of position * f, in 64 bits: k turns of 2 pi are taken off
+// first (positions reach millions, and a large argument would cost more).
 __device__ __forceinline__ void cosSin(int position, float f, float* c, float* s) {
   const double a = static_cast<double>(position) * static_cast<double>(f);
   const double turns = rint(a * 0.15915494309189533577);
-  const double r = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586477, a));
-  sincosf(static_cast<float>(r), s, c);
+  double sd, cd;
+  sincos(fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586477, a)), &sd, &cd);
+  *c = static_cast<float>(cd);
+  *s = static_cast<float>(sd);
 }
 
 // cos and sin of tokens [t0, t0 + n) into smem: cos at [i * half + j], sin at
@@ -74,8 +77,8 @@ __device__ __forceinline__ void rotate(float (&x)[8], int lane, const Rope& r, c
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const float a = x[2 * i], b = x[2 * i + 1];
-        x[2 * i] = a * cc[i] - b * ss[i];
-        x[2 * i + 1] = b * cc[i] + a * ss[i];
+        x[2 * i] = __fsub_rn(__fmul_rn(a, cc[i]), __fmul_rn(b, ss[i]));
+        x[2 * i + 1] = __fadd_rn(__fmul_rn(b, cc[i]), __fmul_rn(a, ss[i]));
       }
     }
     return;
@@ -94,9 +97,21 @@ __device__ __forceinline__ void rotate(float (&x)[8], int lane, const Rope& r, c
       const float4 s = *reinterpret_cast<const float4*>(sinv + j + 4 * v);
       const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[4 * v + i] = x[4 * v + i] * cc[i] + sg * y[4 * v + i] * ss[i];
+      for (int i = 0; i < 4; i++) x[4 * v + i] = __fadd_rn(__fmul_rn(x[4 * v + i], cc[i]), __fmul_rn(sg * y[4 * v + i], ss[i]));
     }
   }
+}
+
+// Sum of a lane's squares: fours in order.
+__device__ __forceinline__ float squares8(const float (&x)[8]) {
+  float s[2];
+#pragma unroll
+  for (int v = 0; v < 2; v++) {
+    s[v] = __fmul_rn(x[4 * v], x[4 * v]);
+#pragma unroll
+    for (int i = 1; i < 4; i++) s[v] = __fadd_rn(s[v], __fmul_rn(x[4 * v + i], x[4 * v + i]));
+  }
+  return __fadd_rn(s[0], s[1]);
 }
 
 template <int LANES>
@@ -115,88 +130,100 @@ struct ForwardArgs {
   int tokens, D, tpb;
 };
 
+// The rows of a block in steps: token and head without a division.
+struct RowWalk {
+  int t, h, dt, dh, heads;
+  __device__ __forceinline__ RowWalk(int row, int step, int heads_)
+      : t(row / heads_), h(row % heads_), dt(step / heads_), dh(step % heads_), heads(heads_) {}
+  __device__ __forceinline__ void next() {
+    t += dt;
+    h += dh;
+    if (h >= heads) {
+      h -= heads;
+      t++;
+    }
+  }
+};
+
 // Block: tpb tokens, all their heads (queries, keys, values in that order).
+// Norm and rotation round after every f32 operation (no contraction), so that
+// the fused write gives the bits of the two calls it stands for.
 template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) forwardKernel(ForwardArgs p) {
+__global__ void __launch_bounds__(kThreads, 4) forwardKernel(ForwardArgs p) {
   extern __shared__ float angles[];
+  constexpr int kRows = kThreads / LANES;
   const int t0 = blockIdx.x * p.tpb, n = min(p.tpb, p.tokens - t0);
+  const int lane = threadIdx.x % LANES;
+  const bool active = 8 * lane < p.D;
+  const int nq = p.in[0].heads, nk = p.in[1].heads;
+  const int rows = n * (nq + nk + p.in[2].heads);
+  RowWalk at(threadIdx.x / LANES, kRows, nq + nk + p.in[2].heads);
+
+  // The next row is under way while one is worked on.
+  auto load = [&]() {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (at.t < n && active) {
+      const int which = (at.h >= nq) + (at.h >= nq + nk), h = at.h - (which > 0 ? nq : 0) - (which > 1 ? nk : 0);
+      const Heads& in = p.in[which];
+      v = *reinterpret_cast<const uint4*>(static_cast<const T*>(in.data) + (t0 + at.t) * in.tok + h * in.head + 8 * lane);
+    }
+    return v;
+  };
+  uint4 ahead = load();
+  uint4 weight[2] = {};
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+    if (p.rope.weight[i] != nullptr && active)
+      weight[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.rope.weight[i]) + 8 * lane);
+  const bool normed = p.rope.weight[0] != nullptr || p.rope.weight[1] != nullptr;
   if (p.rope.half > 0) {
     fillAngles(p.rope, t0, n, p.tpb, angles);
     __syncthreads();
   }
-  constexpr int kRows = kThreads / LANES;
-  const int lane = threadIdx.x % LANES, row0 = threadIdx.x / LANES;
-  const bool active = 8 * lane < p.D;
-  const int heads = p.in[0].heads + p.in[1].heads + p.in[2].heads;
-  const int rows = n * heads;
+  const float share = 1.0f / p.D;
   // Whole warps step together: a row behind the last one is masked.
   for (int base = 0; base < rows; base += kRows) {
-    const int row = base + row0;
-    const bool live = row < rows && active;
-    const int t = row < rows ? row / heads : 0;
-    int h = row < rows ? row % heads : 0, which = 0;
-    if (h >= p.in[0].heads) {
-      h -= p.in[0].heads;
-      which = 1;
-      if (h >= p.in[1].heads) {
-        h -= p.in[1].heads;
-        which = 2;
+    const int t = at.t, which = (at.h >= nq) + (at.h >= nq + nk);
+    const int h = at.h - (which > 0 ? nq : 0) - (which > 1 ? nk : 0);
+    const bool live = t < n && active;
+    uint4 raw = ahead;
+    at.next();
+    if (base + kRows < rows) ahead = load();
+    if (__any_sync(~0u, which < 2)) {
+      float x[8];
+      unpack8<T>(raw, x);
+      if (normed) {
+        const float r = rsqrtf(__fadd_rn(__fmul_rn(rowSum<LANES>(squares8(x)), share), p.rope.eps));
+        if (which < 2 && p.rope.weight[which] != nullptr) {
+          float w[8];
+          unpack8<T>(which ? weight[1] : weight[0], w);
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
+        }
       }
-    }
-    float x[8] = {};
-    if (live) {
-      const Heads& in = p.in[which];
-      const T* src = static_cast<const T*>(in.data) + (t0 + t) * in.tok + h * in.head + 8 * lane;
-      unpack8<T>(*reinterpret_cast<const uint4*>(src), x);
-    }
-    // Every lane of the warp takes part in the shuffles; rows of values (and
-    // rows without a weight or an angle) keep their channels.
-    const void* wp = which < 2 ? p.rope.weight[which] : nullptr;
-    if (p.rope.weight[0] != nullptr || p.rope.weight[1] != nullptr) {
-      float sq = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; i++) sq += x[i] * x[i];
-      sq = rowSum<LANES>(sq);
-      if (wp != nullptr && active) {
-        const float r = rsqrtf(sq / p.D + p.rope.eps);
-        float w[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(wp) + 8 * lane), w);
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = x[i] * r * w[i];
+      if (p.rope.half > 0) {
+        const float* c = angles + min(t, n - 1) * p.rope.half;
+        rotate<LANES>(x, lane, p.rope, c, c + p.tpb * p.rope.half, 1.0f);
+        // a row of values shares the warp, and keeps its bits
+        if (which < 2) raw = pack8<T>(x);
       }
-    }
-    if (p.rope.half > 0) {
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; i++) y[i] = x[i];
-      rotate<LANES>(y, lane, p.rope, angles + t * p.rope.half, angles + (p.tpb + t) * p.rope.half, 1.0f);
-      if (which < 2) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = y[i];
-      }
-    }
-    if (which < 2 && p.out[which].data != nullptr) {
-      if (live) {
+      if (which < 2 && live && p.out[which].data != nullptr) {
         const Heads& out = p.out[which];
-        *reinterpret_cast<uint4*>(static_cast<T*>(out.data) + (t0 + t) * out.tok + h * out.head + 8 * lane) = pack8<T>(x);
+        *reinterpret_cast<uint4*>(static_cast<T*>(out.data) + (t0 + t) * out.tok + h * out.head + 8 * lane) = raw;
       }
     }
-    if (p.cache.data != nullptr) {
-      // The keys as the model's type holds them (values are read in it).
-      const uint4 v = pack8<T>(x);
-      unpack8<T>(v, x);
+    if (p.cache.data != nullptr && __any_sync(~0u, which > 0)) {
       uint32_t params;
-      const uint32_t word = kv4::quantise8(x, ~0u, &params);
+      const uint32_t word = kv4::quantise8<T>(raw, &params);
       const int slot = which > 0 && live ? p.slots[t0 + t] : -1;
       if (slot >= 0 && slot < p.cache.tokens) {
         uint8_t* blk = cacheBlock(p.cache, slot, h);
-        const int at = slot & 15, G = p.D / kv4::kGroup, g = lane >> 3, b = lane & 7;
+        const int place = slot & 15, G = p.D / kv4::kGroup, g = lane >> 3, b = lane & 7;
         const bool keys = which == 1;
-        const int rowAt = keys ? at : 16 + kv4::valueRow(at);
+        const int rowAt = keys ? place : 16 + kv4::valueRow(place);
         const int wordAt = keys ? kv4::keyWord(b, g, G) : kv4::valueWord(b, g, G);
         *reinterpret_cast<uint32_t*>(blk + rowAt * (p.D / 2) + 4 * wordAt) = word;
-        if (b == 0)
-          *reinterpret_cast<uint32_t*>(blk + (keys ? 16 : 17) * p.D + at * (4 * G) + 4 * g) = params;
+        if (b == 0) *reinterpret_cast<uint32_t*>(blk + (keys ? 16 : 17) * p.D + place * (4 * G) + 4 * g) = params;
       }
     }
   }
@@ -206,7 +233,7 @@ struct ReadArgs {
   Cache cache;
   const int* slots;
   Heads out[2];
-  int tokens;
+  int tokens, tpb;
 };
 
 template <typename T>
@@ -219,30 +246,29 @@ __device__ __forceinline__ void store8<float>(float* dst, const float (&x)[8]) {
   *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-template <typename T>
+// Block: tpb tokens, their keys and then their values.
+template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads) readKernel(ReadArgs p) {
-  const int lanes = p.cache.D / 8, heads = p.cache.heads;
-  const long long total = static_cast<long long>(p.tokens) * 2 * heads * lanes;
-  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < total;
-       i += static_cast<long long>(gridDim.x) * kThreads) {
-    const int lane = static_cast<int>(i % lanes);
-    const long long row = i / lanes;
-    const int hh = static_cast<int>(row % (2 * heads)), t = static_cast<int>(row / (2 * heads));
-    const bool keys = hh < heads;
-    const int h = keys ? hh : hh - heads;
-    const int slot = p.slots[t];
+  constexpr int kRows = kThreads / LANES, D = 8 * LANES, G = D / kv4::kGroup;
+  const int t0 = blockIdx.x * p.tpb, n = min(p.tpb, p.tokens - t0);
+  const int lane = threadIdx.x % LANES, g = lane >> 3, b = lane & 7, heads = p.cache.heads;
+  RowWalk at(threadIdx.x / LANES, kRows, 2 * heads);
+  for (; at.t < n; at.next()) {
+    const bool keys = at.h < heads;
+    const int h = keys ? at.h : at.h - heads;
+    const int slot = p.slots[t0 + at.t];
     float x[8] = {};
     if (slot >= 0 && slot < p.cache.tokens) {
       const uint8_t* blk = cacheBlock(p.cache, slot, h);
-      const int D = p.cache.D, at = slot & 15, G = D / kv4::kGroup, g = lane >> 3, b = lane & 7;
-      const int rowAt = keys ? at : 16 + kv4::valueRow(at);
+      const int place = slot & 15;
+      const int rowAt = keys ? place : 16 + kv4::valueRow(place);
       const int wordAt = keys ? kv4::keyWord(b, g, G) : kv4::valueWord(b, g, G);
       const uint32_t word = *reinterpret_cast<const uint32_t*>(blk + rowAt * (D / 2) + 4 * wordAt);
-      const uint32_t params = *reinterpret_cast<const uint32_t*>(blk + (keys ? 16 : 17) * D + at * (4 * G) + 4 * g);
+      const uint32_t params = *reinterpret_cast<const uint32_t*>(blk + (keys ? 16 : 17) * D + place * (4 * G) + 4 * g);
       kv4::dequantise8(word, params, x);
     }
-    const Heads& out = p.out[keys ? 0 : 1];
-    store8<T>(static_cast<T*>(out.data) + t * out.tok + h * out.head + 8 * lane, x);
+    const Heads& out = keys ? p.out[0] : p.out[1];
+    store8<T>(static_cast<T*>(out.data) + (t0 + at.t) * out.tok + h * out.head + 8 * lane, x);
   }
 }
 
@@ -260,60 +286,77 @@ constexpr int kBackwardBlocks = 148 * 4;
 // dx = r (w g - x^ mean(w g x^)), dw = sum g x^ with g = R^-1 dy, x^ = x r,
 // r = 1 / sqrt(mean x^2 + eps).
 template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) backwardKernel(BackwardArgs p) {
+__global__ void __launch_bounds__(kThreads, 3) backwardKernel(BackwardArgs p) {
   extern __shared__ float angles[];
   constexpr int kRows = kThreads / LANES;
   const int lane = threadIdx.x % LANES, row0 = threadIdx.x / LANES;
   const bool active = 8 * lane < p.D;
-  const int heads = p.x[0].heads + p.x[1].heads;
+  const int nq = p.x[0].heads, heads = nq + p.x[1].heads;
+  const float share = 1.0f / p.D;
+  const bool normed = p.rope.weight[0] != nullptr || p.rope.weight[1] != nullptr;
+  uint4 weight[2] = {};
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+    if (p.rope.weight[i] != nullptr && active)
+      weight[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.rope.weight[i]) + 8 * lane);
   float dw[2][8] = {};
   for (int t0 = blockIdx.x * p.tpb; t0 < p.tokens; t0 += gridDim.x * p.tpb) {
-    const int n = min(p.tpb, p.tokens - t0);
+    const int n = min(p.tpb, p.tokens - t0), rows = n * heads;
+    RowWalk at(row0, kRows, heads);
+    // The next row is under way while one is worked on.
+    auto load = [&](uint4& dy, uint4& x) {
+      dy = x = make_uint4(0, 0, 0, 0);
+      if (at.t < n && active) {
+        const int which = at.h >= nq, h = at.h - (which ? nq : 0);
+        const Heads& a = p.dy[which];
+        dy = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.data) + (t0 + at.t) * a.tok + h * a.head + 8 * lane);
+        if (p.rope.weight[which] != nullptr) {
+          const Heads& b = p.x[which];
+          x = *reinterpret_cast<const uint4*>(static_cast<const T*>(b.data) + (t0 + at.t) * b.tok + h * b.head + 8 * lane);
+        }
+      }
+    };
+    uint4 dyAhead, xAhead;
+    load(dyAhead, xAhead);
     __syncthreads();  // the angles of the tokens before are read
     fillAngles(p.rope, t0, n, p.tpb, angles);
     __syncthreads();
-    const int rows = n * heads;
     for (int base = 0; base < rows; base += kRows) {
-      const int row = base + row0;
-      const bool live = row < rows && active;
-      const int t = row < rows ? row / heads : 0;
-      int h = row < rows ? row % heads : 0;
-      const int which = h >= p.x[0].heads;
-      if (which) h -= p.x[0].heads;
-      float g[8] = {}, x[8] = {};
-      const void* wp = p.rope.weight[which];
-      if (live) {
-        const Heads& a = p.dy[which];
-        unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.data) + (t0 + t) * a.tok + h * a.head + 8 * lane), g);
-        if (wp != nullptr) {
-          const Heads& b = p.x[which];
-          unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(b.data) + (t0 + t) * b.tok + h * b.head + 8 * lane), x);
-        }
-      }
-      rotate<LANES>(g, lane, p.rope, angles + t * p.rope.half, angles + (p.tpb + t) * p.rope.half, -1.0f);
-      if (p.rope.weight[0] != nullptr || p.rope.weight[1] != nullptr) {
-        float w[8] = {};
-        if (wp != nullptr && active)
-          unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(wp) + 8 * lane), w);
-        float sq = 0.0f, gx = 0.0f;
+      const int t = at.t, which = at.h >= nq, h = at.h - (which ? nq : 0);
+      const bool live = t < n && active;
+      float g[8], x[8];
+      unpack8<T>(dyAhead, g);
+      unpack8<T>(xAhead, x);
+      at.next();
+      if (base + kRows < rows) load(dyAhead, xAhead);
+      const float* c = angles + min(t, n - 1) * p.rope.half;
+      rotate<LANES>(g, lane, p.rope, c, c + p.tpb * p.rope.half, -1.0f);
+      if (normed) {
+        float w[8], wg[8];
+        unpack8<T>(which ? weight[1] : weight[0], w);
+        float gx = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          sq += x[i] * x[i];
-          gx += g[i] * w[i] * x[i];
+          wg[i] = g[i] * w[i];
+          gx += wg[i] * x[i];
         }
-        sq = rowSum<LANES>(sq);
-        gx = rowSum<LANES>(gx);
-        if (wp != nullptr) {
-          const float r = rsqrtf(sq / p.D + p.rope.eps);
-          const float m = gx * r / p.D;  // mean(w g x^)
+        float sq = squares8(x);
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) {
+          sq += __shfl_xor_sync(~0u, sq, o);
+          gx += __shfl_xor_sync(~0u, gx, o);
+        }
+        if (p.rope.weight[which] != nullptr) {
+          const float r = rsqrtf(sq * share + p.rope.eps);
+          const float m = gx * r * share;  // mean(w g x^)
+          const float on = live ? r : 0.0f;
+          // A row behind the last one counts as zero (its r may be infinite).
 #pragma unroll
           for (int i = 0; i < 8; i++) {
-            const float xh = x[i] * r;
-            if (live) {  // a row behind the last one may hold 0 * inf
-              if (which) dw[1][i] += g[i] * xh;
-              else dw[0][i] += g[i] * xh;
-            }
-            g[i] = r * (g[i] * w[i] - xh * m);
+            const float xh = x[i] * on;
+            if (which) dw[1][i] += g[i] * xh;
+            else dw[0][i] += g[i] * xh;
+            g[i] = r * (wg[i] - xh * m);
           }
         }
       }
@@ -360,12 +403,12 @@ __global__ void weightGradKernel(const float* partial, int blocks, int D, T* dqw
 
 int lanesFor(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
-// Tokens a block takes: about four rows for every group of lanes, so that
-// the angles are shared and loads overlap, but no fewer blocks than SMs.
+// Tokens a block takes: enough rows for a dozen steps, so that the angles are
+// shared and loads overlap, but no fewer blocks than twice the SMs.
 int tokensPerBlock(int tokens, int heads, int D) {
   const int rows = kThreads / lanesFor(D);
   int tpb = 1;
-  while (tpb < 16 && tpb * heads < 4 * rows && tokens / (2 * tpb) >= 148) tpb *= 2;
+  while (tpb < 16 && tpb * heads < 12 * rows && tokens / (2 * tpb) >= 2 * 148) tpb *= 2;
   return tpb;
 }
 
@@ -402,6 +445,12 @@ void launchBackward(const BackwardArgs& p, int grid, cudaStream_t st) {
     case 16: backwardKernel<T, 16><<<grid, kThreads, smem, st>>>(p); break;
     default: backwardKernel<T, 32><<<grid, kThreads, smem, st>>>(p); break;
   }
+}
+
+template <typename T>
+void launchRead(const ReadArgs& p, int grid, cudaStream_t st) {
+  if (p.cache.D == 64) readKernel<T, 8><<<grid, kThreads, 0, st>>>(p);
+  else readKernel<T, 16><<<grid, kThreads, 0, st>>>(p);
 }
 
 bool sixteenBit(vcclDataType_t t) { return t == vcclBfloat16 || t == vcclFloat16; }
@@ -539,14 +588,13 @@ vcclResult_t vcclKv4Read(const vcclKv4_t* cache, const int* slots, const vcclHea
       v->heads != cache->kvHeads)
     return vcclInvalidArgument;
   TraceRange trace("vccl Kv4Read");
-  const ReadArgs p{cacheOf(cache), slots, {headsOf(k), headsOf(v)}, tokens};
-  const long long work = static_cast<long long>(tokens) * 2 * cache->kvHeads * (cache->D / 8);
-  const long long blocks = (work + kThreads - 1) / kThreads;
-  const int grid = static_cast<int>(blocks < 148 * 16 ? blocks : 148 * 16);
+  const int tpb = tokensPerBlock(tokens, 2 * cache->kvHeads, cache->D);
+  const ReadArgs p{cacheOf(cache), slots, {headsOf(k), headsOf(v)}, tokens, tpb};
+  const int grid = (tokens + tpb - 1) / tpb;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (datatype == vcclBfloat16) readKernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(p);
-  else if (datatype == vcclFloat16) readKernel<__half><<<grid, kThreads, 0, st>>>(p);
-  else readKernel<float><<<grid, kThreads, 0, st>>>(p);
+  if (datatype == vcclBfloat16) launchRead<__nv_bfloat16>(p, grid, st);
+  else if (datatype == vcclFloat16) launchRead<__half>(p, grid, st);
+  else launchRead<float>(p, grid, st);
   return launched("vcclKv4Read");
 }
 

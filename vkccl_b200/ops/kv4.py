@@ -17,14 +17,12 @@ graphs.
 
 from __future__ import annotations
 
-from ctypes import byref
 from typing import Optional, Tuple, Union
 
 import torch
 
 from vkccl_b200._lib import lib
-from vkccl_b200.comm import _check
-from vkccl_b200.ops._args import DTYPES, cache4, float16s, heads, on_device, rope_of, stream, vector
+from vkccl_b200.ops._args import DTYPES, cache4, call, float16s, fresh, heads, rope_of, vector
 
 MAX_BATCH = 4096
 
@@ -47,14 +45,12 @@ def kv4_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: tor
     distinct.  A group of 64 channels with a NaN or an infinity reads back as
     NaN.
     """
-    float16s(k, "k")
-    dev, dtype, (t, n, dim) = k.device, k.dtype, k.shape
-    c = cache4(cache, dim, dev)
-    hk, hv = heads(k, "k", dtype, dev, t, dim, c.kvHeads), heads(v, "v", dtype, dev, t, dim, c.kvHeads)
+    dev, dtype = float16s(k, "k"), k.dtype
+    t, _, dim = k.shape
+    c, n, _, _ = cache4(cache, dim, dev)
+    hk, hv = heads(k, "k", dtype, dev, t, dim, n), heads(v, "v", dtype, dev, t, dim, n)
     at = vector(slots, "slots", torch.int32, t, dev)
-    with on_device(dev):
-        _check(lib().vcclKv4Append(byref(c), byref(hk), byref(hv), at, None, None, None, t, DTYPES[dtype], stream(dev)),
-               "vcclKv4Append")
+    call(lib().vcclKv4Append, "vcclKv4Append", dev, c, hk, hv, at, None, None, None, t, DTYPES[dtype])
 
 
 def kv4_append_rope(cache: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -62,19 +58,18 @@ def kv4_append_rope(cache: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
                     k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
                     q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``qk_norm_rope`` of q and k, and ``kv4_append`` of the result and v, in one launch: the same bits.  Returns q_out."""
-    float16s(q, "q")
-    dev, dtype, (t, _, dim) = q.device, q.dtype, q.shape
-    c = cache4(cache, dim, dev)
+    dev, dtype = float16s(q, "q"), q.dtype
+    t, nq, dim = q.shape
+    c, n, _, _ = cache4(cache, dim, dev)
     hq = heads(q, "q", dtype, dev, t, dim)
-    hk, hv = heads(k, "k", dtype, dev, t, dim, c.kvHeads), heads(v, "v", dtype, dev, t, dim, c.kvHeads)
+    hk, hv = heads(k, "k", dtype, dev, t, dim, n), heads(v, "v", dtype, dev, t, dim, n)
     at = vector(slots, "slots", torch.int32, t, dev)
     rope = rope_of(positions, inv_freq, q_weight, k_weight, eps, interleaved, dtype, dev, t, dim)
     if q_out is None:
-        q_out = torch.empty((t, hq.heads, dim), dtype=dtype, device=dev)
-    oq = heads(q_out, "q_out", dtype, dev, t, dim, hq.heads, written=True)
-    with on_device(dev):
-        _check(lib().vcclKv4Append(byref(c), byref(hk), byref(hv), at, byref(rope), byref(hq), byref(oq), t,
-                                   DTYPES[dtype], stream(dev)), "vcclKv4Append")
+        q_out, oq = fresh(q, t, nq, dim)
+    else:
+        oq = heads(q_out, "q_out", dtype, dev, t, dim, nq, True)
+    call(lib().vcclKv4Append, "vcclKv4Append", dev, c, hk, hv, at, rope, hq, oq, t, DTYPES[dtype])
     return q_out
 
 
@@ -84,20 +79,19 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torc
     """The keys and values [T, kv heads, D] that the cache holds at slots [T]; zero where a slot is skipped."""
     if dtype not in DTYPES:
         raise ValueError("dtype must be bf16, fp16 or f32")
-    c = cache4(cache)
-    dev = cache.device
+    c, n, dim, _ = cache4(cache)
+    dev = cache.get_device()
     if not isinstance(slots, torch.Tensor) or slots.dim() != 1:
         raise ValueError("slots must be a one-dimensional int32 tensor")
     t = slots.shape[0]
     at = vector(slots, "slots", torch.int32, t, dev)
     if k_out is None:
-        k_out = torch.empty((t, c.kvHeads, c.D), dtype=dtype, device=dev)
+        k_out = torch.empty((t, n, dim), dtype=dtype, device=cache.device)
     if v_out is None:
-        v_out = torch.empty((t, c.kvHeads, c.D), dtype=dtype, device=dev)
-    ok = heads(k_out, "k_out", dtype, dev, t, c.D, c.kvHeads, written=True)
-    ov = heads(v_out, "v_out", dtype, dev, t, c.D, c.kvHeads, written=True)
-    with on_device(dev):
-        _check(lib().vcclKv4Read(byref(c), at, byref(ok), byref(ov), t, DTYPES[dtype], stream(dev)), "vcclKv4Read")
+        v_out = torch.empty((t, n, dim), dtype=dtype, device=cache.device)
+    ok = heads(k_out, "k_out", dtype, dev, t, dim, n, True)
+    ov = heads(v_out, "v_out", dtype, dev, t, dim, n, True)
+    call(lib().vcclKv4Read, "vcclKv4Read", dev, c, at, ok, ov, t, DTYPES[dtype])
     return k_out, v_out
 
 
@@ -117,32 +111,31 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     on a page outside of the cache are not seen.  With return_lse also the
     natural logarithm of the sum of exponentials, f32 [T, q heads].
     """
-    float16s(q, "q")
-    dev, dtype, (t, n, dim) = q.device, q.dtype, q.shape
-    c = cache4(cache, dim, dev)
+    dev, dtype = float16s(q, "q"), q.dtype
+    t, n, dim = q.shape
+    c, kv_heads, _, page_size = cache4(cache, dim, dev)
     hq = heads(q, "q", dtype, dev, t, dim)
-    if n % c.kvHeads:
-        raise ValueError(f"{n} query heads do not divide over {c.kvHeads} key heads")
+    if n % kv_heads:
+        raise ValueError(f"{n} query heads do not divide over {kv_heads} key heads")
     if (not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32 or block_table.dim() != 2
-            or block_table.device != dev or not block_table.is_contiguous() or 0 in block_table.shape):
-        raise ValueError(f"block_table must be a contiguous int32 tensor [batch, pages per request] on {dev}")
+            or block_table.get_device() != dev or not block_table.is_contiguous() or 0 in block_table.shape):
+        raise ValueError(f"block_table must be a contiguous int32 tensor [batch, pages per request] on CUDA device {dev}")
     batch, width = block_table.shape
     if batch > MAX_BATCH:
         raise ValueError(f"at most {MAX_BATCH} requests, got {batch}")
-    if width * c.pageSize > 2**31 - 1 or t * n > 2**31 - 1:
+    if width * page_size > 2**31 - 1 or t * n > 2**31 - 1:
         raise ValueError("a request's tokens and the rows of all heads must fit in 31 bits")
     a_kv = vector(kv_lens, "kv_lens", torch.int32, batch, dev)
     a_q = vector(q_starts, "q_starts", torch.int32, batch + 1, dev)
-    fresh = out is None
-    if fresh:
-        out = torch.empty((t, n, dim), dtype=dtype, device=dev)
-    ho = heads(out, "out", dtype, dev, t, dim, n, written=True)
-    lse = torch.empty((t, n), dtype=torch.float32, device=dev) if return_lse else None
-    with on_device(dev):
-        h = lib()
-        ws = torch.empty(h.vcclKv4AttentionWorkspace(batch, t, n, c.kvHeads, dim), dtype=torch.uint8, device=dev)
-        _check(h.vcclKv4Attention(byref(hq), byref(c), block_table.data_ptr(), width, a_kv, a_q, batch, t,
-                                  dim ** -0.5 if scale is None else float(scale), byref(ho),
-                                  None if lse is None else lse.data_ptr(), int(fresh), ws.data_ptr(), DTYPES[dtype],
-                                  stream(dev)), "vcclKv4Attention")
+    new = out is None
+    if new:
+        out, ho = fresh(q, t, n, dim)
+    else:
+        ho = heads(out, "out", dtype, dev, t, dim, n, True)
+    lse = torch.empty((t, n), dtype=torch.float32, device=q.device) if return_lse else None
+    h = lib()
+    ws = cache.new_empty(h.vcclKv4AttentionWorkspace(batch, t, n, kv_heads, dim))
+    call(h.vcclKv4Attention, "vcclKv4Attention", dev, hq, c, block_table.data_ptr(), width, a_kv, a_q, batch, t,
+         dim ** -0.5 if scale is None else scale, ho, None if lse is None else lse.data_ptr(), 1 if new else 0,
+         ws.data_ptr(), DTYPES[dtype])
     return (out, lse) if return_lse else out

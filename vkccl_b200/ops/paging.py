@@ -16,8 +16,7 @@ from typing import Optional
 import torch
 
 from vkccl_b200._lib import lib
-from vkccl_b200.comm import _check
-from vkccl_b200.ops._args import on_device, stream, vector
+from vkccl_b200.ops._args import call, vector
 
 MAX_BATCH = 8192
 
@@ -53,12 +52,12 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     """
     if not isinstance(lens, torch.Tensor) or not lens.is_cuda or lens.dim() != 1:
         raise ValueError("lens must be a one-dimensional int32 CUDA tensor")
-    dev, batch = lens.device, lens.shape[0]
+    dev, batch = lens.get_device(), lens.shape[0]
     if not 1 <= batch <= MAX_BATCH:
         raise ValueError(f"1 to {MAX_BATCH} requests, got {batch}")
     if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch
-            or block_table.shape[1] < 1 or block_table.device != dev or not block_table.is_contiguous()):
-        raise ValueError(f"block_table must be a contiguous int32 tensor [{batch}, pages per request] on {dev}")
+            or block_table.shape[1] < 1 or block_table.get_device() != dev or not block_table.is_contiguous()):
+        raise ValueError(f"block_table must be a contiguous int32 tensor [{batch}, pages per request] on CUDA device {dev}")
     width = block_table.shape[1]
     if free_pages.dim() != 1 or free_pages.shape[0] < 1:
         raise ValueError("free_pages must be a one-dimensional int32 tensor with room for every page")
@@ -73,17 +72,17 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
         if finished.dtype not in (torch.bool, torch.uint8):
             raise ValueError("finished must be bool or uint8")
         a_done = vector(finished, "finished", finished.dtype, batch, dev)
+    buffer = lens.new_empty(3 * tokens + 3 * batch + 2)
+    base = buffer.data_ptr()
+    positions, slots, requests, q_starts, kv_lens, after, count = buffer.split(
+        (tokens, tokens, tokens, batch + 1, batch, batch, 1))
+    at = base + 12 * tokens
+    a_after, a_left = at + 4 * (2 * batch + 1), at + 4 * (3 * batch + 1)
     if lens_out is not None:
-        vector(lens_out, "lens_out", i32, batch, dev)
+        after, a_after = lens_out, vector(lens_out, "lens_out", i32, batch, dev)
     if count_out is not None:
-        vector(count_out, "count_out", i32, 1, dev)
-    positions, slots, requests, q_starts, kv_lens, after, count = torch.empty(
-        3 * tokens + 3 * batch + 2, dtype=i32, device=dev).split((tokens, tokens, tokens, batch + 1, batch, batch, 1))
-    after = after if lens_out is None else lens_out
-    count = count if count_out is None else count_out
-    with on_device(dev):
-        _check(lib().vcclPagePlan(a_lens, a_new, a_done, block_table.data_ptr(), a_free, a_count, batch, width, pool,
-                                  page_size, tokens, positions.data_ptr(), slots.data_ptr(), requests.data_ptr(),
-                                  q_starts.data_ptr(), kv_lens.data_ptr(), after.data_ptr(), count.data_ptr(),
-                                  stream(dev)), "vcclPagePlan")
+        count, a_left = count_out, vector(count_out, "count_out", i32, 1, dev)
+    call(lib().vcclPagePlan, "vcclPagePlan", dev, a_lens, a_new, a_done, block_table.data_ptr(), a_free, a_count, batch,
+         width, pool, page_size, tokens, base, base + 4 * tokens, base + 8 * tokens, at, at + 4 * (batch + 1), a_after,
+         a_left)
     return PagePlan(positions, slots, requests, q_starts, kv_lens, after, count)

@@ -14,22 +14,22 @@ need no copy.  The angle is taken in 64 bits, so far positions keep it.
 
 from __future__ import annotations
 
-from ctypes import byref
 from typing import Optional, Tuple
 
 import torch
 
 from vkccl_b200._lib import lib
-from vkccl_b200.comm import _check
-from vkccl_b200.ops._args import DTYPES, float16s, heads, on_device, rope_of, stream
+from vkccl_b200.ops._args import DTYPES, call, float16s, fresh, heads, rope_of
 
 
-def _dim(q: torch.Tensor) -> int:
-    float16s(q, "q")
-    dim = q.shape[2]
+def _sizes(q: torch.Tensor, k: torch.Tensor):
+    dev = float16s(q, "q")
+    t, n, dim = q.shape
     if dim % 8 or not 16 <= dim <= 256:
         raise ValueError(f"the head dimension must be a multiple of 8 from 16 to 256, got {dim}")
-    return dim
+    if not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise ValueError("k must be a tensor [tokens, heads, head dim]")
+    return dev, q.dtype, t, n, k.shape[1], dim
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -43,19 +43,18 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     together, else (j, j + rotated / 2).  An output may be its input; it must
     not overlap it in another way.
     """
-    dim = _dim(q)
-    dev, dtype, t = q.device, q.dtype, q.shape[0]
+    dev, dtype, t, nq, nk, dim = _sizes(q, k)
     hq, hk = heads(q, "q", dtype, dev, t, dim), heads(k, "k", dtype, dev, t, dim)
     rope = rope_of(positions, inv_freq, q_weight, k_weight, eps, interleaved, dtype, dev, t, dim)
     if q_out is None:
-        q_out = torch.empty((t, hq.heads, dim), dtype=dtype, device=dev)
+        q_out, oq = fresh(q, t, nq, dim)
+    else:
+        oq = heads(q_out, "q_out", dtype, dev, t, dim, nq, True)
     if k_out is None:
-        k_out = torch.empty((t, hk.heads, dim), dtype=dtype, device=dev)
-    oq = heads(q_out, "q_out", dtype, dev, t, dim, hq.heads, written=True)
-    ok = heads(k_out, "k_out", dtype, dev, t, dim, hk.heads, written=True)
-    with on_device(dev):
-        _check(lib().vcclQkNormRope(byref(hq), byref(hk), byref(rope), byref(oq), byref(ok), t, dim, DTYPES[dtype],
-                                    stream(dev)), "vcclQkNormRope")
+        k_out, ok = fresh(k, t, nk, dim)
+    else:
+        ok = heads(k_out, "k_out", dtype, dev, t, dim, nk, True)
+    call(lib().vcclQkNormRope, "vcclQkNormRope", dev, hq, hk, rope, oq, ok, t, dim, DTYPES[dtype])
     return q_out, k_out
 
 
@@ -71,26 +70,24 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     join f64) in a fixed order: the same bits on every run.  dq_in may be dq,
     dk_in may be dk.
     """
-    dim = _dim(q)
-    dev, dtype, t = q.device, q.dtype, q.shape[0]
+    dev, dtype, t, nq, nk, dim = _sizes(q, k)
     hq, hk = heads(q, "q", dtype, dev, t, dim), heads(k, "k", dtype, dev, t, dim)
-    gq, gk = heads(dq, "dq", dtype, dev, t, dim, hq.heads), heads(dk, "dk", dtype, dev, t, dim, hk.heads)
+    gq, gk = heads(dq, "dq", dtype, dev, t, dim, nq), heads(dk, "dk", dtype, dev, t, dim, nk)
     rope = rope_of(positions, inv_freq, q_weight, k_weight, eps, interleaved, dtype, dev, t, dim)
     if dq_in is None:
-        dq_in = torch.empty((t, hq.heads, dim), dtype=dtype, device=dev)
+        dq_in, oq = fresh(q, t, nq, dim)
+    else:
+        oq = heads(dq_in, "dq_in", dtype, dev, t, dim, nq, True)
     if dk_in is None:
-        dk_in = torch.empty((t, hk.heads, dim), dtype=dtype, device=dev)
-    oq = heads(dq_in, "dq_in", dtype, dev, t, dim, hq.heads, written=True)
-    ok = heads(dk_in, "dk_in", dtype, dev, t, dim, hk.heads, written=True)
-    dwq = None if q_weight is None else torch.empty(dim, dtype=dtype, device=dev)
-    dwk = None if k_weight is None else torch.empty(dim, dtype=dtype, device=dev)
-    ws = None
-    if q_weight is not None or k_weight is not None:
-        ws = torch.empty(lib().vcclQkNormRopeBackwardWorkspace(dim), dtype=torch.uint8, device=dev)
-    with on_device(dev):
-        _check(lib().vcclQkNormRopeBackward(byref(gq), byref(gk), byref(hq), byref(hk), byref(rope), byref(oq), byref(ok),
-                                            None if dwq is None else dwq.data_ptr(),
-                                            None if dwk is None else dwk.data_ptr(),
-                                            None if ws is None else ws.data_ptr(), t, dim, DTYPES[dtype], stream(dev)),
-               "vcclQkNormRopeBackward")
+        dk_in, ok = fresh(k, t, nk, dim)
+    else:
+        ok = heads(dk_in, "dk_in", dtype, dev, t, dim, nk, True)
+    dwq = None if q_weight is None else q_weight.new_empty(dim)
+    dwk = None if k_weight is None else k_weight.new_empty(dim)
+    h, ws = lib(), None
+    if dwq is not None or dwk is not None:
+        ws = torch.empty(h.vcclQkNormRopeBackwardWorkspace(dim), dtype=torch.uint8, device=q.device)
+    call(h.vcclQkNormRopeBackward, "vcclQkNormRopeBackward", dev, gq, gk, hq, hk, rope, oq, ok,
+         None if dwq is None else dwq.data_ptr(), None if dwk is None else dwk.data_ptr(),
+         None if ws is None else ws.data_ptr(), t, dim, DTYPES[dtype])
     return dq_in, dk_in, dwq, dwk
