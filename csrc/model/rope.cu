@@ -102,23 +102,53 @@ __device__ __forceinline__ void rotate(float (&x)[8], int lane, const Rope& r, c
   }
 }
 
-// Sum of a lane's squares: fours in order.
-__device__ __forceinline__ float squares8(const float (&x)[8]) {
-  float s[2];
+// Sum of a row's squares, in the order in which torch's mean over a row of
+// 64 or 128 adds them on this GPU, so that a program that comes from
+// elementary torch operations keeps its bits, and with them its 4-bit codes
+// (a last bit of the norm moves one bf16 key in 10^5 and one code in 10^6):
+// fours in order (rows of 128; one by one for 64), then the sums of the upper
+// half of the row onto those of the lower half, and so on.  Lanes trade what
+// they do not keep, so a row of 128 takes 5 shuffles, one of 64 takes 10.
+// Other rows: fours in order, then a tree over the lanes.
+__device__ __forceinline__ float four(const float* x) {
+  float s = __fmul_rn(x[0], x[0]);
 #pragma unroll
-  for (int v = 0; v < 2; v++) {
-    s[v] = __fmul_rn(x[4 * v], x[4 * v]);
-#pragma unroll
-    for (int i = 1; i < 4; i++) s[v] = __fadd_rn(s[v], __fmul_rn(x[4 * v + i], x[4 * v + i]));
-  }
-  return __fadd_rn(s[0], s[1]);
+  for (int i = 1; i < 4; i++) s = __fadd_rn(s, __fmul_rn(x[i], x[i]));
+  return s;
 }
 
 template <int LANES>
-__device__ __forceinline__ float rowSum(float v) {
+__device__ __forceinline__ float squaresOfRow(const float (&x)[8], int lane, int D) {
+  if (LANES == 16 && D == 128) {
+    const float a = four(x), b = four(x + 4);
+    const bool up = lane & 8;  // keeps the sums of the second fours
+    float v = up ? b : a;
+    v = __fadd_rn(v, __shfl_xor_sync(~0u, up ? a : b, 8));
 #pragma unroll
-  for (int o = 1; o < LANES; o <<= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
+    for (int o = 4; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(~0u, v, o));
+    return __fadd_rn(v, __shfl_xor_sync(~0u, v, 8));
+  }
+  if (LANES == 8 && D == 64) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = __fmul_rn(x[i], x[i]);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {  // keeps the upper half of what it has where its bit o is set
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < o; i++) {
+        const float got = __shfl_xor_sync(~0u, up ? v[i] : v[i + o], o);
+        v[i] = __fadd_rn(up ? v[i + o] : v[i], got);
+      }
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) v[0] = __fadd_rn(v[0], __shfl_xor_sync(~0u, v[0], o));
+    return v[0];
+  }
+  float s = __fadd_rn(four(x), four(x + 4));
+#pragma unroll
+  for (int o = 1; o < LANES; o <<= 1) s = __fadd_rn(s, __shfl_xor_sync(~0u, s, o));
+  return s;
 }
 
 struct ForwardArgs {
@@ -193,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 4) forwardKernel(ForwardArgs p) {
       float x[8];
       unpack8<T>(raw, x);
       if (normed) {
-        const float r = rsqrtf(__fadd_rn(__fmul_rn(rowSum<LANES>(squares8(x)), share), p.rope.eps));
+        const float r = rsqrtf(__fadd_rn(__fmul_rn(squaresOfRow<LANES>(x, lane, p.D), share), p.rope.eps));
         if (which < 2 && p.rope.weight[which] != nullptr) {
           float w[8];
           unpack8<T>(which ? weight[1] : weight[0], w);
@@ -340,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 3) backwardKernel(BackwardArgs p) {
           wg[i] = g[i] * w[i];
           gx += wg[i] * x[i];
         }
-        float sq = squares8(x);
+        float sq = four(x) + four(x + 4);
 #pragma unroll
         for (int o = 1; o < LANES; o <<= 1) {
           sq += __shfl_xor_sync(~0u, sq, o);
