@@ -611,19 +611,37 @@ __global__ void __launch_bounds__(128) joinKernel(AttnArgs p, int R) {
       const int workers = workersFor(p, total);
       const int w0 = workerOf(a, total, workers), w1 = workerOf(a + nt - 1, total, workers);
       if (w0 == w1) return;  // written by its warp
-      for (int w = w0; w <= w1; w++) {
-        const long long slot = 2LL * w + (rangeStart(w, total, workers) < a ? 1 : 0);
-        const float2 st = p.stats[slot * R + row % R];
-        const float top = fmaxf(m, st.x);
+      // 32 parts at a time: a lane reads the maximum and the sum of one.
+      for (int base = w0; base <= w1; base += 32) {
+        const int w = base + lane, n = min(32, w1 - base + 1);
+        long long slot = 0;
+        float2 st = make_float2(kNone, 0.0f);
+        if (lane < n) {
+          slot = (2LL * w + (rangeStart(w, total, workers) < a ? 1 : 0)) * R + row % R;
+          st = p.stats[slot];
+        }
+        float top = st.x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        top = fmaxf(m, top);
         const float old = exp2Fast(m - top), add = exp2Fast(st.x - top);
         m = top;
-        l = l * old + st.y * add;
-        const float2* src = reinterpret_cast<const float2*>(p.partial + (slot * R + row % R) * D) + lane;
+        float sum = st.y * add;
 #pragma unroll
-        for (int gr = 0; gr < G; gr++) {
-          const float2 v = src[32 * gr];
-          y[2 * gr] = y[2 * gr] * old + v.x * add;
-          y[2 * gr + 1] = y[2 * gr + 1] * old + v.y * add;
+        for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        l = l * old + sum;
+#pragma unroll
+        for (int k = 0; k < 2 * G; k++) y[k] *= old;
+#pragma unroll 8
+        for (int k = 0; k < n; k++) {
+          const float f = __shfl_sync(~0u, add, k);
+          const float2* src = reinterpret_cast<const float2*>(p.partial + __shfl_sync(~0u, slot, k) * D) + lane;
+#pragma unroll
+          for (int gr = 0; gr < G; gr++) {
+            const float2 v = src[32 * gr];
+            y[2 * gr] = fmaf(v.x, f, y[2 * gr]);
+            y[2 * gr + 1] = fmaf(v.y, f, y[2 * gr + 1]);
+          }
         }
       }
     }

@@ -35,146 +35,169 @@ struct PlanArgs {
   int* kvLens;
   int* lensOut;
   int* countOut;
+  int* firstPages;  // [batch] place on the stack of the first page that a request takes
 };
 
-struct Sums {
-  long long a, b, c;
+struct Pair {
+  long long a, b;
 };
 
-// Inclusive prefix sums over the block; *total is the block's sum.
-__device__ __forceinline__ Sums blockScan(Sums v, Sums* warpSums, Sums* total) {
+// Inclusive prefix sums over the block, added to *carry, which moves on.
+__device__ __forceinline__ Pair blockScan(Pair v, Pair* warpSums, Pair* carry) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long a = __shfl_up_sync(~0u, v.a, o), b = __shfl_up_sync(~0u, v.b, o), c = __shfl_up_sync(~0u, v.c, o);
+    const long long a = __shfl_up_sync(~0u, v.a, o), b = __shfl_up_sync(~0u, v.b, o);
     if (lane >= o) {
       v.a += a;
       v.b += b;
-      v.c += c;
     }
   }
-  __syncthreads();  // warpSums of an earlier call are read
   if (lane == 31) warpSums[warp] = v;
   __syncthreads();
-  if (warp == 0) {
-    Sums w = lane < static_cast<int>(blockDim.x >> 5) ? warpSums[lane] : Sums{0, 0, 0};
+  Pair w = warpSums[lane];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long a = __shfl_up_sync(~0u, w.a, o), b = __shfl_up_sync(~0u, w.b, o), c = __shfl_up_sync(~0u, w.c, o);
-      if (lane >= o) {
-        w.a += a;
-        w.b += b;
-        w.c += c;
-      }
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long a = __shfl_up_sync(~0u, w.a, o), b = __shfl_up_sync(~0u, w.b, o);
+    if (lane >= o) {
+      w.a += a;
+      w.b += b;
     }
-    warpSums[lane] = w;
   }
-  __syncthreads();
-  if (warp > 0) {
-    const Sums w = warpSums[warp - 1];
-    v.a += w.a;
-    v.b += w.b;
-    v.c += w.c;
-  }
-  *total = warpSums[(blockDim.x >> 5) - 1];
+  const int before = warp > 0 ? warp - 1 : 0;
+  const long long a = __shfl_sync(~0u, w.a, before), b = __shfl_sync(~0u, w.b, before);
+  const Pair total = {__shfl_sync(~0u, w.a, 31), __shfl_sync(~0u, w.b, 31)};
+  v.a += carry->a + (warp > 0 ? a : 0);
+  v.b += carry->b + (warp > 0 ? b : 0);
+  carry->a += total.a;
+  carry->b += total.b;
+  __syncthreads();  // warpSums may be written again
   return v;
 }
 
 __device__ __forceinline__ long long pagesOf(long long tokens, int page) { return (tokens + page - 1) / page; }
 
-// One block: lengths, grants, the stack and the table.
+// The last i of n whose start is at most x (starts rise; starts[0] <= x).
+__device__ __forceinline__ int findStart(const int* starts, int n, int x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int m = (lo + hi + 1) >> 1;
+    if (starts[m] <= x) lo = m;
+    else hi = m - 1;
+  }
+  return lo;
+}
+
+// One block: lengths, grants and released pages.  A block-wide prefix sum is
+// two shuffles and two barriers; the released pages are moved one a thread,
+// four in flight, whoever's they are (a warp for each request left most warps
+// idle behind a few long ones: 38 us where this takes 9, 256 requests of which
+// 16 end with 230 pages each).
 __global__ void __launch_bounds__(kPlanThreads) planStateKernel(PlanArgs p) {
-  extern __shared__ int scratch[];  // have, first page (of the taken ones), pages to take: batch each
-  int* sHave = scratch;
-  int* sFirst = sHave + p.batch;
-  int* sNeed = sFirst + p.batch;
-  __shared__ Sums warpSums[32];
+  extern __shared__ int scratch[];  // released pages before each request, rows up to and including it
+  int* sReleased = scratch;
+  int* sEnd = sReleased + p.batch;
+  __shared__ Pair warpSums[32];
   __shared__ int taken;
   if (threadIdx.x == 0) taken = 0;
 
   const int count = min(max(*p.freeCount, 0), p.poolSize);
-  // Pages released, per request (in sNeed for the moment) and in all.
-  long long released = 0;
+  Pair sums = {0, 0};
   for (int base = 0; base < p.batch; base += kPlanThreads) {
     const int i = base + threadIdx.x;
-    int r = 0;
-    if (i < p.batch && p.finished != nullptr && p.finished[i])
-      r = static_cast<int>(min(pagesOf(max(p.lens[i], 0), p.page), static_cast<long long>(p.width)));
-    Sums total;
-    const Sums s = blockScan({r, 0, 0}, warpSums, &total);
+    Pair v = {0, 0};
     if (i < p.batch) {
-      sNeed[i] = r;
-      sFirst[i] = static_cast<int>(released + s.a - r);
+      if (p.finished != nullptr && p.finished[i])
+        v.a = min(pagesOf(max(p.lens[i], 0), p.page), static_cast<long long>(p.width));
+      v.b = max(p.newLens[i], 0);
     }
-    released += total.a;
+    const Pair s = blockScan(v, warpSums, &sums);
+    if (i < p.batch) {
+      sReleased[i] = static_cast<int>(min(s.a - v.a, static_cast<long long>(INT_MAX)));
+      sEnd[i] = static_cast<int>(min(s.b, static_cast<long long>(INT_MAX)));
+    }
   }
   __syncthreads();
-  // Onto the stack, a warp a request.
-  for (int i = threadIdx.x >> 5; i < p.batch; i += kPlanThreads / 32)
-    for (int j = threadIdx.x & 31; j < sNeed[i]; j += 32) {
-      const long long at = static_cast<long long>(count) + sFirst[i] + j;
-      if (at < p.poolSize) p.pool[at] = p.table[static_cast<long long>(i) * p.width + j];
+  const int room = p.poolSize - count;
+  const int released = static_cast<int>(min(sums.a, static_cast<long long>(room)));
+  const int stack = count + released;
+  for (int base = threadIdx.x; base < released; base += 4 * kPlanThreads) {
+    int got[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int e = base + u * kPlanThreads;
+      if (e < released) {
+        const int i = findStart(sReleased, p.batch, e);
+        got[u] = p.table[static_cast<long long>(i) * p.width + e - sReleased[i]];
+      }
     }
-  const long long stack = min(count + released, static_cast<long long>(p.poolSize));
-  __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int e = base + u * kPlanThreads;
+      if (e < released) p.pool[count + e] = got[u];
+    }
+  }
 
-  long long rows = 0, asked = 0;
+  Pair asked = {0, 0};
   for (int base = 0; base < p.batch; base += kPlanThreads) {
     const int i = base + threadIdx.x;
-    long long left = 0, n = 0;
+    long long left = 0, n = 0, need = 0;
+    bool fits = false;
     if (i < p.batch) {
       left = p.finished != nullptr && p.finished[i] ? 0 : max(p.lens[i], 0);
       n = max(p.newLens[i], 0);
+      const long long want = pagesOf(left + n, p.page);
+      fits = want <= p.width && sEnd[i] <= p.tokens;
+      need = fits ? want - pagesOf(left, p.page) : 0;
     }
-    Sums total;
-    const long long end = rows + blockScan({n, 0, 0}, warpSums, &total).a;
-    rows += total.a;
-    const long long have = pagesOf(left, p.page), want = pagesOf(left + n, p.page);
-    const bool fits = want <= p.width && end <= p.tokens;
-    const long long need = fits ? want - have : 0;
-    const long long upto = asked + blockScan({need, 0, 0}, warpSums, &total).a;
-    asked += total.a;
+    const long long upto = blockScan({need, 0}, warpSums, &asked).a;
     if (i < p.batch) {
       const bool granted = fits && (need == 0 || upto <= stack);
       if (granted && need > 0) atomicMax(&taken, static_cast<int>(upto));
-      sHave[i] = static_cast<int>(min(have, static_cast<long long>(p.width)));
-      sFirst[i] = static_cast<int>(upto - need);
-      sNeed[i] = granted ? static_cast<int>(need) : 0;
-      p.qStarts[i + 1] = static_cast<int>(min(end, static_cast<long long>(INT_MAX)));
+      sReleased[i] = granted ? static_cast<int>(min(upto - need, static_cast<long long>(INT_MAX))) : 0;
+      p.qStarts[i + 1] = sEnd[i];
       if (i == 0) p.qStarts[0] = 0;
       p.kvLens[i] = granted ? static_cast<int>(left + n) : 0;
       p.lensOut[i] = static_cast<int>(left + (granted ? n : 0));
     }
   }
   __syncthreads();
-  const long long bottom = stack - taken;
-  for (int i = threadIdx.x >> 5; i < p.batch; i += kPlanThreads / 32)
-    for (int j = threadIdx.x & 31; j < sNeed[i]; j += 32)
-      p.table[static_cast<long long>(i) * p.width + sHave[i] + j] = p.pool[bottom + sFirst[i] + j];
-  if (threadIdx.x == 0) *p.countOut = static_cast<int>(bottom);
+  const int bottom = stack - taken;
+  for (int i = threadIdx.x; i < p.batch; i += kPlanThreads) p.firstPages[i] = bottom + sReleased[i];
+  if (threadIdx.x == 0) *p.countOut = bottom;
 }
 
-// Each row's request, position and slot.
-__global__ void planRowsKernel(PlanArgs p) {
+// Each row's request, position and slot; the first row of a page that its
+// request takes puts the page into the table.  What the table held before is
+// read only for pages that the request had, so no block waits for another.
+__global__ void __launch_bounds__(256) planRowsKernel(PlanArgs p) {
+  extern __shared__ int starts[];  // [batch + 1]
+  for (int i = threadIdx.x; i <= p.batch; i += blockDim.x) starts[i] = p.qStarts[i];
+  __syncthreads();
   const int t = blockIdx.x * blockDim.x + threadIdx.x;
   if (t >= p.tokens) return;
-  int lo = 0, hi = p.batch;  // the first request that ends behind t
-  while (lo < hi) {
-    const int m = (lo + hi) >> 1;
-    if (p.qStarts[m + 1] > t) hi = m;
-    else lo = m + 1;
-  }
-  int position = 0, slot = -1;
-  if (lo < p.batch) {
-    const int start = p.qStarts[lo], n = p.qStarts[lo + 1] - start, kv = p.kvLens[lo];
-    if (kv >= n && kv > 0) {
-      position = kv - n + t - start;
-      slot = p.table[static_cast<long long>(lo) * p.width + position / p.page] * p.page + position % p.page;
+  int position = 0, slot = -1, who = -1;
+  if (t < starts[p.batch]) {
+    who = findStart(starts, p.batch, t);
+    const int start = starts[who], n = starts[who + 1] - start, kv = p.kvLens[who];
+    if (kv > 0) {  // granted
+      const int left = kv - n, have = static_cast<int>(pagesOf(left, p.page));
+      position = left + t - start;
+      const int j = position / p.page;
+      int* entry = p.table + static_cast<long long>(who) * p.width + j;
+      int page;
+      if (j < have) {
+        page = *entry;
+      } else {
+        page = p.pool[p.firstPages[who] + j - have];
+        if (t == start || position == j * p.page) *entry = page;
+      }
+      slot = page * p.page + position - j * p.page;
     }
   }
   p.positions[t] = position;
   p.slots[t] = slot;
-  p.requests[t] = lo < p.batch ? lo : -1;
+  p.requests[t] = who;
 }
 
 }  // namespace
@@ -186,26 +209,26 @@ using namespace vccl;
 extern "C" vcclResult_t vcclPagePlan(const int* lens, const int* newLens, const unsigned char* finished, int* table,
                                      int* freePages, const int* freeCount, int batch, int width, int poolSize,
                                      int pageSize, int tokens, int* positions, int* slots, int* requests,
-                                     int* qStarts, int* kvLens, int* lensOut, int* countOut, vcclStream_t stream) {
-  if (!lens || !newLens || !table || !freePages || !freeCount || !qStarts || !kvLens || !lensOut || !countOut ||
+                                     int* qStarts, int* kvLens, int* lensOut, int* countOut, int* firstPages, vcclStream_t stream) {
+  if (!lens || !newLens || !table || !freePages || !freeCount || !qStarts || !kvLens || !lensOut || !countOut || !firstPages ||
       batch <= 0 || batch > model::kPlanMaxBatch || width <= 0 || poolSize <= 0 || pageSize <= 0 || tokens < 0 ||
       static_cast<long long>(poolSize) * pageSize > INT_MAX || static_cast<long long>(width) * pageSize > INT_MAX ||
       (tokens > 0 && (!positions || !slots || !requests)))
     return vcclInvalidArgument;
   TraceRange trace("vccl PagePlan");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const model::PlanArgs p{lens,   newLens,  finished, table,     freePages, freeCount, batch,  width,   poolSize,
-                          pageSize, tokens, positions, slots,    requests,  qStarts,   kvLens, lensOut, countOut};
-  const size_t smem = static_cast<size_t>(batch) * 3 * sizeof(int);
+  const model::PlanArgs p{lens,     newLens, finished,  table, freePages, freeCount, batch,  width,   poolSize, pageSize,
+                          tokens,   positions, slots, requests, qStarts, kvLens, lensOut, countOut, firstPages};
+  const size_t smem = static_cast<size_t>(batch) * 2 * sizeof(int);
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(model::planStateKernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               model::kPlanMaxBatch * 3 * static_cast<int>(sizeof(int)));
+                                               model::kPlanMaxBatch * 2 * static_cast<int>(sizeof(int)));
     if (e != cudaSuccess) {
       VERR("vcclPagePlan: %s", cudaGetErrorString(e));
       return vcclSystemError;
     }
   }
   model::planStateKernel<<<1, model::kPlanThreads, smem, st>>>(p);
-  if (tokens > 0) model::planRowsKernel<<<(tokens + 255) / 256, 256, 0, st>>>(p);
+  if (tokens > 0) model::planRowsKernel<<<(tokens + 255) / 256, 256, (batch + 1) * sizeof(int), st>>>(p);
   return model::launched("vcclPagePlan");
 }

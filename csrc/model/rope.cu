@@ -413,22 +413,26 @@ __global__ void __launch_bounds__(kThreads, 3) backwardKernel(BackwardArgs p) {
   }
 }
 
-// The blocks' sums in a fixed order: the same bits on every run.
+// The blocks' sums in a fixed order: the same bits on every run.  32 channels
+// a block, its 32 warps a share of the sums each.
 template <typename T>
-__global__ void weightGradKernel(const float* partial, int blocks, int D, T* dqw, T* dkw) {
-  const int which = blockIdx.y, d = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) weightGradKernel(const float* partial, int blocks, int D, T* dqw, T* dkw) {
+  const int which = blockIdx.y, lane = threadIdx.x & 31, d = blockIdx.x * 32 + lane, part = threadIdx.x >> 5;
   T* out = which ? dkw : dqw;
   if (out == nullptr) return;
-  __shared__ double sums[8][32];
+  __shared__ double sums[32][33];
   double s = 0.0;
-  if (d < D)
-    for (int b = part; b < blocks; b += 8) s += partial[(static_cast<long long>(b) * 2 + which) * D + d];
-  sums[part][threadIdx.x & 31] = s;
-  __syncthreads();
-  if (part == 0 && d < D) {
-    for (int i = 1; i < 8; i++) s += sums[i][threadIdx.x & 31];
-    out[d] = static_cast<T>(static_cast<float>(s));
+  if (d < D) {
+#pragma unroll 8
+    for (int b = part; b < blocks; b += 32) s += partial[(static_cast<long long>(b) * 2 + which) * D + d];
   }
+  sums[part][lane] = s;
+  __syncthreads();
+  // Warp w adds up channel w.
+  s = sums[lane][part];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  if (lane == 0 && blockIdx.x * 32 + part < D) out[blockIdx.x * 32 + part] = static_cast<T>(static_cast<float>(s));
 }
 
 int lanesFor(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
@@ -573,10 +577,10 @@ vcclResult_t vcclQkNormRopeBackward(const vcclHeads_t* dq, const vcclHeads_t* dk
     const dim3 g((D + 31) / 32, 2);
     const float* part = static_cast<const float*>(workspace);
     if (datatype == vcclBfloat16)
-      weightGradKernel<<<g, 256, 0, st>>>(part, grid, D, static_cast<__nv_bfloat16*>(dqWeight),
+      weightGradKernel<<<g, 1024, 0, st>>>(part, grid, D, static_cast<__nv_bfloat16*>(dqWeight),
                                           static_cast<__nv_bfloat16*>(dkWeight));
     else
-      weightGradKernel<<<g, 256, 0, st>>>(part, grid, D, static_cast<__half*>(dqWeight), static_cast<__half*>(dkWeight));
+      weightGradKernel<<<g, 1024, 0, st>>>(part, grid, D, static_cast<__half*>(dqWeight), static_cast<__half*>(dkWeight));
   }
   return launched("vcclQkNormRopeBackward");
 }

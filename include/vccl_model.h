@@ -41,11 +41,11 @@ extern "C" {
  * lensOut[i] = L_i + (granted ? n_i : 0); *countOut; and for each of the
  * tokens rows its position, slot (-1 if refused or behind the last row) and
  * request (-1 behind the last row).  lensOut may be lens, countOut may be
- * freeCount.  batch <= 8192. */
+ * freeCount.  firstPages[batch] is scratch.  batch <= 8192. */
 vcclResult_t vcclPagePlan(const int* lens, const int* newLens, const unsigned char* finished, int* table,
                           int* freePages, const int* freeCount, int batch, int width, int poolSize, int pageSize,
                           int tokens, int* positions, int* slots, int* requests, int* qStarts, int* kvLens,
-                          int* lensOut, int* countOut, vcclStream_t stream);
+                          int* lensOut, int* countOut, int* firstPages, vcclStream_t stream);
 
 /* A [tokens, heads, D] tensor: pointer and strides in elements. */
 typedef struct {

@@ -153,7 +153,7 @@ def _declare_extensions(h: ctypes.CDLL) -> None:
         "vcclMoeDispatchFp8": [P, P, P, P, P, P, P, I, I, I, I, I, P, P],
         "vcclMoeCombine": [P, P, P, P, P, I, I, I, I, P, P],
         # vccl_model.h
-        "vcclPagePlan": [P, P, P, P, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P],
+        "vcclPagePlan": [P, P, P, P, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, P],
         "vcclQkNormRope": [P, P, P, P, P, I, I, I, P],
         "vcclQkNormRopeBackward": [P, P, P, P, P, P, P, P, P, P, I, I, I, P],
         "vcclKv4Append": [P, P, P, P, P, P, P, I, I, P],

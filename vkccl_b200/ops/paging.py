@@ -72,10 +72,10 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
         if finished.dtype not in (torch.bool, torch.uint8):
             raise ValueError("finished must be bool or uint8")
         a_done = vector(finished, "finished", finished.dtype, batch, dev)
-    buffer = lens.new_empty(3 * tokens + 3 * batch + 2)
+    buffer = lens.new_empty(3 * tokens + 4 * batch + 2)
     base = buffer.data_ptr()
-    positions, slots, requests, q_starts, kv_lens, after, count = buffer.split(
-        (tokens, tokens, tokens, batch + 1, batch, batch, 1))
+    positions, slots, requests, q_starts, kv_lens, after, count, _ = buffer.split(
+        (tokens, tokens, tokens, batch + 1, batch, batch, 1, batch))
     at = base + 12 * tokens
     a_after, a_left = at + 4 * (2 * batch + 1), at + 4 * (3 * batch + 1)
     if lens_out is not None:
@@ -84,5 +84,5 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
         count, a_left = count_out, vector(count_out, "count_out", i32, 1, dev)
     call(lib().vcclPagePlan, "vcclPagePlan", dev, a_lens, a_new, a_done, block_table.data_ptr(), a_free, a_count, batch,
          width, pool, page_size, tokens, base, base + 4 * tokens, base + 8 * tokens, at, at + 4 * (batch + 1), a_after,
-         a_left)
+         a_left, at + 4 * (3 * batch + 2))
     return PagePlan(positions, slots, requests, q_starts, kv_lens, after, count)
