@@ -88,18 +88,17 @@ __device__ __forceinline__ int findStart(const int* starts, int n, int x) {
   return lo;
 }
 
-// One block: lengths, grants and released pages.  A block-wide prefix sum is
-// two shuffles and two barriers; the released pages are moved one a thread,
-// four in flight, whoever's they are (a warp for each request left most warps
-// idle behind a few long ones: 38 us where this takes 9, 256 requests of which
-// 16 end with 230 pages each).
+// Block 0: lengths and grants.  The other blocks move the released pages onto
+// the stack, one a thread, whoever's they are (a warp for each request left
+// most warps idle behind a few long ones); every block takes the prefix sums
+// of the released pages for itself, so none waits for another.
 __global__ void __launch_bounds__(kPlanThreads) planStateKernel(PlanArgs p) {
   extern __shared__ int scratch[];  // released pages before each request, rows up to and including it
   int* sReleased = scratch;
   int* sEnd = sReleased + p.batch;
   __shared__ Pair warpSums[32];
   __shared__ int taken;
-  if (threadIdx.x == 0) taken = 0;
+  if (threadIdx.x == 0) taken = 0;  // read behind several barriers
 
   const int count = min(max(*p.freeCount, 0), p.poolSize);
   Pair sums = {0, 0};
@@ -121,21 +120,12 @@ __global__ void __launch_bounds__(kPlanThreads) planStateKernel(PlanArgs p) {
   const int room = p.poolSize - count;
   const int released = static_cast<int>(min(sums.a, static_cast<long long>(room)));
   const int stack = count + released;
-  for (int base = threadIdx.x; base < released; base += 4 * kPlanThreads) {
-    int got[4];
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const int e = base + u * kPlanThreads;
-      if (e < released) {
-        const int i = findStart(sReleased, p.batch, e);
-        got[u] = p.table[static_cast<long long>(i) * p.width + e - sReleased[i]];
-      }
+  if (blockIdx.x > 0) {
+    for (int e = (blockIdx.x - 1) * kPlanThreads + threadIdx.x; e < released; e += (gridDim.x - 1) * kPlanThreads) {
+      const int i = findStart(sReleased, p.batch, e);
+      p.pool[count + e] = p.table[static_cast<long long>(i) * p.width + e - sReleased[i]];
     }
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const int e = base + u * kPlanThreads;
-      if (e < released) p.pool[count + e] = got[u];
-    }
+    return;
   }
 
   Pair asked = {0, 0};
@@ -228,7 +218,9 @@ extern "C" vcclResult_t vcclPagePlan(const int* lens, const int* newLens, const 
       return vcclSystemError;
     }
   }
-  model::planStateKernel<<<1, model::kPlanThreads, smem, st>>>(p);
+  // A thread for each page that the finished requests may hold, 148 blocks at most.
+  const long long held = finished ? (static_cast<long long>(batch) * width + model::kPlanThreads - 1) / model::kPlanThreads : 0;
+  model::planStateKernel<<<1 + static_cast<int>(held < 147 ? held : 147), model::kPlanThreads, smem, st>>>(p);
   if (tokens > 0) model::planRowsKernel<<<(tokens + 255) / 256, 256, (batch + 1) * sizeof(int), st>>>(p);
   return model::launched("vcclPagePlan");
 }
