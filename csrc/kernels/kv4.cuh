@@ -144,8 +144,10 @@ __device__ __forceinline__ void dequantise8(uint32_t w, uint32_t params, float (
   const float s = bf16Lo(params), m = bf16Hi(params);
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const float c = static_cast<float>((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u);
-    x[i] = __fmaf_rn(c - 7.5f, s, m);
+    const int at = 4 * ((i >> 1) + 4 * (i & 1));
+    // code at bit 1 of 2^22, whose last bit is worth 1/2: 2^22 + code
+    const uint32_t c = (at > 0 ? w >> (at - 1) : w << 1) & 0x1Eu;
+    x[i] = __fmaf_rn(__uint_as_float(0x4A800000u | c) - 4194311.5f, s, m);
   }
 }
 

@@ -15,24 +15,13 @@
 namespace vccl {
 namespace model {
 
-// What a kernel needs of a vcclHeads_t.
-struct Heads {
-  void* data;
-  long long tok;
-  long long head;
-  int heads;
-};
-
-inline Heads headsOf(const vcclHeads_t* h) {
-  if (h == nullptr) return {nullptr, 0, 0, 0};
-  return {h->data, h->tokenStride, h->headStride, h->heads};
-}
-
-// 16-byte vectors: base and strides in whole vectors of 8 elements.
+// 16-byte vectors: base and strides in whole vectors, and strides and head
+// counts that the kernels' index arithmetic holds (products are 64 bits).
 inline bool headsOk(const vcclHeads_t* h, int elemBytes) {
-  if (h == nullptr || h->data == nullptr || h->heads <= 0) return false;
-  const long long vec = 16 / elemBytes;
-  return (reinterpret_cast<uintptr_t>(h->data) & 15u) == 0 && h->tokenStride % vec == 0 && h->headStride % vec == 0;
+  if (h == nullptr || h->data == nullptr || h->heads <= 0 || h->heads > 32768) return false;
+  const long long vec = 16 / elemBytes, most = 1ll << 31;
+  return (reinterpret_cast<uintptr_t>(h->data) & 15u) == 0 && h->tokenStride % vec == 0 && h->headStride % vec == 0 &&
+         h->tokenStride >= 0 && h->tokenStride < most && h->headStride >= 0 && h->headStride < most;
 }
 
 inline vcclResult_t launched(const char* what) {

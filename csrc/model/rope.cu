@@ -9,7 +9,13 @@
 // shuffles among them.  The cosines and sines of a block's tokens are taken
 // once, into shared memory: the angle position * invFreq is a product in 64
 // bits, reduced to [-pi, pi] there, since positions reach millions.
-// All of it is bound by memory: every operand is read or written once.
+//
+// All of it should be bound by memory, every operand being read or written
+// once, and was bound by instructions at first (309 for each warp's step of
+// two rows of 128 channels).  So a warp's step takes rows of one kind
+// (queries, keys or values), whose strides and weights are then uniform, the
+// token and head come from a product with a reciprocal, and the next step's
+// row is loaded before this one is worked on.
 #include "kernels/kv4.cuh"
 #include "model/common.cuh"
 
@@ -33,13 +39,77 @@ struct Cache {
   long long tokens;  // pages * pageSize
   int heads;
   int blocksPerPage;
+  int shift;  // blocksPerPage = 1 << shift, or -1
   int D;
 };
 
 __device__ __forceinline__ uint8_t* cacheBlock(const Cache& c, int slot, int head) {
-  const int block = slot >> 4, page = block / c.blocksPerPage;
-  return c.data + ((static_cast<long long>(page) * c.heads + head) * c.blocksPerPage + block % c.blocksPerPage) *
+  const int block = slot >> 4, page = c.shift >= 0 ? block >> c.shift : block / c.blocksPerPage;
+  return c.data + ((static_cast<long long>(page) * c.heads + head) * c.blocksPerPage + (block - page * c.blocksPerPage)) *
                       kv4::blockBytes(c.D);
+}
+
+// One kind of rows: heads of every token, read or written with strides in
+// elements.
+struct Side {
+  const void* in;
+  void* out;
+  int inTok, inHead, outTok, outHead;
+  int heads;
+  uint32_t recip;  // ceil(2^32 / heads); 0 for one head
+};
+
+// Where a warp's step stands: row r of a kind in a block of tokens.
+struct Row {
+  int kind, t, h;
+  bool live;
+};
+
+template <int KINDS>
+struct Steps {
+  int end[KINDS];  // steps up to and including a kind
+};
+
+template <int KINDS, int LANES>
+__device__ __forceinline__ Steps<KINDS> stepsOf(const Side* side, int n) {
+  constexpr int kPerWarp = 32 / LANES;
+  Steps<KINDS> s;
+  int e = 0;
+#pragma unroll
+  for (int k = 0; k < KINDS; k++) {
+    e += (n * side[k].heads + kPerWarp - 1) / kPerWarp;
+    s.end[k] = e;
+  }
+  return s;
+}
+
+template <int KINDS, int LANES>
+__device__ __forceinline__ Row rowOf(const Side* side, const Steps<KINDS>& s, int step, int n, bool active) {
+  constexpr int kPerWarp = 32 / LANES;
+  Row r;
+  r.kind = 0;
+  int first = 0;
+#pragma unroll
+  for (int k = 1; k < KINDS; k++)
+    if (step >= s.end[k - 1]) {
+      r.kind = k;
+      first = s.end[k - 1];
+    }
+  const int row = (step - first) * kPerWarp + (threadIdx.x & 31) / LANES;
+  const Side& d = side[r.kind];
+  r.t = d.recip ? static_cast<int>(__umulhi(static_cast<uint32_t>(row), d.recip)) : row;
+  r.h = row - r.t * d.heads;
+  r.live = active && r.t < n && step < s.end[KINDS - 1];
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* inOf(const Side& d, int token, int h) {
+  return static_cast<const T*>(d.in) + static_cast<long long>(token) * d.inTok + static_cast<long long>(h) * d.inHead;
+}
+template <typename T>
+__device__ __forceinline__ T* outOf(const Side& d, int token, int h) {
+  return static_cast<T*>(d.out) + static_cast<long long>(token) * d.outTok + static_cast<long long>(h) * d.outHead;
 }
 
 // cos and sin of position * f, in 64 bits: k turns of 2 pi are taken off
@@ -53,32 +123,57 @@ __device__ __forceinline__ void cosSin(int position, float f, float* c, float* s
   *s = static_cast<float>(sd);
 }
 
-// cos and sin of tokens [t0, t0 + n) into smem: cos at [i * half + j], sin at
-// tpb * half further on.
-__device__ __forceinline__ void fillAngles(const Rope& r, int t0, int n, int tpb, float* smem) {
+// Of tokens [t0, t0 + n): cosines, sines, negative sines, half each.
+__device__ __forceinline__ void fillAngles(const Rope& r, int t0, int n, float* smem) {
   for (int i = threadIdx.x; i < n * r.half; i += blockDim.x) {
+    const int t = i / r.half, j = i - t * r.half;
     float c, s;
-    cosSin(r.positions[t0 + i / r.half], r.invFreq[i % r.half], &c, &s);
-    smem[i] = c;
-    smem[tpb * r.half + i] = s;
+    cosSin(r.positions[t0 + t], r.invFreq[j], &c, &s);
+    float* at = smem + t * 3 * r.half + j;
+    at[0] = c;
+    at[r.half] = s;
+    at[2 * r.half] = -s;
   }
 }
 
-// Rotates the channels of a row in place; back: by the negative angle.
-// cosv, sinv: of the row's token.
-template <int LANES>
-__device__ __forceinline__ void rotate(float (&x)[8], int lane, const Rope& r, const float* cosv, const float* sinv,
-                                       float sign) {
+// The weights as f32, D of queries and D of keys.
+template <typename T>
+__device__ __forceinline__ void fillWeights(const Rope& r, int D, float* smem) {
+  for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
+    const T* w = static_cast<const T*>(r.weight[i >= D]);
+    if (w != nullptr) smem[i] = static_cast<float>(w[i >= D ? i - D : i]);
+  }
+}
+
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = a.x;
+  x[1] = a.y;
+  x[2] = a.z;
+  x[3] = a.w;
+  x[4] = b.x;
+  x[5] = b.y;
+  x[6] = b.z;
+  x[7] = b.w;
+}
+
+// Rotates the channels of a row in place; BACK: by the negative angle.
+// angles: of the row's token.  Every operation rounds by itself.
+template <int LANES, bool BACK>
+__device__ __forceinline__ void rotate(float (&x)[8], int lane, const Rope& r, const float* angles) {
+  const float* up = angles + (BACK ? 2 : 1) * r.half;    // what the second channel of a pair takes
+  const float* down = angles + (BACK ? 1 : 2) * r.half;  // what the first one takes
   if (r.interleaved) {
     if (8 * lane < 2 * r.half) {
-      const float4 c = *reinterpret_cast<const float4*>(cosv + 4 * lane);
-      const float4 s = *reinterpret_cast<const float4*>(sinv + 4 * lane);
-      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {sign * s.x, sign * s.y, sign * s.z, sign * s.w};
+      const float4 c = *reinterpret_cast<const float4*>(angles + 4 * lane);
+      const float4 u = *reinterpret_cast<const float4*>(up + 4 * lane);
+      const float4 d = *reinterpret_cast<const float4*>(down + 4 * lane);
+      const float cc[4] = {c.x, c.y, c.z, c.w}, uu[4] = {u.x, u.y, u.z, u.w}, dd[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const float a = x[2 * i], b = x[2 * i + 1];
-        x[2 * i] = __fsub_rn(__fmul_rn(a, cc[i]), __fmul_rn(b, ss[i]));
-        x[2 * i + 1] = __fadd_rn(__fmul_rn(b, cc[i]), __fmul_rn(a, ss[i]));
+        x[2 * i] = __fadd_rn(__fmul_rn(a, cc[i]), __fmul_rn(b, dd[i]));
+        x[2 * i + 1] = __fadd_rn(__fmul_rn(b, cc[i]), __fmul_rn(a, uu[i]));
       }
     }
     return;
@@ -90,15 +185,11 @@ __device__ __forceinline__ void rotate(float (&x)[8], int lane, const Rope& r, c
   for (int i = 0; i < 8; i++) y[i] = __shfl_sync(~0u, x[i], src, LANES);
   if (lane < 2 * h) {
     const int j = 8 * (lane < h ? lane : lane - h);
-    const float sg = lane < h ? -sign : sign;
+    float c[8], s[8];
+    load8(angles + j, c);
+    load8((lane < h ? down : up) + j, s);
 #pragma unroll
-    for (int v = 0; v < 2; v++) {
-      const float4 c = *reinterpret_cast<const float4*>(cosv + j + 4 * v);
-      const float4 s = *reinterpret_cast<const float4*>(sinv + j + 4 * v);
-      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-      for (int i = 0; i < 4; i++) x[4 * v + i] = __fadd_rn(__fmul_rn(x[4 * v + i], cc[i]), __fmul_rn(sg * y[4 * v + i], ss[i]));
-    }
+    for (int i = 0; i < 8; i++) x[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i]));
   }
 }
 
@@ -152,104 +243,75 @@ __device__ __forceinline__ float squaresOfRow(const float (&x)[8], int lane, int
 }
 
 struct ForwardArgs {
-  Heads in[3];   // queries, keys, values (values, and queries, may be absent)
-  Heads out[2];  // queries, keys (keys absent where they go to the cache)
+  Side side[3];  // queries, keys, values; out == nullptr: not written (keys and values go to the cache)
   Rope rope;
   Cache cache;  // data == nullptr: no cache
   const int* slots;
   int tokens, D, tpb;
 };
 
-// The rows of a block in steps: token and head without a division.
-struct RowWalk {
-  int t, h, dt, dh, heads;
-  __device__ __forceinline__ RowWalk(int row, int step, int heads_)
-      : t(row / heads_), h(row % heads_), dt(step / heads_), dh(step % heads_), heads(heads_) {}
-  __device__ __forceinline__ void next() {
-    t += dt;
-    h += dh;
-    if (h >= heads) {
-      h -= heads;
-      t++;
-    }
-  }
-};
-
-// Block: tpb tokens, all their heads (queries, keys, values in that order).
-// Norm and rotation round after every f32 operation (no contraction), so that
-// the fused write gives the bits of the two calls it stands for.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads, 4) forwardKernel(ForwardArgs p) {
-  extern __shared__ float angles[];
-  constexpr int kRows = kThreads / LANES;
+// Block: tpb tokens, all their heads.  Norm and rotation round after every
+// f32 operation (no contraction), so that the fused write gives the bits of
+// the two calls it stands for.
+template <typename T, int LANES, int KINDS>
+__global__ void __launch_bounds__(kThreads, 4) forwardKernel(const __grid_constant__ ForwardArgs p) {
+  extern __shared__ float4 shared[];
+  float* weights = reinterpret_cast<float*>(shared);
+  float* angles = weights + 2 * p.D;
   const int t0 = blockIdx.x * p.tpb, n = min(p.tpb, p.tokens - t0);
   const int lane = threadIdx.x % LANES;
   const bool active = 8 * lane < p.D;
-  const int nq = p.in[0].heads, nk = p.in[1].heads;
-  const int rows = n * (nq + nk + p.in[2].heads);
-  RowWalk at(threadIdx.x / LANES, kRows, nq + nk + p.in[2].heads);
-
-  // The next row is under way while one is worked on.
-  auto load = [&]() {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (at.t < n && active) {
-      const int which = (at.h >= nq) + (at.h >= nq + nk), h = at.h - (which > 0 ? nq : 0) - (which > 1 ? nk : 0);
-      const Heads& in = p.in[which];
-      v = *reinterpret_cast<const uint4*>(static_cast<const T*>(in.data) + (t0 + at.t) * in.tok + h * in.head + 8 * lane);
-    }
-    return v;
-  };
-  uint4 ahead = load();
-  uint4 weight[2] = {};
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-    if (p.rope.weight[i] != nullptr && active)
-      weight[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.rope.weight[i]) + 8 * lane);
+  const Steps<KINDS> steps = stepsOf<KINDS, LANES>(p.side, n);
   const bool normed = p.rope.weight[0] != nullptr || p.rope.weight[1] != nullptr;
+
+  Row ahead;
+  uint4 rawAhead;
+  int slotAhead = -1;
+  auto load = [&](int step) {
+    ahead = rowOf<KINDS, LANES>(p.side, steps, step, n, active);
+    rawAhead = make_uint4(0, 0, 0, 0);
+    if (ahead.live) {
+      rawAhead = *reinterpret_cast<const uint4*>(inOf<T>(p.side[ahead.kind], t0 + ahead.t, ahead.h) + 8 * lane);
+      if (KINDS == 3) slotAhead = p.slots[t0 + ahead.t];
+    }
+  };
+  int step = threadIdx.x >> 5;
+  load(step);
   if (p.rope.half > 0) {
-    fillAngles(p.rope, t0, n, p.tpb, angles);
+    if (normed) fillWeights<T>(p.rope, p.D, weights);
+    fillAngles(p.rope, t0, n, angles);
     __syncthreads();
   }
   const float share = 1.0f / p.D;
-  // Whole warps step together: a row behind the last one is masked.
-  for (int base = 0; base < rows; base += kRows) {
-    const int t = at.t, which = (at.h >= nq) + (at.h >= nq + nk);
-    const int h = at.h - (which > 0 ? nq : 0) - (which > 1 ? nk : 0);
-    const bool live = t < n && active;
-    uint4 raw = ahead;
-    at.next();
-    if (base + kRows < rows) ahead = load();
-    if (__any_sync(~0u, which < 2)) {
+  for (; step < steps.end[KINDS - 1]; step += kThreads / 32) {
+    const Row row = ahead;
+    const int slot = slotAhead;
+    uint4 raw = rawAhead;
+    load(step + kThreads / 32);
+    if (row.kind < 2 && p.rope.half > 0) {
       float x[8];
       unpack8<T>(raw, x);
-      if (normed) {
+      if (p.rope.weight[row.kind] != nullptr) {
         const float r = rsqrtf(__fadd_rn(__fmul_rn(squaresOfRow<LANES>(x, lane, p.D), share), p.rope.eps));
-        if (which < 2 && p.rope.weight[which] != nullptr) {
+        if (active) {
           float w[8];
-          unpack8<T>(which ? weight[1] : weight[0], w);
+          load8(weights + row.kind * p.D + 8 * lane, w);
 #pragma unroll
           for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
         }
       }
-      if (p.rope.half > 0) {
-        const float* c = angles + min(t, n - 1) * p.rope.half;
-        rotate<LANES>(x, lane, p.rope, c, c + p.tpb * p.rope.half, 1.0f);
-        // a row of values shares the warp, and keeps its bits
-        if (which < 2) raw = pack8<T>(x);
-      }
-      if (which < 2 && live && p.out[which].data != nullptr) {
-        const Heads& out = p.out[which];
-        *reinterpret_cast<uint4*>(static_cast<T*>(out.data) + (t0 + t) * out.tok + h * out.head + 8 * lane) = raw;
-      }
+      rotate<LANES, false>(x, lane, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
+      raw = pack8<T>(x);
+      if (row.live && p.side[row.kind].out != nullptr)
+        *reinterpret_cast<uint4*>(outOf<T>(p.side[row.kind], t0 + row.t, row.h) + 8 * lane) = raw;
     }
-    if (p.cache.data != nullptr && __any_sync(~0u, which > 0)) {
+    if (KINDS == 3 && row.kind > 0) {
       uint32_t params;
       const uint32_t word = kv4::quantise8<T>(raw, &params);
-      const int slot = which > 0 && live ? p.slots[t0 + t] : -1;
-      if (slot >= 0 && slot < p.cache.tokens) {
-        uint8_t* blk = cacheBlock(p.cache, slot, h);
+      if (row.live && slot >= 0 && slot < p.cache.tokens) {
+        uint8_t* blk = cacheBlock(p.cache, slot, row.h);
         const int place = slot & 15, G = p.D / kv4::kGroup, g = lane >> 3, b = lane & 7;
-        const bool keys = which == 1;
+        const bool keys = row.kind == 1;
         const int rowAt = keys ? place : 16 + kv4::valueRow(place);
         const int wordAt = keys ? kv4::keyWord(b, g, G) : kv4::valueWord(b, g, G);
         *reinterpret_cast<uint32_t*>(blk + rowAt * (p.D / 2) + 4 * wordAt) = word;
@@ -260,9 +322,9 @@ __global__ void __launch_bounds__(kThreads, 4) forwardKernel(ForwardArgs p) {
 }
 
 struct ReadArgs {
+  Side side[2];  // keys, values: out
   Cache cache;
   const int* slots;
-  Heads out[2];
   int tokens, tpb;
 };
 
@@ -278,18 +340,20 @@ __device__ __forceinline__ void store8<float>(float* dst, const float (&x)[8]) {
 
 // Block: tpb tokens, their keys and then their values.
 template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) readKernel(ReadArgs p) {
-  constexpr int kRows = kThreads / LANES, D = 8 * LANES, G = D / kv4::kGroup;
+__global__ void __launch_bounds__(kThreads) readKernel(const __grid_constant__ ReadArgs p) {
+  constexpr int D = 8 * LANES, G = D / kv4::kGroup;
   const int t0 = blockIdx.x * p.tpb, n = min(p.tpb, p.tokens - t0);
-  const int lane = threadIdx.x % LANES, g = lane >> 3, b = lane & 7, heads = p.cache.heads;
-  RowWalk at(threadIdx.x / LANES, kRows, 2 * heads);
-  for (; at.t < n; at.next()) {
-    const bool keys = at.h < heads;
-    const int h = keys ? at.h : at.h - heads;
-    const int slot = p.slots[t0 + at.t];
+  const int lane = threadIdx.x % LANES, g = lane >> 3, b = lane & 7;
+  const Steps<2> steps = stepsOf<2, LANES>(p.side, n);
+#pragma unroll 2
+  for (int step = threadIdx.x >> 5; step < steps.end[1]; step += kThreads / 32) {
+    const Row row = rowOf<2, LANES>(p.side, steps, step, n, true);
+    if (!row.live) continue;
+    const bool keys = row.kind == 0;
+    const int slot = p.slots[t0 + row.t];
     float x[8] = {};
     if (slot >= 0 && slot < p.cache.tokens) {
-      const uint8_t* blk = cacheBlock(p.cache, slot, h);
+      const uint8_t* blk = cacheBlock(p.cache, slot, row.h);
       const int place = slot & 15;
       const int rowAt = keys ? place : 16 + kv4::valueRow(place);
       const int wordAt = keys ? kv4::keyWord(b, g, G) : kv4::valueWord(b, g, G);
@@ -297,13 +361,13 @@ __global__ void __launch_bounds__(kThreads) readKernel(ReadArgs p) {
       const uint32_t params = *reinterpret_cast<const uint32_t*>(blk + (keys ? 16 : 17) * D + place * (4 * G) + 4 * g);
       kv4::dequantise8(word, params, x);
     }
-    const Heads& out = keys ? p.out[0] : p.out[1];
-    store8<T>(static_cast<T*>(out.data) + (t0 + at.t) * out.tok + h * out.head + 8 * lane, x);
+    store8<T>(outOf<T>(p.side[row.kind], t0 + row.t, row.h) + 8 * lane, x);
   }
 }
 
 struct BackwardArgs {
-  Heads dy[2], x[2], dx[2];
+  Side side[2];    // gradients of the outputs in, of the inputs out
+  Side forward[2];  // the inputs
   Rope rope;
   float* partial;  // [grid][2][D] sums of dy * x^ (where a weight is given)
   int tokens, D, tpb;
@@ -316,88 +380,77 @@ constexpr int kBackwardBlocks = 148 * 4;
 // dx = r (w g - x^ mean(w g x^)), dw = sum g x^ with g = R^-1 dy, x^ = x r,
 // r = 1 / sqrt(mean x^2 + eps).
 template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads, 3) backwardKernel(BackwardArgs p) {
-  extern __shared__ float angles[];
-  constexpr int kRows = kThreads / LANES;
-  const int lane = threadIdx.x % LANES, row0 = threadIdx.x / LANES;
+__global__ void __launch_bounds__(kThreads, 3) backwardKernel(const __grid_constant__ BackwardArgs p) {
+  extern __shared__ float4 shared[];
+  float* weights = reinterpret_cast<float*>(shared);
+  float* angles = weights + 2 * p.D;
+  const int lane = threadIdx.x % LANES;
   const bool active = 8 * lane < p.D;
-  const int nq = p.x[0].heads, heads = nq + p.x[1].heads;
   const float share = 1.0f / p.D;
-  const bool normed = p.rope.weight[0] != nullptr || p.rope.weight[1] != nullptr;
-  uint4 weight[2] = {};
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-    if (p.rope.weight[i] != nullptr && active)
-      weight[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.rope.weight[i]) + 8 * lane);
+  fillWeights<T>(p.rope, p.D, weights);
   float dw[2][8] = {};
   for (int t0 = blockIdx.x * p.tpb; t0 < p.tokens; t0 += gridDim.x * p.tpb) {
-    const int n = min(p.tpb, p.tokens - t0), rows = n * heads;
-    RowWalk at(row0, kRows, heads);
-    // The next row is under way while one is worked on.
-    auto load = [&](uint4& dy, uint4& x) {
-      dy = x = make_uint4(0, 0, 0, 0);
-      if (at.t < n && active) {
-        const int which = at.h >= nq, h = at.h - (which ? nq : 0);
-        const Heads& a = p.dy[which];
-        dy = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.data) + (t0 + at.t) * a.tok + h * a.head + 8 * lane);
-        if (p.rope.weight[which] != nullptr) {
-          const Heads& b = p.x[which];
-          x = *reinterpret_cast<const uint4*>(static_cast<const T*>(b.data) + (t0 + at.t) * b.tok + h * b.head + 8 * lane);
-        }
+    const int n = min(p.tpb, p.tokens - t0);
+    const Steps<2> steps = stepsOf<2, LANES>(p.side, n);
+    Row ahead;
+    uint4 dyAhead, xAhead;
+    auto load = [&](int step) {
+      ahead = rowOf<2, LANES>(p.side, steps, step, n, active);
+      dyAhead = xAhead = make_uint4(0, 0, 0, 0);
+      if (ahead.live) {
+        dyAhead = *reinterpret_cast<const uint4*>(inOf<T>(p.side[ahead.kind], t0 + ahead.t, ahead.h) + 8 * lane);
+        if (p.rope.weight[ahead.kind] != nullptr)
+          xAhead = *reinterpret_cast<const uint4*>(inOf<T>(p.forward[ahead.kind], t0 + ahead.t, ahead.h) + 8 * lane);
       }
     };
-    uint4 dyAhead, xAhead;
-    load(dyAhead, xAhead);
+    int step = threadIdx.x >> 5;
+    load(step);
     __syncthreads();  // the angles of the tokens before are read
-    fillAngles(p.rope, t0, n, p.tpb, angles);
+    fillAngles(p.rope, t0, n, angles);
     __syncthreads();
-    for (int base = 0; base < rows; base += kRows) {
-      const int t = at.t, which = at.h >= nq, h = at.h - (which ? nq : 0);
-      const bool live = t < n && active;
+    for (; step < steps.end[1]; step += kThreads / 32) {
+      const Row row = ahead;
       float g[8], x[8];
       unpack8<T>(dyAhead, g);
       unpack8<T>(xAhead, x);
-      at.next();
-      if (base + kRows < rows) load(dyAhead, xAhead);
-      const float* c = angles + min(t, n - 1) * p.rope.half;
-      rotate<LANES>(g, lane, p.rope, c, c + p.tpb * p.rope.half, -1.0f);
-      if (normed) {
-        float w[8], wg[8];
-        unpack8<T>(which ? weight[1] : weight[0], w);
-        float gx = 0.0f;
+      load(step + kThreads / 32);
+      rotate<LANES, true>(g, lane, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
+      if (p.rope.weight[row.kind] != nullptr) {
+        float w[8] = {};
+        if (active) load8(weights + row.kind * p.D + 8 * lane, w);
+        float sq = 0.0f, gx = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          wg[i] = g[i] * w[i];
-          gx += wg[i] * x[i];
+          sq = fmaf(x[i], x[i], sq);
+          w[i] *= g[i];
+          gx = fmaf(w[i], x[i], gx);
         }
-        float sq = four(x) + four(x + 4);
 #pragma unroll
         for (int o = 1; o < LANES; o <<= 1) {
           sq += __shfl_xor_sync(~0u, sq, o);
           gx += __shfl_xor_sync(~0u, gx, o);
         }
-        if (p.rope.weight[which] != nullptr) {
-          const float r = rsqrtf(sq * share + p.rope.eps);
-          const float m = gx * r * share;  // mean(w g x^)
-          const float on = live ? r : 0.0f;
-          // A row behind the last one counts as zero (its r may be infinite).
+        const float r = rsqrtf(fmaf(sq, share, p.rope.eps));
+        const float m = gx * r * share;  // mean(w g x^)
+        // A row behind the last one counts as zero (its r may be infinite).
+        const float on = row.live ? r : 0.0f;
+        if (row.kind == 0) {
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float xh = x[i] * on;
-            if (which) dw[1][i] += g[i] * xh;
-            else dw[0][i] += g[i] * xh;
-            g[i] = r * (wg[i] - xh * m);
-          }
+          for (int i = 0; i < 8; i++) dw[0][i] = fmaf(g[i], x[i] * on, dw[0][i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++) dw[1][i] = fmaf(g[i], x[i] * on, dw[1][i]);
         }
+#pragma unroll
+        for (int i = 0; i < 8; i++) g[i] = r * fmaf(-(x[i] * on), m, w[i]);
       }
-      if (live) {
-        const Heads& o = p.dx[which];
-        *reinterpret_cast<uint4*>(static_cast<T*>(o.data) + (t0 + t) * o.tok + h * o.head + 8 * lane) = pack8<T>(g);
-      }
+      if (row.live) *reinterpret_cast<uint4*>(outOf<T>(p.side[row.kind], t0 + row.t, row.h) + 8 * lane) = pack8<T>(g);
     }
   }
   if (p.partial == nullptr) return;
   // Rows of the block, then the block's sums to its own place.
+  constexpr int kRows = kThreads / LANES;
+  const int row0 = threadIdx.x / LANES;
   __shared__ float sums[kThreads * 8];
 #pragma unroll
   for (int which = 0; which < 2; which++) {
@@ -446,7 +499,26 @@ int tokensPerBlock(int tokens, int heads, int D) {
   return tpb;
 }
 
-size_t angleBytes(const Rope& r, int tpb) { return static_cast<size_t>(2) * tpb * r.half * sizeof(float); }
+size_t sharedBytes(const Rope& r, int tpb, int D) { return (static_cast<size_t>(3) * tpb * r.half + 2 * D) * sizeof(float); }
+
+// Kinds of rows from the descriptions; an absent one has no heads.
+Side sideOf(const vcclHeads_t* in, const vcclHeads_t* out) {
+  Side s{};
+  if (in != nullptr) {
+    s.in = in->data;
+    s.inTok = static_cast<int>(in->tokenStride);
+    s.inHead = static_cast<int>(in->headStride);
+    s.heads = in->heads;
+  }
+  if (out != nullptr) {
+    s.out = out->data;
+    s.outTok = static_cast<int>(out->tokenStride);
+    s.outHead = static_cast<int>(out->headStride);
+    s.heads = out->heads;
+  }
+  s.recip = s.heads > 1 ? static_cast<uint32_t>(((1ull << 32) + s.heads - 1) / s.heads) : 0;
+  return s;
+}
 
 bool ropeOk(const vcclRope_t* r, int D, int tokens) {
   if (r == nullptr || (tokens > 0 && (r->positions == nullptr)) || r->invFreq == nullptr) return false;
@@ -460,20 +532,23 @@ Rope ropeOf(const vcclRope_t* r) {
   return {r->positions, r->invFreq, {r->qWeight, r->kWeight}, r->half, r->interleaved, r->eps};
 }
 
-template <typename T>
+template <typename T, int KINDS>
 void launchForward(const ForwardArgs& p, cudaStream_t st) {
   const int grid = (p.tokens + p.tpb - 1) / p.tpb;
-  const size_t smem = angleBytes(p.rope, p.tpb);
+  const size_t smem = sharedBytes(p.rope, p.tpb, p.D);
   switch (lanesFor(p.D)) {
-    case 8: forwardKernel<T, 8><<<grid, kThreads, smem, st>>>(p); break;
-    case 16: forwardKernel<T, 16><<<grid, kThreads, smem, st>>>(p); break;
-    default: forwardKernel<T, 32><<<grid, kThreads, smem, st>>>(p); break;
+    case 8: forwardKernel<T, 8, KINDS><<<grid, kThreads, smem, st>>>(p); break;
+    case 16: forwardKernel<T, 16, KINDS><<<grid, kThreads, smem, st>>>(p); break;
+    default:
+      // the cache holds rows of 64 or 128 channels
+      if constexpr (KINDS == 2) forwardKernel<T, 32, KINDS><<<grid, kThreads, smem, st>>>(p);
+      break;
   }
 }
 
 template <typename T>
 void launchBackward(const BackwardArgs& p, int grid, cudaStream_t st) {
-  const size_t smem = angleBytes(p.rope, p.tpb);
+  const size_t smem = sharedBytes(p.rope, p.tpb, p.D);
   switch (lanesFor(p.D)) {
     case 8: backwardKernel<T, 8><<<grid, kThreads, smem, st>>>(p); break;
     case 16: backwardKernel<T, 16><<<grid, kThreads, smem, st>>>(p); break;
@@ -496,8 +571,11 @@ bool cacheOk(const vcclKv4_t* c) {
 }
 
 Cache cacheOf(const vcclKv4_t* c) {
-  return {static_cast<uint8_t*>(c->data), static_cast<long long>(c->pages) * c->pageSize, c->kvHeads,
-          c->pageSize / kv4::kBlockTokens, c->D};
+  const int per = c->pageSize / kv4::kBlockTokens;
+  int shift = 0;
+  while ((1 << shift) < per) shift++;
+  return {static_cast<uint8_t*>(c->data), static_cast<long long>(c->pages) * c->pageSize, c->kvHeads, per,
+          (1 << shift) == per ? shift : -1, c->D};
 }
 
 }  // namespace
@@ -520,17 +598,15 @@ vcclResult_t vcclQkNormRope(const vcclHeads_t* q, const vcclHeads_t* k, const vc
     return vcclInvalidArgument;
   TraceRange trace("vccl QkNormRope");
   ForwardArgs p{};
-  p.in[0] = headsOf(q);
-  p.in[1] = headsOf(k);
-  p.out[0] = headsOf(qOut);
-  p.out[1] = headsOf(kOut);
+  p.side[0] = sideOf(q, qOut);
+  p.side[1] = sideOf(k, kOut);
   p.rope = ropeOf(rope);
   p.tokens = tokens;
   p.D = D;
   p.tpb = tokensPerBlock(tokens, q->heads + k->heads, D);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (datatype == vcclBfloat16) launchForward<__nv_bfloat16>(p, st);
-  else launchForward<__half>(p, st);
+  if (datatype == vcclBfloat16) launchForward<__nv_bfloat16, 2>(p, st);
+  else launchForward<__half, 2>(p, st);
   return launched("vcclQkNormRope");
 }
 
@@ -557,12 +633,10 @@ vcclResult_t vcclQkNormRopeBackward(const vcclHeads_t* dq, const vcclHeads_t* dk
   int grid = 0;
   if (tokens > 0) {
     BackwardArgs p{};
-    p.dy[0] = headsOf(dq);
-    p.dy[1] = headsOf(dk);
-    p.x[0] = headsOf(q);
-    p.x[1] = headsOf(k);
-    p.dx[0] = headsOf(dqIn);
-    p.dx[1] = headsOf(dkIn);
+    p.side[0] = sideOf(dq, dqIn);
+    p.side[1] = sideOf(dk, dkIn);
+    p.forward[0] = sideOf(q, nullptr);
+    p.forward[1] = sideOf(k, nullptr);
     p.rope = ropeOf(rope);
     p.partial = weights ? static_cast<float*>(workspace) : nullptr;
     p.tokens = tokens;
@@ -597,19 +671,18 @@ vcclResult_t vcclKv4Append(const vcclKv4_t* cache, const vcclHeads_t* k, const v
   if (q != nullptr && (!headsOk(q, 2) || !headsOk(qOut, 2) || q->heads != qOut->heads)) return vcclInvalidArgument;
   TraceRange trace("vccl Kv4Append");
   ForwardArgs p{};
-  p.in[0] = headsOf(q);
-  p.in[1] = headsOf(k);
-  p.in[2] = headsOf(v);
-  p.out[0] = headsOf(qOut);
+  p.side[0] = sideOf(q, qOut);
+  p.side[1] = sideOf(k, nullptr);
+  p.side[2] = sideOf(v, nullptr);
   p.rope = ropeOf(rope);
   p.cache = cacheOf(cache);
   p.slots = slots;
   p.tokens = tokens;
   p.D = cache->D;
-  p.tpb = tokensPerBlock(tokens, p.in[0].heads + 2 * cache->kvHeads, cache->D);
+  p.tpb = tokensPerBlock(tokens, p.side[0].heads + 2 * cache->kvHeads, cache->D);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (datatype == vcclBfloat16) launchForward<__nv_bfloat16>(p, st);
-  else launchForward<__half>(p, st);
+  if (datatype == vcclBfloat16) launchForward<__nv_bfloat16, 3>(p, st);
+  else launchForward<__half, 3>(p, st);
   return launched("vcclKv4Append");
 }
 
@@ -623,7 +696,7 @@ vcclResult_t vcclKv4Read(const vcclKv4_t* cache, const int* slots, const vcclHea
     return vcclInvalidArgument;
   TraceRange trace("vccl Kv4Read");
   const int tpb = tokensPerBlock(tokens, 2 * cache->kvHeads, cache->D);
-  const ReadArgs p{cacheOf(cache), slots, {headsOf(k), headsOf(v)}, tokens, tpb};
+  const ReadArgs p{{sideOf(nullptr, k), sideOf(nullptr, v)}, cacheOf(cache), slots, tokens, tpb};
   const int grid = (tokens + tpb - 1) / tpb;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (datatype == vcclBfloat16) launchRead<__nv_bfloat16>(p, grid, st);
