@@ -37,7 +37,8 @@ namespace vccl {
 namespace model {
 namespace {
 
-constexpr int kWarps = 4;          // per block
+constexpr int kWarps = 8;          // per block
+constexpr int kStages = 4;         // blocks of 16 tokens that a warp has under way
 constexpr int kTile = 32;          // tokens in a unit of work
 constexpr int kMaxBatch = 4096;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -168,22 +169,42 @@ struct BlockRegs {
 template <int WORDS>
 __device__ __forceinline__ void loadWords(const uint8_t* p, uint32_t* w) {
   if constexpr (WORDS == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
     w[0] = v.x;
     w[1] = v.y;
     w[2] = v.z;
     w[3] = v.w;
   } else if constexpr (WORDS == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x;
     w[1] = v.y;
   } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// A block in shared memory is as in global memory, but that for D = 128 the
+// 16-byte chunks of value rows 4i + 2 and 4i + 3 change places in twos: lanes
+// of four rows then read from different banks.
+__device__ __forceinline__ int swapTwos(int chunk) { return chunk ^ ((chunk & 8) >> 2); }
+
+template <int G>
+__device__ __forceinline__ void copyBlock(uint8_t* to, const uint8_t* from, int lane) {
+  constexpr int D = 64 * G, kChunks = 18 * D / 16;
+  const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+#pragma unroll
+  for (int j = 0; j < (kChunks + 31) / 32; j++) {
+    const bool values = G == 2 && j >= D / 64 && j < D / 32;  // chunks D / 2 to D
+    const int chunk = 32 * j + lane;
+    if (32 * (j + 1) <= kChunks || chunk < kChunks)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 16 * (32 * j + (values ? swapTwos(lane) : lane))),
+                   "l"(from + 16 * chunk)
+                   : "memory");
   }
 }
 
 template <int G>
-__device__ __forceinline__ void loadBlock(BlockRegs<G>& r, const uint8_t* block, int lane) {
+__device__ __forceinline__ void readBlock(BlockRegs<G>& r, const uint8_t* block, int lane) {
   constexpr int D = 64 * G;
   const int g = lane >> 2, q = lane & 3;
 #pragma unroll
@@ -192,8 +213,9 @@ __device__ __forceinline__ void loadBlock(BlockRegs<G>& r, const uint8_t* block,
     loadWords<G>(block + 16 * D + (g + 8 * i) * (4 * G), r.kp[i]);
     loadWords<G>(block + 17 * D + (g + 8 * i) * (4 * G), r.vp[i]);
   }
+  const int at = G == 2 ? q * (D / 2) + ((g * 8) ^ ((q & 2) << 4)) : q * (D / 2) + g * 4;
 #pragma unroll
-  for (int i = 0; i < 4; i++) loadWords<G>(block + 8 * D + (4 * i + q) * (D / 2) + g * (4 * G), r.v[i]);
+  for (int i = 0; i < 4; i++) loadWords<G>(block + 8 * D + 4 * i * (D / 2) + at, r.v[i]);
 }
 
 // A warp's state for one unit.
@@ -201,7 +223,7 @@ template <int G, int NT>
 struct Unit {
   uint32_t qb[NT][G][4][2];  // Q^T operands: word half h, code pair u -> [2h + u]
   float qs[NT][2];           // log2(e) * scale * 2^24 / (power of two of the row), rows 2q and 2q + 1
-  float sq[NT][G][2];        // log2(e) * scale * sum of the row's group
+  float sq[NT][G][2];        // sum of the row's group, in units of qs
   int limit[NT][2];          // tokens that the row sees
   int most, least;           // of all rows of the unit
   float m[NT][2], l[NT][2];
@@ -259,7 +281,7 @@ __device__ __forceinline__ void loadQuery(Unit<G, NT>& u, const AttnArgs& p, con
       for (int j = 0; j < 16; j++) s += x[gr][j];
       s += __shfl_xor_sync(~0u, s, 1);
       s += __shfl_xor_sync(~0u, s, 2);
-      sq[gr] = s * p.scaleLog2;
+      sq[gr] = s * f * 5.9604644775390625e-8f;
 #pragma unroll
       for (int w = 0; w < 4; w++) {  // word half w / 2, code pair w % 2: channels 4w .. 4w + 3 of the lane's 16
         const float* y = &x[gr][4 * w];
@@ -309,8 +331,9 @@ __device__ __forceinline__ void loadQuery(Unit<G, NT>& u, const AttnArgs& p, con
 template <int G, int NT>
 __device__ __forceinline__ void blockStep(Unit<G, NT>& u, const BlockRegs<G>& r, int t0, int lane) {
   const int g = lane >> 2;
-  float x[NT][4];
-  // S^T, group by group: the scale of a token and group acts on the group's sum.
+  // S^T, group by group: the scale of a token and group acts on the group's
+  // sum.  z is the score in units of qs.
+  float z[NT][4], x[NT][4];
 #pragma unroll
   for (int gr = 0; gr < G; gr++) {
     float acc[NT][4] = {};
@@ -334,11 +357,15 @@ __device__ __forceinline__ void blockStep(Unit<G, NT>& u, const BlockRegs<G>& r,
       for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          const float y = fmaf(acc[n][2 * i + c] * s, u.qs[n][c], off * u.sq[n][gr][c]);
-          x[n][2 * i + c] = gr == 0 ? y : x[n][2 * i + c] + y;
+          const float y = gr == 0 ? off * u.sq[n][gr][c] : fmaf(off, u.sq[n][gr][c], z[n][2 * i + c]);
+          z[n][2 * i + c] = fmaf(acc[n][2 * i + c], s, y);
         }
     }
   }
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int k = 0; k < 4; k++) x[n][k] = fmaf(z[n][k], u.qs[n][k & 1], -u.m[n][k & 1]);
   float s[2][G], mid[2][G];
 #pragma unroll
   for (int i = 0; i < 2; i++)
@@ -368,11 +395,12 @@ __device__ __forceinline__ void blockStep(Unit<G, NT>& u, const BlockRegs<G>& r,
   // The maximum is followed loosely: it moves when a score passes it by 8
   // (weights reach 2^8), and the power of two of the scales when one passes
   // it by 4, so most blocks take neither a reduction nor a rescaling.
-  bool grow = false;
+  float high = fmaxf(x[0][0], x[0][1]);
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int c = 0; c < 2; c++) grow = grow || fmaxf(x[n][c], x[n][2 + c]) > u.m[n][c] + 8.0f;
+    for (int k = n == 0 ? 2 : 0; k < 4; k++) high = fmaxf(high, x[n][k]);
+  bool grow = high > 8.0f;
 #pragma unroll
   for (int gr = 0; gr < G; gr++) grow = grow || fmaxf(s[0][gr], s[1][gr]) > u.lim[gr];
   if (__any_sync(~0u, grow)) {
@@ -389,14 +417,17 @@ __device__ __forceinline__ void blockStep(Unit<G, NT>& u, const BlockRegs<G>& r,
         const float inv = __uint_as_float(static_cast<uint32_t>(min(254 - e, 253)) << 23);
         beta[gr] = u.lim[gr] > 0.0f ? inv / u.inv[gr] : 1.0f;  // a quotient of powers of two
         u.inv[gr] = inv;
-        u.lim[gr] = e < 252 ? __uint_as_float(static_cast<uint32_t>(e + 2) << 23) : INFINITY;
+        u.lim[gr] = e <= 252 ? __uint_as_float(static_cast<uint32_t>(e + 2) << 23) : INFINITY;
       }
     }
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        float top = fmaxf(x[n][c], x[n][2 + c]);
+        float top = kNone;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+          if (x[n][2 * i + c] != -INFINITY) top = fmaxf(top, z[n][2 * i + c] * u.qs[n][c]);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
         const float m = fmaxf(u.m[n][c], top);
@@ -405,6 +436,9 @@ __device__ __forceinline__ void blockStep(Unit<G, NT>& u, const BlockRegs<G>& r,
         u.l[n][c] *= alpha[n][c];
 #pragma unroll
         for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] *= alpha[n][c];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+          if (x[n][2 * i + c] != -INFINITY) x[n][2 * i + c] = fmaf(z[n][2 * i + c], u.qs[n][c], -m);
       }
 #pragma unroll
       for (int gr = 0; gr < G; gr++) {
@@ -424,14 +458,15 @@ __device__ __forceinline__ void blockStep(Unit<G, NT>& u, const BlockRegs<G>& r,
     for (int i = 0; i < 2; i++)
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        const float w = exp2Fast(x[n][2 * i + c] - u.m[n][c]);
+        const float w = exp2Fast(x[n][2 * i + c]);
         x[n][2 * i + c] = w;
         u.l[n][c] += w;
+        if (!edge) {
 #pragma unroll
-        for (int gr = 0; gr < G; gr++) {
-          // at the edge a row must not meet a NaN of a token that it does not see
-          const float add = edge && w == 0.0f ? 0.0f : mid[i][gr];
-          u.mid[n][gr][c] = fmaf(w, add, u.mid[n][gr][c]);
+          for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] = fmaf(w, mid[i][gr], u.mid[n][gr][c]);
+        } else if (w != 0.0f) {  // a row must not meet a NaN of a token that it does not see
+#pragma unroll
+          for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] = fmaf(w, mid[i][gr], u.mid[n][gr][c]);
         }
       }
   // O^T: rows are channels 8g + 2j (from the low halves) and 8g + 2j + 1.
@@ -522,10 +557,19 @@ __device__ __forceinline__ void finish(Unit<G, NT>& u, const AttnArgs& p, const 
     }
 }
 
+constexpr int blocksPerSm(int nt) { return nt == 1 ? 2 : 1; }
+
+template <int G>
+constexpr int ringBytes() {
+  return kStages * 18 * 64 * G;
+}
+
 template <int G, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) attnKernel(AttnArgs p) {
-  extern __shared__ long long prefix[];
-  constexpr int R = 8 * NT;
+__global__ void __launch_bounds__(kWarps * 32, blocksPerSm(NT)) attnKernel(const __grid_constant__ AttnArgs p) {
+  extern __shared__ uint4 shared[];  // the warps' rings, then the prefix sums
+  constexpr int R = 8 * NT, D = 64 * G;
+  uint8_t* ring = reinterpret_cast<uint8_t*>(shared) + (threadIdx.x >> 5) * ringBytes<G>();
+  long long* prefix = reinterpret_cast<long long*>(reinterpret_cast<uint8_t*>(shared) + kWarps * ringBytes<G>());
   scanTiles<kWarps * 32>(p, R, prefix);
   __syncthreads();
   if (blockIdx.x == 0)
@@ -543,38 +587,54 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) attnKernel(AttnA
     const Request r = requestOf(p, b);
     const int nt = tilesOf(r), units = unitsOf(p, r, R);
     const long long off = tile - prefix[b];
-    const int unit = static_cast<int>(off / nt), from = static_cast<int>(off % nt);
-    const int head = unit / units, row0 = (unit % units) * R;
+    const int unit = static_cast<int>(off / nt), from = static_cast<int>(off - static_cast<long long>(unit) * nt);
+    const int head = unit / units, row0 = (unit - head * units) * R;
     const int upto = static_cast<int>(min(static_cast<long long>(nt), from + (last - tile)));
+    const int begin = from * (kTile / kv4::kBlockTokens);
+    const int* pages = p.table + static_cast<long long>(b) * p.width;
 
+    // Lane i looks up block 32 j + i of the range: its page, then its address.
+    // The pages of the next 32 are under way while these are copied.
+    const int known = (r.kv + kv4::kBlockTokens - 1) / kv4::kBlockTokens;
+    auto pageOf = [&](int block) { return block < known ? pages[block / p.blocksPerPage] : -1; };
+    int pageAhead = pageOf(begin + lane);
     Unit<G, NT> u;
     loadQuery<G, NT>(u, p, r, head, row0, lane);
-    // Blocks of this range that some row sees; page numbers come 32 blocks at a time.
+    // Blocks of this range that some row sees.
     const int end = min(upto * (kTile / kv4::kBlockTokens), (u.most + kv4::kBlockTokens - 1) / kv4::kBlockTokens);
-    for (int base = from * (kTile / kv4::kBlockTokens); base < end; base += 32) {
-      const int mine = base + lane;
-      int page = -1;
-      if (mine < end) page = p.table[static_cast<long long>(b) * p.width + mine / p.blocksPerPage];
-      const int count = min(32, end - base);
-      BlockRegs<G> regs[2];
-      auto fetch = [&](BlockRegs<G>& to, int k) {
-        const int pg = __shfl_sync(~0u, page, k);
-        const bool ok = pg >= 0 && pg < p.pages;
-        if (ok)
-          loadBlock<G>(to,
-                       p.cache + ((static_cast<long long>(pg) * p.kvHeads + head) * p.blocksPerPage +
-                                  (base + k) % p.blocksPerPage) * kv4::blockBytes(64 * G),
-                       lane);
-        return ok;
-      };
-      bool ok0 = fetch(regs[0], 0), ok1 = false;
-      for (int k = 0; k < count; k += 2) {
-        if (k + 1 < count) ok1 = fetch(regs[1], k + 1);
-        if (ok0) blockStep<G, NT>(u, regs[0], (base + k) * kv4::kBlockTokens, lane);
-        if (k + 2 < count) ok0 = fetch(regs[0], k + 2);
-        if (k + 1 < count && ok1) blockStep<G, NT>(u, regs[1], (base + k + 1) * kv4::kBlockTokens, lane);
+    long long address = 0;
+    uint32_t there = 0, thereBefore = 0;  // blocks of this look-up, and the last, whose page exists
+    auto issue = [&](int i) {  // i-th block of the range
+      const int block = begin + i;
+      if (block < end) {
+        if ((i & 31) == 0) {
+          const int mine = block + lane, page = pageAhead;
+          const bool ok = page >= 0 && page < p.pages;
+          address = ((static_cast<long long>(page) * p.kvHeads + head) * p.blocksPerPage + mine % p.blocksPerPage) * (18 * D);
+          thereBefore = there;
+          there = __ballot_sync(~0u, ok);
+          pageAhead = pageOf(mine + 32);
+        }
+        const long long at = __shfl_sync(~0u, address, i & 31);
+        if ((there >> (i & 31)) & 1u) copyBlock<G>(ring + (i & (kStages - 1)) * (18 * D), p.cache + at, lane);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++) issue(i);
+    for (int i = 0; begin + i < end; i++) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();  // the block is there for every lane, and the one before has been read by all
+      issue(i + kStages - 1);
+      // the look-up may have moved on to the next 32 blocks
+      const uint32_t mask = ((i ^ (i + kStages - 1)) & 32) && begin + ((i + kStages - 1) & ~31) < end ? thereBefore : there;
+      if ((mask >> (i & 31)) & 1u) {
+        BlockRegs<G> regs;
+        readBlock<G>(regs, ring + (i & (kStages - 1)) * (18 * D), lane);
+        blockStep<G, NT>(u, regs, (begin + i) * kv4::kBlockTokens, lane);
       }
     }
+    __syncwarp();  // the ring is read by all before the next unit's copies
     const bool whole = from == 0 && upto == nt;
     // A range has at most two partial units: the one it starts in, and the one it ends in.
     finish<G, NT>(u, p, r, head, row0, lane, whole ? -1 : tile == first ? 2 * w : 2 * w + 1);
@@ -669,6 +729,16 @@ int rowTiles(int batch, int tokens, int group) {
   return group > 8 || static_cast<long long>(tokens) * group > 8LL * batch ? 2 : 1;
 }
 
+template <int G, int NT>
+cudaError_t launchAttn(const AttnArgs& p, int grid, cudaStream_t st) {
+  const size_t smem = kWarps * ringBytes<G>() + static_cast<size_t>(p.batch + 1) * sizeof(long long);
+  const cudaError_t e = cudaFuncSetAttribute(attnKernel<G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             kWarps * ringBytes<G>() + (kMaxBatch + 1) * static_cast<int>(sizeof(long long)));
+  if (e != cudaSuccess) return e;
+  attnKernel<G, NT><<<grid, kWarps * 32, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 }  // namespace
@@ -683,7 +753,7 @@ extern "C" {
 size_t vcclKv4AttentionWorkspace(int batch, int tokens, int qHeads, int kvHeads, int D) {
   if (batch <= 0 || kvHeads <= 0 || qHeads <= 0 || D <= 0) return 0;
   const int nt = rowTiles(batch, tokens, qHeads / kvHeads);
-  const size_t slots = static_cast<size_t>(smsOfDevice()) * (nt == 1 ? 3 : 2) * kWarps * 2;
+  const size_t slots = static_cast<size_t>(smsOfDevice()) * blocksPerSm(nt) * kWarps * 2;
   return align256((batch + 1) * sizeof(long long)) + align256(slots * 8 * nt * sizeof(float2)) +
          slots * 8 * nt * D * sizeof(float);
 }
@@ -705,7 +775,7 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   TraceRange trace("vccl Kv4Attention");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int group = q->heads / cache->kvHeads, nt = rowTiles(batch, tokens, group), R = 8 * nt;
-  const int grid = smsOfDevice() * (nt == 1 ? 3 : 2);
+  const int grid = smsOfDevice() * blocksPerSm(nt);
   AttnArgs p{};
   p.q = q->data;
   p.qTok = q->tokenStride;
@@ -736,13 +806,12 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   p.stats = reinterpret_cast<float2*>(ws);
   ws += align256(static_cast<size_t>(p.workers) * 2 * R * sizeof(float2));
   p.partial = reinterpret_cast<float*>(ws);
-  const size_t smem = static_cast<size_t>(batch + 1) * sizeof(long long);
-  if (cache->D == 128) {
-    if (nt == 1) attnKernel<2, 1><<<grid, kWarps * 32, smem, st>>>(p);
-    else attnKernel<2, 2><<<grid, kWarps * 32, smem, st>>>(p);
-  } else {
-    if (nt == 1) attnKernel<1, 1><<<grid, kWarps * 32, smem, st>>>(p);
-    else attnKernel<1, 2><<<grid, kWarps * 32, smem, st>>>(p);
+  cudaError_t e;
+  if (cache->D == 128) e = nt == 1 ? launchAttn<2, 1>(p, grid, st) : launchAttn<2, 2>(p, grid, st);
+  else e = nt == 1 ? launchAttn<1, 1>(p, grid, st) : launchAttn<1, 2>(p, grid, st);
+  if (e != cudaSuccess) {
+    VERR("vcclKv4Attention: %s", cudaGetErrorString(e));
+    return vcclSystemError;
   }
   const int rows = static_cast<int>((static_cast<long long>(tokens) * q->heads + 3) / 4);
   if (cache->D == 128) joinKernel<2><<<rows, 128, 0, st>>>(p, R);
