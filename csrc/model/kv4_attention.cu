@@ -37,9 +37,10 @@ namespace vccl {
 namespace model {
 namespace {
 
-constexpr int kWarps = 8;          // per block
-constexpr int kStages = 4;         // blocks of 16 tokens that a warp has under way
-constexpr int kTile = 32;          // tokens in a unit of work
+constexpr int kTile = 32;          // tokens that a warp takes in one step
+constexpr int kWarps = 12;         // per block, one block per SM
+constexpr int kStages = 3;         // tiles that a warp has in shared memory
+constexpr int kBlocks = kTile / kv4::kBlockTokens;  // blocks in a tile
 constexpr int kMaxBatch = 4096;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kNone = -1e30f;    // a maximum over nothing
@@ -141,6 +142,14 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The first product of a sum.
+__device__ __forceinline__ void mmaFirst(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -157,14 +166,6 @@ __device__ __forceinline__ float exp2Fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-
-// The codes and parameters of one block of 16 tokens, as one lane reads them.
-template <int G>
-struct BlockRegs {
-  uint32_t k[2][2 * G];  // tokens g, g + 8: words (group, half)
-  uint32_t v[4][G];      // tokens 2q, 2q + 1, 8 + 2q, 9 + 2q: word of each group
-  uint32_t kp[2][G], vp[2][G];
-};
 
 template <int WORDS>
 __device__ __forceinline__ void loadWords(const uint8_t* p, uint32_t* w) {
@@ -203,19 +204,34 @@ __device__ __forceinline__ void copyBlock(uint8_t* to, const uint8_t* from, int 
   }
 }
 
+// What a lane reads of a block: of keys, tokens g and g + 8, words (group,
+// half); of values, tokens 2q, 2q + 1, 8 + 2q, 9 + 2q, the word of each group;
+// scales and midpoints of tokens g and g + 8.
 template <int G>
-__device__ __forceinline__ void readBlock(BlockRegs<G>& r, const uint8_t* block, int lane) {
+__device__ __forceinline__ void readKeys(uint32_t (&k)[2][2 * G], uint32_t (&kp)[2][G], const uint8_t* block, int lane) {
   constexpr int D = 64 * G;
   const int g = lane >> 2, q = lane & 3;
 #pragma unroll
   for (int i = 0; i < 2; i++) {
-    loadWords<2 * G>(block + (g + 8 * i) * (D / 2) + q * (8 * G), r.k[i]);
-    loadWords<G>(block + 16 * D + (g + 8 * i) * (4 * G), r.kp[i]);
-    loadWords<G>(block + 17 * D + (g + 8 * i) * (4 * G), r.vp[i]);
+    loadWords<2 * G>(block + (g + 8 * i) * (D / 2) + q * (8 * G), k[i]);
+    loadWords<G>(block + 16 * D + (g + 8 * i) * (4 * G), kp[i]);
   }
+}
+
+template <int G>
+__device__ __forceinline__ void readValueParams(uint32_t (&vp)[2][G], const uint8_t* block, int lane) {
+  constexpr int D = 64 * G;
+#pragma unroll
+  for (int i = 0; i < 2; i++) loadWords<G>(block + 17 * D + ((lane >> 2) + 8 * i) * (4 * G), vp[i]);
+}
+
+template <int G>
+__device__ __forceinline__ void readValues(uint32_t (&v)[4][G], const uint8_t* block, int lane) {
+  constexpr int D = 64 * G;
+  const int g = lane >> 2, q = lane & 3;
   const int at = G == 2 ? q * (D / 2) + ((g * 8) ^ ((q & 2) << 4)) : q * (D / 2) + g * 4;
 #pragma unroll
-  for (int i = 0; i < 4; i++) loadWords<G>(block + 8 * D + 4 * i * (D / 2) + at, r.v[i]);
+  for (int i = 0; i < 4; i++) loadWords<G>(block + 8 * D + 4 * i * (D / 2) + at, v[i]);
 }
 
 // A warp's state for one unit.
@@ -227,7 +243,7 @@ struct Unit {
   int limit[NT][2];          // tokens that the row sees
   int most, least;           // of all rows of the unit
   float m[NT][2], l[NT][2];
-  float o[NT][G][4][4];      // 2^24 (16 for odd u) * 2^-r * sum p' c
+  float o[NT][G][4][4];      // 2^-24 * 2^-r * sum p' c; odd j: of c + 16 c', c that of j - 1
   float ones[NT][G][4];      // 2^-r * sum p'
   float mid[NT][G][2];       // sum p mid
   float inv[G], lim[G];      // 2^-r, and the scale above which r grows
@@ -327,87 +343,116 @@ __device__ __forceinline__ void loadQuery(Unit<G, NT>& u, const AttnArgs& p, con
   u.least = min(least, __shfl_xor_sync(~0u, least, 2));
 }
 
-// One block of 16 tokens that starts at token t0 of the request.
+// The two bytes of a word's upper halves, each in the low byte of 16 bits.
+__device__ __forceinline__ uint32_t upperBytes(uint32_t w) { return __byte_perm(w, 0u, 0x4341); }
+
+// A tile of 32 tokens that starts at token t0 of the request.  Two blocks at a
+// time give the scheduler twice the independent work of one, and share the
+// looks at the maximum (one block at a time: 166 us where this takes 137, 64
+// requests of 500 to 16000 tokens, 8 key heads).  there: bit b, block b exists.
 template <int G, int NT>
-__device__ __forceinline__ void blockStep(Unit<G, NT>& u, const BlockRegs<G>& r, int t0, int lane) {
+__device__ __forceinline__ void tileStep(Unit<G, NT>& u, const uint8_t* tile, int t0, uint32_t there, int lane) {
+  constexpr int D = 64 * G, B = kBlocks;
   const int g = lane >> 2;
   // S^T, group by group: the scale of a token and group acts on the group's
-  // sum.  z is the score in units of qs.
-  float z[NT][4], x[NT][4];
+  // sum.  z is the score in units of qs; x what it passes the maximum by.
+  float z[B][NT][4], x[B][NT][4];
 #pragma unroll
-  for (int gr = 0; gr < G; gr++) {
-    float acc[NT][4] = {};
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const uint32_t w0 = r.k[0][2 * gr + h], w1 = r.k[1][2 * gr + h];
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-        mma(acc[n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, u.qb[n][gr][2 * h][0],
-            u.qb[n][gr][2 * h][1]);
-      const uint32_t s0 = w0 >> 8, s1 = w1 >> 8;
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-        mma(acc[n], s0 & 0x000F000Fu, s1 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x00F000F0u, u.qb[n][gr][2 * h + 1][0],
-            u.qb[n][gr][2 * h + 1][1]);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++) {  // tokens g, g + 8
-      const float s = kv4::bf16Lo(r.kp[i][gr]), off = fmaf(-7.5f, s, kv4::bf16Hi(r.kp[i][gr]));
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-          const float y = gr == 0 ? off * u.sq[n][gr][c] : fmaf(off, u.sq[n][gr][c], z[n][2 * i + c]);
-          z[n][2 * i + c] = fmaf(acc[n][2 * i + c], s, y);
-        }
-    }
-  }
-#pragma unroll
-  for (int n = 0; n < NT; n++)
-#pragma unroll
-    for (int k = 0; k < 4; k++) x[n][k] = fmaf(z[n][k], u.qs[n][k & 1], -u.m[n][k & 1]);
-  float s[2][G], mid[2][G];
-#pragma unroll
-  for (int i = 0; i < 2; i++)
+  for (int b = 0; b < B; b++) {
+    uint32_t k[2][2 * G], kp[2][G];
+    readKeys<G>(k, kp, tile + b * 18 * D, lane);
 #pragma unroll
     for (int gr = 0; gr < G; gr++) {
-      s[i][gr] = kv4::bf16Lo(r.vp[i][gr]);
-      mid[i][gr] = kv4::bf16Hi(r.vp[i][gr]);
-    }
-  // Tokens behind some row's last one: their scores are none, and the
-  // parameters of those that no row sees may be anything.
-  const bool edge = t0 + kv4::kBlockTokens > u.least;
-  if (edge) {
+      float acc[NT][4];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int t = t0 + g + 8 * i;
+      for (int h = 0; h < 2; h++) {
+        const uint32_t w0 = k[0][2 * gr + h], w1 = k[1][2 * gr + h];
+        const uint32_t s0 = upperBytes(w0), s1 = upperBytes(w1);
 #pragma unroll
-      for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT; n++) {
+          if (h == 0)
+            mmaFirst(acc[n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, u.qb[n][gr][0][0],
+                     u.qb[n][gr][0][1]);
+          else
+            mma(acc[n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, u.qb[n][gr][2][0],
+                u.qb[n][gr][2][1]);
+          mma(acc[n], s0 & 0x000F000Fu, s1 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x00F000F0u, u.qb[n][gr][2 * h + 1][0],
+              u.qb[n][gr][2 * h + 1][1]);
+        }
+      }
 #pragma unroll
-        for (int c = 0; c < 2; c++)
-          if (t >= u.limit[n][c]) x[n][2 * i + c] = -INFINITY;
-      if (t >= u.most) {
+      for (int i = 0; i < 2; i++) {  // tokens g, g + 8
+        const float s = kv4::bf16Lo(kp[i][gr]), off = fmaf(-7.5f, s, kv4::bf16Hi(kp[i][gr]));
 #pragma unroll
-        for (int gr = 0; gr < G; gr++) s[i][gr] = mid[i][gr] = 0.0f;
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            const float y = gr == 0 ? off * u.sq[n][gr][c] : fmaf(off, u.sq[n][gr][c], z[b][n][2 * i + c]);
+            z[b][n][2 * i + c] = fmaf(acc[n][2 * i + c], s, y);
+          }
       }
     }
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[b][n][e] = fmaf(z[b][n][e], u.qs[n][e & 1], -u.m[n][e & 1]);
+  }
+  float s[B][2][G], mid[B][2][G];
+#pragma unroll
+  for (int b = 0; b < B; b++) {
+    uint32_t vp[2][G];
+    readValueParams<G>(vp, tile + b * 18 * D, lane);
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int gr = 0; gr < G; gr++) {
+        s[b][i][gr] = kv4::bf16Lo(vp[i][gr]);
+        mid[b][i][gr] = kv4::bf16Hi(vp[i][gr]);
+      }
+  }
+  // Tokens behind some row's last one, or on no page: their scores are none,
+  // and the parameters of those that no row sees may be anything.
+  const bool edge = t0 + kTile > u.least || there != (1u << B) - 1;
+  if (edge) {
+#pragma unroll
+    for (int b = 0; b < B; b++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int t = ((there >> b) & 1u) ? t0 + 16 * b + g + 8 * i : INT_MAX;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int c = 0; c < 2; c++)
+            if (t >= u.limit[n][c]) x[b][n][2 * i + c] = -INFINITY;
+        if (t >= u.most) {
+#pragma unroll
+          for (int gr = 0; gr < G; gr++) s[b][i][gr] = mid[b][i][gr] = 0.0f;
+        }
+      }
   }
   // The maximum is followed loosely: it moves when a score passes it by 8
   // (weights reach 2^8), and the power of two of the scales when one passes
-  // it by 4, so most blocks take neither a reduction nor a rescaling.
-  float high = fmaxf(x[0][0], x[0][1]);
+  // it by 4, so most tiles take neither a reduction nor a rescaling.
+  float high = x[0][0][0], wide[G];
 #pragma unroll
-  for (int n = 0; n < NT; n++)
+  for (int b = 0; b < B; b++)
 #pragma unroll
-    for (int k = n == 0 ? 2 : 0; k < 4; k++) high = fmaxf(high, x[n][k]);
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) high = fmaxf(high, x[b][n][e]);
   bool grow = high > 8.0f;
 #pragma unroll
-  for (int gr = 0; gr < G; gr++) grow = grow || fmaxf(s[0][gr], s[1][gr]) > u.lim[gr];
+  for (int gr = 0; gr < G; gr++) {
+    wide[gr] = s[0][0][gr];
+#pragma unroll
+    for (int b = 0; b < B; b++) wide[gr] = fmaxf(wide[gr], fmaxf(s[b][0][gr], s[b][1][gr]));
+    grow = grow || wide[gr] > u.lim[gr];
+  }
   if (__any_sync(~0u, grow)) {
-    float alpha[NT][2], beta[G];
+    float beta[G];
 #pragma unroll
     for (int gr = 0; gr < G; gr++) {
-      float top = fmaxf(s[0][gr], s[1][gr]);
+      float top = wide[gr];
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
       beta[gr] = 1.0f;
@@ -422,27 +467,32 @@ __device__ __forceinline__ void blockStep(Unit<G, NT>& u, const BlockRegs<G>& r,
     }
 #pragma unroll
     for (int n = 0; n < NT; n++) {
+      float alpha[2];
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         float top = kNone;
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-          if (x[n][2 * i + c] != -INFINITY) top = fmaxf(top, z[n][2 * i + c] * u.qs[n][c]);
+        for (int b = 0; b < B; b++)
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+            if (x[b][n][2 * i + c] != -INFINITY) top = fmaxf(top, z[b][n][2 * i + c] * u.qs[n][c]);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
         const float m = fmaxf(u.m[n][c], top);
-        alpha[n][c] = exp2Fast(u.m[n][c] - m);
+        alpha[c] = exp2Fast(u.m[n][c] - m);
         u.m[n][c] = m;
-        u.l[n][c] *= alpha[n][c];
+        u.l[n][c] *= alpha[c];
 #pragma unroll
-        for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] *= alpha[n][c];
+        for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] *= alpha[c];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-          if (x[n][2 * i + c] != -INFINITY) x[n][2 * i + c] = fmaf(z[n][2 * i + c], u.qs[n][c], -m);
+        for (int b = 0; b < B; b++)
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+            if (x[b][n][2 * i + c] != -INFINITY) x[b][n][2 * i + c] = fmaf(z[b][n][2 * i + c], u.qs[n][c], -m);
       }
 #pragma unroll
       for (int gr = 0; gr < G; gr++) {
-        const float f[2] = {alpha[n][0] * beta[gr], alpha[n][1] * beta[gr]};
+        const float f[2] = {alpha[0] * beta[gr], alpha[1] * beta[gr]};
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           u.ones[n][gr][k] *= f[k & 1];
@@ -453,47 +503,51 @@ __device__ __forceinline__ void blockStep(Unit<G, NT>& u, const BlockRegs<G>& r,
     }
   }
 #pragma unroll
-  for (int n = 0; n < NT; n++)
+  for (int b = 0; b < B; b++) {
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int c = 0; c < 2; c++) {
-        const float w = exp2Fast(x[n][2 * i + c]);
-        x[n][2 * i + c] = w;
-        u.l[n][c] += w;
-        if (!edge) {
+      for (int i = 0; i < 2; i++)
 #pragma unroll
-          for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] = fmaf(w, mid[i][gr], u.mid[n][gr][c]);
-        } else if (w != 0.0f) {  // a row must not meet a NaN of a token that it does not see
+        for (int c = 0; c < 2; c++) {
+          const float w = exp2Fast(x[b][n][2 * i + c]);
+          x[b][n][2 * i + c] = w;
+          u.l[n][c] += w;
+          if (!edge || w != 0.0f) {  // a row must not meet a NaN of a token that it does not see
 #pragma unroll
-          for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] = fmaf(w, mid[i][gr], u.mid[n][gr][c]);
+            for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] = fmaf(w, mid[b][i][gr], u.mid[n][gr][c]);
+          }
         }
+    // O^T: rows are channels 8g + 2j (from the low halves of the words) and
+    // 8g + 2j + 1.  Odd j take a byte's two codes together, c + 16 c': the end
+    // takes c back out.
+    uint32_t v[4][G];
+    readValues<G>(v, tile + b * 18 * D, lane);
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) {
+      const float f0 = s[b][0][gr] * u.inv[gr], f1 = s[b][1][gr] * u.inv[gr];
+      uint32_t b0[NT], b1[NT];
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        float w[4] = {x[b][n][0] * f0, x[b][n][1] * f0, x[b][n][2] * f1, x[b][n][3] * f1};
+        if (edge) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) w[k] = x[b][n][k] == 0.0f ? 0.0f : w[k];
+        }
+        b0[n] = transpose8x8(packHalf(w[0], w[1]));
+        b1[n] = transpose8x8(packHalf(w[2], w[3]));
+        mma(u.ones[n][gr], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, b0[n], b1[n]);
       }
-  // O^T: rows are channels 8g + 2j (from the low halves) and 8g + 2j + 1.
+      const uint32_t x0 = __byte_perm(v[0][gr], v[1][gr], 0x5410), y0 = __byte_perm(v[0][gr], v[1][gr], 0x7632);
+      const uint32_t x1 = __byte_perm(v[2][gr], v[3][gr], 0x5410), y1 = __byte_perm(v[2][gr], v[3][gr], 0x7632);
+      const uint32_t xs0 = upperBytes(x0), ys0 = upperBytes(y0), xs1 = upperBytes(x1), ys1 = upperBytes(y1);
 #pragma unroll
-  for (int gr = 0; gr < G; gr++) {
-    const float f0 = s[0][gr] * u.inv[gr], f1 = s[1][gr] * u.inv[gr];
-    uint32_t b0[NT], b1[NT];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      float w[4] = {x[n][0] * f0, x[n][1] * f0, x[n][2] * f1, x[n][3] * f1};
-      if (edge) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) w[k] = x[n][k] == 0.0f ? 0.0f : w[k];
+      for (int n = 0; n < NT; n++) {
+        mma(u.o[n][gr][0], x0 & 0x000F000Fu, y0 & 0x000F000Fu, x1 & 0x000F000Fu, y1 & 0x000F000Fu, b0[n], b1[n]);
+        mma(u.o[n][gr][1], x0 & 0x00FF00FFu, y0 & 0x00FF00FFu, x1 & 0x00FF00FFu, y1 & 0x00FF00FFu, b0[n], b1[n]);
+        mma(u.o[n][gr][2], xs0 & 0x000F000Fu, ys0 & 0x000F000Fu, xs1 & 0x000F000Fu, ys1 & 0x000F000Fu, b0[n], b1[n]);
+        mma(u.o[n][gr][3], xs0, ys0, xs1, ys1, b0[n], b1[n]);
       }
-      b0[n] = transpose8x8(packHalf(w[0], w[1]));
-      b1[n] = transpose8x8(packHalf(w[2], w[3]));
-      mma(u.ones[n][gr], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, b0[n], b1[n]);
-    }
-    const uint32_t x0 = __byte_perm(r.v[0][gr], r.v[1][gr], 0x5410), y0 = __byte_perm(r.v[0][gr], r.v[1][gr], 0x7632);
-    const uint32_t x1 = __byte_perm(r.v[2][gr], r.v[3][gr], 0x5410), y1 = __byte_perm(r.v[2][gr], r.v[3][gr], 0x7632);
-    const uint32_t xs0 = x0 >> 8, ys0 = y0 >> 8, xs1 = x1 >> 8, ys1 = y1 >> 8;
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      mma(u.o[n][gr][0], x0 & 0x000F000Fu, y0 & 0x000F000Fu, x1 & 0x000F000Fu, y1 & 0x000F000Fu, b0[n], b1[n]);
-      mma(u.o[n][gr][1], x0 & 0x00F000F0u, y0 & 0x00F000F0u, x1 & 0x00F000F0u, y1 & 0x00F000F0u, b0[n], b1[n]);
-      mma(u.o[n][gr][2], xs0 & 0x000F000Fu, ys0 & 0x000F000Fu, xs1 & 0x000F000Fu, ys1 & 0x000F000Fu, b0[n], b1[n]);
-      mma(u.o[n][gr][3], xs0 & 0x00F000F0u, ys0 & 0x00F000F0u, xs1 & 0x00F000F0u, ys1 & 0x00F000F0u, b0[n], b1[n]);
     }
   }
 }
@@ -534,10 +588,13 @@ __device__ __forceinline__ void finish(Unit<G, NT>& u, const AttnArgs& p, const 
         const float base = fmaf(-7.5f * u.ones[n][gr][c], back, mid[gr]);
         float y[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float f = (j & 1) ? 1048576.0f : 16777216.0f;
-          y[2 * j] = fmaf(u.o[n][gr][j][c] * f, back, base) * norm;
-          y[2 * j + 1] = fmaf(u.o[n][gr][j][2 + c] * f, back, base) * norm;
+        for (int j = 0; j < 8; j++) {
+          // channel 8g + j: the sum of its code, times 2^-24
+          const float* o = u.o[n][gr][j >> 1];
+          const float* low = u.o[n][gr][(j >> 1) & ~1];
+          const int at = 2 * (j & 1) + c;
+          const float sum = (j & 2) ? (o[at] - low[at]) * 1048576.0f : o[at] * 16777216.0f;
+          y[j] = fmaf(sum, back, base) * norm;
         }
         if (slot < 0) {
           const long long at = (r.start + i) * p.oTok + h * p.oHead + 64 * gr + 8 * g;
@@ -557,23 +614,24 @@ __device__ __forceinline__ void finish(Unit<G, NT>& u, const AttnArgs& p, const 
     }
 }
 
-constexpr int blocksPerSm(int nt) { return nt == 1 ? 2 : 1; }
+// Two row tiles need the registers of three warps for two.
+constexpr int warpsFor(int nt) { return nt == 1 ? kWarps : 8; }
 
 template <int G>
-constexpr int ringBytes() {
-  return kStages * 18 * 64 * G;
+constexpr int tileBytes() {
+  return kBlocks * 18 * 64 * G;
 }
 
 template <int G, int NT>
-__global__ void __launch_bounds__(kWarps * 32, blocksPerSm(NT)) attnKernel(const __grid_constant__ AttnArgs p) {
+__global__ void __launch_bounds__(warpsFor(NT) * 32, 1) attnKernel(const __grid_constant__ AttnArgs p) {
   extern __shared__ uint4 shared[];  // the warps' rings, then the prefix sums
-  constexpr int R = 8 * NT, D = 64 * G;
-  uint8_t* ring = reinterpret_cast<uint8_t*>(shared) + (threadIdx.x >> 5) * ringBytes<G>();
-  long long* prefix = reinterpret_cast<long long*>(reinterpret_cast<uint8_t*>(shared) + kWarps * ringBytes<G>());
-  scanTiles<kWarps * 32>(p, R, prefix);
+  constexpr int R = 8 * NT, D = 64 * G, kThreads = warpsFor(NT) * 32;
+  uint8_t* ring = reinterpret_cast<uint8_t*>(shared) + (threadIdx.x >> 5) * (kStages * tileBytes<G>());
+  long long* prefix = reinterpret_cast<long long*>(reinterpret_cast<uint8_t*>(shared) + warpsFor(NT) * kStages * tileBytes<G>());
+  scanTiles<kThreads>(p, R, prefix);
   __syncthreads();
   if (blockIdx.x == 0)
-    for (int b = threadIdx.x; b <= p.batch; b += kWarps * 32) p.prefix[b] = prefix[b];
+    for (int b = threadIdx.x; b <= p.batch; b += kThreads) p.prefix[b] = prefix[b];
   const long long total = prefix[p.batch];
   if (total == 0) return;
   const int lane = threadIdx.x & 31;
@@ -590,49 +648,52 @@ __global__ void __launch_bounds__(kWarps * 32, blocksPerSm(NT)) attnKernel(const
     const int unit = static_cast<int>(off / nt), from = static_cast<int>(off - static_cast<long long>(unit) * nt);
     const int head = unit / units, row0 = (unit - head * units) * R;
     const int upto = static_cast<int>(min(static_cast<long long>(nt), from + (last - tile)));
-    const int begin = from * (kTile / kv4::kBlockTokens);
     const int* pages = p.table + static_cast<long long>(b) * p.width;
 
     // Lane i looks up block 32 j + i of the range: its page, then its address.
     // The pages of the next 32 are under way while these are copied.
     const int known = (r.kv + kv4::kBlockTokens - 1) / kv4::kBlockTokens;
     auto pageOf = [&](int block) { return block < known ? pages[block / p.blocksPerPage] : -1; };
-    int pageAhead = pageOf(begin + lane);
+    int pageAhead = pageOf(from * kBlocks + lane);
     Unit<G, NT> u;
     loadQuery<G, NT>(u, p, r, head, row0, lane);
-    // Blocks of this range that some row sees.
-    const int end = min(upto * (kTile / kv4::kBlockTokens), (u.most + kv4::kBlockTokens - 1) / kv4::kBlockTokens);
+    // Tiles of this range that some row sees.
+    const int count = min(upto, (u.most + kTile - 1) / kTile) - from;
     long long address = 0;
     uint32_t there = 0, thereBefore = 0;  // blocks of this look-up, and the last, whose page exists
-    auto issue = [&](int i) {  // i-th block of the range
-      const int block = begin + i;
-      if (block < end) {
-        if ((i & 31) == 0) {
-          const int mine = block + lane, page = pageAhead;
+    int in = 0, out = 0;                  // places in the ring
+    auto issue = [&](int i) {             // i-th tile of the range
+      if (i < count) {
+        const int at = (i * kBlocks) & 31;
+        if (at == 0) {
+          const int mine = (from + i) * kBlocks + lane, page = pageAhead;
           const bool ok = page >= 0 && page < p.pages;
           address = ((static_cast<long long>(page) * p.kvHeads + head) * p.blocksPerPage + mine % p.blocksPerPage) * (18 * D);
           thereBefore = there;
           there = __ballot_sync(~0u, ok);
           pageAhead = pageOf(mine + 32);
         }
-        const long long at = __shfl_sync(~0u, address, i & 31);
-        if ((there >> (i & 31)) & 1u) copyBlock<G>(ring + (i & (kStages - 1)) * (18 * D), p.cache + at, lane);
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) {
+          const long long from = __shfl_sync(~0u, address, at + b);
+          if ((there >> (at + b)) & 1u) copyBlock<G>(ring + in * tileBytes<G>() + b * 18 * D, p.cache + from, lane);
+        }
       }
+      in = in + 1 == kStages ? 0 : in + 1;
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
     for (int i = 0; i < kStages - 1; i++) issue(i);
-    for (int i = 0; begin + i < end; i++) {
+    for (int i = 0; i < count; i++) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-      __syncwarp();  // the block is there for every lane, and the one before has been read by all
-      issue(i + kStages - 1);
+      __syncwarp();  // the tile is there for every lane, and the one before has been read by all
+      const int next = i + kStages - 1;
+      issue(next);
       // the look-up may have moved on to the next 32 blocks
-      const uint32_t mask = ((i ^ (i + kStages - 1)) & 32) && begin + ((i + kStages - 1) & ~31) < end ? thereBefore : there;
-      if ((mask >> (i & 31)) & 1u) {
-        BlockRegs<G> regs;
-        readBlock<G>(regs, ring + (i & (kStages - 1)) * (18 * D), lane);
-        blockStep<G, NT>(u, regs, (begin + i) * kv4::kBlockTokens, lane);
-      }
+      const bool moved = ((i ^ next) & (32 / kBlocks)) && (next & ~(32 / kBlocks - 1)) < count;
+      const uint32_t mask = ((moved ? thereBefore : there) >> ((i * kBlocks) & 31)) & ((1u << kBlocks) - 1);
+      if (mask != 0) tileStep<G, NT>(u, ring + out * tileBytes<G>(), (from + i) * kTile, mask, lane);
+      out = out + 1 == kStages ? 0 : out + 1;
     }
     __syncwarp();  // the ring is read by all before the next unit's copies
     const bool whole = from == 0 && upto == nt;
@@ -731,11 +792,12 @@ int rowTiles(int batch, int tokens, int group) {
 
 template <int G, int NT>
 cudaError_t launchAttn(const AttnArgs& p, int grid, cudaStream_t st) {
-  const size_t smem = kWarps * ringBytes<G>() + static_cast<size_t>(p.batch + 1) * sizeof(long long);
+  constexpr int kRings = warpsFor(NT) * kStages * tileBytes<G>();
+  const size_t smem = kRings + static_cast<size_t>(p.batch + 1) * sizeof(long long);
   const cudaError_t e = cudaFuncSetAttribute(attnKernel<G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kWarps * ringBytes<G>() + (kMaxBatch + 1) * static_cast<int>(sizeof(long long)));
+                                             kRings + (kMaxBatch + 1) * static_cast<int>(sizeof(long long)));
   if (e != cudaSuccess) return e;
-  attnKernel<G, NT><<<grid, kWarps * 32, smem, st>>>(p);
+  attnKernel<G, NT><<<grid, warpsFor(NT) * 32, smem, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -753,7 +815,7 @@ extern "C" {
 size_t vcclKv4AttentionWorkspace(int batch, int tokens, int qHeads, int kvHeads, int D) {
   if (batch <= 0 || kvHeads <= 0 || qHeads <= 0 || D <= 0) return 0;
   const int nt = rowTiles(batch, tokens, qHeads / kvHeads);
-  const size_t slots = static_cast<size_t>(smsOfDevice()) * blocksPerSm(nt) * kWarps * 2;
+  const size_t slots = static_cast<size_t>(smsOfDevice()) * warpsFor(nt) * 2;
   return align256((batch + 1) * sizeof(long long)) + align256(slots * 8 * nt * sizeof(float2)) +
          slots * 8 * nt * D * sizeof(float);
 }
@@ -775,7 +837,7 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   TraceRange trace("vccl Kv4Attention");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int group = q->heads / cache->kvHeads, nt = rowTiles(batch, tokens, group), R = 8 * nt;
-  const int grid = smsOfDevice() * blocksPerSm(nt);
+  const int grid = smsOfDevice();
   AttnArgs p{};
   p.q = q->data;
   p.qTok = q->tokenStride;
@@ -796,7 +858,7 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   p.group = group;
   p.pages = cache->pages;
   p.blocksPerPage = cache->pageSize / kv4::kBlockTokens;
-  p.workers = grid * kWarps;
+  p.workers = grid * warpsFor(nt);
   p.half16 = datatype == vcclFloat16;
   p.zeroTail = zeroTail;
   p.scaleLog2 = scale * 1.44269504088896340736f;
