@@ -81,15 +81,28 @@ __device__ __forceinline__ int unitsOf(const AttnArgs& p, const Request& r, int 
 
 __device__ __forceinline__ int tilesOf(const Request& r) { return (r.kv + kTile - 1) / kTile; }
 
-__device__ __forceinline__ long long rangeStart(long long w, long long total, int workers) { return w * total / workers; }
-__device__ __forceinline__ int workerOf(long long tile, long long total, int workers) {
-  return static_cast<int>(((tile + 1) * workers - 1) / total);
+// A quotient that is mostly one of 32-bit numbers (a 64-bit division takes
+// over a hundred instructions).
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
 }
 
-// Every warp that takes part has at least one tile.
-__device__ __forceinline__ int workersFor(const AttnArgs& p, long long total) {
-  return static_cast<int>(min(static_cast<long long>(p.workers), total));
-}
+// Tiles to warps: every warp that takes part has `each` tiles, the first
+// `more` of them one more.
+struct Split {
+  int workers;
+  long long each, more;
+  __device__ __forceinline__ Split(long long total, int most) {
+    workers = static_cast<int>(min(static_cast<long long>(most), total));
+    each = quotient(total, workers);
+    more = total - each * workers;
+  }
+  __device__ __forceinline__ long long start(int w) const { return w * each + min(static_cast<long long>(w), more); }
+  __device__ __forceinline__ int owner(long long tile) const {
+    const long long ahead = more * (each + 1);
+    return static_cast<int>(tile < ahead ? quotient(tile, each + 1) : more + quotient(tile - ahead, each));
+  }
+};
 
 // prefix[b] = tiles of the requests before b (all heads and row tiles).
 template <int THREADS>
@@ -167,21 +180,15 @@ __device__ __forceinline__ float exp2Fast(float x) {
   return r;
 }
 
+// Shared memory by its 32-bit address: one register and an immediate.
 template <int WORDS>
-__device__ __forceinline__ void loadWords(const uint8_t* p, uint32_t* w) {
-  if constexpr (WORDS == 4) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x;
-    w[1] = v.y;
-    w[2] = v.z;
-    w[3] = v.w;
-  } else if constexpr (WORDS == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x;
-    w[1] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
+__device__ __forceinline__ void loadWords(uint32_t at, uint32_t* w) {
+  if constexpr (WORDS == 4)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+  else if constexpr (WORDS == 2)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
 }
 
 // A block in shared memory is as in global memory, but that for D = 128 the
@@ -189,49 +196,55 @@ __device__ __forceinline__ void loadWords(const uint8_t* p, uint32_t* w) {
 // of four rows then read from different banks.
 __device__ __forceinline__ int swapTwos(int chunk) { return chunk ^ ((chunk & 8) >> 2); }
 
+// to: of the block, plus 16 * lane; from: likewise.
 template <int G>
-__device__ __forceinline__ void copyBlock(uint8_t* to, const uint8_t* from, int lane) {
+__device__ __forceinline__ void copyBlock(uint32_t to, const uint8_t* from, int lane) {
   constexpr int D = 64 * G, kChunks = 18 * D / 16;
-  const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  const uint32_t swapped = to + 16 * (swapTwos(lane) - lane);
 #pragma unroll
   for (int j = 0; j < (kChunks + 31) / 32; j++) {
     const bool values = G == 2 && j >= D / 64 && j < D / 32;  // chunks D / 2 to D
-    const int chunk = 32 * j + lane;
-    if (32 * (j + 1) <= kChunks || chunk < kChunks)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 16 * (32 * j + (values ? swapTwos(lane) : lane))),
-                   "l"(from + 16 * chunk)
-                   : "memory");
+    if (32 * (j + 1) <= kChunks || 32 * j + lane < kChunks)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((values ? swapped : to) + 512 * j), "l"(from + 512 * j) : "memory");
   }
 }
 
 // What a lane reads of a block: of keys, tokens g and g + 8, words (group,
 // half); of values, tokens 2q, 2q + 1, 8 + 2q, 9 + 2q, the word of each group;
 // scales and midpoints of tokens g and g + 8.
+struct LaneOffsets {
+  uint32_t keys, params, values;
+};
+
 template <int G>
-__device__ __forceinline__ void readKeys(uint32_t (&k)[2][2 * G], uint32_t (&kp)[2][G], const uint8_t* block, int lane) {
+__device__ __forceinline__ LaneOffsets offsetsOf(int lane) {
   constexpr int D = 64 * G;
   const int g = lane >> 2, q = lane & 3;
+  return {static_cast<uint32_t>(g * (D / 2) + q * (8 * G)), static_cast<uint32_t>(g * (4 * G)),
+          static_cast<uint32_t>(q * (D / 2) + (G == 2 ? (g * 8) ^ ((q & 2) << 4) : g * 4))};
+}
+
+template <int G>
+__device__ __forceinline__ void readKeys(uint32_t (&k)[2][2 * G], uint32_t (&kp)[2][G], uint32_t block, const LaneOffsets& at) {
+  constexpr int D = 64 * G;
 #pragma unroll
   for (int i = 0; i < 2; i++) {
-    loadWords<2 * G>(block + (g + 8 * i) * (D / 2) + q * (8 * G), k[i]);
-    loadWords<G>(block + 16 * D + (g + 8 * i) * (4 * G), kp[i]);
+    loadWords<2 * G>(block + at.keys + 4 * i * D, k[i]);
+    loadWords<G>(block + at.params + 16 * D + 32 * G * i, kp[i]);
   }
 }
 
 template <int G>
-__device__ __forceinline__ void readValueParams(uint32_t (&vp)[2][G], const uint8_t* block, int lane) {
-  constexpr int D = 64 * G;
+__device__ __forceinline__ void readValueParams(uint32_t (&vp)[2][G], uint32_t block, const LaneOffsets& at) {
 #pragma unroll
-  for (int i = 0; i < 2; i++) loadWords<G>(block + 17 * D + ((lane >> 2) + 8 * i) * (4 * G), vp[i]);
+  for (int i = 0; i < 2; i++) loadWords<G>(block + at.params + 17 * 64 * G + 32 * G * i, vp[i]);
 }
 
 template <int G>
-__device__ __forceinline__ void readValues(uint32_t (&v)[4][G], const uint8_t* block, int lane) {
+__device__ __forceinline__ void readValues(uint32_t (&v)[4][G], uint32_t block, const LaneOffsets& at) {
   constexpr int D = 64 * G;
-  const int g = lane >> 2, q = lane & 3;
-  const int at = G == 2 ? q * (D / 2) + ((g * 8) ^ ((q & 2) << 4)) : q * (D / 2) + g * 4;
 #pragma unroll
-  for (int i = 0; i < 4; i++) loadWords<G>(block + 8 * D + 4 * i * (D / 2) + at, v[i]);
+  for (int i = 0; i < 4; i++) loadWords<G>(block + at.values + 8 * D + 2 * i * D, v[i]);
 }
 
 // A warp's state for one unit.
@@ -346,12 +359,68 @@ __device__ __forceinline__ void loadQuery(Unit<G, NT>& u, const AttnArgs& p, con
 // The two bytes of a word's upper halves, each in the low byte of 16 bits.
 __device__ __forceinline__ uint32_t upperBytes(uint32_t w) { return __byte_perm(w, 0u, 0x4341); }
 
+// The second half of a tile: weights of the scores x, and their products with
+// the values.  EDGE: some row does not see some token.
+template <int G, int NT, bool EDGE>
+__device__ __forceinline__ void weighValues(Unit<G, NT>& u, float (&x)[kBlocks][NT][4], const float (&s)[kBlocks][2][G],
+                                            const float (&mid)[kBlocks][2][G], uint32_t tile, const LaneOffsets& at) {
+  constexpr int D = 64 * G, B = kBlocks;
+#pragma unroll
+  for (int b = 0; b < B; b++) {
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          const float w = exp2Fast(x[b][n][2 * i + c]);
+          x[b][n][2 * i + c] = w;
+          u.l[n][c] += w;
+          if (!EDGE || w != 0.0f) {  // a row must not meet a NaN of a token that it does not see
+#pragma unroll
+            for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] = fmaf(w, mid[b][i][gr], u.mid[n][gr][c]);
+          }
+        }
+    // O^T: rows are channels 8g + 2j (from the low halves of the words) and
+    // 8g + 2j + 1.  Odd j take a byte's two codes together, c + 16 c': the end
+    // takes c back out.
+    uint32_t v[4][G];
+    readValues<G>(v, tile + b * 18 * D, at);
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) {
+      const float f0 = s[b][0][gr] * u.inv[gr], f1 = s[b][1][gr] * u.inv[gr];
+      uint32_t b0[NT], b1[NT];
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        float w[4] = {x[b][n][0] * f0, x[b][n][1] * f0, x[b][n][2] * f1, x[b][n][3] * f1};
+        if (EDGE) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) w[k] = x[b][n][k] == 0.0f ? 0.0f : w[k];
+        }
+        b0[n] = transpose8x8(packHalf(w[0], w[1]));
+        b1[n] = transpose8x8(packHalf(w[2], w[3]));
+        mma(u.ones[n][gr], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, b0[n], b1[n]);
+      }
+      const uint32_t x0 = __byte_perm(v[0][gr], v[1][gr], 0x5410), y0 = __byte_perm(v[0][gr], v[1][gr], 0x7632);
+      const uint32_t x1 = __byte_perm(v[2][gr], v[3][gr], 0x5410), y1 = __byte_perm(v[2][gr], v[3][gr], 0x7632);
+      const uint32_t xs0 = upperBytes(x0), ys0 = upperBytes(y0), xs1 = upperBytes(x1), ys1 = upperBytes(y1);
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        mma(u.o[n][gr][0], x0 & 0x000F000Fu, y0 & 0x000F000Fu, x1 & 0x000F000Fu, y1 & 0x000F000Fu, b0[n], b1[n]);
+        mma(u.o[n][gr][1], x0 & 0x00FF00FFu, y0 & 0x00FF00FFu, x1 & 0x00FF00FFu, y1 & 0x00FF00FFu, b0[n], b1[n]);
+        mma(u.o[n][gr][2], xs0 & 0x000F000Fu, ys0 & 0x000F000Fu, xs1 & 0x000F000Fu, ys1 & 0x000F000Fu, b0[n], b1[n]);
+        mma(u.o[n][gr][3], xs0, ys0, xs1, ys1, b0[n], b1[n]);
+      }
+    }
+  }
+}
+
 // A tile of 32 tokens that starts at token t0 of the request.  Two blocks at a
 // time give the scheduler twice the independent work of one, and share the
 // looks at the maximum (one block at a time: 166 us where this takes 137, 64
 // requests of 500 to 16000 tokens, 8 key heads).  there: bit b, block b exists.
 template <int G, int NT>
-__device__ __forceinline__ void tileStep(Unit<G, NT>& u, const uint8_t* tile, int t0, uint32_t there, int lane) {
+__device__ __forceinline__ void tileStep(Unit<G, NT>& u, uint32_t tile, const LaneOffsets& at, int t0, uint32_t there, int lane) {
   constexpr int D = 64 * G, B = kBlocks;
   const int g = lane >> 2;
   // S^T, group by group: the scale of a token and group acts on the group's
@@ -360,7 +429,7 @@ __device__ __forceinline__ void tileStep(Unit<G, NT>& u, const uint8_t* tile, in
 #pragma unroll
   for (int b = 0; b < B; b++) {
     uint32_t k[2][2 * G], kp[2][G];
-    readKeys<G>(k, kp, tile + b * 18 * D, lane);
+    readKeys<G>(k, kp, tile + b * 18 * D, at);
 #pragma unroll
     for (int gr = 0; gr < G; gr++) {
       float acc[NT][4];
@@ -401,7 +470,7 @@ __device__ __forceinline__ void tileStep(Unit<G, NT>& u, const uint8_t* tile, in
 #pragma unroll
   for (int b = 0; b < B; b++) {
     uint32_t vp[2][G];
-    readValueParams<G>(vp, tile + b * 18 * D, lane);
+    readValueParams<G>(vp, tile + b * 18 * D, at);
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -502,54 +571,8 @@ __device__ __forceinline__ void tileStep(Unit<G, NT>& u, const uint8_t* tile, in
       }
     }
   }
-#pragma unroll
-  for (int b = 0; b < B; b++) {
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-          const float w = exp2Fast(x[b][n][2 * i + c]);
-          x[b][n][2 * i + c] = w;
-          u.l[n][c] += w;
-          if (!edge || w != 0.0f) {  // a row must not meet a NaN of a token that it does not see
-#pragma unroll
-            for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] = fmaf(w, mid[b][i][gr], u.mid[n][gr][c]);
-          }
-        }
-    // O^T: rows are channels 8g + 2j (from the low halves of the words) and
-    // 8g + 2j + 1.  Odd j take a byte's two codes together, c + 16 c': the end
-    // takes c back out.
-    uint32_t v[4][G];
-    readValues<G>(v, tile + b * 18 * D, lane);
-#pragma unroll
-    for (int gr = 0; gr < G; gr++) {
-      const float f0 = s[b][0][gr] * u.inv[gr], f1 = s[b][1][gr] * u.inv[gr];
-      uint32_t b0[NT], b1[NT];
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        float w[4] = {x[b][n][0] * f0, x[b][n][1] * f0, x[b][n][2] * f1, x[b][n][3] * f1};
-        if (edge) {
-#pragma unroll
-          for (int k = 0; k < 4; k++) w[k] = x[b][n][k] == 0.0f ? 0.0f : w[k];
-        }
-        b0[n] = transpose8x8(packHalf(w[0], w[1]));
-        b1[n] = transpose8x8(packHalf(w[2], w[3]));
-        mma(u.ones[n][gr], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, b0[n], b1[n]);
-      }
-      const uint32_t x0 = __byte_perm(v[0][gr], v[1][gr], 0x5410), y0 = __byte_perm(v[0][gr], v[1][gr], 0x7632);
-      const uint32_t x1 = __byte_perm(v[2][gr], v[3][gr], 0x5410), y1 = __byte_perm(v[2][gr], v[3][gr], 0x7632);
-      const uint32_t xs0 = upperBytes(x0), ys0 = upperBytes(y0), xs1 = upperBytes(x1), ys1 = upperBytes(y1);
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        mma(u.o[n][gr][0], x0 & 0x000F000Fu, y0 & 0x000F000Fu, x1 & 0x000F000Fu, y1 & 0x000F000Fu, b0[n], b1[n]);
-        mma(u.o[n][gr][1], x0 & 0x00FF00FFu, y0 & 0x00FF00FFu, x1 & 0x00FF00FFu, y1 & 0x00FF00FFu, b0[n], b1[n]);
-        mma(u.o[n][gr][2], xs0 & 0x000F000Fu, ys0 & 0x000F000Fu, xs1 & 0x000F000Fu, ys1 & 0x000F000Fu, b0[n], b1[n]);
-        mma(u.o[n][gr][3], xs0, ys0, xs1, ys1, b0[n], b1[n]);
-      }
-    }
-  }
+  if (edge) weighValues<G, NT, true>(u, x, s, mid, tile, at);
+  else weighValues<G, NT, false>(u, x, s, mid, tile, at);
 }
 
 template <typename T>
@@ -625,8 +648,9 @@ constexpr int tileBytes() {
 template <int G, int NT>
 __global__ void __launch_bounds__(warpsFor(NT) * 32, 1) attnKernel(const __grid_constant__ AttnArgs p) {
   extern __shared__ uint4 shared[];  // the warps' rings, then the prefix sums
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may be set up beside this
   constexpr int R = 8 * NT, D = 64 * G, kThreads = warpsFor(NT) * 32;
-  uint8_t* ring = reinterpret_cast<uint8_t*>(shared) + (threadIdx.x >> 5) * (kStages * tileBytes<G>());
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(shared)) + (threadIdx.x >> 5) * (kStages * tileBytes<G>());
   long long* prefix = reinterpret_cast<long long*>(reinterpret_cast<uint8_t*>(shared) + warpsFor(NT) * kStages * tileBytes<G>());
   scanTiles<kThreads>(p, R, prefix);
   __syncthreads();
@@ -635,17 +659,20 @@ __global__ void __launch_bounds__(warpsFor(NT) * 32, 1) attnKernel(const __grid_
   const long long total = prefix[p.batch];
   if (total == 0) return;
   const int lane = threadIdx.x & 31;
+  const LaneOffsets offsets = offsetsOf<G>(lane);
+  const uint8_t* mine = p.cache + 16 * lane;
   // Neighbouring ranges go to different blocks, so that few tiles spread over the SMs.
-  const int w = (threadIdx.x >> 5) * gridDim.x + blockIdx.x, workers = workersFor(p, total);
-  if (w >= workers) return;
-  const long long first = rangeStart(w, total, workers), last = rangeStart(w + 1, total, workers);
+  const int w = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
+  const Split split(total, p.workers);
+  if (w >= split.workers) return;
+  const long long first = split.start(w), last = split.start(w + 1);
   long long tile = first;
   while (tile < last) {
     const int b = findRequest(prefix, p.batch, tile);
     const Request r = requestOf(p, b);
     const int nt = tilesOf(r), units = unitsOf(p, r, R);
     const long long off = tile - prefix[b];
-    const int unit = static_cast<int>(off / nt), from = static_cast<int>(off - static_cast<long long>(unit) * nt);
+    const int unit = static_cast<int>(quotient(off, nt)), from = static_cast<int>(off - static_cast<long long>(unit) * nt);
     const int head = unit / units, row0 = (unit - head * units) * R;
     const int upto = static_cast<int>(min(static_cast<long long>(nt), from + (last - tile)));
     const int* pages = p.table + static_cast<long long>(b) * p.width;
@@ -666,17 +693,17 @@ __global__ void __launch_bounds__(warpsFor(NT) * 32, 1) attnKernel(const __grid_
       if (i < count) {
         const int at = (i * kBlocks) & 31;
         if (at == 0) {
-          const int mine = (from + i) * kBlocks + lane, page = pageAhead;
+          const int block = (from + i) * kBlocks + lane, page = pageAhead;
           const bool ok = page >= 0 && page < p.pages;
-          address = ((static_cast<long long>(page) * p.kvHeads + head) * p.blocksPerPage + mine % p.blocksPerPage) * (18 * D);
+          address = ((static_cast<long long>(page) * p.kvHeads + head) * p.blocksPerPage + block % p.blocksPerPage) * (18 * D);
           thereBefore = there;
           there = __ballot_sync(~0u, ok);
-          pageAhead = pageOf(mine + 32);
+          pageAhead = pageOf(block + 32);
         }
 #pragma unroll
         for (int b = 0; b < kBlocks; b++) {
           const long long from = __shfl_sync(~0u, address, at + b);
-          if ((there >> (at + b)) & 1u) copyBlock<G>(ring + in * tileBytes<G>() + b * 18 * D, p.cache + from, lane);
+          if ((there >> (at + b)) & 1u) copyBlock<G>(ring + in * tileBytes<G>() + b * 18 * D + 16 * lane, mine + from, lane);
         }
       }
       in = in + 1 == kStages ? 0 : in + 1;
@@ -692,7 +719,7 @@ __global__ void __launch_bounds__(warpsFor(NT) * 32, 1) attnKernel(const __grid_
       // the look-up may have moved on to the next 32 blocks
       const bool moved = ((i ^ next) & (32 / kBlocks)) && (next & ~(32 / kBlocks - 1)) < count;
       const uint32_t mask = ((moved ? thereBefore : there) >> ((i * kBlocks) & 31)) & ((1u << kBlocks) - 1);
-      if (mask != 0) tileStep<G, NT>(u, ring + out * tileBytes<G>(), (from + i) * kTile, mask, lane);
+      if (mask != 0) tileStep<G, NT>(u, ring + out * tileBytes<G>(), offsets, (from + i) * kTile, mask, lane);
       out = out + 1 == kStages ? 0 : out + 1;
     }
     __syncwarp();  // the ring is read by all before the next unit's copies
@@ -720,6 +747,7 @@ __global__ void __launch_bounds__(128) joinKernel(AttnArgs p, int R) {
   }
   float y[2 * G] = {};
   float m = kNone, l = 0.0f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial sums are there
   const Request r = lo < p.batch ? requestOf(p, lo) : Request{0, 0, 0};
   if (t < r.start || t >= r.start + r.rows) {
     if (!p.zeroTail) return;
@@ -729,8 +757,8 @@ __global__ void __launch_bounds__(128) joinKernel(AttnArgs p, int R) {
       const int row = (t - r.start) * p.group + h % p.group, units = unitsOf(p, r, R);
       const long long total = p.prefix[p.batch];
       const long long a = p.prefix[lo] + (static_cast<long long>(h / p.group) * units + row / R) * nt;
-      const int workers = workersFor(p, total);
-      const int w0 = workerOf(a, total, workers), w1 = workerOf(a + nt - 1, total, workers);
+      const Split split(total, p.workers);
+      const int w0 = split.owner(a), w1 = split.owner(a + nt - 1);
       if (w0 == w1) return;  // written by its warp
       // 32 parts at a time: a lane reads the maximum and the sum of one.
       for (int base = w0; base <= w1; base += 32) {
@@ -738,7 +766,7 @@ __global__ void __launch_bounds__(128) joinKernel(AttnArgs p, int R) {
         long long slot = 0;
         float2 st = make_float2(kNone, 0.0f);
         if (lane < n) {
-          slot = (2LL * w + (rangeStart(w, total, workers) < a ? 1 : 0)) * R + row % R;
+          slot = (2LL * w + (split.start(w) < a ? 1 : 0)) * R + row % R;
           st = p.stats[slot];
         }
         float top = st.x;
@@ -875,10 +903,23 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
     VERR("vcclKv4Attention: %s", cudaGetErrorString(e));
     return vcclSystemError;
   }
-  const int rows = static_cast<int>((static_cast<long long>(tokens) * q->heads + 3) / 4);
-  if (cache->D == 128) joinKernel<2><<<rows, 128, 0, st>>>(p, R);
-  else joinKernel<1><<<rows, 128, 0, st>>>(p, R);
-  return launched("vcclKv4Attention");
+  // Launched beside the kernel before it: its blocks find their requests
+  // while that one ends, and wait for its results.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(tokens) * q->heads + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cache->D == 128 ? cudaLaunchKernelEx(&cfg, joinKernel<2>, p, R) : cudaLaunchKernelEx(&cfg, joinKernel<1>, p, R);
+  if (e != cudaSuccess) {
+    VERR("vcclKv4Attention: %s", cudaGetErrorString(e));
+    return vcclSystemError;
+  }
+  return vcclSuccess;
 }
 
 }  // extern "C"
