@@ -730,71 +730,95 @@ __global__ void __launch_bounds__(warpsFor(NT) * 32, 1) attnKernel(const __grid_
   }
 }
 
-// Joins the partial sums of every row whose unit was cut, and clears the rows
-// that see nothing or stand behind the last request.  A warp takes one row.
-template <int G>
-__global__ void __launch_bounds__(128) joinKernel(AttnArgs p, int R) {
-  constexpr int D = 64 * G;
-  const int lane = threadIdx.x & 31;
-  const long long id = blockIdx.x * 4LL + (threadIdx.x >> 5);
-  if (id >= static_cast<long long>(p.tokens) * p.qHeads) return;
-  const int t = static_cast<int>(id / p.qHeads), h = static_cast<int>(id % p.qHeads);
-  int lo = 0, hi = p.batch;  // the first request that ends behind t
-  while (lo < hi) {
-    const int m = (lo + hi) >> 1;
-    if (p.qStarts[m + 1] > t) hi = m;
-    else lo = m + 1;
+// The request whose rows hold t (batch if none), by a whole warp: 32 starts
+// are looked at together, so 1024 requests take two looks.
+__device__ __forceinline__ int requestOfRow(const AttnArgs& p, int t, int lane) {
+  int lo = 0, n = p.batch;  // it is one of lo .. lo + n - 1, or none of them
+  while (n > 32) {
+    const int step = (n + 31) >> 5, at = lo + min(lane * step, n - 1);
+    const uint32_t before = __ballot_sync(~0u, lane * step < n && p.qStarts[at] <= t);
+    if (before == 0) return p.batch;
+    const int piece = 31 - __clz(before);
+    n = min(step, n - piece * step);
+    lo += piece * step;
   }
+  const uint32_t ahead = __ballot_sync(~0u, lane < n && p.qStarts[lo + lane + 1] > t);
+  return ahead == 0 ? p.batch : lo + __ffs(ahead) - 1;
+}
+
+// Joins the partial sums of every row whose unit was cut, and clears the rows
+// that see nothing or stand behind the last request.  A block of four warps
+// takes one row where parts are many (WIDE: few rows in all), else each warp
+// takes one.  The loads of a row depend on one another three deep: starts and
+// lengths, maxima and sums, outputs.
+template <int G, bool WIDE>
+__global__ void __launch_bounds__(128) joinKernel(const __grid_constant__ AttnArgs p, int R) {
+  constexpr int D = 64 * G;
+  __shared__ float sums[WIDE ? 4 : 1][WIDE ? D : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long id = WIDE ? blockIdx.x : blockIdx.x * 4LL + warp;
+  if (id >= static_cast<long long>(p.tokens) * p.qHeads) return;
+  const int t = static_cast<int>(id / p.qHeads), h = static_cast<int>(id - static_cast<long long>(t) * p.qHeads);
+  const int b = requestOfRow(p, t, lane);
+  const Request r = b < p.batch ? requestOf(p, b) : Request{0, 0, 0};
+  const bool inside = t >= r.start && t < r.start + r.rows;
+  if (!inside && !p.zeroTail) return;
+  const int nt = inside ? tilesOf(r) : 0;
   float y[2 * G] = {};
   float m = kNone, l = 0.0f;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial sums are there
-  const Request r = lo < p.batch ? requestOf(p, lo) : Request{0, 0, 0};
-  if (t < r.start || t >= r.start + r.rows) {
-    if (!p.zeroTail) return;
-  } else {
-    const int nt = tilesOf(r);
-    if (nt > 0) {
-      const int row = (t - r.start) * p.group + h % p.group, units = unitsOf(p, r, R);
-      const long long total = p.prefix[p.batch];
-      const long long a = p.prefix[lo] + (static_cast<long long>(h / p.group) * units + row / R) * nt;
-      const Split split(total, p.workers);
-      const int w0 = split.owner(a), w1 = split.owner(a + nt - 1);
-      if (w0 == w1) return;  // written by its warp
-      // 32 parts at a time: a lane reads the maximum and the sum of one.
-      for (int base = w0; base <= w1; base += 32) {
-        const int w = base + lane, n = min(32, w1 - base + 1);
-        long long slot = 0;
-        float2 st = make_float2(kNone, 0.0f);
-        if (lane < n) {
-          slot = (2LL * w + (split.start(w) < a ? 1 : 0)) * R + row % R;
-          st = p.stats[slot];
-        }
-        float top = st.x;
+  if (nt > 0) {
+    const int row = (t - r.start) * p.group + h % p.group, units = unitsOf(p, r, R);
+    const long long total = p.prefix[p.batch];
+    const long long a = p.prefix[b] + (static_cast<long long>(h / p.group) * units + row / R) * nt;
+    const Split split(total, p.workers);
+    const int w0 = split.owner(a), w1 = split.owner(a + nt - 1);
+    if (w0 == w1) return;  // written by its warp
+    // 32 parts at a time: a lane reads the maximum and the sum of one.
+    for (int base = w0; base <= w1; base += 32) {
+      const int w = base + lane, n = min(32, w1 - base + 1);
+      long long slot = 0;
+      float2 st = make_float2(kNone, 0.0f);
+      if (lane < n) {
+        slot = (2LL * w + (split.start(w) < a ? 1 : 0)) * R + row % R;
+        st = p.stats[slot];
+      }
+      float top = st.x;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        top = fmaxf(m, top);
-        const float old = exp2Fast(m - top), add = exp2Fast(st.x - top);
-        m = top;
-        float sum = st.y * add;
+      for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+      top = fmaxf(m, top);
+      const float old = exp2Fast(m - top), add = exp2Fast(st.x - top);
+      m = top;
+      float sum = st.y * add;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        l = l * old + sum;
+      for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
+      l = l * old + sum;
 #pragma unroll
-        for (int k = 0; k < 2 * G; k++) y[k] *= old;
+      for (int k = 0; k < 2 * G; k++) y[k] *= old;
 #pragma unroll 8
-        for (int k = 0; k < n; k++) {
-          const float f = __shfl_sync(~0u, add, k);
-          const float2* src = reinterpret_cast<const float2*>(p.partial + __shfl_sync(~0u, slot, k) * D) + lane;
+      for (int k = WIDE ? warp : 0; k < n; k += WIDE ? 4 : 1) {
+        const float f = __shfl_sync(~0u, add, k);
+        const float2* src = reinterpret_cast<const float2*>(p.partial + __shfl_sync(~0u, slot, k) * D) + lane;
 #pragma unroll
-          for (int gr = 0; gr < G; gr++) {
-            const float2 v = src[32 * gr];
-            y[2 * gr] = fmaf(v.x, f, y[2 * gr]);
-            y[2 * gr + 1] = fmaf(v.y, f, y[2 * gr + 1]);
-          }
+        for (int gr = 0; gr < G; gr++) {
+          const float2 v = src[32 * gr];
+          y[2 * gr] = fmaf(v.x, f, y[2 * gr]);
+          y[2 * gr + 1] = fmaf(v.y, f, y[2 * gr + 1]);
         }
       }
     }
+    if (WIDE) {  // the warps' shares, in order
+#pragma unroll
+      for (int k = 0; k < 2 * G; k++) sums[warp][64 * (k >> 1) + 2 * lane + (k & 1)] = y[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 2 * G; k++) {
+        const int d = 64 * (k >> 1) + 2 * lane + (k & 1);
+        y[k] = (sums[0][d] + sums[WIDE ? 1 : 0][d]) + (sums[WIDE ? 2 : 0][d] + sums[WIDE ? 3 : 0][d]);
+      }
+    }
   }
+  if (WIDE && warp > 0) return;
   const bool none = l == 0.0f;
   const float norm = none ? 0.0f : 1.0f / l;
   const long long at = t * p.oTok + h * p.oHead + 2 * lane;
@@ -906,7 +930,11 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   // Launched beside the kernel before it: its blocks find their requests
   // while that one ends, and wait for its results.
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(tokens) * q->heads + 3) / 4));
+  // A block a row while every SM gets no more than four (8 rows of 29 parts:
+  // 7 us with a warp a row, 4 with a block).
+  const long long rows = static_cast<long long>(tokens) * q->heads;
+  const bool wide = rows <= 4LL * smsOfDevice();
+  cfg.gridDim = dim3(static_cast<unsigned>(wide ? rows : (rows + 3) / 4));
   cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -914,7 +942,8 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cache->D == 128 ? cudaLaunchKernelEx(&cfg, joinKernel<2>, p, R) : cudaLaunchKernelEx(&cfg, joinKernel<1>, p, R);
+  if (cache->D == 128) e = wide ? cudaLaunchKernelEx(&cfg, joinKernel<2, true>, p, R) : cudaLaunchKernelEx(&cfg, joinKernel<2, false>, p, R);
+  else e = wide ? cudaLaunchKernelEx(&cfg, joinKernel<1, true>, p, R) : cudaLaunchKernelEx(&cfg, joinKernel<1, false>, p, R);
   if (e != cudaSuccess) {
     VERR("vcclKv4Attention: %s", cudaGetErrorString(e));
     return vcclSystemError;
