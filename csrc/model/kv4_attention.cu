@@ -29,6 +29,7 @@
 // joins in order.
 #include <cfloat>
 #include <climits>
+#include <mutex>
 
 #include "kernels/kv4.cuh"
 #include "model/common.cuh"
@@ -61,6 +62,12 @@ struct AttnArgs {
   int width, batch, tokens, qHeads, kvHeads, group, pages, blocksPerPage;
   int workers, half16, zeroTail;
   float scaleLog2;
+  // Requests of at least longRows query rows a key head go to chunkKernel (0: none do).
+  int longRows, splits;
+  int* chunkStarts;     // [batch + 1] units before each request
+  float2* chunkStats;   // [units][256] maximum (log2), sum, with splits > 1
+  float* chunkPartial;  // [units][256][D]
+  int* errorFlag;       // mapped host word, set when a wait ran out
 };
 
 // What a request brings: its first row, its rows, its tokens.
@@ -74,7 +81,12 @@ __device__ __forceinline__ Request requestOf(const AttnArgs& p, int b) {
   return {s, e - s, static_cast<int>(min(static_cast<long long>(max(p.kvLens[b], 0)), most))};
 }
 
+__device__ __forceinline__ bool isLong(const AttnArgs& p, const Request& r) {
+  return p.longRows > 0 && static_cast<long long>(r.rows) * p.group >= p.longRows;
+}
+
 __device__ __forceinline__ int unitsOf(const AttnArgs& p, const Request& r, int R) {
+  if (isLong(p, r)) return 0;
   const long long rows = static_cast<long long>(r.rows) * p.group;
   return static_cast<int>((rows + R - 1) / R);
 }
@@ -746,6 +758,20 @@ __device__ __forceinline__ int requestOfRow(const AttnArgs& p, int t, int lane) 
   return ahead == 0 ? p.batch : lo + __ffs(ahead) - 1;
 }
 
+// A joined row: a lane has channels 2 lane and 2 lane + 1 of every group.
+template <int G>
+__device__ __forceinline__ void storeRow(const AttnArgs& p, int t, int h, int lane, const float (&y)[2 * G], float m, float l) {
+  const bool none = l == 0.0f;
+  const float norm = none ? 0.0f : 1.0f / l;
+  const long long at = t * p.oTok + h * p.oHead + 2 * lane;
+#pragma unroll
+  for (int gr = 0; gr < G; gr++) {
+    if (p.half16) *reinterpret_cast<__half2*>(static_cast<__half*>(p.out) + at + 64 * gr) = __floats2half2_rn(y[2 * gr] * norm, y[2 * gr + 1] * norm);
+    else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) + at + 64 * gr) = __floats2bfloat162_rn(y[2 * gr] * norm, y[2 * gr + 1] * norm);
+  }
+  if (lane == 0 && p.lse != nullptr) p.lse[static_cast<long long>(t) * p.qHeads + h] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
 // Joins the partial sums of every row whose unit was cut, and clears the rows
 // that see nothing or stand behind the last request.  A block of four warps
 // takes one row where parts are many (WIDE: few rows in all), else each warp
@@ -762,7 +788,7 @@ __global__ void __launch_bounds__(128) joinKernel(const __grid_constant__ AttnAr
   const int b = requestOfRow(p, t, lane);
   const Request r = b < p.batch ? requestOf(p, b) : Request{0, 0, 0};
   const bool inside = t >= r.start && t < r.start + r.rows;
-  if (!inside && !p.zeroTail) return;
+  if (inside ? isLong(p, r) : !p.zeroTail) return;
   const int nt = inside ? tilesOf(r) : 0;
   float y[2 * G] = {};
   float m = kNone, l = 0.0f;
@@ -819,21 +845,93 @@ __global__ void __launch_bounds__(128) joinKernel(const __grid_constant__ AttnAr
     }
   }
   if (WIDE && warp > 0) return;
-  const bool none = l == 0.0f;
-  const float norm = none ? 0.0f : 1.0f / l;
-  const long long at = t * p.oTok + h * p.oHead + 2 * lane;
-#pragma unroll
-  for (int gr = 0; gr < G; gr++) {
-    if (p.half16) *reinterpret_cast<__half2*>(static_cast<__half*>(p.out) + at + 64 * gr) = __floats2half2_rn(y[2 * gr] * norm, y[2 * gr + 1] * norm);
-    else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) + at + 64 * gr) = __floats2bfloat162_rn(y[2 * gr] * norm, y[2 * gr + 1] * norm);
-  }
-  if (lane == 0 && p.lse != nullptr) p.lse[static_cast<long long>(t) * p.qHeads + h] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+  storeRow<G>(p, t, h, lane, y, m, l);
 }
+
+}  // namespace
+}  // namespace model
+}  // namespace vccl
+
+#include "kernels/kv4_chunk.cuh"
+
+namespace vccl {
+namespace model {
+namespace {
 
 int smsOfDevice() {
   int dev = 0, n = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
   return n;
+}
+
+// Requests with this many query rows a key head go to the tensor-core kernel
+// (a quarter of its 256-row units), and it is launched where the requests
+// bring kLongMean rows on average (a launch that finds none costs 3 us).
+constexpr int kLongRows = 64, kLongMean = 24;
+
+struct ChunkPlan {
+  bool use;
+  int splits;
+  long long units;  // at most, shares included
+};
+
+ChunkPlan chunkPlan(int batch, int tokens, int qHeads, int kvHeads) {
+  const long long rows = static_cast<long long>(tokens) * (qHeads / kvHeads);
+  if (rows < kLongRows || rows < static_cast<long long>(kLongMean) * batch) return {false, 1, 0};
+  const long long most = rows / kLongRows;
+  const long long units = kvHeads * (rows / kChunkRows + (batch < most ? batch : most));
+  // Fewer units than twice the SMs: the keys are shared out as well.
+  const long long s = 2LL * smsOfDevice() / units;
+  const int splits = static_cast<int>(s < 1 ? 1 : s > 16 ? 16 : s);
+  return {true, splits, units * splits};
+}
+
+// One abort word per device in mapped host memory: a launch that gave up a
+// wait sets it, and the next call on that device reads it.  Not made while a
+// stream is captured (the launch then reports nothing).
+std::mutex gFlagMu;
+int* gHostFlags[64] = {};
+int* gDevFlags[64] = {};
+
+int* chunkErrorFlag(cudaStream_t st) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  dev &= 63;
+  std::lock_guard<std::mutex> lock(gFlagMu);
+  if (gDevFlags[dev] == nullptr) {
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) return nullptr;
+    int* h = nullptr;
+    int* d = nullptr;
+    if (cudaHostAlloc(reinterpret_cast<void**>(&h), 64, cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) return nullptr;
+    *h = 0;
+    if (cudaHostGetDevicePointer(reinterpret_cast<void**>(&d), h, 0) != cudaSuccess) return nullptr;
+    gHostFlags[dev] = h;
+    gDevFlags[dev] = d;
+  }
+  return gDevFlags[dev];
+}
+
+bool takeChunkError() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  dev &= 63;
+  std::lock_guard<std::mutex> lock(gFlagMu);
+  volatile int* h = gHostFlags[dev];
+  if (h == nullptr || *h == 0) return false;
+  *h = 0;
+  return true;
+}
+
+template <int G>
+cudaError_t launchChunk(const AttnArgs& p, long long units, cudaStream_t st) {
+  const int fixed = ChunkSmem<G>::kStarts + 1024;
+  const cudaError_t e = cudaFuncSetAttribute(chunkKernel<G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             fixed + (kMaxBatch + 1) * static_cast<int>(sizeof(int)));
+  if (e != cudaSuccess) return e;
+  const int sms = smsOfDevice();
+  chunkKernel<G><<<static_cast<int>(units < sms ? units : sms), kChunkThreads, fixed + (p.batch + 1) * sizeof(int), st>>>(p);
+  return cudaGetLastError();
 }
 
 // Two tiles of 8 query rows where a request brings more than 8 rows of a key
@@ -865,11 +963,13 @@ using namespace vccl::model;
 extern "C" {
 
 size_t vcclKv4AttentionWorkspace(int batch, int tokens, int qHeads, int kvHeads, int D) {
-  if (batch <= 0 || kvHeads <= 0 || qHeads <= 0 || D <= 0) return 0;
+  if (batch <= 0 || tokens < 0 || kvHeads <= 0 || qHeads < kvHeads || D <= 0) return 0;
   const int nt = rowTiles(batch, tokens, qHeads / kvHeads);
-  const size_t slots = static_cast<size_t>(smsOfDevice()) * warpsFor(nt) * 2;
-  return align256((batch + 1) * sizeof(long long)) + align256(slots * 8 * nt * sizeof(float2)) +
-         slots * 8 * nt * D * sizeof(float);
+  const size_t slots = static_cast<size_t>(smsOfDevice()) * warpsFor(nt) * 2 * 8 * nt;
+  const ChunkPlan cp = chunkPlan(batch, tokens, qHeads, kvHeads);
+  const size_t chunkSlots = cp.use && cp.splits > 1 ? static_cast<size_t>(cp.units) * kChunkRows : 0;
+  return align256((batch + 1) * sizeof(long long)) + align256(slots * sizeof(float2)) + align256(slots * D * sizeof(float)) +
+         align256((batch + 1) * sizeof(int)) + align256(chunkSlots * sizeof(float2)) + chunkSlots * D * sizeof(float);
 }
 
 vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, const int* table, int width,
@@ -886,6 +986,10 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   if (!headsOk(q, 2) || !headsOk(out, 2) || q->heads != out->heads || q->heads % cache->kvHeads != 0 || !table ||
       !kvLens || !qStarts || !workspace || static_cast<long long>(tokens) * q->heads > INT_MAX)
     return vcclInvalidArgument;
+  if (takeChunkError()) {
+    VERR("vcclKv4Attention: an earlier call on this device gave up (a pipeline wait ran out); its output is invalid");
+    return vcclInternalError;
+  }
   TraceRange trace("vccl Kv4Attention");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int group = q->heads / cache->kvHeads, nt = rowTiles(batch, tokens, group), R = 8 * nt;
@@ -920,6 +1024,24 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   p.stats = reinterpret_cast<float2*>(ws);
   ws += align256(static_cast<size_t>(p.workers) * 2 * R * sizeof(float2));
   p.partial = reinterpret_cast<float*>(ws);
+  ws += align256(static_cast<size_t>(p.workers) * 2 * R * cache->D * sizeof(float));
+  const ChunkPlan cp = chunkPlan(batch, tokens, q->heads, cache->kvHeads);
+  if (cp.use) {
+    p.longRows = kLongRows;
+    p.splits = cp.splits;
+    p.chunkStarts = reinterpret_cast<int*>(ws);
+    ws += align256((batch + 1) * sizeof(int));
+    const size_t chunkSlots = cp.splits > 1 ? static_cast<size_t>(cp.units) * kChunkRows : 0;
+    p.chunkStats = reinterpret_cast<float2*>(ws);
+    ws += align256(chunkSlots * sizeof(float2));
+    p.chunkPartial = reinterpret_cast<float*>(ws);
+    p.errorFlag = chunkErrorFlag(st);
+    const cudaError_t c = cache->D == 128 ? launchChunk<2>(p, cp.units, st) : launchChunk<1>(p, cp.units, st);
+    if (c != cudaSuccess) {
+      VERR("vcclKv4Attention: %s", cudaGetErrorString(c));
+      return vcclSystemError;
+    }
+  }
   cudaError_t e;
   if (cache->D == 128) e = nt == 1 ? launchAttn<2, 1>(p, grid, st) : launchAttn<2, 2>(p, grid, st);
   else e = nt == 1 ? launchAttn<1, 1>(p, grid, st) : launchAttn<1, 2>(p, grid, st);
@@ -947,6 +1069,12 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   if (e != cudaSuccess) {
     VERR("vcclKv4Attention: %s", cudaGetErrorString(e));
     return vcclSystemError;
+  }
+  if (cp.use && cp.splits > 1) {
+    const unsigned blocks = static_cast<unsigned>((rows + 3) / 4);
+    if (cache->D == 128) chunkJoinKernel<2><<<blocks, 128, 0, st>>>(p);
+    else chunkJoinKernel<1><<<blocks, 128, 0, st>>>(p);
+    return launched("vcclKv4Attention");
   }
   return vcclSuccess;
 }

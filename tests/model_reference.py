@@ -93,11 +93,12 @@ def stored_values(x):
 
 
 def attention(q, k, v, kv_lens, q_starts, scale):
-    """q [T, Hq, D]; k, v: a list of [len, H, D] per request (f64).  Returns out, lse and, for a bound on the error,
-    sum p |v| (the size of the terms that are added up)."""
+    """q [T, Hq, D]; k, v: a list of [len, H, D] per request (f64).  Returns out, lse and, for bounds on the error,
+    sum p |v| (the size of the terms that are added up) and sqrt(sum p^2 (v - out)^2) (what independent errors of the
+    scores move out by)."""
     t, hq, d = q.shape
     out = torch.zeros(t, hq, d, dtype=torch.float64, device=q.device)
-    size = torch.zeros_like(out)
+    size, spread = torch.zeros_like(out), torch.zeros_like(out)
     lse = torch.full((t, hq), -math.inf, dtype=torch.float64, device=q.device)
     for b, n in enumerate(kv_lens):
         a, e = q_starts[b], q_starts[b + 1]
@@ -114,4 +115,5 @@ def attention(q, k, v, kv_lens, q_starts, scale):
             lse[i] = torch.logsumexp(sc, -1)
             out[i] = torch.einsum("hn,nhd->hd", p, vv[:see])
             size[i] = torch.einsum("hn,nhd->hd", p, vv[:see].abs())
-    return out, lse, size
+            spread[i] = torch.einsum("hn,nhd->hd", p ** 2, (vv[:see] - out[i]) ** 2).sqrt()
+    return out, lse, size, spread

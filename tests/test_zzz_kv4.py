@@ -389,7 +389,7 @@ def filled(g, kv_lens, page, hk, dim, extra_pages=2, dtype=torch.bfloat16, width
 def check_attention(got, lse, q, ks, vs, kv_lens, q_starts, scale=None):
     d = q.shape[-1]
     scale = d ** -0.5 if scale is None else scale
-    want, wlse, size = ref.attention(q, ks, vs, kv_lens, q_starts, scale)
+    want, wlse, size, spread = ref.attention(q, ks, vs, kv_lens, q_starts, scale)
     # The largest sum of absolute products behind a score: (7.5 scale + |mid|) bounds a value, and with it f32 keeps a
     # score to 2^-19 of it (products of exact codes, a handful of f32 roundings and 128 additions of 2^-24 each).
     most = [x.abs().amax() * 3 if x.numel() else torch.zeros((), dtype=torch.float64, device="cuda") for x in ks]
@@ -401,9 +401,24 @@ def check_attention(got, lse, q, ks, vs, kv_lens, q_starts, scale=None):
     # subnormal end (2^-25 a token), scores, and the stored type
     slack = want.abs() * half_step(q.dtype) * (1 + 2**-6) + size * 2.0**-11 + vmax * 2.0**-11 * 2 * (1 / math.sqrt(max(n, 1)) + 2.0**-4) \
         + n * 2.0**-25 * vmax + (size + vmax * 2.0**-4) * score + 2.0**-25
+    # Requests with many rows are computed from keys and values in f16, as o + s (code - 8) with o = mid + s / 2 rounded
+    # once (|o| <= 1.1 max |x|) and the sum rounded once: 2^-11 (|o| + |x|) at most, and in weights of 2^-11.  Of a key's
+    # 64 channels the roundings of the sums are independent (variance step^2 / 3) and that of o is one for all; scores
+    # are then off by sigma, the output by sigma * spread: 6 sigma.
+    heads = ks[0].shape[1]
+    long = torch.zeros(q.shape[0], 1, 1, dtype=torch.float64, device="cuda")
+    if q.shape[0] * (q.shape[1] // heads) >= 64:
+        for a, e in zip(q_starts, q_starts[1:]):
+            if (e - a) * (q.shape[1] // heads) >= 64:
+                long[a:e] = 1.0
+    kmax = max([x.abs().max().item() for x in ks if x.numel()] + [0.0])
+    x = q.double()
+    groups = x.unflatten(-1, (-1, 64)).sum(-1)
+    sigma = abs(scale) * 2.0**-11 / math.sqrt(3) * kmax * (x.pow(2).sum(-1) + 1.1**2 * groups.pow(2).sum(-1)).sqrt()
+    slack = slack + long * (2.0**-11 * (2 * size + 1.1 * vmax) + 6 * sigma[..., None] * spread)
     close(got, want, slack, "out")
     if lse is not None:
-        close(lse, wlse, score[..., 0] + wlse.abs().nan_to_num(posinf=0) * 2.0**-20 + 2.0**-19, "lse")
+        close(lse, wlse, score[..., 0] + long[..., 0] * 6 * sigma + wlse.abs().nan_to_num(posinf=0) * 2.0**-20 + 2.0**-19, "lse")
 
 
 def starts(q_lens):
@@ -663,7 +678,7 @@ def test_serving_steps_match_dense_attention(captured):
             vs.append(ref.stored_values(torch.stack([h[1] for h in history[i]])) if history[i] else empty)
         assert lens.tolist() == kv_lens
         q64 = ref.norm_rope(qkv[:, :hq], w, 1e-6, pos, freq, False)
-        want, _, _ = ref.attention(q64, ks, vs, kv_lens, qs, dim ** -0.5)
+        want = ref.attention(q64, ks, vs, kv_lens, qs, dim ** -0.5)[0]
         # bf16 queries and outputs, and keys whose 4-bit code may fall to the neighbour where the f32 and f64 rotations
         # round to neighbouring bf16 numbers: bounded in the norm of each row
         err = (out[:qs[-1]].double() - want[:qs[-1]]).norm(dim=-1) / (want[:qs[-1]].norm(dim=-1) + 1e-3)
