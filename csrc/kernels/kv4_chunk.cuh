@@ -17,12 +17,16 @@
 // run in order, so the scores of the next keys may take the place of weights
 // just used.
 //
-// Numbers.  f16 holds 11 bits, one more than what 4-bit values rounded to
-// bf16 would keep; its range is handled by powers of two: a query row is
-// scaled to 2^12, 32 neighbouring tokens (what a warp turns, and what a
-// softmax thread takes at once) share a power of two for keys and one for
-// values, which the softmax puts into its scale and into the weights.  Scores,
-// maxima, sums and outputs are f32.  The maximum is followed loosely (by 8 in
+// Numbers.  f16 holds 11 bits, and a scale of 8 bits times a code between -8
+// and 7 (3 bits and a power of two) is exact in them.  So a key is the product
+// s (code - 8), and what is the same for 64 channels, o = mid + s / 2, meets
+// the sum of the query's channels in a few more columns of the product (both
+// as two f16 each, 22 bits): scores are exact to f32.  Values are o + s (code -
+// 8), o and the sum rounded to f16.  f16's range is handled by powers of two:
+// a query row is scaled to 2^8, 32 neighbouring tokens (what a warp turns, and
+// what a softmax thread takes at once) share a power of two for keys and one
+// for values, which the softmax puts into its scale and into the weights.
+// Scores, maxima, sums and outputs are f32.  The maximum is followed loosely (by 8 in
 // the base-2 logarithm), so the output is rescaled rarely.
 #pragma once
 
@@ -100,6 +104,37 @@ __device__ __forceinline__ uint64_t smemDescMn(uint32_t addr) {
   return d;
 }
 
+// K-major operand of 16 columns without a swizzle: 8 rows of 16 bytes to an
+// atom, the next 8 columns 128 bytes on, the next 8 rows 256.
+__device__ __forceinline__ uint64_t smemDescPlain(uint32_t addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3fffu);
+  d |= static_cast<uint64_t>(128u >> 4) << 16;
+  d |= static_cast<uint64_t>(256u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  return d;
+}
+constexpr int kPlainBytes = 128 * 32;
+__device__ __forceinline__ int plainRow(int row) { return (row >> 3) * 256 + (row & 7) * 16; }
+
+__device__ __forceinline__ float halfOf(float x) { return __half2float(__float2half_rn(x)); }
+
+// Columns that carry sum over groups of a_g b_g, a and b as two f16 each; a
+// side's columns of one group are (high, high, low) or (high, low, high).
+template <int G, bool QUERY>
+__device__ __forceinline__ void storeSums(uint8_t* block, int row, const float (&x)[G]) {
+  float y[8] = {};
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    const float high = halfOf(x[g]), low = x[g] - high;
+    y[3 * g] = high;
+    y[3 * g + 1] = QUERY ? high : low;
+    y[3 * g + 2] = QUERY ? low : high;
+  }
+  *reinterpret_cast<uint4*>(block + plainRow(row)) = pack8<__half>(y);
+  *reinterpret_cast<uint4*>(block + plainRow(row) + 128) = make_uint4(0, 0, 0, 0);
+}
+
 // 2^e for -126 <= e <= 127 (clamped).
 __device__ __forceinline__ float powerOfTwo(int e) {
   return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23);
@@ -112,7 +147,9 @@ struct ChunkSmem {
   static constexpr int kQ = 0;          // [2 row tiles][G]
   static constexpr int kK = kQ + 2 * G * kBlock;  // [2 stages][G]
   static constexpr int kV = kK + 2 * G * kBlock;
-  static constexpr int kInfo = kV + 2 * G * kBlock;
+  static constexpr int kQSums = kV + 2 * G * kBlock;  // [2 row tiles]
+  static constexpr int kKSums = kQSums + 2 * kPlainBytes;  // [2 stages]
+  static constexpr int kInfo = kKSums + 2 * kPlainBytes;
   static constexpr int kStarts = kInfo + 1024;  // units before each request
 };
 
@@ -173,16 +210,16 @@ __device__ __forceinline__ ChunkUnit chunkUnit(const AttnArgs& p, const int* sta
 }
 
 // One token's row of codes -> f16 in shared memory: 8 channels a store.
-// scale, mid: of its groups, already divided by the power of two; KEYS: the
-// order of the words.
+// scale, offset: of its groups, already divided by the power of two.  KEYS:
+// the order of the words, and products alone (the offsets go to storeSums).
 template <int G, bool KEYS>
-__device__ __forceinline__ void widen(const uint32_t (&w)[8 * G], const float (&scale)[G], const float (&mid)[G], uint8_t* block,
+__device__ __forceinline__ void widen(const uint32_t (&w)[8 * G], const float (&scale)[G], const float (&offset)[G], uint8_t* block,
                                       int t) {
   __half2 s[G], o[G];
 #pragma unroll
   for (int g = 0; g < G; g++) {
     s[g] = __float2half2_rn(scale[g]);
-    o[g] = __float2half2_rn(fmaf(0.5f, scale[g], mid[g]));  // value = o + s (code - 8)
+    o[g] = __float2half2_rn(offset[g]);
   }
   const __half2 minus8 = __float2half2_rn(-1032.0f), sixteenth = __float2half2_rn(0.0625f), minus72 = __float2half2_rn(-72.0f);
 #pragma unroll
@@ -194,7 +231,8 @@ __device__ __forceinline__ void widen(const uint32_t (&w)[8 * G], const float (&
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       const __half2 c = *reinterpret_cast<const __half2*>(&h[k]);  // 1024 + code, or 1024 + 16 code: both exact
-      const __half2 v = __hfma2((k & 1) ? __hfma2(c, sixteenth, minus72) : __hadd2(c, minus8), s[g], o[g]);
+      const __half2 d = (k & 1) ? __hfma2(c, sixteenth, minus72) : __hadd2(c, minus8);
+      const __half2 v = KEYS ? __hmul2(d, s[g]) : __hfma2(d, s[g], o[g]);
       h[k] = *reinterpret_cast<const uint32_t*>(&v);
     }
     *reinterpret_cast<uint4*>(block + g * ChunkSmem<G>::kBlock + t * 128 + ((b ^ (t & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
@@ -204,6 +242,71 @@ __device__ __forceinline__ void widen(const uint32_t (&w)[8 * G], const float (&
 // A wait of a whole warp: every lane goes on, or none does.
 __device__ __forceinline__ bool warpWait(uint64_t* bar, uint32_t parity, volatile int* abortFlag) {
   return __all_sync(~0u, sm100::mbarWait(bar, parity, abortFlag));
+}
+
+// Keys of 32 that a row sees, of which `left` are in its range.
+__device__ __forceinline__ uint32_t seenOf(uint32_t valid, int left) {
+  return valid & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1);
+}
+
+// First look at a row's scores: the maximum over the keys that it sees, in
+// the base-2 logarithm.  EDGE: some row of the warp does not see some key.
+// Scores come 32 at a time, the next under way.
+template <bool EDGE>
+__device__ __forceinline__ float tileMaximum(uint32_t scores, const ChunkInfo& info, float unit, int left) {
+  uint32_t s[2][32];
+  float top = kNone;
+  tmemLoad32(scores, s[0]);
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    sm100::tmemLoadWait();
+    if (k < 3) tmemLoad32(scores + 32 * (k + 1), s[(k + 1) & 1]);
+    const uint32_t seen = EDGE ? seenOf(info.valid[k], left - 32 * k) : ~0u;
+    float x[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+      const float v = __uint_as_float(s[k & 1][i]);
+      x[i & 1] = fmaxf(x[i & 1], !EDGE || ((seen >> i) & 1u) ? v : -INFINITY);
+    }
+    const float most = fmaxf(x[0], x[1]);
+    if (most > -INFINITY) top = fmaxf(top, most * unit * powerOfTwo(info.keyExp[k]));
+  }
+  return top;
+}
+
+// Second look: the weights, to TMEM in the place of the scores; returns their
+// sum.  off: minus the maximum; ref: the power of two that the outputs have.
+template <bool EDGE>
+__device__ __forceinline__ float tileWeights(uint32_t scores, const ChunkInfo& info, float unit, int left, float m, int ref) {
+  uint32_t s[2][32];
+  float sum = 0.0f;
+  tmemLoad32(scores, s[0]);
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    sm100::tmemLoadWait();
+    if (k < 3) tmemLoad32(scores + 32 * (k + 1), s[(k + 1) & 1]);
+    const uint32_t seen = EDGE ? seenOf(info.valid[k], left - 32 * k) : ~0u;
+    const int ve = info.valueExp[k], shift = ve == kNoExponent ? 0 : max(ve - ref, -100);
+    const float scale = unit * powerOfTwo(info.keyExp[k]), off = static_cast<float>(shift) - m;
+    float part[2] = {0.0f, 0.0f};
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      float a = exp2Fast(fmaf(__uint_as_float(s[k & 1][2 * i]), scale, off));
+      float b = exp2Fast(fmaf(__uint_as_float(s[k & 1][2 * i + 1]), scale, off));
+      if (EDGE) {
+        if (!((seen >> (2 * i)) & 1u)) a = 0.0f;
+        if (!((seen >> (2 * i + 1)) & 1u)) b = 0.0f;
+      }
+      part[0] += a;
+      part[1] += b;
+      w[i] = packHalf(a, b);
+    }
+    sum = fmaf(part[0] + part[1], powerOfTwo(-shift), sum);
+    // Scores 32 (k + 1) on are under way or to come: the weights end before them.
+    tmemStore16(scores + 16 * k, w);
+  }
+  return sum;
 }
 
 template <int G>
@@ -287,8 +390,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       int ref = kNoExponent;  // the outputs are in units of 2^ref
       uint32_t poison = 0;
       if (c.from < c.upto) {
-        // The row's channels, scaled to 2^12 at most, as the left operand.
-        float amax = 0.0f;
+        // The row's channels, scaled to 2^8, and their sums as the left operand.
+        float amax = 0.0f, sums[G] = {};
         const uint16_t* src = static_cast<const uint16_t*>(p.q) + static_cast<long long>(c.r.start + token) * p.qTok + static_cast<long long>(h) * p.qHead;
         uint4 raw[8 * G];
 #pragma unroll
@@ -298,12 +401,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
           if (p.half16) unpack8<__half>(raw[i], x);
           else unpack8<__nv_bfloat16>(raw[i], x);
 #pragma unroll
-          for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[e]));
+          for (int e = 0; e < 8; e++) {
+            amax = fmaxf(amax, fabsf(x[e]));
+            sums[i / 8] += x[e];
+          }
         }
         const int e = exponentOf(amax);
         const bool plain = amax == 0.0f || e > 120 || e < -100;
-        const float f = (plain ? 1.0f : powerOfTwo(12 - e)) * (p.scaleLog2 < 0.0f ? -1.0f : 1.0f);
-        unit = (plain ? 1.0f : powerOfTwo(e - 12)) * fabsf(p.scaleLog2);
+        const float f = (plain ? 1.0f : powerOfTwo(8 - e)) * (p.scaleLog2 < 0.0f ? -1.0f : 1.0f);
+        unit = (plain ? 1.0f : powerOfTwo(e - 8)) * fabsf(p.scaleLog2);
 #pragma unroll
         for (int i = 0; i < 8 * G; i++) {
           float x[8];
@@ -313,6 +419,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
           for (int k = 0; k < 8; k++) x[k] *= f;
           *reinterpret_cast<uint4*>(smem + L::kQ + (t * G + i / 8) * L::kBlock + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = pack8<__half>(x);
         }
+#pragma unroll
+        for (int g = 0; g < G; g++) sums[g] *= f;
+        storeSums<G, true>(smem + L::kQSums + t * kPlainBytes, row, sums);
         sm100::fenceProxyAsyncShared();
         sm100::mbarArrive(&ctl.qFull[t]);
         for (int j = c.from; j < c.upto; j++, seq++) {
@@ -323,36 +432,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
           sCount++;
           sm100::tcFenceAfter();
           const ChunkInfo& info = ctl.info[seq & 3];
-          float scale[4];
-          int valueExp[4], newRef = ref;
-          uint32_t mask[4];
-          bool all = true;
+          const int left = limit - j * kChunkKeys;  // keys of the tile in the row's range
+          const uint32_t valid = info.valid[0] & info.valid[1] & info.valid[2] & info.valid[3];
+          const bool edge = __any_sync(~0u, left < kChunkKeys || valid != ~0u);
+          int newRef = ref;
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            scale[k] = unit * powerOfTwo(info.keyExp[k]);
-            valueExp[k] = info.valueExp[k];
-            newRef = max(newRef, valueExp[k]);
-            const int left = limit - (j * kChunkKeys + 32 * k);  // keys of these 32 that the row sees
-            mask[k] = info.valid[k] & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1);
-            all = all && mask[k] == ~0u;
-          }
-          const bool edge = __any_sync(~0u, !all);
-          float top = kNone;
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            uint32_t s[32];
-            tmemLoad32(scores + 32 * k, s);
-            sm100::tmemLoadWait();
-            float x = -INFINITY;
-            if (edge) {
-#pragma unroll
-              for (int i = 0; i < 32; i++) x = fmaxf(x, (mask[k] >> i) & 1u ? __uint_as_float(s[i]) : -INFINITY);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; i++) x = fmaxf(x, __uint_as_float(s[i]));
-            }
-            if (x > -INFINITY) top = fmaxf(top, x * scale[k]);
-          }
+          for (int k = 0; k < 4; k++) newRef = max(newRef, info.valueExp[k]);
+          const float top = edge ? tileMaximum<true>(scores, info, unit, left) : tileMaximum<false>(scores, info, unit, left);
           if (__any_sync(~0u, top > m + 8.0f || newRef > ref)) {
             const float next = fmaxf(m, top), shrink = exp2Fast(m - next);
             if (j > c.from) {
@@ -372,32 +458,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
             m = next;
             ref = newRef;
           }
+          l += edge ? tileWeights<true>(scores, info, unit, left, m, ref) : tileWeights<false>(scores, info, unit, left, m, ref);
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            uint32_t s[32], w[16];
-            tmemLoad32(scores + 32 * k, s);
-            sm100::tmemLoadWait();
-            const int shift = valueExp[k] == kNoExponent ? 0 : max(valueExp[k] - ref, -100);
-            const float off = static_cast<float>(shift) - m;
-            float sum0 = 0.0f, sum1 = 0.0f;
+          for (int g = 0; g < G; g++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-              float a = exp2Fast(fmaf(__uint_as_float(s[2 * i]), scale[k], off));
-              float b = exp2Fast(fmaf(__uint_as_float(s[2 * i + 1]), scale[k], off));
-              if (edge) {
-                if (!((mask[k] >> (2 * i)) & 1u)) a = 0.0f;
-                if (!((mask[k] >> (2 * i + 1)) & 1u)) b = 0.0f;
-              }
-              sum0 += a;
-              sum1 += b;
-              w[i] = packHalf(a, b);
-            }
-            l = fmaf(sum0 + sum1, powerOfTwo(-shift), l);
-            tmemStore16(scores + 16 * k, w);
-#pragma unroll
-            for (int g = 0; g < G; g++)
-              if (info.bad[g][k] & mask[k]) poison |= 1u << g;
-          }
+            for (int k = 0; k < 4; k++)
+              if (info.bad[g][k] & seenOf(info.valid[k], left - 32 * k)) poison |= 1u << g;
           tmemStoreWait();
           sm100::tcFenceBefore();
           sm100::mbarArrive(&ctl.pFull[t]);
@@ -551,14 +617,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
 #pragma unroll
       for (int g = 0; g < G; g++) {
         ks[g] *= kf;
-        km[g] *= kf;
+        km[g] = fmaf(0.5f, ks[g], km[g] * kf);  // value = m + s (code - 8) from here on
         vs[g] *= vf;
-        vm[g] *= vf;
+        vm[g] = fmaf(0.5f, vs[g], vm[g] * vf);
       }
       const int st = seq & 1;
       const uint32_t parity = ((seq >> 1) & 1u) ^ 1u;
       if (!warpWait(&ctl.kEmpty[st], parity, abortFlag)) break;
       widen<G, true>(raw.k, ks, km, smem + L::kK + st * G * L::kBlock, tid);
+      storeSums<G, false>(smem + L::kKSums + st * kPlainBytes, tid, km);
       sm100::fenceProxyAsyncShared();
       sm100::mbarArrive(&ctl.kFull[st]);
       if (!warpWait(&ctl.vEmpty[st], parity, abortFlag)) break;
@@ -571,6 +638,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
   } else if (lane == 0) {
     // ---------------- products ----------------
     constexpr uint32_t kScores = idescF16(128, 128, false), kOutputs = idescF16(128, D, true);
+    const uint32_t qSums = sm100::smemAddr(smem + L::kQSums), kSums = sm100::smemAddr(smem + L::kKSums);
     const uint32_t qBase = sm100::smemAddr(smem + L::kQ), kBase = sm100::smemAddr(smem + L::kK), vBase = sm100::smemAddr(smem + L::kV);
     uint32_t seq = 0, qCount[2] = {0, 0}, pCount[2] = {0, 0};
     bool ok = true;
@@ -581,6 +649,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         for (int k = 0; k < 4; k++)
           mmaF16(tmem + t * 128, sm100::smemDescSw128(qBase + (t * G + g) * L::kBlock + 32 * k),
                  sm100::smemDescSw128(kBase + ((s & 1) * G + g) * L::kBlock + 32 * k), kScores, g + k > 0);
+      mmaF16(tmem + t * 128, smemDescPlain(qSums + t * kPlainBytes), smemDescPlain(kSums + (s & 1) * kPlainBytes), kScores, 1);
       sm100::mmaCommit(&ctl.sFull[t]);
     };
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
