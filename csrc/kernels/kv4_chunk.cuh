@@ -73,17 +73,24 @@ __device__ __forceinline__ void tmemStore32(uint32_t taddr, const uint32_t (&r)[
 }
 __device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// f16 products: A in shared memory or TMEM, B in shared memory.
-__device__ __forceinline__ void mmaF16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// f16 products: A in shared memory or TMEM, B in shared memory.  Shared-memory
+// descriptors come as two words, of which only the first moves from product to
+// product: the one thread that issues them would else be what the tensor cores
+// wait for (a product of 128 x 128 x 16 takes 64 clocks; with 64-bit
+// descriptors made anew the thread took 100 for each).
+template <bool ACCUMULATE>
+__device__ __forceinline__ void mmaF16(uint32_t d, uint32_t aLo, uint32_t aHi, uint32_t bLo, uint32_t bHi, uint32_t idesc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %6, 0;\n mov.b64 a, {%1, %2};\n mov.b64 b, {%3, %4};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}\n" ::"r"(d),
+      "r"(aLo), "r"(aHi), "r"(bLo), "r"(bHi), "r"(idesc), "n"(ACCUMULATE ? 1 : 0)
       : "memory");
 }
-__device__ __forceinline__ void mmaF16Tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mmaF16Tmem(uint32_t d, uint32_t a, uint32_t bLo, uint32_t bHi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n mov.b64 b, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(bLo), "r"(bHi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -642,14 +649,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
     const uint32_t qBase = sm100::smemAddr(smem + L::kQ), kBase = sm100::smemAddr(smem + L::kK), vBase = sm100::smemAddr(smem + L::kV);
     uint32_t seq = 0, qCount[2] = {0, 0}, pCount[2] = {0, 0};
     bool ok = true;
+    // Words of the descriptors: addresses count 16 bytes.
+    const uint64_t rows = sm100::smemDescSw128(0), plain = smemDescPlain(0), major = smemDescMn(0);
+    const uint32_t rowsLo = static_cast<uint32_t>(rows), rowsHi = static_cast<uint32_t>(rows >> 32);
+    const uint32_t plainLo = static_cast<uint32_t>(plain), plainHi = static_cast<uint32_t>(plain >> 32);
+    const uint32_t majorLo = static_cast<uint32_t>(major), majorHi = static_cast<uint32_t>(major >> 32);
+    constexpr uint32_t kStep = L::kBlock >> 4;
     auto issueScores = [&](int t, uint32_t s) {
+      const uint32_t d = tmem + t * 128, q = rowsLo + (qBase >> 4) + t * (G * kStep), k = rowsLo + (kBase >> 4) + (s & 1) * (G * kStep);
+      mmaF16<false>(d, q, rowsHi, k, rowsHi, kScores);
 #pragma unroll
-      for (int g = 0; g < G; g++)
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          mmaF16(tmem + t * 128, sm100::smemDescSw128(qBase + (t * G + g) * L::kBlock + 32 * k),
-                 sm100::smemDescSw128(kBase + ((s & 1) * G + g) * L::kBlock + 32 * k), kScores, g + k > 0);
-      mmaF16(tmem + t * 128, smemDescPlain(qSums + t * kPlainBytes), smemDescPlain(kSums + (s & 1) * kPlainBytes), kScores, 1);
+      for (int i = 1; i < 4 * G; i++)
+        mmaF16<true>(d, q + (i >> 2) * kStep + 2 * (i & 3), rowsHi, k + (i >> 2) * kStep + 2 * (i & 3), rowsHi, kScores);
+      mmaF16<true>(d, plainLo + (qSums >> 4) + t * (kPlainBytes >> 4), plainHi, plainLo + (kSums >> 4) + (s & 1) * (kPlainBytes >> 4),
+                   plainHi, kScores);
       sm100::mmaCommit(&ctl.sFull[t]);
     };
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
@@ -670,8 +683,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
           sm100::tcFenceAfter();
 #pragma unroll
           for (int k = 0; k < 8; k++)
-            mmaF16Tmem(tmem + kOut + t * D, tmem + t * 128 + 8 * k, smemDescMn(vBase + (seq & 1) * G * L::kBlock + 2048 * k), kOutputs,
-                       j + k > 0);
+            mmaF16Tmem(tmem + kOut + t * D, tmem + t * 128 + 8 * k, majorLo + (vBase >> 4) + (seq & 1) * (G * kStep) + 128 * k, majorHi,
+                       kOutputs, k > 0 ? 1u : static_cast<uint32_t>(j));
           if (j + 1 == n) sm100::mmaCommit(&ctl.oFull[t]);
           if (t + 1 == c.tiles) sm100::mmaCommit(&ctl.vEmpty[seq & 1]);
           if (j + 1 < n) {
