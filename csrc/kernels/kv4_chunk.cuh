@@ -3,19 +3,20 @@
 // generation tensor cores (included by kv4_attention.cu).
 //
 // A unit is 256 query rows (two tiles of 128) of one request and key head
-// against a range of keys, 128 at a time.  Roles of a block of 13 warps:
+// against a range of keys, 64 at a time.  Roles of a block of 13 warps:
 //   warps 0-3, 4-7  softmax of the first and the second row tile, a thread a
 //                   row: scores from TMEM, weights back to TMEM as f16, in
 //                   the place of the scores;
-//   warps 8-11      a thread a token: codes from global memory (one tile
-//                   ahead in registers) to f16 in shared memory, in the
-//                   128-byte swizzle that the products read;
-//   warp 12         one thread issues S = Q K^T (N = 128) and O += P V (P
-//                   from TMEM, V with channels as the major axis).
-// While one row tile's products run the other's softmax does; the order PV0,
-// S0, PV1, S1 of the products keeps both busy, and the products of one thread
-// run in order, so the scores of the next keys may take the place of weights
-// just used.
+//   warps 8-9       a thread a token: key codes from global memory (one tile
+//   10-11           ahead in registers) to f16 in shared memory, in the
+//                   128-byte swizzle that the products read; value codes;
+//   warp 12         one thread issues S = Q K^T (N = 64) and O += P V (P from
+//                   TMEM, V with channels as the major axis).
+// A row tile has two places for scores, so the products of the keys after next
+// go on beside the softmax of these (with 128 keys and one place the softmax
+// waited 1700 of 7800 clocks for its scores, and read them twice for want of
+// registers).  The products of one thread run in order, so scores may take the
+// place of weights just used.
 //
 // Numbers.  f16 holds 11 bits, and a scale of 8 bits times a code between -8
 // and 7 (3 bits and a power of two) is exact in them.  So a key is the product
@@ -38,7 +39,8 @@ namespace model {
 namespace {
 
 constexpr int kChunkRows = 256;
-constexpr int kChunkKeys = 128;
+constexpr int kChunkKeys = 64;
+constexpr int kChunkStages = 4;     // tiles of keys, and of values, in shared memory
 constexpr int kChunkThreads = 13 * 32;
 constexpr int kNoExponent = -1000;  // of 32 tokens that are all zero
 
@@ -100,11 +102,11 @@ __host__ __device__ constexpr uint32_t idescF16(int m, int n, bool transposeB) {
 }
 
 // N-major operand in the 128-byte swizzle: atoms of 64 channels by 8 tokens;
-// the next 64 channels 16 KiB on (leading), the next 8 tokens 1 KiB on (stride).
+// the next 64 channels 8 KiB on (leading), the next 8 tokens 1 KiB on (stride).
 __device__ __forceinline__ uint64_t smemDescMn(uint32_t addr) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((addr >> 4) & 0x3fffu);
-  d |= static_cast<uint64_t>(16384u >> 4) << 16;
+  d |= static_cast<uint64_t>(8192u >> 4) << 16;
   d |= static_cast<uint64_t>(1024u >> 4) << 32;
   d |= static_cast<uint64_t>(1u) << 46;
   d |= static_cast<uint64_t>(2u) << 61;
@@ -121,7 +123,6 @@ __device__ __forceinline__ uint64_t smemDescPlain(uint32_t addr) {
   d |= static_cast<uint64_t>(1u) << 46;
   return d;
 }
-constexpr int kPlainBytes = 128 * 32;
 __device__ __forceinline__ int plainRow(int row) { return (row >> 3) * 256 + (row & 7) * 16; }
 
 __device__ __forceinline__ float halfOf(float x) { return __half2float(__float2half_rn(x)); }
@@ -150,26 +151,30 @@ __device__ __forceinline__ int exponentOf(float x) { return static_cast<int>((__
 
 template <int G>
 struct ChunkSmem {
-  static constexpr int kBlock = 16384;  // 128 rows of 64 f16
-  static constexpr int kQ = 0;          // [2 row tiles][G]
-  static constexpr int kK = kQ + 2 * G * kBlock;  // [2 stages][G]
-  static constexpr int kV = kK + 2 * G * kBlock;
-  static constexpr int kQSums = kV + 2 * G * kBlock;  // [2 row tiles]
-  static constexpr int kKSums = kQSums + 2 * kPlainBytes;  // [2 stages]
-  static constexpr int kInfo = kKSums + 2 * kPlainBytes;
+  static constexpr int kQBlock = 16384;  // 128 rows of 64 f16
+  static constexpr int kBlock = 8192;    // 64 tokens of 64 f16
+  static constexpr int kQ = 0;           // [2 row tiles][G]
+  static constexpr int kK = kQ + 2 * G * kQBlock;  // [stages][G]
+  static constexpr int kV = kK + kChunkStages * G * kBlock;
+  static constexpr int kQSums = kV + kChunkStages * G * kBlock;  // [2 row tiles]
+  static constexpr int kKSums = kQSums + 2 * 128 * 32;           // [stages]
+  static constexpr int kInfo = kKSums + kChunkStages * 64 * 32;
   static constexpr int kStarts = kInfo + 1024;  // units before each request
 };
 
-// What the tokens of a tile bring, by 32 (one warp's).
+// What the tokens of a tile bring, by 32.
 struct ChunkInfo {
-  uint32_t valid[4];   // the token is there
-  uint32_t bad[2][4];  // its values of a group are not finite (and zero in the product)
-  int keyExp[4], valueExp[4];
+  uint32_t valid[2];   // the token is there
+  uint32_t bad[2][2];  // its values of a group are not finite (and zero in the product)
+  int keyExp[2], valueExp[2];
 };
 
 struct ChunkControl {
-  ChunkInfo info[4];
-  uint64_t qFull[2], kFull[2], kEmpty[2], vFull[2], vEmpty[2], sFull[2], pFull[2], oFull[2], drain;
+  ChunkInfo info[kChunkStages];
+  uint64_t kFull[kChunkStages], kEmpty[kChunkStages], vFull[kChunkStages], vEmpty[kChunkStages];
+  // A wait tells a phase of a barrier from the one before it alone, so what
+  // can be two tiles ahead has a barrier for each place.
+  uint64_t qFull[2], sFull[2][2], pFull[2][2], pvDone[2][2], drain;
   uint32_t tmem;
   int abort;
 };
@@ -256,69 +261,68 @@ __device__ __forceinline__ uint32_t seenOf(uint32_t valid, int left) {
   return valid & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1);
 }
 
-// First look at a row's scores: the maximum over the keys that it sees, in
-// the base-2 logarithm.  EDGE: some row of the warp does not see some key.
-// Scores come 32 at a time, the next under way.
+// The maximum of a row's scores over the keys that it sees, in the base-2
+// logarithm.  EDGE: some row of the warp does not see some key.
 template <bool EDGE>
-__device__ __forceinline__ float tileMaximum(uint32_t scores, const ChunkInfo& info, float unit, int left) {
-  uint32_t s[2][32];
+__device__ __forceinline__ float tileMaximum(uint32_t (&s)[2][32], const ChunkInfo& info, const float (&scale)[2], int left) {
   float top = kNone;
-  tmemLoad32(scores, s[0]);
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    sm100::tmemLoadWait();
-    if (k < 3) tmemLoad32(scores + 32 * (k + 1), s[(k + 1) & 1]);
+  for (int k = 0; k < 2; k++) {
     const uint32_t seen = EDGE ? seenOf(info.valid[k], left - 32 * k) : ~0u;
-    float x[2] = {-INFINITY, -INFINITY};
+    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < 32; i++) {
-      const float v = __uint_as_float(s[k & 1][i]);
-      x[i & 1] = fmaxf(x[i & 1], !EDGE || ((seen >> i) & 1u) ? v : -INFINITY);
+      if (EDGE && !((seen >> i) & 1u)) s[k][i] = 0xFF800000u;  // -inf
+      x[i & 3] = fmaxf(x[i & 3], __uint_as_float(s[k][i]));
     }
-    const float most = fmaxf(x[0], x[1]);
-    if (most > -INFINITY) top = fmaxf(top, most * unit * powerOfTwo(info.keyExp[k]));
+    const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    if (most > -INFINITY) top = fmaxf(top, most * scale[k]);
   }
   return top;
 }
 
-// Second look: the weights, to TMEM in the place of the scores; returns their
-// sum.  off: minus the maximum; ref: the power of two that the outputs have.
-template <bool EDGE>
-__device__ __forceinline__ float tileWeights(uint32_t scores, const ChunkInfo& info, float unit, int left, float m, int ref) {
-  uint32_t s[2][32];
+// The weights of the scores, to TMEM in their place; returns their sum.  ref:
+// the power of two that the outputs have.
+__device__ __forceinline__ float tileWeights(const uint32_t (&s)[2][32], uint32_t scores, const ChunkInfo& info, const float (&scale)[2],
+                                             float m, int ref) {
   float sum = 0.0f;
-  tmemLoad32(scores, s[0]);
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    sm100::tmemLoadWait();
-    if (k < 3) tmemLoad32(scores + 32 * (k + 1), s[(k + 1) & 1]);
-    const uint32_t seen = EDGE ? seenOf(info.valid[k], left - 32 * k) : ~0u;
+  for (int k = 0; k < 2; k++) {
     const int ve = info.valueExp[k], shift = ve == kNoExponent ? 0 : max(ve - ref, -100);
-    const float scale = unit * powerOfTwo(info.keyExp[k]), off = static_cast<float>(shift) - m;
-    float part[2] = {0.0f, 0.0f};
+    const float off = static_cast<float>(shift) - m;
+    float part[4] = {};
     uint32_t w[16];
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-      float a = exp2Fast(fmaf(__uint_as_float(s[k & 1][2 * i]), scale, off));
-      float b = exp2Fast(fmaf(__uint_as_float(s[k & 1][2 * i + 1]), scale, off));
-      if (EDGE) {
-        if (!((seen >> (2 * i)) & 1u)) a = 0.0f;
-        if (!((seen >> (2 * i + 1)) & 1u)) b = 0.0f;
-      }
-      part[0] += a;
-      part[1] += b;
+      const float a = exp2Fast(fmaf(__uint_as_float(s[k][2 * i]), scale[k], off));
+      const float b = exp2Fast(fmaf(__uint_as_float(s[k][2 * i + 1]), scale[k], off));
+      part[2 * (i & 1)] += a;
+      part[2 * (i & 1) + 1] += b;
       w[i] = packHalf(a, b);
     }
-    sum = fmaf(part[0] + part[1], powerOfTwo(-shift), sum);
-    // Scores 32 (k + 1) on are under way or to come: the weights end before them.
+    sum = fmaf((part[0] + part[1]) + (part[2] + part[3]), powerOfTwo(-shift), sum);
     tmemStore16(scores + 16 * k, w);
   }
   return sum;
 }
 
+// Power of two of 32 tokens' keys or values: scaled by it, the largest is
+// below 2^13.  scale, mid: of the lane's token, finite or not a number.
+template <int G>
+__device__ __forceinline__ int exponentOf32(const float (&scale)[G], const float (&mid)[G], int none) {
+  float top = 0.0f;
+#pragma unroll
+  for (int g = 0; g < G; g++) top = fmaxf(top, fmaf(8.5f, fabsf(scale[g]), fabsf(mid[g])));
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  return top == 0.0f || !(top < INFINITY) ? none : max(exponentOf(top), -100) - 12;
+}
+
+// A token's row of codes with its parameters; a value thread has those of the
+// keys too (it writes down what the softmax needs of both).
 template <int G>
 struct RawToken {
-  uint32_t k[8 * G], v[8 * G], kp[G], vp[G];
+  uint32_t w[8 * G], params[G], keyParams[G];
   bool there;
 };
 
@@ -334,15 +338,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
+    for (int i = 0; i < kChunkStages; i++) {
+      sm100::mbarInit(&ctl.kFull[i], 64);
+      sm100::mbarInit(&ctl.kEmpty[i], 1);
+      sm100::mbarInit(&ctl.vFull[i], 64);
+      sm100::mbarInit(&ctl.vEmpty[i], 1);
+    }
     for (int i = 0; i < 2; i++) {
       sm100::mbarInit(&ctl.qFull[i], 128);
-      sm100::mbarInit(&ctl.kFull[i], 128);
-      sm100::mbarInit(&ctl.kEmpty[i], 1);
-      sm100::mbarInit(&ctl.vFull[i], 128);
-      sm100::mbarInit(&ctl.vEmpty[i], 1);
-      sm100::mbarInit(&ctl.sFull[i], 1);
-      sm100::mbarInit(&ctl.pFull[i], 128);
-      sm100::mbarInit(&ctl.oFull[i], 1);
+      sm100::mbarInit(&ctl.sFull[i][0], 1);
+      sm100::mbarInit(&ctl.sFull[i][1], 1);
+      sm100::mbarInit(&ctl.pFull[i][0], 128);
+      sm100::mbarInit(&ctl.pFull[i][1], 128);
+      sm100::mbarInit(&ctl.pvDone[i][0], 1);
+      sm100::mbarInit(&ctl.pvDone[i][1], 1);
     }
     sm100::mbarInit(&ctl.drain, 1);
     ctl.abort = 0;
@@ -378,115 +387,137 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
   if (warp < 8) {
     // ---------------- softmax ----------------
     const int t = warp >> 2, row = threadIdx.x & 127;
-    const uint32_t scores = tmem + t * 128 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t output = tmem + kOut + t * D + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    uint32_t seq = 0;               // tiles of keys of the block so far: the place of their info
-    uint32_t sCount = 0, oCount = 0;  // scores and outputs of this row tile so far
-    bool ok = true;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-      const ChunkUnit c = chunkUnit(p, starts, u);
-      if (t >= c.tiles) {
-        seq += c.upto - c.from;  // the info ring moves on
-        continue;
-      }
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t output = tmem + kOut + t * D + lanes;
+    uint32_t seq = 0;    // tiles of keys of the block so far: the place of their info
+    uint32_t count = 0;  // of those, the ones with this row tile
+    float unit = 1.0f;   // what a score counts in the base-2 logarithm
+    int limit = 0;       // keys that the row sees
+    // A unit's queries: the row's channels, scaled to 2^8, and their sums as
+    // the left operand.
+    auto loadQuery = [&](const ChunkUnit& c) {
       const long long mine = static_cast<long long>(c.row0) + t * 128 + row;
       const bool live = mine < static_cast<long long>(c.r.rows) * p.group;
       const int token = live ? static_cast<int>(mine / p.group) : 0, h = c.head * p.group + (live ? static_cast<int>(mine % p.group) : 0);
-      const int limit = live ? min(max(c.r.kv - c.r.rows + token + 1, 0), c.r.kv) : c.r.kv;
-      float m = kNone, l = 0.0f, unit = 1.0f;
+      limit = live ? min(max(c.r.kv - c.r.rows + token + 1, 0), c.r.kv) : c.r.kv;
+      float amax = 0.0f, sums[G] = {};
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + static_cast<long long>(c.r.start + token) * p.qTok + static_cast<long long>(h) * p.qHead;
+      uint4 raw[8 * G];
+#pragma unroll
+      for (int i = 0; i < 8 * G; i++) raw[i] = live ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 8 * G; i++) {
+        float x[8];
+        if (p.half16) unpack8<__half>(raw[i], x);
+        else unpack8<__nv_bfloat16>(raw[i], x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          amax = fmaxf(amax, fabsf(x[e]));
+          sums[i / 8] += x[e];
+        }
+      }
+      const int e = exponentOf(amax);
+      const bool plain = amax == 0.0f || e > 120 || e < -100;
+      const float f = (plain ? 1.0f : powerOfTwo(8 - e)) * (p.scaleLog2 < 0.0f ? -1.0f : 1.0f);
+      unit = (plain ? 1.0f : powerOfTwo(e - 8)) * fabsf(p.scaleLog2);
+#pragma unroll
+      for (int i = 0; i < 8 * G; i++) {
+        float x[8];
+        if (p.half16) unpack8<__half>(raw[i], x);
+        else unpack8<__nv_bfloat16>(raw[i], x);
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] *= f;
+        *reinterpret_cast<uint4*>(smem + L::kQ + (t * G + i / 8) * L::kQBlock + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = pack8<__half>(x);
+      }
+#pragma unroll
+      for (int g = 0; g < G; g++) sums[g] *= f;
+      storeSums<G, true>(smem + L::kQSums + t * (128 * 32), row, sums);
+      sm100::fenceProxyAsyncShared();
+      sm100::mbarArrive(&ctl.qFull[t]);
+    };
+    // The next unit with keys for this row tile, from unit u on; its queries
+    // are loaded as soon as the last scores of the unit before are there.
+    bool ok = true;
+    int u = blockIdx.x;
+    if (u < units) {
+      const ChunkUnit c = chunkUnit(p, starts, u);
+      if (t < c.tiles && c.from < c.upto) loadQuery(c);
+    }
+    for (; u < units && ok; u += gridDim.x) {
+      const ChunkUnit c = chunkUnit(p, starts, u);
+      const bool any = t < c.tiles && c.from < c.upto;
+      const int mineLimit = limit;
+      const float mineUnit = unit;
+      float m = kNone, l = 0.0f;
       int ref = kNoExponent;  // the outputs are in units of 2^ref
       uint32_t poison = 0;
-      if (c.from < c.upto) {
-        // The row's channels, scaled to 2^8, and their sums as the left operand.
-        float amax = 0.0f, sums[G] = {};
-        const uint16_t* src = static_cast<const uint16_t*>(p.q) + static_cast<long long>(c.r.start + token) * p.qTok + static_cast<long long>(h) * p.qHead;
-        uint4 raw[8 * G];
-#pragma unroll
-        for (int i = 0; i < 8 * G; i++) {
-          raw[i] = live ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
-          float x[8];
-          if (p.half16) unpack8<__half>(raw[i], x);
-          else unpack8<__nv_bfloat16>(raw[i], x);
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            amax = fmaxf(amax, fabsf(x[e]));
-            sums[i / 8] += x[e];
-          }
-        }
-        const int e = exponentOf(amax);
-        const bool plain = amax == 0.0f || e > 120 || e < -100;
-        const float f = (plain ? 1.0f : powerOfTwo(8 - e)) * (p.scaleLog2 < 0.0f ? -1.0f : 1.0f);
-        unit = (plain ? 1.0f : powerOfTwo(e - 8)) * fabsf(p.scaleLog2);
-#pragma unroll
-        for (int i = 0; i < 8 * G; i++) {
-          float x[8];
-          if (p.half16) unpack8<__half>(raw[i], x);
-          else unpack8<__nv_bfloat16>(raw[i], x);
-#pragma unroll
-          for (int k = 0; k < 8; k++) x[k] *= f;
-          *reinterpret_cast<uint4*>(smem + L::kQ + (t * G + i / 8) * L::kBlock + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = pack8<__half>(x);
-        }
-#pragma unroll
-        for (int g = 0; g < G; g++) sums[g] *= f;
-        storeSums<G, true>(smem + L::kQSums + t * kPlainBytes, row, sums);
-        sm100::fenceProxyAsyncShared();
-        sm100::mbarArrive(&ctl.qFull[t]);
-        for (int j = c.from; j < c.upto; j++, seq++) {
-          if (!warpWait(&ctl.sFull[t], sCount & 1u, abortFlag)) {
-            ok = false;
-            break;
-          }
-          sCount++;
+      if (!any) {
+        seq += c.upto - c.from;
+      } else {
+        for (int j = c.from; j < c.upto; j++, seq++, count++) {
+          const uint32_t scores = tmem + t * 128 + (count & 1) * 64 + lanes;
+          ok = warpWait(&ctl.sFull[t][count & 1], (count >> 1) & 1u, abortFlag) &&
+               warpWait(&ctl.vFull[seq & 3], (seq >> 2) & 1u, abortFlag);
+          if (!ok) break;
           sm100::tcFenceAfter();
+          uint32_t s[2][32];
+          tmemLoad32(scores, s[0]);
+          tmemLoad32(scores + 32, s[1]);
           const ChunkInfo& info = ctl.info[seq & 3];
-          const int left = limit - j * kChunkKeys;  // keys of the tile in the row's range
-          const uint32_t valid = info.valid[0] & info.valid[1] & info.valid[2] & info.valid[3];
-          const bool edge = __any_sync(~0u, left < kChunkKeys || valid != ~0u);
-          int newRef = ref;
-#pragma unroll
-          for (int k = 0; k < 4; k++) newRef = max(newRef, info.valueExp[k]);
-          const float top = edge ? tileMaximum<true>(scores, info, unit, left) : tileMaximum<false>(scores, info, unit, left);
+          const int left = mineLimit - j * kChunkKeys;  // keys of the tile in the row's range
+          const bool edge = __any_sync(~0u, left < kChunkKeys || (info.valid[0] & info.valid[1]) != ~0u);
+          const int newRef = max(ref, max(info.valueExp[0], info.valueExp[1]));
+          const float scale[2] = {mineUnit * powerOfTwo(info.keyExp[0]), mineUnit * powerOfTwo(info.keyExp[1])};
+          sm100::tmemLoadWait();
+          const float top = edge ? tileMaximum<true>(s, info, scale, left) : tileMaximum<false>(s, info, scale, left);
           if (__any_sync(~0u, top > m + 8.0f || newRef > ref)) {
             const float next = fmaxf(m, top), shrink = exp2Fast(m - next);
             if (j > c.from) {
+              // the products with the weights before these have ended
+              ok = warpWait(&ctl.pvDone[t][(count - 1) & 1], ((count - 1) >> 1) & 1u, abortFlag);
+              if (!ok) break;
+              sm100::tcFenceAfter();
               const float factor = shrink * (ref == kNoExponent ? 1.0f : powerOfTwo(max(ref - newRef, -126)));
 #pragma unroll 1
-              for (int k = 0; k < D / 32; k++) {
-                uint32_t o[32];
-                tmemLoad32(output + 32 * k, o);
+              for (int k = 0; k < D / 16; k++) {
+                uint32_t o[16];
+                sm100::tmemLoad16(output + 16 * k, o);
                 sm100::tmemLoadWait();
 #pragma unroll
-                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                tmemStore32(output + 32 * k, o);
+                for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                tmemStore16(output + 16 * k, o);
               }
-              tmemStoreWait();
             }
             l *= shrink;
             m = next;
             ref = newRef;
           }
-          l += edge ? tileWeights<true>(scores, info, unit, left, m, ref) : tileWeights<false>(scores, info, unit, left, m, ref);
+          l += tileWeights(s, scores, info, scale, m, ref);
 #pragma unroll
           for (int g = 0; g < G; g++)
 #pragma unroll
-            for (int k = 0; k < 4; k++)
+            for (int k = 0; k < 2; k++)
               if (info.bad[g][k] & seenOf(info.valid[k], left - 32 * k)) poison |= 1u << g;
           tmemStoreWait();
           sm100::tcFenceBefore();
-          sm100::mbarArrive(&ctl.pFull[t]);
+          sm100::mbarArrive(&ctl.pFull[t][count & 1]);
         }
+      }
+      if (!ok) break;
+      if (u + gridDim.x < units) {
+        const ChunkUnit next = chunkUnit(p, starts, u + gridDim.x);
+        if (t < next.tiles && next.from < next.upto) loadQuery(next);
       }
       // The result, or this share of it.
-      const bool any = c.from < c.upto;
-      if (!ok || (!any && p.splits > 1)) continue;  // an empty share counts as absent
+      if (t >= c.tiles || (!any && p.splits > 1)) continue;  // an empty share counts as absent
       if (any) {
-        if (!warpWait(&ctl.oFull[t], oCount & 1u, abortFlag)) {
-          ok = false;
-          continue;
-        }
-        oCount++;
+        ok = warpWait(&ctl.pvDone[t][(count - 1) & 1], ((count - 1) >> 1) & 1u, abortFlag);
+        if (!ok) break;
         sm100::tcFenceAfter();
       }
+      const long long mine = static_cast<long long>(c.row0) + t * 128 + row;
+      const bool live = mine < static_cast<long long>(c.r.rows) * p.group;
+      const int token = live ? static_cast<int>(mine / p.group) : 0, h = c.head * p.group + (live ? static_cast<int>(mine % p.group) : 0);
       const bool whole = p.splits == 1, none = l == 0.0f;
       const float factor = (whole ? (none ? 0.0f : 1.0f / l) : 1.0f) * (ref == kNoExponent ? 1.0f : powerOfTwo(ref));
       const long long slot = static_cast<long long>(u) * kChunkRows + t * 128 + row;
@@ -525,8 +556,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
     }
   } else if (warp < 12) {
     // ---------------- codes to f16 ----------------
-    const int tid = threadIdx.x - 256, w = warp - 8;
-    // The tile whose page number is under way: two tiles ahead of the one that is turned.
+    const bool keys = warp < 10;
+    const int tid = threadIdx.x & 63, w = warp & 1;
+    // The tile after next: its token's page number is under way.
     int u = blockIdx.x, j = 0, upto = 0, head = 0, kv = 0;
     const int* pages = nullptr;
     bool exists = false;
@@ -552,34 +584,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
     };
     auto fetch = [&](RawToken<G>& r) {
       r.there = exists && page >= 0 && page < p.pages;
-      if (r.there) {
-        const int place = token % (p.blocksPerPage * 16);
-        const uint8_t* block = p.cache + ((static_cast<long long>(page) * p.kvHeads + head) * p.blocksPerPage + (place >> 4)) * (18 * D);
-        const int at = place & 15;
-        const uint4* k = reinterpret_cast<const uint4*>(block + at * (D / 2));
-        const uint4* v = reinterpret_cast<const uint4*>(block + 8 * D + kv4::valueRow(at) * (D / 2));
+      const int place = token % (p.blocksPerPage * 16), at = place & 15;
+      const uint8_t* block = p.cache + ((static_cast<long long>(r.there ? page : 0) * p.kvHeads + head) * p.blocksPerPage + (place >> 4)) * (18 * D);
+      const uint4* codes = reinterpret_cast<const uint4*>(block + (keys ? at : 16 + kv4::valueRow(at)) * (D / 2));
 #pragma unroll
-        for (int i = 0; i < 2 * G; i++) {
-          const uint4 a = __ldg(k + i), b = __ldg(v + i);
-          r.k[4 * i] = a.x;
-          r.k[4 * i + 1] = a.y;
-          r.k[4 * i + 2] = a.z;
-          r.k[4 * i + 3] = a.w;
-          r.v[4 * i] = b.x;
-          r.v[4 * i + 1] = b.y;
-          r.v[4 * i + 2] = b.z;
-          r.v[4 * i + 3] = b.w;
-        }
+      for (int i = 0; i < 2 * G; i++) {
+        uint4 a = make_uint4(0, 0, 0, 0);  // codes of 0 with nothing to scale
+        if (r.there) a = __ldg(codes + i);
+        r.w[4 * i] = a.x;
+        r.w[4 * i + 1] = a.y;
+        r.w[4 * i + 2] = a.z;
+        r.w[4 * i + 3] = a.w;
+      }
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-          r.kp[g] = __ldg(reinterpret_cast<const uint32_t*>(block + 16 * D + at * (4 * G)) + g);
-          r.vp[g] = __ldg(reinterpret_cast<const uint32_t*>(block + 17 * D + at * (4 * G)) + g);
-        }
-      } else {  // zeros: codes of 0 with nothing to scale
-#pragma unroll
-        for (int i = 0; i < 8 * G; i++) r.k[i] = r.v[i] = 0;
-#pragma unroll
-        for (int g = 0; g < G; g++) r.kp[g] = r.vp[g] = 0;
+      for (int g = 0; g < G; g++) {
+        r.keyParams[g] = r.there ? __ldg(reinterpret_cast<const uint32_t*>(block + 16 * D + at * (4 * G)) + g) : 0;
+        r.params[g] = r.there && !keys ? __ldg(reinterpret_cast<const uint32_t*>(block + 17 * D + at * (4 * G)) + g) : 0;
       }
     };
     RawToken<G> raw, next;
@@ -591,119 +611,134 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       const bool follows = exists;
       fetch(next);
       if (exists) advance();
-      // Parameters of the 32 tokens of this warp, and their powers of two.
-      float ks[G], km[G], vs[G], vm[G], kTop = 0.0f, vTop = 0.0f;
-      ChunkInfo& info = ctl.info[seq & 3];
+      const int st = seq & 3;
+      const uint32_t parity = ((seq >> 2) & 1u) ^ 1u;
+      float s[G], m[G];
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        ks[g] = kv4::bf16Lo(raw.kp[g]);
-        km[g] = kv4::bf16Hi(raw.kp[g]);
-        vs[g] = kv4::bf16Lo(raw.vp[g]);
-        vm[g] = kv4::bf16Hi(raw.vp[g]);
-        const bool bad = !(isfinite(vs[g]) && isfinite(vm[g]));
-        if (bad) vs[g] = vm[g] = 0.0f;
-        const uint32_t whose = __ballot_sync(~0u, bad);
-        if (lane == 0) info.bad[g][w] = whose;
-        kTop = fmaxf(kTop, fmaf(8.5f, fabsf(ks[g]), fabsf(km[g])));
-        vTop = fmaxf(vTop, fmaf(8.5f, fabsf(vs[g]), fabsf(vm[g])));
+        s[g] = kv4::bf16Lo(raw.keyParams[g]);
+        m[g] = kv4::bf16Hi(raw.keyParams[g]);
       }
+      const int ke = exponentOf32<G>(s, m, 0);
+      if (keys) {
+        const float f = powerOfTwo(-ke);
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        kTop = fmaxf(kTop, __shfl_xor_sync(~0u, kTop, o));
-        vTop = fmaxf(vTop, __shfl_xor_sync(~0u, vTop, o));
-      }
-      const int ke = kTop == 0.0f || !(kTop < INFINITY) ? 0 : max(exponentOf(kTop), -100) - 12;
-      const int ve = vTop == 0.0f ? kNoExponent : max(exponentOf(vTop), -100) - 12;
-      const uint32_t there = __ballot_sync(~0u, raw.there);
-      if (lane == 0) {
-        info.valid[w] = there;
-        info.keyExp[w] = ke;
-        info.valueExp[w] = ve;
-      }
-      const float kf = powerOfTwo(-ke), vf = ve == kNoExponent ? 1.0f : powerOfTwo(-ve);
+        for (int g = 0; g < G; g++) {
+          s[g] *= f;
+          m[g] = fmaf(0.5f, s[g], m[g] * f);  // value = m + s (code - 8) from here on
+        }
+        if (!warpWait(&ctl.kEmpty[st], parity, abortFlag)) break;
+        widen<G, true>(raw.w, s, m, smem + L::kK + st * G * L::kBlock, tid);
+        storeSums<G, false>(smem + L::kKSums + st * (64 * 32), tid, m);
+        sm100::fenceProxyAsyncShared();
+        sm100::mbarArrive(&ctl.kFull[st]);
+      } else {
+        uint32_t bad[G];
 #pragma unroll
-      for (int g = 0; g < G; g++) {
-        ks[g] *= kf;
-        km[g] = fmaf(0.5f, ks[g], km[g] * kf);  // value = m + s (code - 8) from here on
-        vs[g] *= vf;
-        vm[g] = fmaf(0.5f, vs[g], vm[g] * vf);
+        for (int g = 0; g < G; g++) {
+          s[g] = kv4::bf16Lo(raw.params[g]);
+          m[g] = kv4::bf16Hi(raw.params[g]);
+          const bool not_finite = !(isfinite(s[g]) && isfinite(m[g]));
+          if (not_finite) s[g] = m[g] = 0.0f;
+          bad[g] = __ballot_sync(~0u, not_finite);
+        }
+        const int ve = exponentOf32<G>(s, m, kNoExponent);
+        const float f = ve == kNoExponent ? 1.0f : powerOfTwo(-ve);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          s[g] *= f;
+          m[g] = fmaf(0.5f, s[g], m[g] * f);
+        }
+        const uint32_t present = __ballot_sync(~0u, raw.there);
+        if (!warpWait(&ctl.vEmpty[st], parity, abortFlag)) break;
+        if (lane == 0) {  // what was there is read: its weights have been used
+          ChunkInfo& info = ctl.info[st];
+          info.valid[w] = present;
+          info.keyExp[w] = ke;
+          info.valueExp[w] = ve;
+#pragma unroll
+          for (int g = 0; g < G; g++) info.bad[g][w] = bad[g];
+        }
+        widen<G, false>(raw.w, s, m, smem + L::kV + st * G * L::kBlock, tid);
+        sm100::fenceProxyAsyncShared();
+        sm100::mbarArrive(&ctl.vFull[st]);
       }
-      const int st = seq & 1;
-      const uint32_t parity = ((seq >> 1) & 1u) ^ 1u;
-      if (!warpWait(&ctl.kEmpty[st], parity, abortFlag)) break;
-      widen<G, true>(raw.k, ks, km, smem + L::kK + st * G * L::kBlock, tid);
-      storeSums<G, false>(smem + L::kKSums + st * kPlainBytes, tid, km);
-      sm100::fenceProxyAsyncShared();
-      sm100::mbarArrive(&ctl.kFull[st]);
-      if (!warpWait(&ctl.vEmpty[st], parity, abortFlag)) break;
-      widen<G, false>(raw.v, vs, vm, smem + L::kV + st * G * L::kBlock, tid);
-      sm100::fenceProxyAsyncShared();
-      sm100::mbarArrive(&ctl.vFull[st]);
       raw = next;
       here = follows;
     }
   } else if (lane == 0) {
     // ---------------- products ----------------
-    constexpr uint32_t kScores = idescF16(128, 128, false), kOutputs = idescF16(128, D, true);
-    const uint32_t qSums = sm100::smemAddr(smem + L::kQSums), kSums = sm100::smemAddr(smem + L::kKSums);
-    const uint32_t qBase = sm100::smemAddr(smem + L::kQ), kBase = sm100::smemAddr(smem + L::kK), vBase = sm100::smemAddr(smem + L::kV);
-    uint32_t seq = 0, qCount[2] = {0, 0}, pCount[2] = {0, 0};
-    bool ok = true;
+    constexpr uint32_t kScores = idescF16(128, kChunkKeys, false), kOutputs = idescF16(128, D, true);
     // Words of the descriptors: addresses count 16 bytes.
     const uint64_t rows = sm100::smemDescSw128(0), plain = smemDescPlain(0), major = smemDescMn(0);
-    const uint32_t rowsLo = static_cast<uint32_t>(rows), rowsHi = static_cast<uint32_t>(rows >> 32);
-    const uint32_t plainLo = static_cast<uint32_t>(plain), plainHi = static_cast<uint32_t>(plain >> 32);
-    const uint32_t majorLo = static_cast<uint32_t>(major), majorHi = static_cast<uint32_t>(major >> 32);
-    constexpr uint32_t kStep = L::kBlock >> 4;
-    auto issueScores = [&](int t, uint32_t s) {
-      const uint32_t d = tmem + t * 128, q = rowsLo + (qBase >> 4) + t * (G * kStep), k = rowsLo + (kBase >> 4) + (s & 1) * (G * kStep);
+    const uint32_t rowsHi = static_cast<uint32_t>(rows >> 32), plainHi = static_cast<uint32_t>(plain >> 32), majorHi = static_cast<uint32_t>(major >> 32);
+    const uint32_t base = sm100::smemAddr(smem) >> 4;
+    const uint32_t qLo = static_cast<uint32_t>(rows) + base + (L::kQ >> 4), kLo = static_cast<uint32_t>(rows) + base + (L::kK >> 4);
+    const uint32_t vLo = static_cast<uint32_t>(major) + base + (L::kV >> 4);
+    const uint32_t qsLo = static_cast<uint32_t>(plain) + base + (L::kQSums >> 4), ksLo = static_cast<uint32_t>(plain) + base + (L::kKSums >> 4);
+    constexpr uint32_t kQStep = L::kQBlock >> 4, kStep = L::kBlock >> 4;
+    uint32_t seq = 0, qCount[2] = {0, 0}, sCount[2] = {0, 0}, pCount[2] = {0, 0};
+    bool ok = true;
+    auto issueScores = [&](int t, uint32_t st) {
+      const uint32_t d = tmem + t * 128 + (sCount[t] & 1) * 64, q = qLo + t * (G * kQStep), k = kLo + st * (G * kStep);
       mmaF16<false>(d, q, rowsHi, k, rowsHi, kScores);
 #pragma unroll
       for (int i = 1; i < 4 * G; i++)
-        mmaF16<true>(d, q + (i >> 2) * kStep + 2 * (i & 3), rowsHi, k + (i >> 2) * kStep + 2 * (i & 3), rowsHi, kScores);
-      mmaF16<true>(d, plainLo + (qSums >> 4) + t * (kPlainBytes >> 4), plainHi, plainLo + (kSums >> 4) + (s & 1) * (kPlainBytes >> 4),
-                   plainHi, kScores);
-      sm100::mmaCommit(&ctl.sFull[t]);
+        mmaF16<true>(d, q + (i >> 2) * kQStep + 2 * (i & 3), rowsHi, k + (i >> 2) * kStep + 2 * (i & 3), rowsHi, kScores);
+      mmaF16<true>(d, qsLo + t * (128 * 32 >> 4), plainHi, ksLo + st * (64 * 32 >> 4), plainHi, kScores);
+      sm100::mmaCommit(&ctl.sFull[t][sCount[t] & 1]);
+      sCount[t]++;
     };
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const ChunkUnit c = chunkUnit(p, starts, u);
       const int n = c.upto - c.from;
       if (n <= 0) continue;
-      for (int t = 0; t < c.tiles && ok; t++) ok = sm100::mbarWait(&ctl.qFull[t], qCount[t]++ & 1u, abortFlag);
-      ok = ok && sm100::mbarWait(&ctl.kFull[seq & 1], (seq >> 1) & 1u, abortFlag);
-      if (!ok) break;
-      sm100::tcFenceAfter();
-      for (int t = 0; t < c.tiles; t++) issueScores(t, seq);
-      sm100::mmaCommit(&ctl.kEmpty[seq & 1]);
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+        if (t < c.tiles && ok) ok = sm100::mbarWait(&ctl.qFull[t], qCount[t]++ & 1u, abortFlag);
+      for (int i = 0; i < 2 && i < n && ok; i++) {
+        const uint32_t s = seq + i;
+        ok = sm100::mbarWait(&ctl.kFull[s & 3], (s >> 2) & 1u, abortFlag);
+        if (!ok) break;
+        sm100::tcFenceAfter();
+        issueScores(0, s & 3);
+        if (c.tiles > 1) issueScores(1, s & 3);
+        sm100::mmaCommit(&ctl.kEmpty[s & 3]);
+      }
       for (int j = 0; j < n && ok; j++, seq++) {
-        for (int t = 0; t < c.tiles; t++) {
-          ok = sm100::mbarWait(&ctl.pFull[t], pCount[t]++ & 1u, abortFlag);
-          if (ok && t == 0) ok = sm100::mbarWait(&ctl.vFull[seq & 1], (seq >> 1) & 1u, abortFlag);
+        const uint32_t st = seq & 3, far = (seq + 2) & 3;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          if (t >= c.tiles || !ok) break;
+          const uint32_t place = pCount[t] & 1, weights = tmem + t * 128 + place * 64;
+          ok = sm100::mbarWait(&ctl.pFull[t][place], (pCount[t] >> 1) & 1u, abortFlag);
+          pCount[t]++;
+          if (ok && t == 0) ok = sm100::mbarWait(&ctl.vFull[st], (seq >> 2) & 1u, abortFlag);
           if (!ok) break;
           sm100::tcFenceAfter();
 #pragma unroll
-          for (int k = 0; k < 8; k++)
-            mmaF16Tmem(tmem + kOut + t * D, tmem + t * 128 + 8 * k, majorLo + (vBase >> 4) + (seq & 1) * (G * kStep) + 128 * k, majorHi,
-                       kOutputs, k > 0 ? 1u : static_cast<uint32_t>(j));
-          if (j + 1 == n) sm100::mmaCommit(&ctl.oFull[t]);
-          if (t + 1 == c.tiles) sm100::mmaCommit(&ctl.vEmpty[seq & 1]);
-          if (j + 1 < n) {
+          for (int k = 0; k < kChunkKeys / 16; k++)
+            mmaF16Tmem(tmem + kOut + t * D, weights + 8 * k, vLo + st * (G * kStep) + 128 * k, majorHi, kOutputs,
+                       k > 0 ? 1u : static_cast<uint32_t>(j));
+          sm100::mmaCommit(&ctl.pvDone[t][place]);
+          if (t + 1 == c.tiles) sm100::mmaCommit(&ctl.vEmpty[st]);
+          if (j + 2 < n) {
             if (t == 0) {
-              ok = sm100::mbarWait(&ctl.kFull[(seq + 1) & 1], ((seq + 1) >> 1) & 1u, abortFlag);
+              ok = sm100::mbarWait(&ctl.kFull[far], ((seq + 2) >> 2) & 1u, abortFlag);
               if (!ok) break;
               sm100::tcFenceAfter();
             }
-            issueScores(t, seq + 1);
-            if (t + 1 == c.tiles) sm100::mmaCommit(&ctl.kEmpty[(seq + 1) & 1]);
+            issueScores(t, far);
+            if (t + 1 == c.tiles) sm100::mmaCommit(&ctl.kEmpty[far]);
           }
         }
       }
     }
-    if (!ok) {  // let the products that were issued end before the block does
-      sm100::mmaCommit(&ctl.drain);
-      volatile int never = 0;
-      sm100::mbarWait(&ctl.drain, 0, &never, 200000000ull);
-    }
+    // Every product and arrival that was issued ends before the block does:
+    // the barriers' memory is the next block's.
+    sm100::mmaCommit(&ctl.drain);
+    volatile int never = 0;
+    sm100::mbarWait(&ctl.drain, 0, &never, 200000000ull);
   }
   __syncwarp();
   sm100::tcFenceBefore();
