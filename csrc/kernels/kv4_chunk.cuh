@@ -3,15 +3,17 @@
 // generation tensor cores (included by kv4_attention.cu).
 //
 // A unit is 256 query rows (two tiles of 128) of one request and key head
-// against a range of keys, 64 at a time.  Roles of a block of 13 warps:
+// against a range of keys, 64 at a time.  Roles of a block of 14 warps:
 //   warps 0-3, 4-7  softmax of the first and the second row tile, a thread a
 //                   row: scores from TMEM, weights back to TMEM as f16, in
 //                   the place of the scores;
 //   warps 8-9       a thread a token: key codes from global memory (one tile
 //   10-11           ahead in registers) to f16 in shared memory, in the
 //                   128-byte swizzle that the products read; value codes;
-//   warp 12         one thread issues S = Q K^T (N = 64) and O += P V (P from
-//                   TMEM, V with channels as the major axis).
+//   warps 12, 13    issue S = Q K^T (N = 64) and O += P V (P from TMEM, V with
+//                   channels as the major axis) of a row tile each: one thread
+//                   for both took 80 to 100 clocks a product, more than the
+//                   tensor cores do.
 // A row tile has two places for scores, so the products of the keys after next
 // go on beside the softmax of these (with 128 keys and one place the softmax
 // waited 1700 of 7800 clocks for its scores, and read them twice for want of
@@ -41,8 +43,8 @@ namespace {
 constexpr int kChunkRows = 256;
 constexpr int kChunkKeys = 64;
 constexpr int kChunkStages = 4;     // tiles of keys, and of values, in shared memory
-constexpr int kChunkThreads = 13 * 32;
-constexpr int kNoExponent = -1000;  // of 32 tokens that are all zero
+constexpr int kChunkThreads = 14 * 32;
+constexpr int kLeastExponent = -112;  // of 32 tokens that are all zero, or next to it
 
 // 32 lanes x 32 bit, 32 consecutive columns per thread.
 __device__ __forceinline__ void tmemLoad32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -163,10 +165,12 @@ struct ChunkSmem {
 };
 
 // What the tokens of a tile bring, by 32.
-struct ChunkInfo {
-  uint32_t valid[2];   // the token is there
-  uint32_t bad[2][2];  // its values of a group are not finite (and zero in the product)
-  int keyExp[2], valueExp[2];
+struct alignas(16) ChunkInfo {
+  uint32_t valid[2];               // the token is there
+  float keyUnit[2];                // the power of two that its keys are divided by
+  float valueExp[2];               // the logarithm of that of its values
+  uint32_t pad[2];
+  uint32_t bad[2][2];              // its values of a group are not finite (and zero in the product)
 };
 
 struct ChunkControl {
@@ -174,7 +178,7 @@ struct ChunkControl {
   uint64_t kFull[kChunkStages], kEmpty[kChunkStages], vFull[kChunkStages], vEmpty[kChunkStages];
   // A wait tells a phase of a barrier from the one before it alone, so what
   // can be two tiles ahead has a barrier for each place.
-  uint64_t qFull[2], sFull[2][2], pFull[2][2], pvDone[2][2], drain;
+  uint64_t qFull[2], sFull[2][2], pFull[2][2], pvDone[2][2], drain[2];
   uint32_t tmem;
   int abort;
 };
@@ -253,6 +257,7 @@ __device__ __forceinline__ void widen(const uint32_t (&w)[8 * G], const float (&
 
 // A wait of a whole warp: every lane goes on, or none does.
 __device__ __forceinline__ bool warpWait(uint64_t* bar, uint32_t parity, volatile int* abortFlag) {
+  if (__all_sync(~0u, sm100::mbarTryWait(bar, parity))) return true;
   return __all_sync(~0u, sm100::mbarWait(bar, parity, abortFlag));
 }
 
@@ -262,13 +267,14 @@ __device__ __forceinline__ uint32_t seenOf(uint32_t valid, int left) {
 }
 
 // The maximum of a row's scores over the keys that it sees, in the base-2
-// logarithm.  EDGE: some row of the warp does not see some key.
+// logarithm; the others become -inf.  EDGE: some row of the warp does not see
+// some key.
 template <bool EDGE>
-__device__ __forceinline__ float tileMaximum(uint32_t (&s)[2][32], const ChunkInfo& info, const float (&scale)[2], int left) {
+__device__ __forceinline__ float tileMaximum(uint32_t (&s)[2][32], const uint2& valid, const float (&scale)[2], int left) {
   float top = kNone;
 #pragma unroll
   for (int k = 0; k < 2; k++) {
-    const uint32_t seen = EDGE ? seenOf(info.valid[k], left - 32 * k) : ~0u;
+    const uint32_t seen = EDGE ? seenOf(k ? valid.y : valid.x, left - 32 * k) : ~0u;
     float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < 32; i++) {
@@ -276,46 +282,92 @@ __device__ __forceinline__ float tileMaximum(uint32_t (&s)[2][32], const ChunkIn
       x[i & 3] = fmaxf(x[i & 3], __uint_as_float(s[k][i]));
     }
     const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    if (most > -INFINITY) top = fmaxf(top, most * scale[k]);
+    if (!EDGE || most > -INFINITY) top = fmaxf(top, most * scale[k]);
   }
   return top;
 }
 
-// The weights of the scores, to TMEM in their place; returns their sum.  ref:
-// the power of two that the outputs have.
-__device__ __forceinline__ float tileWeights(const uint32_t (&s)[2][32], uint32_t scores, const ChunkInfo& info, const float (&scale)[2],
-                                             float m, int ref) {
-  float sum = 0.0f;
+// The weights of 32 scores, to TMEM in their place; returns their sum.
+__device__ __forceinline__ float halfWeights(const uint32_t (&s)[32], uint32_t at, float scale, float off) {
+  float part[4] = {};
+  uint32_t w[16];
 #pragma unroll
-  for (int k = 0; k < 2; k++) {
-    const int ve = info.valueExp[k], shift = ve == kNoExponent ? 0 : max(ve - ref, -100);
-    const float off = static_cast<float>(shift) - m;
-    float part[4] = {};
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const float a = exp2Fast(fmaf(__uint_as_float(s[k][2 * i]), scale[k], off));
-      const float b = exp2Fast(fmaf(__uint_as_float(s[k][2 * i + 1]), scale[k], off));
-      part[2 * (i & 1)] += a;
-      part[2 * (i & 1) + 1] += b;
-      w[i] = packHalf(a, b);
-    }
-    sum = fmaf((part[0] + part[1]) + (part[2] + part[3]), powerOfTwo(-shift), sum);
-    tmemStore16(scores + 16 * k, w);
+  for (int i = 0; i < 16; i++) {
+    const float a = exp2Fast(fmaf(__uint_as_float(s[2 * i]), scale, off));
+    const float b = exp2Fast(fmaf(__uint_as_float(s[2 * i + 1]), scale, off));
+    part[2 * (i & 1)] += a;
+    part[2 * (i & 1) + 1] += b;
+    w[i] = packHalf(a, b);
   }
-  return sum;
+  tmemStore16(at, w);
+  return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// Power of two of 32 tokens' keys or values: scaled by it, the largest is
-// below 2^13.  scale, mid: of the lane's token, finite or not a number.
+// What a softmax thread keeps of its row.
+struct RowState {
+  float m, l;      // maximum followed loosely (base-2 logarithm), sum
+  float ref;       // the outputs are in units of 2^ref
+  uint32_t poison; // groups whose values are not finite
+};
+
+// One tile's scores to weights.  Returns false if a wait ran out.
+template <int G, bool EDGE>
+__device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32_t output, const ChunkInfo& info, const uint2& valid,
+                                            float unit, int left, bool first, uint64_t* before, uint32_t beforeParity,
+                                            volatile int* abortFlag) {
+  constexpr int D = 64 * G;
+  uint32_t s[2][32];
+  tmemLoad32(scores, s[0]);
+  tmemLoad32(scores + 32, s[1]);
+  const float2 keyUnit = *reinterpret_cast<const float2*>(info.keyUnit), valueExp = *reinterpret_cast<const float2*>(info.valueExp);
+  const uint4 bad = *reinterpret_cast<const uint4*>(info.bad);
+  const float scale[2] = {unit * keyUnit.x, unit * keyUnit.y};
+  const float ref = fmaxf(r.ref, fmaxf(valueExp.x, valueExp.y));
+  sm100::tmemLoadWait();
+  const float top = tileMaximum<EDGE>(s, valid, scale, left);
+  if (__any_sync(~0u, top > r.m + 8.0f || ref > r.ref)) {
+    const float next = fmaxf(r.m, top), shrink = exp2Fast(r.m - next);
+    if (!first) {
+      // the products with the weights before these have ended
+      if (!warpWait(before, beforeParity, abortFlag)) return false;
+      sm100::tcFenceAfter();
+      const float factor = shrink * exp2Fast(r.ref - ref);
+#pragma unroll 1
+      for (int k = 0; k < D / 16; k++) {
+        uint32_t o[16];
+        sm100::tmemLoad16(output + 16 * k, o);
+        sm100::tmemLoadWait();
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+        tmemStore16(output + 16 * k, o);
+      }
+    }
+    r.l *= shrink;
+    r.m = next;
+    r.ref = ref;
+  }
+  // Weights of values in smaller units are smaller; 2^100 apart they vanish.
+  const float shift0 = fmaxf(valueExp.x - r.ref, -100.0f), shift1 = fmaxf(valueExp.y - r.ref, -100.0f);
+  const float sum0 = halfWeights(s[0], scores, scale[0], shift0 - r.m);
+  const float sum1 = halfWeights(s[1], scores + 16, scale[1], shift1 - r.m);
+  r.l = fmaf(sum0, exp2Fast(-shift0), fmaf(sum1, exp2Fast(-shift1), r.l));
+  if ((bad.x | bad.y | bad.z | bad.w) != 0) {
+    const uint32_t seen0 = seenOf(valid.x, left), seen1 = seenOf(valid.y, left - 32);
+    if ((bad.x & seen0) | (bad.y & seen1)) r.poison |= 1u;
+    if ((bad.z & seen0) | (bad.w & seen1)) r.poison |= 2u;
+  }
+  return true;
+}
+
+// Logarithm of the power of two of 32 tokens' keys or values: divided by it,
+// the largest is below 2^13.  scale, mid: of the lane's token.
 template <int G>
-__device__ __forceinline__ int exponentOf32(const float (&scale)[G], const float (&mid)[G], int none) {
+__device__ __forceinline__ int exponentOf32(const float (&scale)[G], const float (&mid)[G]) {
   float top = 0.0f;
 #pragma unroll
   for (int g = 0; g < G; g++) top = fmaxf(top, fmaf(8.5f, fabsf(scale[g]), fabsf(mid[g])));
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-  return top == 0.0f || !(top < INFINITY) ? none : max(exponentOf(top), -100) - 12;
+  // positive floats are ordered like their bits
+  return max(exponentOf(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top)))) - 12, kLeastExponent);
 }
 
 // A token's row of codes with its parameters; a value thread has those of the
@@ -325,6 +377,97 @@ struct RawToken {
   uint32_t w[8 * G], params[G], keyParams[G];
   bool there;
 };
+
+// The products of row tile T, by one warp: all of it waits, one thread issues.
+// The block has all 512 columns of TMEM, from column 0 on, so places in it are
+// constants.
+template <int G, int T>
+__device__ __forceinline__ void issueProducts(const AttnArgs& p, const int* starts, int units, const uint8_t* smem, ChunkControl& ctl) {
+  constexpr int D = 64 * G;
+  using L = ChunkSmem<G>;
+  constexpr uint32_t kScores = idescF16(128, kChunkKeys, false), kOutputs = idescF16(128, D, true);
+  constexpr uint32_t kQStep = L::kQBlock >> 4, kStep = L::kBlock >> 4;
+  volatile int* abortFlag = &ctl.abort;
+  // Words of the descriptors: addresses count 16 bytes.
+  const uint64_t rows = sm100::smemDescSw128(0), plain = smemDescPlain(0), major = smemDescMn(0);
+  const uint32_t rowsHi = static_cast<uint32_t>(rows >> 32), plainHi = static_cast<uint32_t>(plain >> 32), majorHi = static_cast<uint32_t>(major >> 32);
+  const uint32_t base = sm100::smemAddr(smem) >> 4;
+  const uint32_t q = static_cast<uint32_t>(rows) + base + (L::kQ >> 4) + T * G * kQStep;
+  const uint32_t qSums = static_cast<uint32_t>(plain) + base + (L::kQSums >> 4) + T * (128 * 32 >> 4);
+  uint32_t seq = 0, qCount = 0, sCount = 0, pCount = 0;
+  // Scores of the keys in a stage, to the place that is free.
+  auto issueScores = [&](uint32_t st) {
+    const uint32_t d = T * 128 + (sCount & 1) * 64;
+    const uint32_t k = static_cast<uint32_t>(rows) + base + (L::kK >> 4) + st * (G * kStep);
+    const uint32_t kSums = static_cast<uint32_t>(plain) + base + (L::kKSums >> 4) + st * (64 * 32 >> 4);
+    if (sm100::electOne()) {
+      mmaF16<false>(d, q, rowsHi, k, rowsHi, kScores);
+#pragma unroll
+      for (int i = 1; i < 4 * G; i++)
+        mmaF16<true>(d, q + (i >> 2) * kQStep + 2 * (i & 3), rowsHi, k + (i >> 2) * kStep + 2 * (i & 3), rowsHi, kScores);
+      mmaF16<true>(d, qSums, plainHi, kSums, plainHi, kScores);
+      sm100::mmaCommit(&ctl.sFull[T][sCount & 1]);
+      sm100::mmaCommit(&ctl.kEmpty[st]);
+    }
+    __syncwarp();
+    sCount++;
+  };
+  bool ok = true;
+  for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+    const ChunkUnit c = chunkUnit(p, starts, u);
+    const int n = c.upto - c.from;
+    if (T >= c.tiles) {  // nothing of this row tile: its share of every stage is let go once it is there
+      for (int j = 0; j < n && ok; j++, seq++) {
+        const uint32_t st = seq & 3, parity = (seq >> 2) & 1u;
+        ok = warpWait(&ctl.kFull[st], parity, abortFlag) && warpWait(&ctl.vFull[st], parity, abortFlag);
+        if (ok && sm100::electOne()) {
+          sm100::mbarArrive(&ctl.kEmpty[st]);
+          sm100::mbarArrive(&ctl.vEmpty[st]);
+        }
+        __syncwarp();
+      }
+      continue;
+    }
+    if (n <= 0) continue;
+    ok = warpWait(&ctl.qFull[T], qCount++ & 1u, abortFlag);
+    for (int i = 0; i < 2 && i < n && ok; i++) {
+      const uint32_t s = seq + i;
+      ok = warpWait(&ctl.kFull[s & 3], (s >> 2) & 1u, abortFlag);
+      if (!ok) break;
+      sm100::tcFenceAfter();
+      issueScores(s & 3);
+    }
+    for (int j = 0; j < n && ok; j++, seq++) {
+      const uint32_t st = seq & 3, place = pCount & 1, weights = T * 128 + place * 64;
+      ok = warpWait(&ctl.pFull[T][place], (pCount >> 1) & 1u, abortFlag) && warpWait(&ctl.vFull[st], (seq >> 2) & 1u, abortFlag);
+      if (!ok) break;
+      pCount++;
+      sm100::tcFenceAfter();
+      const uint32_t v = static_cast<uint32_t>(major) + base + (L::kV >> 4) + st * (G * kStep);
+      if (sm100::electOne()) {
+#pragma unroll
+        for (int k = 0; k < kChunkKeys / 16; k++)
+          mmaF16Tmem(256 + T * D, weights + 8 * k, v + 128 * k, majorHi, kOutputs, k > 0 ? 1u : static_cast<uint32_t>(j));
+        sm100::mmaCommit(&ctl.pvDone[T][place]);
+        sm100::mmaCommit(&ctl.vEmpty[st]);
+      }
+      __syncwarp();
+      if (j + 2 < n) {
+        const uint32_t far = (seq + 2) & 3;
+        ok = warpWait(&ctl.kFull[far], ((seq + 2) >> 2) & 1u, abortFlag);
+        if (!ok) break;
+        sm100::tcFenceAfter();
+        issueScores(far);
+      }
+    }
+  }
+  // Every product and arrival that was issued ends before the block does: the
+  // barriers' memory is the next block's.
+  if (sm100::electOne()) sm100::mmaCommit(&ctl.drain[T]);
+  __syncwarp();
+  volatile int never = 0;
+  sm100::mbarWait(&ctl.drain[T], 0, &never, 200000000ull);
+}
 
 template <int G>
 __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_constant__ AttnArgs p) {
@@ -340,9 +483,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
   if (threadIdx.x == 0) {
     for (int i = 0; i < kChunkStages; i++) {
       sm100::mbarInit(&ctl.kFull[i], 64);
-      sm100::mbarInit(&ctl.kEmpty[i], 1);
+      sm100::mbarInit(&ctl.kEmpty[i], 2);
       sm100::mbarInit(&ctl.vFull[i], 64);
-      sm100::mbarInit(&ctl.vEmpty[i], 1);
+      sm100::mbarInit(&ctl.vEmpty[i], 2);
     }
     for (int i = 0; i < 2; i++) {
       sm100::mbarInit(&ctl.qFull[i], 128);
@@ -353,7 +496,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       sm100::mbarInit(&ctl.pvDone[i][0], 1);
       sm100::mbarInit(&ctl.pvDone[i][1], 1);
     }
-    sm100::mbarInit(&ctl.drain, 1);
+    sm100::mbarInit(&ctl.drain[0], 1);
+    sm100::mbarInit(&ctl.drain[1], 1);
     ctl.abort = 0;
     sm100::fenceBarrierInit();
   }
@@ -381,6 +525,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
   __syncthreads();
   sm100::tcFenceAfter();
   const uint32_t tmem = ctl.tmem;
+  if (threadIdx.x == 0 && tmem != 0) ctl.abort = 1;  // all columns start at the first
   const int units = starts[p.batch];
   constexpr uint32_t kOut = 256;  // columns of the outputs, behind two times 128 of scores
 
@@ -448,9 +593,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       const bool any = t < c.tiles && c.from < c.upto;
       const int mineLimit = limit;
       const float mineUnit = unit;
-      float m = kNone, l = 0.0f;
-      int ref = kNoExponent;  // the outputs are in units of 2^ref
-      uint32_t poison = 0;
+      RowState state = {kNone, 0.0f, static_cast<float>(kLeastExponent), 0};
       if (!any) {
         seq += c.upto - c.from;
       } else {
@@ -460,44 +603,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
                warpWait(&ctl.vFull[seq & 3], (seq >> 2) & 1u, abortFlag);
           if (!ok) break;
           sm100::tcFenceAfter();
-          uint32_t s[2][32];
-          tmemLoad32(scores, s[0]);
-          tmemLoad32(scores + 32, s[1]);
           const ChunkInfo& info = ctl.info[seq & 3];
+          const uint2 valid = *reinterpret_cast<const uint2*>(info.valid);
           const int left = mineLimit - j * kChunkKeys;  // keys of the tile in the row's range
-          const bool edge = __any_sync(~0u, left < kChunkKeys || (info.valid[0] & info.valid[1]) != ~0u);
-          const int newRef = max(ref, max(info.valueExp[0], info.valueExp[1]));
-          const float scale[2] = {mineUnit * powerOfTwo(info.keyExp[0]), mineUnit * powerOfTwo(info.keyExp[1])};
-          sm100::tmemLoadWait();
-          const float top = edge ? tileMaximum<true>(s, info, scale, left) : tileMaximum<false>(s, info, scale, left);
-          if (__any_sync(~0u, top > m + 8.0f || newRef > ref)) {
-            const float next = fmaxf(m, top), shrink = exp2Fast(m - next);
-            if (j > c.from) {
-              // the products with the weights before these have ended
-              ok = warpWait(&ctl.pvDone[t][(count - 1) & 1], ((count - 1) >> 1) & 1u, abortFlag);
-              if (!ok) break;
-              sm100::tcFenceAfter();
-              const float factor = shrink * (ref == kNoExponent ? 1.0f : powerOfTwo(max(ref - newRef, -126)));
-#pragma unroll 1
-              for (int k = 0; k < D / 16; k++) {
-                uint32_t o[16];
-                sm100::tmemLoad16(output + 16 * k, o);
-                sm100::tmemLoadWait();
-#pragma unroll
-                for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                tmemStore16(output + 16 * k, o);
-              }
-            }
-            l *= shrink;
-            m = next;
-            ref = newRef;
-          }
-          l += tileWeights(s, scores, info, scale, m, ref);
-#pragma unroll
-          for (int g = 0; g < G; g++)
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-              if (info.bad[g][k] & seenOf(info.valid[k], left - 32 * k)) poison |= 1u << g;
+          uint64_t* before = &ctl.pvDone[t][(count - 1) & 1];
+          const uint32_t parity = ((count - 1) >> 1) & 1u;
+          if (__any_sync(~0u, left < kChunkKeys || (valid.x & valid.y) != ~0u))
+            ok = tileSoftmax<G, true>(state, scores, output, info, valid, mineUnit, left, j == c.from, before, parity, abortFlag);
+          else
+            ok = tileSoftmax<G, false>(state, scores, output, info, valid, mineUnit, left, j == c.from, before, parity, abortFlag);
+          if (!ok) break;
           tmemStoreWait();
           sm100::tcFenceBefore();
           sm100::mbarArrive(&ctl.pFull[t][count & 1]);
@@ -518,8 +633,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       const long long mine = static_cast<long long>(c.row0) + t * 128 + row;
       const bool live = mine < static_cast<long long>(c.r.rows) * p.group;
       const int token = live ? static_cast<int>(mine / p.group) : 0, h = c.head * p.group + (live ? static_cast<int>(mine % p.group) : 0);
+      const float m = state.m, l = state.l;
       const bool whole = p.splits == 1, none = l == 0.0f;
-      const float factor = (whole ? (none ? 0.0f : 1.0f / l) : 1.0f) * (ref == kNoExponent ? 1.0f : powerOfTwo(ref));
+      const float factor = (whole ? (none ? 0.0f : 1.0f / l) : 1.0f) * powerOfTwo(static_cast<int>(state.ref));
       const long long slot = static_cast<long long>(u) * kChunkRows + t * 128 + row;
 #pragma unroll 1
       for (int k = 0; k < D / 32; k++) {
@@ -529,7 +645,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
           tmemLoad32(output + 32 * k, o);
           sm100::tmemLoadWait();
         }
-        const bool spoilt = (poison >> (k / 2)) & 1u;
+        const bool spoilt = (state.poison >> (k / 2)) & 1u;
 #pragma unroll
         for (int i = 0; i < 32; i++) y[i] = none ? 0.0f : spoilt ? NAN : __uint_as_float(o[i]) * factor;
         if (live) {
@@ -563,6 +679,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
     const int* pages = nullptr;
     bool exists = false;
     int token = 0, page = -1;
+    const int pageTokens = p.blocksPerPage * 16;
+    auto pageOfToken = [&](int x) { return p.pageShift >= 0 ? x >> p.pageShift : x / pageTokens; };
     auto advance = [&]() {
       j++;
       while (j >= upto) {
@@ -580,11 +698,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       }
       exists = true;
       token = j * kChunkKeys + tid;
-      page = token < kv ? pages[token / (p.blocksPerPage * 16)] : -1;
+      page = token < kv ? pages[pageOfToken(token)] : -1;
     };
     auto fetch = [&](RawToken<G>& r) {
       r.there = exists && page >= 0 && page < p.pages;
-      const int place = token % (p.blocksPerPage * 16), at = place & 15;
+      const int place = token - pageOfToken(token) * pageTokens, at = place & 15;
       const uint8_t* block = p.cache + ((static_cast<long long>(r.there ? page : 0) * p.kvHeads + head) * p.blocksPerPage + (place >> 4)) * (18 * D);
       const uint4* codes = reinterpret_cast<const uint4*>(block + (keys ? at : 16 + kv4::valueRow(at)) * (D / 2));
 #pragma unroll
@@ -619,7 +737,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         s[g] = kv4::bf16Lo(raw.keyParams[g]);
         m[g] = kv4::bf16Hi(raw.keyParams[g]);
       }
-      const int ke = exponentOf32<G>(s, m, 0);
+      const int ke = exponentOf32<G>(s, m);
       if (keys) {
         const float f = powerOfTwo(-ke);
 #pragma unroll
@@ -642,8 +760,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
           if (not_finite) s[g] = m[g] = 0.0f;
           bad[g] = __ballot_sync(~0u, not_finite);
         }
-        const int ve = exponentOf32<G>(s, m, kNoExponent);
-        const float f = ve == kNoExponent ? 1.0f : powerOfTwo(-ve);
+        const int ve = exponentOf32<G>(s, m);
+        const float f = powerOfTwo(-ve);
 #pragma unroll
         for (int g = 0; g < G; g++) {
           s[g] *= f;
@@ -654,10 +772,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         if (lane == 0) {  // what was there is read: its weights have been used
           ChunkInfo& info = ctl.info[st];
           info.valid[w] = present;
-          info.keyExp[w] = ke;
-          info.valueExp[w] = ve;
+          info.keyUnit[w] = powerOfTwo(ke);
+          info.valueExp[w] = static_cast<float>(ve);
 #pragma unroll
-          for (int g = 0; g < G; g++) info.bad[g][w] = bad[g];
+          for (int g = 0; g < 2; g++) info.bad[g][w] = g < G ? bad[g < G ? g : 0] : 0;
         }
         widen<G, false>(raw.w, s, m, smem + L::kV + st * G * L::kBlock, tid);
         sm100::fenceProxyAsyncShared();
@@ -666,79 +784,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       raw = next;
       here = follows;
     }
-  } else if (lane == 0) {
-    // ---------------- products ----------------
-    constexpr uint32_t kScores = idescF16(128, kChunkKeys, false), kOutputs = idescF16(128, D, true);
-    // Words of the descriptors: addresses count 16 bytes.
-    const uint64_t rows = sm100::smemDescSw128(0), plain = smemDescPlain(0), major = smemDescMn(0);
-    const uint32_t rowsHi = static_cast<uint32_t>(rows >> 32), plainHi = static_cast<uint32_t>(plain >> 32), majorHi = static_cast<uint32_t>(major >> 32);
-    const uint32_t base = sm100::smemAddr(smem) >> 4;
-    const uint32_t qLo = static_cast<uint32_t>(rows) + base + (L::kQ >> 4), kLo = static_cast<uint32_t>(rows) + base + (L::kK >> 4);
-    const uint32_t vLo = static_cast<uint32_t>(major) + base + (L::kV >> 4);
-    const uint32_t qsLo = static_cast<uint32_t>(plain) + base + (L::kQSums >> 4), ksLo = static_cast<uint32_t>(plain) + base + (L::kKSums >> 4);
-    constexpr uint32_t kQStep = L::kQBlock >> 4, kStep = L::kBlock >> 4;
-    uint32_t seq = 0, qCount[2] = {0, 0}, sCount[2] = {0, 0}, pCount[2] = {0, 0};
-    bool ok = true;
-    auto issueScores = [&](int t, uint32_t st) {
-      const uint32_t d = tmem + t * 128 + (sCount[t] & 1) * 64, q = qLo + t * (G * kQStep), k = kLo + st * (G * kStep);
-      mmaF16<false>(d, q, rowsHi, k, rowsHi, kScores);
-#pragma unroll
-      for (int i = 1; i < 4 * G; i++)
-        mmaF16<true>(d, q + (i >> 2) * kQStep + 2 * (i & 3), rowsHi, k + (i >> 2) * kStep + 2 * (i & 3), rowsHi, kScores);
-      mmaF16<true>(d, qsLo + t * (128 * 32 >> 4), plainHi, ksLo + st * (64 * 32 >> 4), plainHi, kScores);
-      sm100::mmaCommit(&ctl.sFull[t][sCount[t] & 1]);
-      sCount[t]++;
-    };
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-      const ChunkUnit c = chunkUnit(p, starts, u);
-      const int n = c.upto - c.from;
-      if (n <= 0) continue;
-#pragma unroll
-      for (int t = 0; t < 2; t++)
-        if (t < c.tiles && ok) ok = sm100::mbarWait(&ctl.qFull[t], qCount[t]++ & 1u, abortFlag);
-      for (int i = 0; i < 2 && i < n && ok; i++) {
-        const uint32_t s = seq + i;
-        ok = sm100::mbarWait(&ctl.kFull[s & 3], (s >> 2) & 1u, abortFlag);
-        if (!ok) break;
-        sm100::tcFenceAfter();
-        issueScores(0, s & 3);
-        if (c.tiles > 1) issueScores(1, s & 3);
-        sm100::mmaCommit(&ctl.kEmpty[s & 3]);
-      }
-      for (int j = 0; j < n && ok; j++, seq++) {
-        const uint32_t st = seq & 3, far = (seq + 2) & 3;
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-          if (t >= c.tiles || !ok) break;
-          const uint32_t place = pCount[t] & 1, weights = tmem + t * 128 + place * 64;
-          ok = sm100::mbarWait(&ctl.pFull[t][place], (pCount[t] >> 1) & 1u, abortFlag);
-          pCount[t]++;
-          if (ok && t == 0) ok = sm100::mbarWait(&ctl.vFull[st], (seq >> 2) & 1u, abortFlag);
-          if (!ok) break;
-          sm100::tcFenceAfter();
-#pragma unroll
-          for (int k = 0; k < kChunkKeys / 16; k++)
-            mmaF16Tmem(tmem + kOut + t * D, weights + 8 * k, vLo + st * (G * kStep) + 128 * k, majorHi, kOutputs,
-                       k > 0 ? 1u : static_cast<uint32_t>(j));
-          sm100::mmaCommit(&ctl.pvDone[t][place]);
-          if (t + 1 == c.tiles) sm100::mmaCommit(&ctl.vEmpty[st]);
-          if (j + 2 < n) {
-            if (t == 0) {
-              ok = sm100::mbarWait(&ctl.kFull[far], ((seq + 2) >> 2) & 1u, abortFlag);
-              if (!ok) break;
-              sm100::tcFenceAfter();
-            }
-            issueScores(t, far);
-            if (t + 1 == c.tiles) sm100::mmaCommit(&ctl.kEmpty[far]);
-          }
-        }
-      }
-    }
-    // Every product and arrival that was issued ends before the block does:
-    // the barriers' memory is the next block's.
-    sm100::mmaCommit(&ctl.drain);
-    volatile int never = 0;
-    sm100::mbarWait(&ctl.drain, 0, &never, 200000000ull);
+  } else if (warp == 12) {
+    issueProducts<G, 0>(p, starts, units, smem, ctl);
+  } else {
+    issueProducts<G, 1>(p, starts, units, smem, ctl);
   }
   __syncwarp();
   sm100::tcFenceBefore();

@@ -60,6 +60,7 @@ struct AttnArgs {
   float2* stats;      // [2 * workers][R] maximum (log2), sum
   float* partial;     // [2 * workers][R][D]
   int width, batch, tokens, qHeads, kvHeads, group, pages, blocksPerPage;
+  int pageShift;  // tokens of a page = 1 << pageShift, or -1
   int workers, half16, zeroTail;
   float scaleLog2;
   // Requests of at least longRows query rows a key head go to chunkKernel (0: none do).
@@ -1014,6 +1015,7 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   p.group = group;
   p.pages = cache->pages;
   p.blocksPerPage = cache->pageSize / kv4::kBlockTokens;
+  p.pageShift = (cache->pageSize & (cache->pageSize - 1)) == 0 ? __builtin_ctz(cache->pageSize) : -1;
   p.workers = grid * warpsFor(nt);
   p.half16 = datatype == vcclFloat16;
   p.zeroTail = zeroTail;
