@@ -43,7 +43,7 @@ namespace {
 constexpr int kChunkRows = 256;
 constexpr int kChunkKeys = 64;
 constexpr int kChunkStages = 4;     // tiles of keys, and of values, in shared memory
-constexpr int kChunkThreads = 14 * 32;
+constexpr int kChunkThreads = 16 * 32;
 constexpr int kLeastExponent = -112;  // of 32 tokens that are all zero, or next to it
 
 // 32 lanes x 32 bit, 32 consecutive columns per thread.
@@ -266,41 +266,61 @@ __device__ __forceinline__ uint32_t seenOf(uint32_t valid, int left) {
   return valid & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1);
 }
 
-// The maximum of a row's scores over the keys that it sees, in the base-2
-// logarithm; the others become -inf.  EDGE: some row of the warp does not see
-// some key.
+// 32 scores of a row; those of keys that it does not see become -inf.
 template <bool EDGE>
-__device__ __forceinline__ float tileMaximum(uint32_t (&s)[2][32], const uint2& valid, const float (&scale)[2], int left) {
-  float top = kNone;
+__device__ __forceinline__ void loadScores(uint32_t at, uint32_t (&s)[32], uint32_t seen) {
+  tmemLoad32(at, s);
+  sm100::tmemLoadWait();
+  if (EDGE) {
 #pragma unroll
-  for (int k = 0; k < 2; k++) {
-    const uint32_t seen = EDGE ? seenOf(k ? valid.y : valid.x, left - 32 * k) : ~0u;
-    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int i = 0; i < 32; i++) {
-      if (EDGE && !((seen >> i) & 1u)) s[k][i] = 0xFF800000u;  // -inf
-      x[i & 3] = fmaxf(x[i & 3], __uint_as_float(s[k][i]));
-    }
-    const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    if (!EDGE || most > -INFINITY) top = fmaxf(top, most * scale[k]);
+    for (int i = 0; i < 32; i++)
+      if (!((seen >> i) & 1u)) s[i] = 0xFF800000u;
   }
-  return top;
+}
+
+// Two f32 in one register pair, worked on by one instruction.
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair(float x) { return pair(__float_as_uint(x), __float_as_uint(x)); }
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  uint32_t lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // The weights of 32 scores, to TMEM in their place; returns their sum.
 __device__ __forceinline__ float halfWeights(const uint32_t (&s)[32], uint32_t at, float scale, float off) {
-  float part[4] = {};
+  uint64_t part[2] = {0, 0};
+  const uint64_t by = pair(scale), plus = pair(off);
   uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 16; i++) {
-    const float a = exp2Fast(fmaf(__uint_as_float(s[2 * i]), scale, off));
-    const float b = exp2Fast(fmaf(__uint_as_float(s[2 * i + 1]), scale, off));
-    part[2 * (i & 1)] += a;
-    part[2 * (i & 1) + 1] += b;
+    const float2 x = unpair(fma2(pair(s[2 * i], s[2 * i + 1]), by, plus));
+    const float a = exp2Fast(x.x), b = exp2Fast(x.y);
+    part[i & 1] = add2(part[i & 1], pair(__float_as_uint(a), __float_as_uint(b)));
     w[i] = packHalf(a, b);
   }
   tmemStore16(at, w);
-  return (part[0] + part[1]) + (part[2] + part[3]);
+  const float2 sum = unpair(add2(part[0], part[1]));
+  return sum.x + sum.y;
 }
 
 // What a softmax thread keeps of its row.
@@ -316,15 +336,24 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
                                             float unit, int left, bool first, uint64_t* before, uint32_t beforeParity,
                                             volatile int* abortFlag) {
   constexpr int D = 64 * G;
-  uint32_t s[2][32];
-  tmemLoad32(scores, s[0]);
-  tmemLoad32(scores + 32, s[1]);
   const float2 keyUnit = *reinterpret_cast<const float2*>(info.keyUnit), valueExp = *reinterpret_cast<const float2*>(info.valueExp);
   const uint4 bad = *reinterpret_cast<const uint4*>(info.bad);
-  const float scale[2] = {unit * keyUnit.x, unit * keyUnit.y};
+  const float scale0 = unit * keyUnit.x, scale1 = unit * keyUnit.y;
   const float ref = fmaxf(r.ref, fmaxf(valueExp.x, valueExp.y));
-  sm100::tmemLoadWait();
-  const float top = tileMaximum<EDGE>(s, valid, scale, left);
+  const uint32_t seen0 = EDGE ? seenOf(valid.x, left) : ~0u, seen1 = EDGE ? seenOf(valid.y, left - 32) : ~0u;
+  float top = kNone;
+#pragma unroll 1
+  for (int k = 0; k < 2; k++) {
+    uint32_t s[32];
+    loadScores<EDGE>(scores + 32 * k, s, k ? seen1 : seen0);
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = __uint_as_float(s[i]);
+#pragma unroll
+    for (int i = 4; i < 32; i += 2) x[(i >> 1) & 3] = max3(x[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+    const float most = max3(x[0], x[1], fmaxf(x[2], x[3]));
+    if (!EDGE || most > -INFINITY) top = fmaxf(top, most * (k ? scale1 : scale0));
+  }
   if (__any_sync(~0u, top > r.m + 8.0f || ref > r.ref)) {
     const float next = fmaxf(r.m, top), shrink = exp2Fast(r.m - next);
     if (!first) {
@@ -348,11 +377,14 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
   }
   // Weights of values in smaller units are smaller; 2^100 apart they vanish.
   const float shift0 = fmaxf(valueExp.x - r.ref, -100.0f), shift1 = fmaxf(valueExp.y - r.ref, -100.0f);
-  const float sum0 = halfWeights(s[0], scores, scale[0], shift0 - r.m);
-  const float sum1 = halfWeights(s[1], scores + 16, scale[1], shift1 - r.m);
-  r.l = fmaf(sum0, exp2Fast(-shift0), fmaf(sum1, exp2Fast(-shift1), r.l));
+#pragma unroll 1
+  for (int k = 0; k < 2; k++) {
+    uint32_t s[32];
+    loadScores<EDGE>(scores + 32 * k, s, k ? seen1 : seen0);
+    const float shift = k ? shift1 : shift0;
+    r.l = fmaf(halfWeights(s, scores + 16 * k, k ? scale1 : scale0, shift - r.m), exp2Fast(-shift), r.l);
+  }
   if ((bad.x | bad.y | bad.z | bad.w) != 0) {
-    const uint32_t seen0 = seenOf(valid.x, left), seen1 = seenOf(valid.y, left - 32);
     if ((bad.x & seen0) | (bad.y & seen1)) r.poison |= 1u;
     if ((bad.z & seen0) | (bad.w & seen1)) r.poison |= 2u;
   }
@@ -377,6 +409,18 @@ struct RawToken {
   uint32_t w[8 * G], params[G], keyParams[G];
   bool there;
 };
+
+// Registers a thread, of the 128 that each of the four warpgroups starts with.
+constexpr int kSoftmaxRegisters = 160, kWidenRegisters = 112, kIssueRegisters = 80;
+static_assert(2 * kSoftmaxRegisters + kWidenRegisters + kIssueRegisters == 4 * 128, "what one gives the others take");
+template <int N>
+__device__ __forceinline__ void moreRegisters() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewerRegisters() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 // The products of row tile T, by one warp: all of it waits, one thread issues.
 // The block has all 512 columns of TMEM, from column 0 on, so places in it are
@@ -531,6 +575,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
 
   if (warp < 8) {
     // ---------------- softmax ----------------
+    moreRegisters<kSoftmaxRegisters>();
     const int t = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t output = tmem + kOut + t * D + lanes;
@@ -672,6 +717,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
     }
   } else if (warp < 12) {
     // ---------------- codes to f16 ----------------
+    fewerRegisters<kWidenRegisters>();
     const bool keys = warp < 10;
     const int tid = threadIdx.x & 63, w = warp & 1;
     // The tile after next: its token's page number is under way.
@@ -784,10 +830,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       raw = next;
       here = follows;
     }
-  } else if (warp == 12) {
-    issueProducts<G, 0>(p, starts, units, smem, ctl);
   } else {
-    issueProducts<G, 1>(p, starts, units, smem, ctl);
+    fewerRegisters<kIssueRegisters>();
+    if (warp == 12) issueProducts<G, 0>(p, starts, units, smem, ctl);
+    if (warp == 13) issueProducts<G, 1>(p, starts, units, smem, ctl);
   }
   __syncwarp();
   sm100::tcFenceBefore();
