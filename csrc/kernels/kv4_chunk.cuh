@@ -174,7 +174,7 @@ struct alignas(16) ChunkInfo {
 };
 
 struct ChunkControl {
-  ChunkInfo info[kChunkStages];
+  ChunkInfo info[2 * kChunkStages];  // written with the keys, read until the weights are there
   uint64_t kFull[kChunkStages], kEmpty[kChunkStages], vFull[kChunkStages], vEmpty[kChunkStages];
   // A wait tells a phase of a barrier from the one before it alone, so what
   // can be two tiles ahead has a barrier for each place.
@@ -208,14 +208,14 @@ __device__ __forceinline__ ChunkUnit chunkUnit(const AttnArgs& p, const int* sta
   }
   c.b = lo;
   c.r = requestOf(p, lo);
-  const long long rows = static_cast<long long>(c.r.rows) * p.group;
-  const int perHead = static_cast<int>((rows + kChunkRows - 1) / kChunkRows);
+  const int rows = c.r.rows * p.group;  // at most tokens * q heads
+  const int perHead = (rows + kChunkRows - 1) / kChunkRows;
   int i = u - starts[lo];
   const int share = i % p.splits;
   i /= p.splits;
   c.head = i / perHead;
   c.row0 = (perHead - 1 - i % perHead) * kChunkRows;
-  const int left = static_cast<int>(min(rows - c.row0, static_cast<long long>(kChunkRows)));
+  const int left = min(rows - c.row0, kChunkRows);
   c.tiles = left > 128 ? 2 : 1;
   const int last = (c.row0 + left - 1) / p.group;  // the unit's last token
   const int seen = min(max(c.r.kv - c.r.rows + last + 1, 0), c.r.kv);
@@ -223,6 +223,13 @@ __device__ __forceinline__ ChunkUnit chunkUnit(const AttnArgs& p, const int* sta
   c.from = min(share * each, all);
   c.upto = min(c.from + each, all);
   return c;
+}
+
+// The unit that this block takes in a round: rounds go to and fro, since the
+// units of a head come heaviest first.
+__device__ __forceinline__ int unitOfRound(int round) {
+  const int n = gridDim.x, b = blockIdx.x;
+  return round * n + ((round & 1) ? n - 1 - b : b);
 }
 
 // One token's row of codes -> f16 in shared memory: 8 channels a store.
@@ -402,11 +409,12 @@ __device__ __forceinline__ int exponentOf32(const float (&scale)[G], const float
   return max(exponentOf(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top)))) - 12, kLeastExponent);
 }
 
-// A token's row of codes with its parameters; a value thread has those of the
-// keys too (it writes down what the softmax needs of both).
+// A token's row of codes with its parameters; a key thread has those of the
+// values too (it writes down what the softmax needs of both, before the scores
+// can be there).
 template <int G>
 struct RawToken {
-  uint32_t w[8 * G], params[G], keyParams[G];
+  uint32_t w[8 * G], keyParams[G], valueParams[G];
   bool there;
 };
 
@@ -457,7 +465,7 @@ __device__ __forceinline__ void issueProducts(const AttnArgs& p, const int* star
     sCount++;
   };
   bool ok = true;
-  for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+  for (int round = 0, u = unitOfRound(0); u < units && ok; u = unitOfRound(++round)) {
     const ChunkUnit c = chunkUnit(p, starts, u);
     const int n = c.upto - c.from;
     if (T >= c.tiles) {  // nothing of this row tile: its share of every stage is let go once it is there
@@ -586,9 +594,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
     // A unit's queries: the row's channels, scaled to 2^8, and their sums as
     // the left operand.
     auto loadQuery = [&](const ChunkUnit& c) {
-      const long long mine = static_cast<long long>(c.row0) + t * 128 + row;
-      const bool live = mine < static_cast<long long>(c.r.rows) * p.group;
-      const int token = live ? static_cast<int>(mine / p.group) : 0, h = c.head * p.group + (live ? static_cast<int>(mine % p.group) : 0);
+      const int mine = c.row0 + t * 128 + row;
+      const bool live = mine < c.r.rows * p.group;
+      const int token = live ? mine / p.group : 0, h = c.head * p.group + (live ? mine - token * p.group : 0);
       limit = live ? min(max(c.r.kv - c.r.rows + token + 1, 0), c.r.kv) : c.r.kv;
       float amax = 0.0f, sums[G] = {};
       const uint16_t* src = static_cast<const uint16_t*>(p.q) + static_cast<long long>(c.r.start + token) * p.qTok + static_cast<long long>(h) * p.qHead;
@@ -628,12 +636,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
     // The next unit with keys for this row tile, from unit u on; its queries
     // are loaded as soon as the last scores of the unit before are there.
     bool ok = true;
-    int u = blockIdx.x;
+    int round = 0, u = unitOfRound(0);
     if (u < units) {
       const ChunkUnit c = chunkUnit(p, starts, u);
       if (t < c.tiles && c.from < c.upto) loadQuery(c);
     }
-    for (; u < units && ok; u += gridDim.x) {
+    for (; u < units && ok; u = unitOfRound(++round)) {
       const ChunkUnit c = chunkUnit(p, starts, u);
       const bool any = t < c.tiles && c.from < c.upto;
       const int mineLimit = limit;
@@ -644,11 +652,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       } else {
         for (int j = c.from; j < c.upto; j++, seq++, count++) {
           const uint32_t scores = tmem + t * 128 + (count & 1) * 64 + lanes;
-          ok = warpWait(&ctl.sFull[t][count & 1], (count >> 1) & 1u, abortFlag) &&
-               warpWait(&ctl.vFull[seq & 3], (seq >> 2) & 1u, abortFlag);
+          ok = warpWait(&ctl.sFull[t][count & 1], (count >> 1) & 1u, abortFlag);
           if (!ok) break;
           sm100::tcFenceAfter();
-          const ChunkInfo& info = ctl.info[seq & 3];
+          const ChunkInfo& info = ctl.info[seq & 7];
           const uint2 valid = *reinterpret_cast<const uint2*>(info.valid);
           const int left = mineLimit - j * kChunkKeys;  // keys of the tile in the row's range
           uint64_t* before = &ctl.pvDone[t][(count - 1) & 1];
@@ -664,8 +671,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         }
       }
       if (!ok) break;
-      if (u + gridDim.x < units) {
-        const ChunkUnit next = chunkUnit(p, starts, u + gridDim.x);
+      if (unitOfRound(round + 1) < units) {
+        const ChunkUnit next = chunkUnit(p, starts, unitOfRound(round + 1));
         if (t < next.tiles && next.from < next.upto) loadQuery(next);
       }
       // The result, or this share of it.
@@ -675,9 +682,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         if (!ok) break;
         sm100::tcFenceAfter();
       }
-      const long long mine = static_cast<long long>(c.row0) + t * 128 + row;
-      const bool live = mine < static_cast<long long>(c.r.rows) * p.group;
-      const int token = live ? static_cast<int>(mine / p.group) : 0, h = c.head * p.group + (live ? static_cast<int>(mine % p.group) : 0);
+      const int mine = c.row0 + t * 128 + row;
+      const bool live = mine < c.r.rows * p.group;
+      const int token = live ? mine / p.group : 0, h = c.head * p.group + (live ? mine - token * p.group : 0);
       const float m = state.m, l = state.l;
       const bool whole = p.splits == 1, none = l == 0.0f;
       const float factor = (whole ? (none ? 0.0f : 1.0f / l) : 1.0f) * powerOfTwo(static_cast<int>(state.ref));
@@ -721,7 +728,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
     const bool keys = warp < 10;
     const int tid = threadIdx.x & 63, w = warp & 1;
     // The tile after next: its token's page number is under way.
-    int u = blockIdx.x, j = 0, upto = 0, head = 0, kv = 0;
+    int round = 0, u = unitOfRound(0), j = 0, upto = 0, head = 0, kv = 0;
     const int* pages = nullptr;
     bool exists = false;
     int token = 0, page = -1;
@@ -735,7 +742,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
           return;
         }
         const ChunkUnit c = chunkUnit(p, starts, u);
-        u += gridDim.x;
+        u = unitOfRound(++round);
         j = c.from;
         upto = c.upto;
         head = c.head;
@@ -762,8 +769,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       }
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        r.keyParams[g] = r.there ? __ldg(reinterpret_cast<const uint32_t*>(block + 16 * D + at * (4 * G)) + g) : 0;
-        r.params[g] = r.there && !keys ? __ldg(reinterpret_cast<const uint32_t*>(block + 17 * D + at * (4 * G)) + g) : 0;
+        r.keyParams[g] = r.there && keys ? __ldg(reinterpret_cast<const uint32_t*>(block + 16 * D + at * (4 * G)) + g) : 0;
+        r.valueParams[g] = r.there ? __ldg(reinterpret_cast<const uint32_t*>(block + 17 * D + at * (4 * G)) + g) : 0;
       }
     };
     RawToken<G> raw, next;
@@ -778,51 +785,51 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       const int st = seq & 3;
       const uint32_t parity = ((seq >> 2) & 1u) ^ 1u;
       float s[G], m[G];
+      uint32_t bad[G];
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        s[g] = kv4::bf16Lo(raw.keyParams[g]);
-        m[g] = kv4::bf16Hi(raw.keyParams[g]);
+        s[g] = kv4::bf16Lo(raw.valueParams[g]);
+        m[g] = kv4::bf16Hi(raw.valueParams[g]);
+        const bool odd = !(isfinite(s[g]) && isfinite(m[g]));
+        if (odd) s[g] = m[g] = 0.0f;
+        bad[g] = __ballot_sync(~0u, odd);
       }
-      const int ke = exponentOf32<G>(s, m);
+      const int ve = exponentOf32<G>(s, m);
       if (keys) {
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          s[g] = kv4::bf16Lo(raw.keyParams[g]);
+          m[g] = kv4::bf16Hi(raw.keyParams[g]);
+        }
+        const int ke = exponentOf32<G>(s, m);
         const float f = powerOfTwo(-ke);
 #pragma unroll
         for (int g = 0; g < G; g++) {
           s[g] *= f;
           m[g] = fmaf(0.5f, s[g], m[g] * f);  // value = m + s (code - 8) from here on
         }
-        if (!warpWait(&ctl.kEmpty[st], parity, abortFlag)) break;
-        widen<G, true>(raw.w, s, m, smem + L::kK + st * G * L::kBlock, tid);
-        storeSums<G, false>(smem + L::kKSums + st * (64 * 32), tid, m);
-        sm100::fenceProxyAsyncShared();
-        sm100::mbarArrive(&ctl.kFull[st]);
-      } else {
-        uint32_t bad[G];
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-          s[g] = kv4::bf16Lo(raw.params[g]);
-          m[g] = kv4::bf16Hi(raw.params[g]);
-          const bool not_finite = !(isfinite(s[g]) && isfinite(m[g]));
-          if (not_finite) s[g] = m[g] = 0.0f;
-          bad[g] = __ballot_sync(~0u, not_finite);
-        }
-        const int ve = exponentOf32<G>(s, m);
-        const float f = powerOfTwo(-ve);
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-          s[g] *= f;
-          m[g] = fmaf(0.5f, s[g], m[g] * f);
-        }
         const uint32_t present = __ballot_sync(~0u, raw.there);
-        if (!warpWait(&ctl.vEmpty[st], parity, abortFlag)) break;
-        if (lane == 0) {  // what was there is read: its weights have been used
-          ChunkInfo& info = ctl.info[st];
+        if (!warpWait(&ctl.kEmpty[st], parity, abortFlag)) break;
+        if (lane == 0) {
+          ChunkInfo& info = ctl.info[seq & 7];
           info.valid[w] = present;
           info.keyUnit[w] = powerOfTwo(ke);
           info.valueExp[w] = static_cast<float>(ve);
 #pragma unroll
           for (int g = 0; g < 2; g++) info.bad[g][w] = g < G ? bad[g < G ? g : 0] : 0;
         }
+        widen<G, true>(raw.w, s, m, smem + L::kK + st * G * L::kBlock, tid);
+        storeSums<G, false>(smem + L::kKSums + st * (64 * 32), tid, m);
+        sm100::fenceProxyAsyncShared();
+        sm100::mbarArrive(&ctl.kFull[st]);
+      } else {
+        const float f = powerOfTwo(-ve);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          s[g] *= f;
+          m[g] = fmaf(0.5f, s[g], m[g] * f);
+        }
+        if (!warpWait(&ctl.vEmpty[st], parity, abortFlag)) break;
         widen<G, false>(raw.w, s, m, smem + L::kV + st * G * L::kBlock, tid);
         sm100::fenceProxyAsyncShared();
         sm100::mbarArrive(&ctl.vFull[st]);
