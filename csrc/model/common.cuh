@@ -24,6 +24,12 @@ inline bool headsOk(const vcclHeads_t* h, int elemBytes) {
          h->tokenStride >= 0 && h->tokenStride < most && h->headStride >= 0 && h->headStride < most;
 }
 
+inline bool cacheOk(const vcclKv4_t* c) {
+  return c != nullptr && c->data != nullptr && (reinterpret_cast<uintptr_t>(c->data) & 15u) == 0 && c->pages > 0 &&
+         c->pageSize > 0 && c->pageSize % 16 == 0 && c->kvHeads > 0 && (c->D == 64 || c->D == 128) &&
+         static_cast<long long>(c->pages) * c->pageSize <= INT32_MAX;
+}
+
 inline vcclResult_t launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return vcclSuccess;

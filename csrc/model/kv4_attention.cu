@@ -977,9 +977,7 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
                               const int* kvLens, const int* qStarts, int batch, int tokens, float scale,
                               const vcclHeads_t* out, float* lse, int zeroTail, void* workspace,
                               vcclDataType_t datatype, vcclStream_t stream) {
-  if (cache == nullptr || cache->data == nullptr || (reinterpret_cast<uintptr_t>(cache->data) & 15u) != 0 ||
-      cache->pages <= 0 || cache->pageSize <= 0 || cache->pageSize % kv4::kBlockTokens != 0 || cache->kvHeads <= 0 ||
-      (cache->D != 64 && cache->D != 128) || tokens < 0 || batch <= 0 || batch > kMaxBatch || width <= 0 ||
+  if (!cacheOk(cache) || tokens < 0 || batch <= 0 || batch > kMaxBatch || width <= 0 ||
       static_cast<long long>(width) * cache->pageSize > INT_MAX ||
       (datatype != vcclBfloat16 && datatype != vcclFloat16))
     return vcclInvalidArgument;

@@ -564,12 +564,6 @@ void launchRead(const ReadArgs& p, int grid, cudaStream_t st) {
 
 bool sixteenBit(vcclDataType_t t) { return t == vcclBfloat16 || t == vcclFloat16; }
 
-bool cacheOk(const vcclKv4_t* c) {
-  return c != nullptr && c->data != nullptr && (reinterpret_cast<uintptr_t>(c->data) & 15u) == 0 && c->pages > 0 &&
-         c->pageSize > 0 && c->pageSize % kv4::kBlockTokens == 0 && c->kvHeads > 0 && (c->D == 64 || c->D == 128) &&
-         static_cast<long long>(c->pages) * c->pageSize <= INT32_MAX;
-}
-
 Cache cacheOf(const vcclKv4_t* c) {
   const int per = c->pageSize / kv4::kBlockTokens;
   int shift = 0;

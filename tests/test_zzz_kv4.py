@@ -724,3 +724,58 @@ def test_backward_captured_and_replayed():
     want = qk_norm_rope_backward(dq, dk, q, k, pos, freq, q_weight=w, k_weight=w)
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_decode_model_with_cache(qk_norm):
+    """TPLlamaDecode.step_cached on one rank: a prompt and two single tokens of two requests (one ends, its place is
+    taken by a new prompt) against the same layers with attention in 64 bits over what was stored."""
+    import vkccl_b200 as v
+    from vkccl_b200.models.llama_decode import DecodeConfig, TPLlamaDecode
+    from vkccl_b200.ops.fused import all_reduce_add_rms_norm
+    from vkccl_b200.ops.gemm import gemm_bf16, gemm_silu_mul
+
+    cfg = DecodeConfig(hidden=1024, intermediate=2048, heads=8, kv_heads=2, head_dim=128, layers=2, qk_norm=qk_norm,
+                       page_size=16)
+    comm = v.Communicator(1, v.get_unique_id(), 0, cuda_device=0)
+    try:
+        model, g = TPLlamaDecode(comm, cfg, seed=3), gen(40)
+        cache = model.new_cache(2, 12, 96)
+        stored = [[([], []) for _ in range(2)] for _ in range(cfg.layers)]  # layer, request -> keys, values
+        held = [0, 0]
+        for new, ends in (([37, 5], []), ([1, 1], []), ([1, 20], [1])):
+            rows = sum(new) + 3
+            x, xn = randn(g, rows, cfg.hidden), randn(g, rows, cfg.hidden)
+            xr, xnr = x.clone(), xn.clone()
+            done = torch.tensor([i in ends for i in range(2)], device="cuda")
+            got = model.step_cached(x, xn, cache, ints(new), finished=done)
+            qs = starts(new)
+            for i in ends:
+                held[i] = 0
+                for layer in stored:
+                    layer[i] = ([], [])
+            pos = ints(sum(([held[i] + t for t in range(new[i])] for i in range(2)), []) + [0] * 3)
+            held = [held[i] + new[i] for i in range(2)]
+            for L, layer in zip(model.layers, stored):
+                qkv = gemm_bf16(xnr, L["qkv"]).view(rows, 12, 128)
+                q64 = ref.norm_rope(qkv[:, :8], L.get("qn"), cfg.eps, pos, model.inv_freq, False)
+                k64 = ref.norm_rope(qkv[:, 8:10], L.get("kn"), cfg.eps, pos, model.inv_freq, False).bfloat16()
+                ks, vs = [], []
+                for i in range(2):
+                    layer[i][0].append(ref.stored_values(k64[qs[i]:qs[i + 1]]))
+                    layer[i][1].append(ref.stored_values(qkv[qs[i]:qs[i + 1], 10:]))
+                    ks.append(torch.cat(layer[i][0]))
+                    vs.append(torch.cat(layer[i][1]))
+                attn = ref.attention(q64.bfloat16(), ks, vs, held, qs, 128 ** -0.5)[0].bfloat16()
+                part = gemm_bf16(attn.view(rows, -1), L["o"])
+                xnr = all_reduce_add_rms_norm(comm, part, xr, L["ln1"], cfg.eps)
+                part = gemm_bf16(gemm_silu_mul(xnr, L["gu"]), L["d"])
+                xnr = all_reduce_add_rms_norm(comm, part, xr, L["ln2"], cfg.eps)
+            assert cache.lens.tolist() == held
+            # The two differ where attention rounds to the neighbouring bf16 number (half a step, 2^-8, of its part of
+            # the residual) and a 4-bit code to its neighbour; through two layers in the norm of a row.
+            n = sum(new)
+            err = (got[:n].double() - xnr[:n].double()).norm(dim=-1) / xnr[:n].double().norm(dim=-1)
+            assert err.max().item() < 4 * 2.0**-8, err.max().item()
+    finally:
+        comm.destroy()

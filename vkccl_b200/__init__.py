@@ -7,7 +7,9 @@ it with ctypes and adds torch integration:
 * ``vkccl_b200.comm``       – Communicator, UniqueId, DataType, RedOp, groups
 * ``vkccl_b200.torch_comm`` – vLLM ``VcclCommunicator`` device communicator
 * ``vkccl_b200.ops``        – fused tensor-parallel kernels (GEMM+RS, AG+GEMM,
-                              AR+residual+RMSNorm, MoE fp8 dispatch/combine)
+                              AR+residual+RMSNorm, MoE fp8 dispatch/combine) and a
+                              decode step's (page plan, norm + rotation, 4-bit
+                              key/value cache and attention over it)
 * ``vkccl_b200.models``     – Llama / Mixtral shaped layers built on them
 * ``vkccl_b200.parallel``   – process-group and sharding helpers
 * ``vkccl_b200.utils``      – device timing and clock sampling

@@ -11,6 +11,10 @@ runs decode, and replayed.  Reported: mean step time over --iters replays
 same layers on cuBLAS + NCCL all-reduce + torch RMSNorm, plus the relative
 difference between the two paths' hidden states after one layer and after
 all layers (random weights make 80 layers amplify rounding differences).
+
+With --context N also the step with its attention over the 4-bit paged cache
+(``step_cached``), every request holding N tokens; the page plan is part of
+the captured step, and each replay adds a token to every request.
 """
 
 from __future__ import annotations
@@ -60,6 +64,7 @@ def main() -> int:
     ap.add_argument("--layers", type=int, default=80)
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
+    ap.add_argument("--context", type=int, default=0, help="tokens that each request holds; 0: no step with attention")
     a = ap.parse_args()
     rank, world, local = (int(os.environ.get(k, d)) for k, d in (("RANK", 0), ("WORLD_SIZE", 1), ("LOCAL_RANK", 0)))
     torch.cuda.set_device(local)
@@ -101,6 +106,22 @@ def main() -> int:
         out["results"][str(b)] = {"vccl_us": round(t_v, 1), "nccl_cublas_us": round(t_n, 1),
                                   "speedup": round(t_n / t_v, 3), "roofline_fraction": round(roof_us / t_v, 3),
                                   "rel_diff_one_layer": err1, "rel_diff_final_state": err}
+        if a.context > 0:
+            room = a.context + a.iters + 3 * a.warmup + 64
+            per = -(-room // model.cfg.page_size)
+            cache = model.new_cache(b, b * per, room)
+            for layer in cache.layers:  # some finite contents: codes at random, scales and midpoints 0.0625
+                layer.copy_(torch.randint(0, 256, layer.shape[1:], device="cuda", dtype=torch.uint8, generator=g))
+                layer[..., 16 * model.cfg.head_dim:].view(torch.bfloat16).fill_(0.0625)
+            grow = torch.full((b,), a.context, dtype=torch.int32, device="cuda")
+            cache.plan(grow, b * a.context)  # pages and lengths of what is held
+            one = torch.ones(b, dtype=torch.int32, device="cuda")
+            xc = x0.clone()
+            t_c = graph_time(lambda: model.step_cached(xc, xn0, cache, one), a.iters, a.warmup)
+            kv_bytes = sum(layer[0, 0, 0].numel() // 16 * layer.shape[1] for layer in cache.layers) * b * a.context
+            out["results"][str(b)].update({"context": a.context, "vccl_cached_us": round(t_c, 1),
+                                           "cached_roofline_fraction": round((roof_us + kv_bytes / hbm_gbs * 1e-3) / t_c, 3)})
+            del cache
         if rank == 0:
             print(json.dumps({"batch": b, **out["results"][str(b)]}), flush=True)
     if rank == 0:
