@@ -93,10 +93,14 @@ __device__ __forceinline__ void pairToFloat<__half>(uint32_t v, float* lo, float
 // A group whose scale or midpoint is not finite is stored as NaN.
 //
 // Eight divisions a lane made the write of a prompt bound by instructions
-// (109 us for 16384 tokens of 8 heads with the read back).  So the quotient
-// is a product with 1 / scale, whose sum with 7.5 is off by less than 2^-20;
-// only where that sum is within 2^-16 of a code's border (one bf16 element in
-// about 200: x - mid is then a whole number of scales) the division decides.
+// (64 us for 16384 tokens of 8 heads, where the bytes take 13).  So
+// code / 15 = (x - mid) / (15 scale) + 1/2 is a product with 1 / (15 scale),
+// held to [0, 1] by the instruction's saturation; 15 times that plus 96 rounds
+// to a multiple of 2^-17, which is more than it is off by: where the code is
+// on the border of two it comes out as k + 1/2 exactly, and the next addition
+// rounds it to even as rint does.  What comes out as k + 1/2 without being it
+// (x - mid is then not a whole number of scales; one group in millions) and
+// scales next to the smallest take the division.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const uint4& raw, uint32_t* params) {
   uint32_t lo2 = min2<T>(min2<T>(raw.x, raw.y), min2<T>(raw.z, raw.w));
@@ -119,21 +123,42 @@ __device__ __forceinline__ uint32_t quantise8(const uint4& raw, uint32_t* params
   }
   *params = static_cast<uint32_t>(__bfloat16_as_ushort(sb)) | (static_cast<uint32_t>(__bfloat16_as_ushort(mb)) << 16);
   const float d = s > 0.0f ? s : 1.0f;
-  const float inv = __frcp_rn(d);
+  const float share = __frcp_rn(15.0f * d);
   const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
-  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number in the low bits
-  uint32_t w = 0u - 0x4B400000u * 0x11111111u;
+  // 1.5 * 2^23 - 96: 96 + code becomes a whole number in the low bits.
+  constexpr float kWhole = 12582816.0f;
+  float a[8], t[8], u[8], worst = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; i++) {
     float x[2];
     pairToFloat<T>(in[i >> 1], &x[0], &x[1]);
-    const float a = __fsub_rn(x[i & 1], m);
-    const float t = fminf(fmaxf(__fmaf_rn(a, inv, 7.5f), 0.0f), 15.0f);
-    float u = __fadd_rn(t, kMagic);
-    if (!(fabsf(__fsub_rn(t, __fsub_rn(u, kMagic))) < 0.5f - 1.52587890625e-5f))
-      u = __fadd_rn(fminf(fmaxf(rintf(__fadd_rn(__fdiv_rn(a, d), 7.5f)), 0.0f), 15.0f), kMagic);
-    w += __float_as_uint(u) << (4 * ((i >> 1) + 4 * (i & 1)));
+    a[i] = __fsub_rn(x[i & 1], m);
+    t[i] = __fmaf_rn(__saturatef(__fmaf_rn(a[i], share, 0.5f)), 15.0f, 96.0f);
+    u[i] = __fadd_rn(t[i], kWhole);
+    worst = fmaxf(worst, fabsf(__fsub_rn(t[i], __fsub_rn(u[i], kWhole))));
   }
+  if (worst == 0.5f || d < 1e-30f) {
+    bool exact = d >= 1e-30f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const bool border = fabsf(__fsub_rn(t[i], __fsub_rn(u[i], kWhole))) == 0.5f;
+      exact = exact && !(border && __fmaf_rn(__fsub_rn(103.5f, t[i]), d, a[i]) != 0.0f);
+    }
+    if (!exact) {
+#pragma unroll 1
+      for (int k = 0; k < 8; k++) {
+        float q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) q = i == k ? a[i] : q;
+        q = __fadd_rn(fminf(fmaxf(rintf(__fadd_rn(__fdiv_rn(q, d), 7.5f)), 0.0f), 15.0f), kWhole + 96.0f);
+#pragma unroll
+        for (int i = 0; i < 8; i++) u[i] = i == k ? q : u[i];
+      }
+    }
+  }
+  uint32_t w = 0u - 0x4B400000u * 0x11111111u;
+#pragma unroll
+  for (int i = 0; i < 8; i++) w += __float_as_uint(u[i]) << (4 * ((i >> 1) + 4 * (i & 1)));
   return w;
 }
 

@@ -4,9 +4,12 @@
 // pass, or alone).
 //
 // A row (one head of one token) is held by LANES neighbouring lanes with 8
-// channels each (16-byte loads and stores); the mean square, the partner
-// channels of the rotation and the group extremes of the 4-bit rounding are
-// shuffles among them.  The cosines and sines of a block's tokens are taken
+// channels each.  Where the row goes on as it is, a lane has 4 channels of the
+// row's first half and the same 4 of its second (two 8-byte loads): the two
+// channels of a pair then meet in a lane, and a row of 128 takes 4 shuffles
+// instead of 13, which shared the shared-memory pipe with the cosines (88 us
+// before, 8192 tokens of 72 heads).  Where it goes to the cache a lane has 8
+// neighbouring channels, as a word of codes does.  The cosines and sines of a block's tokens are taken
 // once, into shared memory: the angle position * invFreq is a product in 64
 // bits, reduced to [-pi, pi] there, since positions reach millions.
 //
@@ -242,37 +245,200 @@ __device__ __forceinline__ float squaresOfRow(const float (&x)[8], int lane, int
   return s;
 }
 
-struct ForwardArgs {
-  Side side[3];  // queries, keys, values; out == nullptr: not written (keys and values go to the cache)
+// ---- rows in halves: channels 4 lane .. + 3 and D / 2 + 4 lane .. + 3 --------
+
+template <typename T>
+__device__ __forceinline__ uint4 loadHalves(const T* row, int lane, int D) {
+  const uint2 a = *reinterpret_cast<const uint2*>(row + 4 * lane), b = *reinterpret_cast<const uint2*>(row + D / 2 + 4 * lane);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+template <typename T>
+__device__ __forceinline__ void storeHalves(T* row, int lane, int D, const uint4& v) {
+  *reinterpret_cast<uint2*>(row + 4 * lane) = make_uint2(v.x, v.y);
+  *reinterpret_cast<uint2*>(row + D / 2 + 4 * lane) = make_uint2(v.z, v.w);
+}
+__device__ __forceinline__ void loadHalves(const float* row, int lane, int D, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(row + 4 * lane), b = *reinterpret_cast<const float4*>(row + D / 2 + 4 * lane);
+  x[0] = a.x;
+  x[1] = a.y;
+  x[2] = a.z;
+  x[3] = a.w;
+  x[4] = b.x;
+  x[5] = b.y;
+  x[6] = b.z;
+  x[7] = b.w;
+}
+
+// The same sums in the same order as squaresOfRow.
+template <int LANES>
+__device__ __forceinline__ float squaresOfHalves(const float (&x)[8], int lane, int D) {
+  if (LANES == 8 && D == 64) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = __fadd_rn(__fmul_rn(x[i], x[i]), __fmul_rn(x[4 + i], x[4 + i]));
+#pragma unroll
+    for (int o = 4; o > 1; o >>= 1) {  // keeps the upper half of what it has where its bit o is set
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < o / 2; i++) {
+        const float got = __shfl_xor_sync(~0u, up ? v[i] : v[i + o / 2], o);
+        v[i] = __fadd_rn(up ? v[i + o / 2] : v[i], got);
+      }
+    }
+    v[0] = __fadd_rn(v[0], __shfl_xor_sync(~0u, v[0], 1));
+    v[0] = __fadd_rn(v[0], __shfl_xor_sync(~0u, v[0], 4));
+    return __fadd_rn(v[0], __shfl_xor_sync(~0u, v[0], 2));
+  }
+  float s = __fadd_rn(four(x), four(x + 4));
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) s = __fadd_rn(s, __shfl_xor_sync(~0u, s, o));
+  return s;
+}
+
+// rotate() for rows in halves.
+template <int LANES, bool BACK>
+__device__ __forceinline__ void rotateHalves(float (&x)[8], int lane, int D, const Rope& r, const float* angles) {
+  const float* up = angles + (BACK ? 2 : 1) * r.half;    // what the second channel of a pair takes
+  const float* down = angles + (BACK ? 1 : 2) * r.half;  // what the first one takes
+  if (r.interleaved) {
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+      const int first = (v ? D / 2 : 0) + 4 * lane;
+      if (first < 2 * r.half && 8 * lane < D) {
+        const float2 c = *reinterpret_cast<const float2*>(angles + first / 2);
+        const float2 u = *reinterpret_cast<const float2*>(up + first / 2), d = *reinterpret_cast<const float2*>(down + first / 2);
+        const float cc[2] = {c.x, c.y}, uu[2] = {u.x, u.y}, dd[2] = {d.x, d.y};
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const float a = x[4 * v + 2 * i], b = x[4 * v + 2 * i + 1];
+          x[4 * v + 2 * i] = __fadd_rn(__fmul_rn(a, cc[i]), __fmul_rn(b, dd[i]));
+          x[4 * v + 2 * i + 1] = __fadd_rn(__fmul_rn(b, cc[i]), __fmul_rn(a, uu[i]));
+        }
+      }
+    }
+    return;
+  }
+  if (2 * r.half == D) {
+    if (8 * lane < D) {
+      const float4 c = *reinterpret_cast<const float4*>(angles + 4 * lane), s = *reinterpret_cast<const float4*>(up + 4 * lane);
+      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float a = x[i], b = x[4 + i];
+        x[i] = __fsub_rn(__fmul_rn(a, cc[i]), __fmul_rn(b, ss[i]));
+        x[4 + i] = __fadd_rn(__fmul_rn(b, cc[i]), __fmul_rn(a, ss[i]));
+      }
+    }
+    return;
+  }
+  // Some channels rotate: the partners of a lane's channels are in other lanes.
+  float y[8];
+#pragma unroll
+  for (int v = 0; v < 2; v++) {
+    const int first = (v ? D / 2 : 0) + 4 * lane;
+    const int partner = first < r.half ? first + r.half : first < 2 * r.half ? first - r.half : first;
+    const int at = min(partner >= D / 2 ? partner - D / 2 : partner, D / 2 - 4) / 4;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float a = __shfl_sync(~0u, x[i], at, LANES), b = __shfl_sync(~0u, x[4 + i], at, LANES);
+      y[4 * v + i] = partner >= D / 2 ? b : a;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < 2; v++) {
+    const int first = (v ? D / 2 : 0) + 4 * lane;
+    if (first < 2 * r.half && 8 * lane < D) {
+      const bool low = first < r.half;
+      const int j = low ? first : first - r.half;
+      const float4 c = *reinterpret_cast<const float4*>(angles + j), s = *reinterpret_cast<const float4*>((low ? down : up) + j);
+      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[4 * v + i] = __fadd_rn(__fmul_rn(x[4 * v + i], cc[i]), __fmul_rn(y[4 * v + i], ss[i]));
+    }
+  }
+}
+
+struct NormRopeArgs {
+  Side side[2];  // queries, keys
   Rope rope;
-  Cache cache;  // data == nullptr: no cache
-  const int* slots;
   int tokens, D, tpb;
 };
 
 // Block: tpb tokens, all their heads.  Norm and rotation round after every
-// f32 operation (no contraction), so that the fused write gives the bits of
-// the two calls it stands for.
-template <typename T, int LANES, int KINDS>
-__global__ void __launch_bounds__(kThreads, 4) forwardKernel(const __grid_constant__ ForwardArgs p) {
+// f32 operation (no contraction): the bits of elementary operations, and of
+// the write to the cache.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kThreads, 4) normRopeKernel(const __grid_constant__ NormRopeArgs p) {
   extern __shared__ float4 shared[];
   float* weights = reinterpret_cast<float*>(shared);
   float* angles = weights + 2 * p.D;
   const int t0 = blockIdx.x * p.tpb, n = min(p.tpb, p.tokens - t0);
   const int lane = threadIdx.x % LANES;
   const bool active = 8 * lane < p.D;
-  const Steps<KINDS> steps = stepsOf<KINDS, LANES>(p.side, n);
+  const Steps<2> steps = stepsOf<2, LANES>(p.side, n);
+
+  Row ahead;
+  uint4 rawAhead;
+  auto load = [&](int step) {
+    ahead = rowOf<2, LANES>(p.side, steps, step, n, active);
+    rawAhead = make_uint4(0, 0, 0, 0);
+    if (ahead.live) rawAhead = loadHalves(inOf<T>(p.side[ahead.kind], t0 + ahead.t, ahead.h), lane, p.D);
+  };
+  int step = threadIdx.x >> 5;
+  load(step);
+  fillWeights<T>(p.rope, p.D, weights);
+  fillAngles(p.rope, t0, n, angles);
+  __syncthreads();
+  const float share = 1.0f / p.D;
+  for (; step < steps.end[1]; step += kThreads / 32) {
+    const Row row = ahead;
+    float x[8];
+    unpack8<T>(rawAhead, x);
+    load(step + kThreads / 32);
+    if (p.rope.weight[row.kind] != nullptr) {
+      const float r = rsqrtf(__fadd_rn(__fmul_rn(squaresOfHalves<LANES>(x, lane, p.D), share), p.rope.eps));
+      if (active) {
+        float w[8];
+        loadHalves(weights + row.kind * p.D, lane, p.D, w);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
+      }
+    }
+    rotateHalves<LANES, false>(x, lane, p.D, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
+    if (row.live) storeHalves(outOf<T>(p.side[row.kind], t0 + row.t, row.h), lane, p.D, pack8<T>(x));
+  }
+}
+
+struct AppendArgs {
+  Side side[3];  // queries, keys, values (of which queries alone are written as they are)
+  Rope rope;
+  Cache cache;
+  const int* slots;
+  int tokens, D, tpb;
+};
+
+// Block: tpb tokens, all their heads; without a rotation keys and values go to
+// the cache as they are.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kThreads, 4) appendKernel(const __grid_constant__ AppendArgs p) {
+  extern __shared__ float4 shared[];
+  float* weights = reinterpret_cast<float*>(shared);
+  float* angles = weights + 2 * p.D;
+  const int t0 = blockIdx.x * p.tpb, n = min(p.tpb, p.tokens - t0);
+  const int lane = threadIdx.x % LANES;
+  const bool active = 8 * lane < p.D;
+  const Steps<3> steps = stepsOf<3, LANES>(p.side, n);
   const bool normed = p.rope.weight[0] != nullptr || p.rope.weight[1] != nullptr;
 
   Row ahead;
   uint4 rawAhead;
   int slotAhead = -1;
   auto load = [&](int step) {
-    ahead = rowOf<KINDS, LANES>(p.side, steps, step, n, active);
+    ahead = rowOf<3, LANES>(p.side, steps, step, n, active);
     rawAhead = make_uint4(0, 0, 0, 0);
     if (ahead.live) {
       rawAhead = *reinterpret_cast<const uint4*>(inOf<T>(p.side[ahead.kind], t0 + ahead.t, ahead.h) + 8 * lane);
-      if (KINDS == 3) slotAhead = p.slots[t0 + ahead.t];
+      slotAhead = p.slots[t0 + ahead.t];
     }
   };
   int step = threadIdx.x >> 5;
@@ -283,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 4) forwardKernel(const __grid_consta
     __syncthreads();
   }
   const float share = 1.0f / p.D;
-  for (; step < steps.end[KINDS - 1]; step += kThreads / 32) {
+  for (; step < steps.end[3 - 1]; step += kThreads / 32) {
     const Row row = ahead;
     const int slot = slotAhead;
     uint4 raw = rawAhead;
@@ -305,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 4) forwardKernel(const __grid_consta
       if (row.live && p.side[row.kind].out != nullptr)
         *reinterpret_cast<uint4*>(outOf<T>(p.side[row.kind], t0 + row.t, row.h) + 8 * lane) = raw;
     }
-    if (KINDS == 3 && row.kind > 0) {
+    if (row.kind > 0) {
       uint32_t params;
       const uint32_t word = kv4::quantise8<T>(raw, &params);
       if (row.live && slot >= 0 && slot < p.cache.tokens) {
@@ -398,9 +564,9 @@ __global__ void __launch_bounds__(kThreads, 3) backwardKernel(const __grid_const
       ahead = rowOf<2, LANES>(p.side, steps, step, n, active);
       dyAhead = xAhead = make_uint4(0, 0, 0, 0);
       if (ahead.live) {
-        dyAhead = *reinterpret_cast<const uint4*>(inOf<T>(p.side[ahead.kind], t0 + ahead.t, ahead.h) + 8 * lane);
+        dyAhead = loadHalves(inOf<T>(p.side[ahead.kind], t0 + ahead.t, ahead.h), lane, p.D);
         if (p.rope.weight[ahead.kind] != nullptr)
-          xAhead = *reinterpret_cast<const uint4*>(inOf<T>(p.forward[ahead.kind], t0 + ahead.t, ahead.h) + 8 * lane);
+          xAhead = loadHalves(inOf<T>(p.forward[ahead.kind], t0 + ahead.t, ahead.h), lane, p.D);
       }
     };
     int step = threadIdx.x >> 5;
@@ -414,10 +580,10 @@ __global__ void __launch_bounds__(kThreads, 3) backwardKernel(const __grid_const
       unpack8<T>(dyAhead, g);
       unpack8<T>(xAhead, x);
       load(step + kThreads / 32);
-      rotate<LANES, true>(g, lane, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
+      rotateHalves<LANES, true>(g, lane, p.D, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
       if (p.rope.weight[row.kind] != nullptr) {
         float w[8] = {};
-        if (active) load8(weights + row.kind * p.D + 8 * lane, w);
+        if (active) loadHalves(weights + row.kind * p.D, lane, p.D, w);
         float sq = 0.0f, gx = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -444,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 3) backwardKernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < 8; i++) g[i] = r * fmaf(-(x[i] * on), m, w[i]);
       }
-      if (row.live) *reinterpret_cast<uint4*>(outOf<T>(p.side[row.kind], t0 + row.t, row.h) + 8 * lane) = pack8<T>(g);
+      if (row.live) storeHalves(outOf<T>(p.side[row.kind], t0 + row.t, row.h), lane, p.D, pack8<T>(g));
     }
   }
   if (p.partial == nullptr) return;
@@ -456,7 +622,8 @@ __global__ void __launch_bounds__(kThreads, 3) backwardKernel(const __grid_const
   for (int which = 0; which < 2; which++) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; i++) sums[row0 * (LANES * 8) + 8 * lane + i] = dw[which][i];
+    for (int i = 0; i < 8; i++)
+      if (active) sums[row0 * (LANES * 8) + (i < 4 ? 0 : p.D / 2) + 4 * lane + (i & 3)] = dw[which][i];
     __syncthreads();
     for (int d = threadIdx.x; d < p.D; d += kThreads) {
       float s = 0.0f;
@@ -532,18 +699,23 @@ Rope ropeOf(const vcclRope_t* r) {
   return {r->positions, r->invFreq, {r->qWeight, r->kWeight}, r->half, r->interleaved, r->eps};
 }
 
-template <typename T, int KINDS>
-void launchForward(const ForwardArgs& p, cudaStream_t st) {
+template <typename T>
+void launchNormRope(const NormRopeArgs& p, cudaStream_t st) {
   const int grid = (p.tokens + p.tpb - 1) / p.tpb;
   const size_t smem = sharedBytes(p.rope, p.tpb, p.D);
   switch (lanesFor(p.D)) {
-    case 8: forwardKernel<T, 8, KINDS><<<grid, kThreads, smem, st>>>(p); break;
-    case 16: forwardKernel<T, 16, KINDS><<<grid, kThreads, smem, st>>>(p); break;
-    default:
-      // the cache holds rows of 64 or 128 channels
-      if constexpr (KINDS == 2) forwardKernel<T, 32, KINDS><<<grid, kThreads, smem, st>>>(p);
-      break;
+    case 8: normRopeKernel<T, 8><<<grid, kThreads, smem, st>>>(p); break;
+    case 16: normRopeKernel<T, 16><<<grid, kThreads, smem, st>>>(p); break;
+    default: normRopeKernel<T, 32><<<grid, kThreads, smem, st>>>(p); break;
   }
+}
+
+template <typename T>
+void launchAppend(const AppendArgs& p, cudaStream_t st) {
+  const int grid = (p.tokens + p.tpb - 1) / p.tpb;
+  const size_t smem = sharedBytes(p.rope, p.tpb, p.D);
+  if (p.D == 64) appendKernel<T, 8><<<grid, kThreads, smem, st>>>(p);
+  else appendKernel<T, 16><<<grid, kThreads, smem, st>>>(p);
 }
 
 template <typename T>
@@ -591,7 +763,7 @@ vcclResult_t vcclQkNormRope(const vcclHeads_t* q, const vcclHeads_t* k, const vc
       k->heads != kOut->heads)
     return vcclInvalidArgument;
   TraceRange trace("vccl QkNormRope");
-  ForwardArgs p{};
+  NormRopeArgs p{};
   p.side[0] = sideOf(q, qOut);
   p.side[1] = sideOf(k, kOut);
   p.rope = ropeOf(rope);
@@ -599,8 +771,8 @@ vcclResult_t vcclQkNormRope(const vcclHeads_t* q, const vcclHeads_t* k, const vc
   p.D = D;
   p.tpb = tokensPerBlock(tokens, q->heads + k->heads, D);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (datatype == vcclBfloat16) launchForward<__nv_bfloat16, 2>(p, st);
-  else launchForward<__half, 2>(p, st);
+  if (datatype == vcclBfloat16) launchNormRope<__nv_bfloat16>(p, st);
+  else launchNormRope<__half>(p, st);
   return launched("vcclQkNormRope");
 }
 
@@ -664,7 +836,7 @@ vcclResult_t vcclKv4Append(const vcclKv4_t* cache, const vcclHeads_t* k, const v
     return vcclInvalidArgument;
   if (q != nullptr && (!headsOk(q, 2) || !headsOk(qOut, 2) || q->heads != qOut->heads)) return vcclInvalidArgument;
   TraceRange trace("vccl Kv4Append");
-  ForwardArgs p{};
+  AppendArgs p{};
   p.side[0] = sideOf(q, qOut);
   p.side[1] = sideOf(k, nullptr);
   p.side[2] = sideOf(v, nullptr);
@@ -675,8 +847,8 @@ vcclResult_t vcclKv4Append(const vcclKv4_t* cache, const vcclHeads_t* k, const v
   p.D = cache->D;
   p.tpb = tokensPerBlock(tokens, p.side[0].heads + 2 * cache->kvHeads, cache->D);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (datatype == vcclBfloat16) launchForward<__nv_bfloat16, 3>(p, st);
-  else launchForward<__half, 3>(p, st);
+  if (datatype == vcclBfloat16) launchAppend<__nv_bfloat16>(p, st);
+  else launchAppend<__half>(p, st);
   return launched("vcclKv4Append");
 }
 
