@@ -19,6 +19,8 @@
 // (queries, keys or values), whose strides and weights are then uniform, the
 // token and head come from a product with a reciprocal, and the next step's
 // row is loaded before this one is worked on.
+#include <type_traits>
+
 #include "kernels/kv4.cuh"
 #include "model/common.cuh"
 
@@ -62,48 +64,49 @@ struct Side {
   uint32_t recip;  // ceil(2^32 / heads); 0 for one head
 };
 
-// Where a warp's step stands: row r of a kind in a block of tokens.
+// Where a lane's row stands in a block of tokens.
 struct Row {
-  int kind, t, h;
+  int t, h;
   bool live;
 };
 
-template <int KINDS>
-struct Steps {
-  int end[KINDS];  // steps up to and including a kind
-};
-
-template <int KINDS, int LANES>
-__device__ __forceinline__ Steps<KINDS> stepsOf(const Side* side, int n) {
-  constexpr int kPerWarp = 32 / LANES;
-  Steps<KINDS> s;
-  int e = 0;
-#pragma unroll
-  for (int k = 0; k < KINDS; k++) {
-    e += (n * side[k].heads + kPerWarp - 1) / kPerWarp;
-    s.end[k] = e;
-  }
-  return s;
-}
-
-template <int KINDS, int LANES>
-__device__ __forceinline__ Row rowOf(const Side* side, const Steps<KINDS>& s, int step, int n, bool active) {
-  constexpr int kPerWarp = 32 / LANES;
+template <int LANES>
+__device__ __forceinline__ Row rowOf(const Side& d, int step, int n, bool active) {
+  const int row = step * (32 / LANES) + (threadIdx.x & 31) / LANES;
   Row r;
-  r.kind = 0;
-  int first = 0;
-#pragma unroll
-  for (int k = 1; k < KINDS; k++)
-    if (step >= s.end[k - 1]) {
-      r.kind = k;
-      first = s.end[k - 1];
-    }
-  const int row = (step - first) * kPerWarp + (threadIdx.x & 31) / LANES;
-  const Side& d = side[r.kind];
   r.t = d.recip ? static_cast<int>(__umulhi(static_cast<uint32_t>(row), d.recip)) : row;
   r.h = row - r.t * d.heads;
-  r.live = active && r.t < n && step < s.end[KINDS - 1];
+  r.live = active && r.t < n;
   return r;
+}
+
+template <int LANES>
+__device__ __forceinline__ int stepsOf(const Side& d, int n) {
+  return (n * d.heads + 32 / LANES - 1) / (32 / LANES);
+}
+
+// A warp's steps of one kind after `before` steps of the kinds ahead, which
+// the block's warps took in turn.  load(row) fetches, work(row) uses what was
+// fetched one step before.  A kind is a constant of the code: its strides and
+// weights are operands, not look-ups (14 a step of 205 instructions).
+template <int LANES, typename Load, typename Work>
+__device__ __forceinline__ void eachRow(const Side& d, int before, int n, bool active, Load&& load, Work&& work) {
+  constexpr int kWarps = kThreads / 32;
+  const int end = stepsOf<LANES>(d, n);
+  int step = ((threadIdx.x >> 5) - before) & (kWarps - 1);
+  if (step >= end) return;
+  Row ahead = rowOf<LANES>(d, step, n, active);
+  load(ahead);
+  while (step < end) {
+    const Row row = ahead;
+    step += kWarps;
+    work(row, [&]() {
+      if (step < end) {
+        ahead = rowOf<LANES>(d, step, n, active);
+        load(ahead);
+      }
+    });
+  }
 }
 
 template <typename T>
@@ -375,38 +378,34 @@ __global__ void __launch_bounds__(kThreads, 4) normRopeKernel(const __grid_const
   const int t0 = blockIdx.x * p.tpb, n = min(p.tpb, p.tokens - t0);
   const int lane = threadIdx.x % LANES;
   const bool active = 8 * lane < p.D;
-  const Steps<2> steps = stepsOf<2, LANES>(p.side, n);
-
-  Row ahead;
-  uint4 rawAhead;
-  auto load = [&](int step) {
-    ahead = rowOf<2, LANES>(p.side, steps, step, n, active);
-    rawAhead = make_uint4(0, 0, 0, 0);
-    if (ahead.live) rawAhead = loadHalves(inOf<T>(p.side[ahead.kind], t0 + ahead.t, ahead.h), lane, p.D);
-  };
-  int step = threadIdx.x >> 5;
-  load(step);
   fillWeights<T>(p.rope, p.D, weights);
   fillAngles(p.rope, t0, n, angles);
   __syncthreads();
   const float share = 1.0f / p.D;
-  for (; step < steps.end[1]; step += kThreads / 32) {
-    const Row row = ahead;
-    float x[8];
-    unpack8<T>(rawAhead, x);
-    load(step + kThreads / 32);
-    if (p.rope.weight[row.kind] != nullptr) {
-      const float r = rsqrtf(__fadd_rn(__fmul_rn(squaresOfHalves<LANES>(x, lane, p.D), share), p.rope.eps));
-      if (active) {
-        float w[8];
-        loadHalves(weights + row.kind * p.D, lane, p.D, w);
+  auto rows = [&](const Side& d, const void* weight, const float* w0, int before) {
+    uint4 ahead;
+    eachRow<LANES>(
+        d, before, n, active,
+        [&](const Row& r) { ahead = r.live ? loadHalves(inOf<T>(d, t0 + r.t, r.h), lane, p.D) : make_uint4(0, 0, 0, 0); },
+        [&](const Row& row, auto&& next) {
+          float x[8];
+          unpack8<T>(ahead, x);
+          next();
+          if (weight != nullptr) {
+            const float r = rsqrtf(__fadd_rn(__fmul_rn(squaresOfHalves<LANES>(x, lane, p.D), share), p.rope.eps));
+            if (active) {
+              float w[8];
+              loadHalves(w0, lane, p.D, w);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
-      }
-    }
-    rotateHalves<LANES, false>(x, lane, p.D, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
-    if (row.live) storeHalves(outOf<T>(p.side[row.kind], t0 + row.t, row.h), lane, p.D, pack8<T>(x));
-  }
+              for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
+            }
+          }
+          rotateHalves<LANES, false>(x, lane, p.D, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
+          if (row.live) storeHalves(outOf<T>(d, t0 + row.t, row.h), lane, p.D, pack8<T>(x));
+        });
+  };
+  rows(p.side[0], p.rope.weight[0], weights, 0);
+  rows(p.side[1], p.rope.weight[1], weights + p.D, stepsOf<LANES>(p.side[0], n));
 }
 
 struct AppendArgs {
@@ -426,65 +425,75 @@ __global__ void __launch_bounds__(kThreads, 4) appendKernel(const __grid_constan
   float* angles = weights + 2 * p.D;
   const int t0 = blockIdx.x * p.tpb, n = min(p.tpb, p.tokens - t0);
   const int lane = threadIdx.x % LANES;
-  const bool active = 8 * lane < p.D;
-  const Steps<3> steps = stepsOf<3, LANES>(p.side, n);
-  const bool normed = p.rope.weight[0] != nullptr || p.rope.weight[1] != nullptr;
-
-  Row ahead;
-  uint4 rawAhead;
-  int slotAhead = -1;
-  auto load = [&](int step) {
-    ahead = rowOf<3, LANES>(p.side, steps, step, n, active);
-    rawAhead = make_uint4(0, 0, 0, 0);
-    if (ahead.live) {
-      rawAhead = *reinterpret_cast<const uint4*>(inOf<T>(p.side[ahead.kind], t0 + ahead.t, ahead.h) + 8 * lane);
-      slotAhead = p.slots[t0 + ahead.t];
-    }
-  };
-  int step = threadIdx.x >> 5;
-  load(step);
-  if (p.rope.half > 0) {
-    if (normed) fillWeights<T>(p.rope, p.D, weights);
+  const int G = p.D / kv4::kGroup, g = lane >> 3, b = lane & 7;
+  const bool turned = p.rope.half > 0;
+  if (turned) {
+    fillWeights<T>(p.rope, p.D, weights);
     fillAngles(p.rope, t0, n, angles);
     __syncthreads();
   }
   const float share = 1.0f / p.D;
-  for (; step < steps.end[3 - 1]; step += kThreads / 32) {
-    const Row row = ahead;
-    const int slot = slotAhead;
-    uint4 raw = rawAhead;
-    load(step + kThreads / 32);
-    if (row.kind < 2 && p.rope.half > 0) {
-      float x[8];
-      unpack8<T>(raw, x);
-      if (p.rope.weight[row.kind] != nullptr) {
-        const float r = rsqrtf(__fadd_rn(__fmul_rn(squaresOfRow<LANES>(x, lane, p.D), share), p.rope.eps));
-        if (active) {
-          float w[8];
-          load8(weights + row.kind * p.D + 8 * lane, w);
+  // Norm and rotation of a row of queries or keys.
+  auto turn = [&](uint4& raw, const Row& row, const void* weight, const float* w0) {
+    float x[8];
+    unpack8<T>(raw, x);
+    if (weight != nullptr) {
+      const float r = rsqrtf(__fadd_rn(__fmul_rn(squaresOfRow<LANES>(x, lane, p.D), share), p.rope.eps));
+      float w[8];
+      load8(w0 + 8 * lane, w);
 #pragma unroll
-          for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
-        }
-      }
-      rotate<LANES, false>(x, lane, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
-      raw = pack8<T>(x);
-      if (row.live && p.side[row.kind].out != nullptr)
-        *reinterpret_cast<uint4*>(outOf<T>(p.side[row.kind], t0 + row.t, row.h) + 8 * lane) = raw;
+      for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
     }
-    if (row.kind > 0) {
-      uint32_t params;
-      const uint32_t word = kv4::quantise8<T>(raw, &params);
-      if (row.live && slot >= 0 && slot < p.cache.tokens) {
-        uint8_t* blk = cacheBlock(p.cache, slot, row.h);
-        const int place = slot & 15, G = p.D / kv4::kGroup, g = lane >> 3, b = lane & 7;
-        const bool keys = row.kind == 1;
-        const int rowAt = keys ? place : 16 + kv4::valueRow(place);
-        const int wordAt = keys ? kv4::keyWord(b, g, G) : kv4::valueWord(b, g, G);
-        *reinterpret_cast<uint32_t*>(blk + rowAt * (p.D / 2) + 4 * wordAt) = word;
-        if (b == 0) *reinterpret_cast<uint32_t*>(blk + (keys ? 16 : 17) * p.D + place * (4 * G) + 4 * g) = params;
-      }
-    }
+    rotate<LANES, false>(x, lane, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
+    raw = pack8<T>(x);
+  };
+  uint4 ahead;
+  int slotAhead = -1;
+  int before = 0;
+  if (turned) {
+    const Side& d = p.side[0];
+    eachRow<LANES>(
+        d, before, n, true,
+        [&](const Row& r) { ahead = r.live ? *reinterpret_cast<const uint4*>(inOf<T>(d, t0 + r.t, r.h) + 8 * lane) : make_uint4(0, 0, 0, 0); },
+        [&](const Row& row, auto&& next) {
+          uint4 raw = ahead;
+          next();
+          turn(raw, row, p.rope.weight[0], weights);
+          if (row.live) *reinterpret_cast<uint4*>(outOf<T>(d, t0 + row.t, row.h) + 8 * lane) = raw;
+        });
+    before = stepsOf<LANES>(d, n);
   }
+  auto store = [&](const Side& d, auto keys) {
+    // the row and the word of a lane's codes in a block, but for the token
+    const int wordAt = 4 * (keys ? kv4::keyWord(b, g, G) : kv4::valueWord(b, g, G));
+    eachRow<LANES>(
+        d, before, n, true,
+        [&](const Row& r) {
+          ahead = make_uint4(0, 0, 0, 0);
+          slotAhead = -1;
+          if (r.live) {
+            ahead = *reinterpret_cast<const uint4*>(inOf<T>(d, t0 + r.t, r.h) + 8 * lane);
+            slotAhead = p.slots[t0 + r.t];
+          }
+        },
+        [&](const Row& row, auto&& next) {
+          uint4 raw = ahead;
+          const int slot = slotAhead;
+          next();
+          if (keys && turned) turn(raw, row, p.rope.weight[1], weights + p.D);
+          uint32_t params;
+          const uint32_t word = kv4::quantise8<T>(raw, &params);
+          if (slot >= 0 && slot < p.cache.tokens) {
+            uint8_t* blk = cacheBlock(p.cache, slot, row.h);
+            const int place = slot & 15, rowAt = keys ? place : 16 + kv4::valueRow(place);
+            *reinterpret_cast<uint32_t*>(blk + rowAt * (p.D / 2) + wordAt) = word;
+            if (b == 0) *reinterpret_cast<uint32_t*>(blk + (keys ? 16 : 17) * p.D + place * (4 * G) + 4 * g) = params;
+          }
+        });
+    before += stepsOf<LANES>(d, n);
+  };
+  store(p.side[1], std::true_type{});
+  store(p.side[2], std::false_type{});
 }
 
 struct ReadArgs {
@@ -510,25 +519,30 @@ __global__ void __launch_bounds__(kThreads) readKernel(const __grid_constant__ R
   constexpr int D = 8 * LANES, G = D / kv4::kGroup;
   const int t0 = blockIdx.x * p.tpb, n = min(p.tpb, p.tokens - t0);
   const int lane = threadIdx.x % LANES, g = lane >> 3, b = lane & 7;
-  const Steps<2> steps = stepsOf<2, LANES>(p.side, n);
-#pragma unroll 2
-  for (int step = threadIdx.x >> 5; step < steps.end[1]; step += kThreads / 32) {
-    const Row row = rowOf<2, LANES>(p.side, steps, step, n, true);
-    if (!row.live) continue;
-    const bool keys = row.kind == 0;
-    const int slot = p.slots[t0 + row.t];
-    float x[8] = {};
-    if (slot >= 0 && slot < p.cache.tokens) {
-      const uint8_t* blk = cacheBlock(p.cache, slot, row.h);
-      const int place = slot & 15;
-      const int rowAt = keys ? place : 16 + kv4::valueRow(place);
-      const int wordAt = keys ? kv4::keyWord(b, g, G) : kv4::valueWord(b, g, G);
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(blk + rowAt * (D / 2) + 4 * wordAt);
-      const uint32_t params = *reinterpret_cast<const uint32_t*>(blk + (keys ? 16 : 17) * D + place * (4 * G) + 4 * g);
-      kv4::dequantise8(word, params, x);
-    }
-    store8<T>(outOf<T>(p.side[row.kind], t0 + row.t, row.h) + 8 * lane, x);
-  }
+  auto rows = [&](const Side& d, auto keys, int before) {
+    const int wordAt = 4 * (keys ? kv4::keyWord(b, g, G) : kv4::valueWord(b, g, G));
+    uint32_t wordAhead = 0, paramsAhead = 0;
+    eachRow<LANES>(
+        d, before, n, true,
+        [&](const Row& row) {
+          wordAhead = paramsAhead = 0;  // reads as 0
+          const int slot = row.live ? p.slots[t0 + row.t] : -1;
+          if (slot >= 0 && slot < p.cache.tokens) {
+            const uint8_t* blk = cacheBlock(p.cache, slot, row.h);
+            const int place = slot & 15, rowAt = keys ? place : 16 + kv4::valueRow(place);
+            wordAhead = *reinterpret_cast<const uint32_t*>(blk + rowAt * (D / 2) + wordAt);
+            paramsAhead = *reinterpret_cast<const uint32_t*>(blk + (keys ? 16 : 17) * D + place * (4 * G) + 4 * g);
+          }
+        },
+        [&](const Row& row, auto&& next) {
+          float x[8];
+          kv4::dequantise8(wordAhead, paramsAhead, x);
+          next();
+          if (row.live) store8<T>(outOf<T>(d, t0 + row.t, row.h) + 8 * lane, x);
+        });
+  };
+  rows(p.side[0], std::true_type{}, 0);
+  rows(p.side[1], std::false_type{}, stepsOf<LANES>(p.side[0], n));
 }
 
 struct BackwardArgs {
@@ -557,61 +571,57 @@ __global__ void __launch_bounds__(kThreads, 3) backwardKernel(const __grid_const
   float dw[2][8] = {};
   for (int t0 = blockIdx.x * p.tpb; t0 < p.tokens; t0 += gridDim.x * p.tpb) {
     const int n = min(p.tpb, p.tokens - t0);
-    const Steps<2> steps = stepsOf<2, LANES>(p.side, n);
-    Row ahead;
-    uint4 dyAhead, xAhead;
-    auto load = [&](int step) {
-      ahead = rowOf<2, LANES>(p.side, steps, step, n, active);
-      dyAhead = xAhead = make_uint4(0, 0, 0, 0);
-      if (ahead.live) {
-        dyAhead = loadHalves(inOf<T>(p.side[ahead.kind], t0 + ahead.t, ahead.h), lane, p.D);
-        if (p.rope.weight[ahead.kind] != nullptr)
-          xAhead = loadHalves(inOf<T>(p.forward[ahead.kind], t0 + ahead.t, ahead.h), lane, p.D);
-      }
-    };
-    int step = threadIdx.x >> 5;
-    load(step);
     __syncthreads();  // the angles of the tokens before are read
     fillAngles(p.rope, t0, n, angles);
     __syncthreads();
-    for (; step < steps.end[1]; step += kThreads / 32) {
-      const Row row = ahead;
-      float g[8], x[8];
-      unpack8<T>(dyAhead, g);
-      unpack8<T>(xAhead, x);
-      load(step + kThreads / 32);
-      rotateHalves<LANES, true>(g, lane, p.D, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
-      if (p.rope.weight[row.kind] != nullptr) {
-        float w[8] = {};
-        if (active) loadHalves(weights + row.kind * p.D, lane, p.D, w);
-        float sq = 0.0f, gx = 0.0f;
+    auto rows = [&](const Side& d, const Side& forward, const void* weight, const float* w0, float (&dw)[8], int before) {
+      uint4 dyAhead, xAhead;
+      eachRow<LANES>(
+          d, before, n, active,
+          [&](const Row& r) {
+            dyAhead = xAhead = make_uint4(0, 0, 0, 0);
+            if (r.live) {
+              dyAhead = loadHalves(inOf<T>(d, t0 + r.t, r.h), lane, p.D);
+              if (weight != nullptr) xAhead = loadHalves(inOf<T>(forward, t0 + r.t, r.h), lane, p.D);
+            }
+          },
+          [&](const Row& row, auto&& next) {
+            float g[8], x[8];
+            unpack8<T>(dyAhead, g);
+            unpack8<T>(xAhead, x);
+            next();
+            rotateHalves<LANES, true>(g, lane, p.D, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
+            if (weight != nullptr) {
+              float w[8] = {};
+              if (active) loadHalves(w0, lane, p.D, w);
+              float sq = 0.0f, gx = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          sq = fmaf(x[i], x[i], sq);
-          w[i] *= g[i];
-          gx = fmaf(w[i], x[i], gx);
-        }
+              for (int i = 0; i < 8; i++) {
+                sq = fmaf(x[i], x[i], sq);
+                w[i] *= g[i];
+                gx = fmaf(w[i], x[i], gx);
+              }
 #pragma unroll
-        for (int o = 1; o < LANES; o <<= 1) {
-          sq += __shfl_xor_sync(~0u, sq, o);
-          gx += __shfl_xor_sync(~0u, gx, o);
-        }
-        const float r = rsqrtf(fmaf(sq, share, p.rope.eps));
-        const float m = gx * r * share;  // mean(w g x^)
-        // A row behind the last one counts as zero (its r may be infinite).
-        const float on = row.live ? r : 0.0f;
-        if (row.kind == 0) {
+              for (int o = 1; o < LANES; o <<= 1) {
+                sq += __shfl_xor_sync(~0u, sq, o);
+                gx += __shfl_xor_sync(~0u, gx, o);
+              }
+              const float r = rsqrtf(fmaf(sq, share, p.rope.eps));
+              // A row behind the last one counts as zero (its r may be infinite).
+              const float on = row.live ? r : 0.0f;
+              const float m = gx * on * on * share;  // r mean(w g x^): dx = r w g - x r m
+              const float mr = m * on;
 #pragma unroll
-          for (int i = 0; i < 8; i++) dw[0][i] = fmaf(g[i], x[i] * on, dw[0][i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; i++) dw[1][i] = fmaf(g[i], x[i] * on, dw[1][i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) g[i] = r * fmaf(-(x[i] * on), m, w[i]);
-      }
-      if (row.live) storeHalves(outOf<T>(p.side[row.kind], t0 + row.t, row.h), lane, p.D, pack8<T>(g));
-    }
+              for (int i = 0; i < 8; i++) {
+                dw[i] = fmaf(g[i] * on, x[i], dw[i]);
+                g[i] = fmaf(-x[i], mr, r * w[i]);
+              }
+            }
+            if (row.live) storeHalves(outOf<T>(d, t0 + row.t, row.h), lane, p.D, pack8<T>(g));
+          });
+    };
+    rows(p.side[0], p.forward[0], p.rope.weight[0], weights, dw[0], 0);
+    rows(p.side[1], p.forward[1], p.rope.weight[1], weights + p.D, dw[1], stepsOf<LANES>(p.side[0], n));
   }
   if (p.partial == nullptr) return;
   // Rows of the block, then the block's sums to its own place.
