@@ -901,7 +901,11 @@ int* chunkErrorFlag(cudaStream_t st) {
   std::lock_guard<std::mutex> lock(gFlagMu);
   if (gDevFlags[dev] == nullptr) {
     cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(st, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) return nullptr;
+    if (cudaStreamIsCapturing(st, &cs) != cudaSuccess) {
+      cudaGetLastError();  // another stream's capture forbids the question
+      return nullptr;
+    }
+    if (cs != cudaStreamCaptureStatusNone) return nullptr;
     int* h = nullptr;
     int* d = nullptr;
     if (cudaHostAlloc(reinterpret_cast<void**>(&h), 64, cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) return nullptr;
@@ -978,7 +982,7 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
                               const vcclHeads_t* out, float* lse, int zeroTail, void* workspace,
                               vcclDataType_t datatype, vcclStream_t stream) {
   if (!cacheOk(cache) || tokens < 0 || batch <= 0 || batch > kMaxBatch || width <= 0 ||
-      static_cast<long long>(width) * cache->pageSize > INT_MAX ||
+      static_cast<long long>(width) * cache->pageSize > (1 << 30) ||  // token numbers and a tile more fit an int
       (datatype != vcclBfloat16 && datatype != vcclFloat16))
     return vcclInvalidArgument;
   if (tokens == 0) return vcclSuccess;

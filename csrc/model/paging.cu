@@ -35,7 +35,10 @@ struct PlanArgs {
   int* kvLens;
   int* lensOut;
   int* countOut;
-  int* firstPages;  // [batch] place on the stack of the first page that a request takes
+  // [2 * batch + 1] place on the stack of the first page that a request takes;
+  // lengths and count after the step.  lensOut may be lens and countOut
+  // freeCount, which every block of the first kernel reads: the second writes.
+  int* scratch;
 };
 
 struct Pair {
@@ -148,13 +151,13 @@ __global__ void __launch_bounds__(kPlanThreads) planStateKernel(PlanArgs p) {
       p.qStarts[i + 1] = sEnd[i];
       if (i == 0) p.qStarts[0] = 0;
       p.kvLens[i] = granted ? static_cast<int>(left + n) : 0;
-      p.lensOut[i] = static_cast<int>(left + (granted ? n : 0));
+      p.scratch[p.batch + i] = static_cast<int>(left + (granted ? n : 0));
     }
   }
   __syncthreads();
   const int bottom = stack - taken;
-  for (int i = threadIdx.x; i < p.batch; i += kPlanThreads) p.firstPages[i] = bottom + sReleased[i];
-  if (threadIdx.x == 0) *p.countOut = bottom;
+  for (int i = threadIdx.x; i < p.batch; i += kPlanThreads) p.scratch[i] = bottom + sReleased[i];
+  if (threadIdx.x == 0) p.scratch[2 * p.batch] = bottom;
 }
 
 // Each row's request, position and slot; the first row of a page that its
@@ -165,6 +168,8 @@ __global__ void __launch_bounds__(256) planRowsKernel(PlanArgs p) {
   for (int i = threadIdx.x; i <= p.batch; i += blockDim.x) starts[i] = p.qStarts[i];
   __syncthreads();
   const int t = blockIdx.x * blockDim.x + threadIdx.x;
+  for (int i = t; i < p.batch; i += gridDim.x * blockDim.x) p.lensOut[i] = p.scratch[p.batch + i];
+  if (t == 0) *p.countOut = p.scratch[2 * p.batch];
   if (t >= p.tokens) return;
   int position = 0, slot = -1, who = -1;
   if (t < starts[p.batch]) {
@@ -179,7 +184,7 @@ __global__ void __launch_bounds__(256) planRowsKernel(PlanArgs p) {
       if (j < have) {
         page = *entry;
       } else {
-        page = p.pool[p.firstPages[who] + j - have];
+        page = p.pool[p.scratch[who] + j - have];
         if (t == start || position == j * p.page) *entry = page;
       }
       slot = page * p.page + position - j * p.page;
@@ -199,8 +204,8 @@ using namespace vccl;
 extern "C" vcclResult_t vcclPagePlan(const int* lens, const int* newLens, const unsigned char* finished, int* table,
                                      int* freePages, const int* freeCount, int batch, int width, int poolSize,
                                      int pageSize, int tokens, int* positions, int* slots, int* requests,
-                                     int* qStarts, int* kvLens, int* lensOut, int* countOut, int* firstPages, vcclStream_t stream) {
-  if (!lens || !newLens || !table || !freePages || !freeCount || !qStarts || !kvLens || !lensOut || !countOut || !firstPages ||
+                                     int* qStarts, int* kvLens, int* lensOut, int* countOut, int* scratch, vcclStream_t stream) {
+  if (!lens || !newLens || !table || !freePages || !freeCount || !qStarts || !kvLens || !lensOut || !countOut || !scratch ||
       batch <= 0 || batch > model::kPlanMaxBatch || width <= 0 || poolSize <= 0 || pageSize <= 0 || tokens < 0 ||
       static_cast<long long>(poolSize) * pageSize > INT_MAX || static_cast<long long>(width) * pageSize > INT_MAX ||
       (tokens > 0 && (!positions || !slots || !requests)))
@@ -208,7 +213,7 @@ extern "C" vcclResult_t vcclPagePlan(const int* lens, const int* newLens, const 
   TraceRange trace("vccl PagePlan");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const model::PlanArgs p{lens,     newLens, finished,  table, freePages, freeCount, batch,  width,   poolSize, pageSize,
-                          tokens,   positions, slots, requests, qStarts, kvLens, lensOut, countOut, firstPages};
+                          tokens,   positions, slots, requests, qStarts, kvLens, lensOut, countOut, scratch};
   const size_t smem = static_cast<size_t>(batch) * 2 * sizeof(int);
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(model::planStateKernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -221,6 +226,6 @@ extern "C" vcclResult_t vcclPagePlan(const int* lens, const int* newLens, const 
   // A thread for each page that the finished requests may hold, 148 blocks at most.
   const long long held = finished ? (static_cast<long long>(batch) * width + model::kPlanThreads - 1) / model::kPlanThreads : 0;
   model::planStateKernel<<<1 + static_cast<int>(held < 147 ? held : 147), model::kPlanThreads, smem, st>>>(p);
-  if (tokens > 0) model::planRowsKernel<<<(tokens + 255) / 256, 256, (batch + 1) * sizeof(int), st>>>(p);
+  model::planRowsKernel<<<tokens > 0 ? (tokens + 255) / 256 : 1, 256, (batch + 1) * sizeof(int), st>>>(p);
   return model::launched("vcclPagePlan");
 }

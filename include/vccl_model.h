@@ -41,11 +41,11 @@ extern "C" {
  * lensOut[i] = L_i + (granted ? n_i : 0); *countOut; and for each of the
  * tokens rows its position, slot (-1 if refused or behind the last row) and
  * request (-1 behind the last row).  lensOut may be lens, countOut may be
- * freeCount.  firstPages[batch] is scratch.  batch <= 8192. */
+ * freeCount.  scratch: 2 * batch + 1 words.  batch <= 8192. */
 vcclResult_t vcclPagePlan(const int* lens, const int* newLens, const unsigned char* finished, int* table,
                           int* freePages, const int* freeCount, int batch, int width, int poolSize, int pageSize,
                           int tokens, int* positions, int* slots, int* requests, int* qStarts, int* kvLens,
-                          int* lensOut, int* countOut, int* firstPages, vcclStream_t stream);
+                          int* lensOut, int* countOut, int* scratch, vcclStream_t stream);
 
 /* A [tokens, heads, D] tensor: pointer and strides in elements. */
 typedef struct {
@@ -114,7 +114,7 @@ vcclResult_t vcclKv4Read(const vcclKv4_t* cache, const int* slots, const vcclHea
  * A row that sees nothing is 0 with lse = -inf.  Rows behind the last
  * request: 0 and -inf with zeroTail, else left as they are.  Tokens on a page
  * outside of the cache are not seen.  q heads a multiple of kvHeads,
- * batch <= 4096.  workspace: vcclKv4AttentionWorkspace bytes. */
+ * batch <= 4096, width * pageSize <= 2^30.  workspace: vcclKv4AttentionWorkspace bytes. */
 size_t vcclKv4AttentionWorkspace(int batch, int tokens, int qHeads, int kvHeads, int D);
 vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, const int* table, int width,
                               const int* kvLens, const int* qStarts, int batch, int tokens, float scale,

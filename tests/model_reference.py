@@ -39,10 +39,11 @@ def plan(lens, new, finished, table, free, count, page, tokens):
                 table[i][have + j] = stack[bottom + first[i] + j]
         kv.append(left[i] + max(new[i], 0) if ok else 0)
         after.append(left[i] + (max(new[i], 0) if ok else 0))
-    pos, slots, who = [], [], []
-    for t in range(tokens):
-        i = next((i for i in range(len(lens)) if starts[i] <= t < starts[i + 1]), -1)
-        who.append(i)
+    pos, slots, who = [], [], [-1] * tokens
+    for i in range(len(lens)):
+        for t in range(starts[i], min(starts[i + 1], tokens)):
+            who[t] = i
+    for t, i in enumerate(who):
         if i >= 0 and grants[i][0]:
             p = left[i] + t - starts[i]
             pos.append(p)
@@ -93,12 +94,11 @@ def stored_values(x):
 
 
 def attention(q, k, v, kv_lens, q_starts, scale):
-    """q [T, Hq, D]; k, v: a list of [len, H, D] per request (f64).  Returns out, lse and, for bounds on the error,
-    sum p |v| (the size of the terms that are added up) and sqrt(sum p^2 (v - out)^2) (what independent errors of the
-    scores move out by)."""
+    """q [T, Hq, D]; k, v: a list of [len, H, D] per request (f64).  Returns out, lse and, for a bound on the error,
+    sum p |v| (the size of the terms that are added up)."""
     t, hq, d = q.shape
     out = torch.zeros(t, hq, d, dtype=torch.float64, device=q.device)
-    size, spread = torch.zeros_like(out), torch.zeros_like(out)
+    size = torch.zeros_like(out)
     lse = torch.full((t, hq), -math.inf, dtype=torch.float64, device=q.device)
     for b, n in enumerate(kv_lens):
         a, e = q_starts[b], q_starts[b + 1]
@@ -115,5 +115,4 @@ def attention(q, k, v, kv_lens, q_starts, scale):
             lse[i] = torch.logsumexp(sc, -1)
             out[i] = torch.einsum("hn,nhd->hd", p, vv[:see])
             size[i] = torch.einsum("hn,nhd->hd", p, vv[:see].abs())
-            spread[i] = torch.einsum("hn,nhd->hd", p ** 2, (vv[:see] - out[i]) ** 2).sqrt()
-    return out, lse, size, spread
+    return out, lse, size

@@ -22,7 +22,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from vkccl_b200._lib import lib
-from vkccl_b200.ops._args import DTYPES, cache4, call, float16s, fresh, heads, rope_of, vector
+from vkccl_b200.ops._args import DTYPES, cache4, call, on_device, float16s, fresh, heads, rope_of, vector
 
 MAX_BATCH = 4096
 
@@ -123,8 +123,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     batch, width = block_table.shape
     if batch > MAX_BATCH:
         raise ValueError(f"at most {MAX_BATCH} requests, got {batch}")
-    if width * page_size > 2**31 - 1 or t * n > 2**31 - 1:
-        raise ValueError("a request's tokens and the rows of all heads must fit in 31 bits")
+    if width * page_size > 2**30 or t * n > 2**31 - 1:
+        raise ValueError("a request has at most 2^30 tokens, and the rows of all heads fit in 31 bits")
     a_kv = vector(kv_lens, "kv_lens", torch.int32, batch, dev)
     a_q = vector(q_starts, "q_starts", torch.int32, batch + 1, dev)
     new = out is None
@@ -134,7 +134,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
         ho = heads(out, "out", dtype, dev, t, dim, n, True)
     lse = torch.empty((t, n), dtype=torch.float32, device=q.device) if return_lse else None
     h = lib()
-    ws = cache.new_empty(h.vcclKv4AttentionWorkspace(batch, t, n, kv_heads, dim))
+    with on_device(dev):  # the scratch goes by the device's SMs
+        ws = cache.new_empty(h.vcclKv4AttentionWorkspace(batch, t, n, kv_heads, dim))
     call(h.vcclKv4Attention, "vcclKv4Attention", dev, hq, c, block_table.data_ptr(), width, a_kv, a_q, batch, t,
          dim ** -0.5 if scale is None else scale, ho, None if lse is None else lse.data_ptr(), 1 if new else 0,
          ws.data_ptr(), DTYPES[dtype])

@@ -72,10 +72,10 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
         if finished.dtype not in (torch.bool, torch.uint8):
             raise ValueError("finished must be bool or uint8")
         a_done = vector(finished, "finished", finished.dtype, batch, dev)
-    buffer = lens.new_empty(3 * tokens + 4 * batch + 2)
+    buffer = lens.new_empty(3 * tokens + 5 * batch + 3)
     base = buffer.data_ptr()
     positions, slots, requests, q_starts, kv_lens, after, count, _ = buffer.split(
-        (tokens, tokens, tokens, batch + 1, batch, batch, 1, batch))
+        (tokens, tokens, tokens, batch + 1, batch, batch, 1, 2 * batch + 1))
     at = base + 12 * tokens
     a_after, a_left = at + 4 * (2 * batch + 1), at + 4 * (3 * batch + 1)
     if lens_out is not None:
