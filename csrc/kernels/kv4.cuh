@@ -93,7 +93,7 @@ __device__ __forceinline__ void pairToFloat<__half>(uint32_t v, float* lo, float
 // A group whose scale or midpoint is not finite is stored as NaN.
 //
 // Eight divisions a lane made the write of a prompt bound by instructions
-// (64 us for 16384 tokens of 8 heads, where the bytes take 13).  So
+// (64 us for 16384 tokens of 8 heads, 46 now; the bytes take 13).  So
 // code / 15 = (x - mid) / (15 scale) + 1/2 is a product with 1 / (15 scale),
 // held to [0, 1] by the instruction's saturation; 15 times that plus 96 rounds
 // to a multiple of 2^-17, which is more than it is off by: where the code is

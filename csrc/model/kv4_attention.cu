@@ -430,7 +430,7 @@ __device__ __forceinline__ void weighValues(Unit<G, NT>& u, float (&x)[kBlocks][
 
 // A tile of 32 tokens that starts at token t0 of the request.  Two blocks at a
 // time give the scheduler twice the independent work of one, and share the
-// looks at the maximum (one block at a time: 166 us where this takes 137, 64
+// looks at the maximum (one block at a time: 166 us where this took 146, 64
 // requests of 500 to 16000 tokens, 8 key heads).  there: bit b, block b exists.
 template <int G, int NT>
 __device__ __forceinline__ void tileStep(Unit<G, NT>& u, uint32_t tile, const LaneOffsets& at, int t0, uint32_t there, int lane) {
