@@ -27,6 +27,7 @@
 // lengths are; a warp that gets a whole unit writes the result, the others
 // write partial sums (unnormalised output, maximum, sum) that a second kernel
 // joins in order.
+#include <atomic>
 #include <cfloat>
 #include <climits>
 #include <mutex>
@@ -928,11 +929,24 @@ bool takeChunkError() {
   return true;
 }
 
+// Raises a kernel's shared-memory limit, once for each device.
+template <typename Kernel>
+cudaError_t allowShared(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <int G>
 cudaError_t launchChunk(const AttnArgs& p, long long units, cudaStream_t st) {
   const int fixed = ChunkSmem<G>::kStarts + 1024;
-  const cudaError_t e = cudaFuncSetAttribute(chunkKernel<G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             fixed + (kMaxBatch + 1) * static_cast<int>(sizeof(int)));
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allowShared(chunkKernel<G>, fixed + (kMaxBatch + 1) * static_cast<int>(sizeof(int)), done);
   if (e != cudaSuccess) return e;
   const int sms = smsOfDevice();
   chunkKernel<G><<<static_cast<int>(units < sms ? units : sms), kChunkThreads, fixed + (p.batch + 1) * sizeof(int), st>>>(p);
@@ -949,8 +963,8 @@ template <int G, int NT>
 cudaError_t launchAttn(const AttnArgs& p, int grid, cudaStream_t st) {
   constexpr int kRings = warpsFor(NT) * kStages * tileBytes<G>();
   const size_t smem = kRings + static_cast<size_t>(p.batch + 1) * sizeof(long long);
-  const cudaError_t e = cudaFuncSetAttribute(attnKernel<G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kRings + (kMaxBatch + 1) * static_cast<int>(sizeof(long long)));
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allowShared(attnKernel<G, NT>, kRings + (kMaxBatch + 1) * static_cast<int>(sizeof(long long)), done);
   if (e != cudaSuccess) return e;
   attnKernel<G, NT><<<grid, warpsFor(NT) * 32, smem, st>>>(p);
   return cudaGetLastError();

@@ -519,6 +519,10 @@ __global__ void __launch_bounds__(kThreads) readKernel(const __grid_constant__ R
   constexpr int D = 8 * LANES, G = D / kv4::kGroup;
   const int t0 = blockIdx.x * p.tpb, n = min(p.tpb, p.tokens - t0);
   const int lane = threadIdx.x % LANES, g = lane >> 3, b = lane & 7;
+  // The slots first, so that a row's codes are one load away.
+  __shared__ int slots[16];
+  if (threadIdx.x < n) slots[threadIdx.x] = p.slots[t0 + threadIdx.x];
+  __syncthreads();
   auto rows = [&](const Side& d, auto keys, int before) {
     const int wordAt = 4 * (keys ? kv4::keyWord(b, g, G) : kv4::valueWord(b, g, G));
     uint32_t wordAhead = 0, paramsAhead = 0;
@@ -526,7 +530,7 @@ __global__ void __launch_bounds__(kThreads) readKernel(const __grid_constant__ R
         d, before, n, true,
         [&](const Row& row) {
           wordAhead = paramsAhead = 0;  // reads as 0
-          const int slot = row.live ? p.slots[t0 + row.t] : -1;
+          const int slot = row.live ? slots[row.t] : -1;
           if (slot >= 0 && slot < p.cache.tokens) {
             const uint8_t* blk = cacheBlock(p.cache, slot, row.h);
             const int place = slot & 15, rowAt = keys ? place : 16 + kv4::valueRow(place);

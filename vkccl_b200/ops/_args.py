@@ -99,9 +99,9 @@ def heads(t, name: str, dtype: torch.dtype, index: int, tokens: int, dim: int, n
     return _HEADS(at, s0, s1, count)
 
 
-def fresh(like: torch.Tensor, tokens: int, n: int, dim: int):
-    """A new contiguous [tokens, n, D] tensor in like's type, and its structure."""
-    t = like.new_empty((tokens, n, dim))
+def fresh(like: torch.Tensor, tokens: int, n: int, dim: int, dtype=None):
+    """A new contiguous [tokens, n, D] tensor on like's device, in its type unless another is given, and its structure."""
+    t = like.new_empty((tokens, n, dim), dtype=dtype)
     return t, _HEADS(t.data_ptr(), n * dim, dim, n)
 
 

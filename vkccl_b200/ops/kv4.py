@@ -22,7 +22,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from vkccl_b200._lib import lib
-from vkccl_b200.ops._args import DTYPES, cache4, call, on_device, float16s, fresh, heads, rope_of, vector
+from vkccl_b200.ops._args import DTYPES, cache4, call, current_device, float16s, fresh, heads, on_device, rope_of, vector
 
 MAX_BATCH = 4096
 
@@ -86,11 +86,13 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torc
     t = slots.shape[0]
     at = vector(slots, "slots", torch.int32, t, dev)
     if k_out is None:
-        k_out = torch.empty((t, n, dim), dtype=dtype, device=cache.device)
+        k_out, ok = fresh(cache, t, n, dim, dtype)
+    else:
+        ok = heads(k_out, "k_out", dtype, dev, t, dim, n, True)
     if v_out is None:
-        v_out = torch.empty((t, n, dim), dtype=dtype, device=cache.device)
-    ok = heads(k_out, "k_out", dtype, dev, t, dim, n, True)
-    ov = heads(v_out, "v_out", dtype, dev, t, dim, n, True)
+        v_out, ov = fresh(cache, t, n, dim, dtype)
+    else:
+        ov = heads(v_out, "v_out", dtype, dev, t, dim, n, True)
     call(lib().vcclKv4Read, "vcclKv4Read", dev, c, at, ok, ov, t, DTYPES[dtype])
     return k_out, v_out
 
@@ -132,10 +134,14 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
         out, ho = fresh(q, t, n, dim)
     else:
         ho = heads(out, "out", dtype, dev, t, dim, n, True)
-    lse = torch.empty((t, n), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((t, n), dtype=torch.float32) if return_lse else None
     h = lib()
-    with on_device(dev):  # the scratch goes by the device's SMs
-        ws = cache.new_empty(h.vcclKv4AttentionWorkspace(batch, t, n, kv_heads, dim))
+    if current_device() == dev:
+        size = h.vcclKv4AttentionWorkspace(batch, t, n, kv_heads, dim)
+    else:  # the scratch goes by the device's SMs
+        with on_device(dev):
+            size = h.vcclKv4AttentionWorkspace(batch, t, n, kv_heads, dim)
+    ws = cache.new_empty(size)
     call(h.vcclKv4Attention, "vcclKv4Attention", dev, hq, c, block_table.data_ptr(), width, a_kv, a_q, batch, t,
          dim ** -0.5 if scale is None else scale, ho, None if lse is None else lse.data_ptr(), 1 if new else 0,
          ws.data_ptr(), DTYPES[dtype])
