@@ -285,28 +285,6 @@ __device__ __forceinline__ void loadScores(uint32_t at, uint32_t (&s)[32], uint3
   }
 }
 
-// Two f32 in one register pair, worked on by one instruction.
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ uint64_t pair(float x) { return pair(__float_as_uint(x), __float_as_uint(x)); }
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  uint32_t lo, hi;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
-  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -345,7 +323,10 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
   constexpr int D = 64 * G;
   const float2 keyUnit = *reinterpret_cast<const float2*>(info.keyUnit), valueExp = *reinterpret_cast<const float2*>(info.valueExp);
   const uint4 bad = *reinterpret_cast<const uint4*>(info.bad);
-  const float scale0 = unit * keyUnit.x, scale1 = unit * keyUnit.y;
+  // Not zero (a softmax scale of zero, or one next to it): unseen scores are
+  // -inf, and scores times the smallest number count nothing.
+  auto above = [](float x) { return x < FLT_MIN ? FLT_MIN : x; };
+  const float scale0 = above(unit * keyUnit.x), scale1 = above(unit * keyUnit.y);
   const float ref = fmaxf(r.ref, fmaxf(valueExp.x, valueExp.y));
   const uint32_t seen0 = EDGE ? seenOf(valid.x, left) : ~0u, seen1 = EDGE ? seenOf(valid.y, left - 32) : ~0u;
   float top = kNone;

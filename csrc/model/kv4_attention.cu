@@ -889,29 +889,35 @@ ChunkPlan chunkPlan(int batch, int tokens, int qHeads, int kvHeads) {
 }
 
 // One abort word per device in mapped host memory: a launch that gave up a
-// wait sets it, and the next call on that device reads it.  Not made while a
-// stream is captured (the launch then reports nothing).
+// wait sets it, and the next call on that device reads it.  Made at the first
+// launch, which may be a captured one: an allocation of host memory puts
+// nothing on a stream, so captures (this thread's and others') allow it in
+// relaxed mode.
 std::mutex gFlagMu;
 int* gHostFlags[64] = {};
 int* gDevFlags[64] = {};
 
-int* chunkErrorFlag(cudaStream_t st) {
+int* chunkErrorFlag() {
   int dev = 0;
   cudaGetDevice(&dev);
   dev &= 63;
   std::lock_guard<std::mutex> lock(gFlagMu);
   if (gDevFlags[dev] == nullptr) {
-    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(st, &cs) != cudaSuccess) {
-      cudaGetLastError();  // another stream's capture forbids the question
-      return nullptr;
-    }
-    if (cs != cudaStreamCaptureStatusNone) return nullptr;
     int* h = nullptr;
     int* d = nullptr;
-    if (cudaHostAlloc(reinterpret_cast<void**>(&h), 64, cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) return nullptr;
-    *h = 0;
-    if (cudaHostGetDevicePointer(reinterpret_cast<void**>(&d), h, 0) != cudaSuccess) return nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&h), 64, cudaHostAllocMapped | cudaHostAllocPortable);
+    if (e == cudaSuccess) {
+      *h = 0;
+      e = cudaHostGetDevicePointer(reinterpret_cast<void**>(&d), h, 0);
+      if (e != cudaSuccess) cudaFreeHost(h);
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
     gHostFlags[dev] = h;
     gDevFlags[dev] = d;
   }
@@ -1053,7 +1059,11 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
     p.chunkStats = reinterpret_cast<float2*>(ws);
     ws += align256(chunkSlots * sizeof(float2));
     p.chunkPartial = reinterpret_cast<float*>(ws);
-    p.errorFlag = chunkErrorFlag(st);
+    p.errorFlag = chunkErrorFlag();
+    if (p.errorFlag == nullptr) {
+      VERR("vcclKv4Attention: no host memory for the word that reports a launch that gave up");
+      return vcclSystemError;
+    }
     const cudaError_t c = cache->D == 128 ? launchChunk<2>(p, cp.units, st) : launchChunk<1>(p, cp.units, st);
     if (c != cudaSuccess) {
       VERR("vcclKv4Attention: %s", cudaGetErrorString(c));

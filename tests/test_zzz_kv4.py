@@ -530,6 +530,20 @@ def test_attention_extreme_sizes():
         check_attention(out, lse, q, [k.double()], [v.double()], [n], [0, 1], scale=scale)
 
 
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [40, 3, 70]])
+def test_attention_scale_is_any_number(scale, q_lens):
+    """A negative scale turns the order of the scores, zero makes all weights equal; both kernels."""
+    from vkccl_b200.ops.kv4 import kv4_attention
+
+    g = gen(23)
+    kv_lens, qs = [700, 90, 333], starts(q_lens)
+    cache, table, ks, vs = filled(g, kv_lens, 32, 1, 128)
+    q = randn(g, qs[-1], 8, 128)
+    out, lse = kv4_attention(q, cache, table, ints(kv_lens), ints(qs), return_lse=True, scale=scale)
+    check_attention(out, lse, q, ks, vs, kv_lens, qs, scale=scale)
+
+
 def test_attention_nan_where_it_belongs():
     """A NaN key or value reaches the rows that see it, and only those; garbage behind the end reaches none."""
     from vkccl_b200.ops.kv4 import kv4_attention, kv4_append
@@ -694,6 +708,36 @@ def test_serving_steps_match_dense_attention(captured):
         # round to neighbouring bf16 numbers: bounded in the norm of each row
         err = (out[:qs[-1]].double() - want[:qs[-1]]).norm(dim=-1) / (want[:qs[-1]].norm(dim=-1) + 1e-3)
         assert err.max().item() < 4 * 2.0**-8, err.max().item()
+
+
+FIRST_CAPTURED = """
+import torch
+from vkccl_b200.ops.kv4 import kv4_alloc, kv4_append, kv4_attention
+torch.manual_seed(1)
+cache = kv4_alloc(8, 32, 1, 128)
+k = torch.randn(256, 1, 128, device="cuda").bfloat16()
+kv4_append(cache, k, k, torch.arange(256, device="cuda", dtype=torch.int32))
+q = torch.randn(100, 8, 128, device="cuda").bfloat16()
+table = torch.arange(8, device="cuda", dtype=torch.int32).view(1, 8)
+lens, starts = torch.tensor([256], device="cuda", dtype=torch.int32), torch.tensor([0, 100], device="cuda", dtype=torch.int32)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = kv4_attention(q, cache, table, lens, starts)
+graph.replay()
+want = kv4_attention(q, cache, table, lens, starts)
+torch.cuda.synchronize()
+assert got.abs().max() > 0 and torch.equal(got, want)
+"""
+
+
+def test_first_call_of_a_process_may_be_captured():
+    """The word that reports a launch that gave up is made by the first call, inside the capture."""
+    import subprocess
+    import sys
+
+    done = subprocess.run([sys.executable, "-c", FIRST_CAPTURED], capture_output=True, text=True, timeout=200)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_two_streams_and_shared_inputs():

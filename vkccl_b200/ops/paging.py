@@ -55,11 +55,11 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     dev, batch = lens.get_device(), lens.shape[0]
     if not 1 <= batch <= MAX_BATCH:
         raise ValueError(f"1 to {MAX_BATCH} requests, got {batch}")
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch
+    if (not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch
             or block_table.shape[1] < 1 or block_table.get_device() != dev or not block_table.is_contiguous()):
         raise ValueError(f"block_table must be a contiguous int32 tensor [{batch}, pages per request] on CUDA device {dev}")
     width = block_table.shape[1]
-    if free_pages.dim() != 1 or free_pages.shape[0] < 1:
+    if not isinstance(free_pages, torch.Tensor) or free_pages.dim() != 1 or free_pages.shape[0] < 1:
         raise ValueError("free_pages must be a one-dimensional int32 tensor with room for every page")
     pool, page_size, tokens = free_pages.shape[0], int(page_size), int(tokens)
     if page_size < 1 or tokens < 0 or pool * page_size > 2**31 - 1 or width * page_size > 2**31 - 1:
@@ -69,7 +69,7 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     a_free, a_count = vector(free_pages, "free_pages", i32, pool, dev), vector(free_count, "free_count", i32, 1, dev)
     a_done = None
     if finished is not None:
-        if finished.dtype not in (torch.bool, torch.uint8):
+        if not isinstance(finished, torch.Tensor) or finished.dtype not in (torch.bool, torch.uint8):
             raise ValueError("finished must be bool or uint8")
         a_done = vector(finished, "finished", finished.dtype, batch, dev)
     buffer = lens.new_empty(3 * tokens + 5 * batch + 3)
