@@ -94,7 +94,9 @@ __device__ __forceinline__ int findStart(const int* starts, int n, int x) {
 // Block 0: lengths and grants.  The other blocks move the released pages onto
 // the stack, one a thread, whoever's they are (a warp for each request left
 // most warps idle behind a few long ones); every block takes the prefix sums
-// of the released pages for itself, so none waits for another.
+// of the released pages for itself, so none waits for another.  Latency bounds
+// the plan: 7 us for both kernels with 256 requests, 14 with 2000 requests of
+// 107777 rows that release 28 thousand pages (38 with a warp a request).
 __global__ void __launch_bounds__(kPlanThreads) planStateKernel(PlanArgs p) {
   extern __shared__ int scratch[];  // released pages before each request, rows up to and including it
   int* sReleased = scratch;
