@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "common/log.h"
 #include "common/trace.h"
 #include "vccl_model.h"
@@ -35,6 +37,19 @@ inline vcclResult_t launched(const char* what) {
   if (e == cudaSuccess) return vcclSuccess;
   VERR("%s: %s", what, cudaGetErrorString(e));
   return vcclSystemError;
+}
+
+// Raises a kernel's shared-memory limit, once for each device.
+template <typename Kernel>
+inline cudaError_t allowShared(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 // T is __nv_bfloat16 or __half.

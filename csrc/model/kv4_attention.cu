@@ -32,7 +32,6 @@
 // 64 heads on 8; the widening of codes bounds it (300 instructions a block of
 // 16 tokens, half of them on the ALU pipe).  One request of 900 tokens takes
 // 12 us, which is the latency of two launches and eight dependent loads.
-#include <atomic>
 #include <cfloat>
 #include <climits>
 #include <mutex>
@@ -938,19 +937,6 @@ bool takeChunkError() {
   if (h == nullptr || *h == 0) return false;
   *h = 0;
   return true;
-}
-
-// Raises a kernel's shared-memory limit, once for each device.
-template <typename Kernel>
-cudaError_t allowShared(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
-  return e;
 }
 
 template <int G>

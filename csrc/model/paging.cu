@@ -217,17 +217,19 @@ extern "C" vcclResult_t vcclPagePlan(const int* lens, const int* newLens, const 
   const model::PlanArgs p{lens,     newLens, finished,  table, freePages, freeCount, batch,  width,   poolSize, pageSize,
                           tokens,   positions, slots, requests, qStarts, kvLens, lensOut, countOut, scratch};
   const size_t smem = static_cast<size_t>(batch) * 2 * sizeof(int);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(model::planStateKernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               model::kPlanMaxBatch * 2 * static_cast<int>(sizeof(int)));
-    if (e != cudaSuccess) {
-      VERR("vcclPagePlan: %s", cudaGetErrorString(e));
-      return vcclSystemError;
-    }
+  // For every batch: what a kernel has without asking, 48 KiB, holds its static shared memory too.
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = model::allowShared(model::planStateKernel, model::kPlanMaxBatch * 2 * static_cast<int>(sizeof(int)), done);
+  if (e != cudaSuccess) {
+    VERR("vcclPagePlan: %s", cudaGetErrorString(e));
+    return vcclSystemError;
   }
   // A thread for each page that the finished requests may hold, 148 blocks at most.
   const long long held = finished ? (static_cast<long long>(batch) * width + model::kPlanThreads - 1) / model::kPlanThreads : 0;
   model::planStateKernel<<<1 + static_cast<int>(held < 147 ? held : 147), model::kPlanThreads, smem, st>>>(p);
+  // The rows are made from what the first kernel writes: without it they are not launched.
+  const vcclResult_t state = model::launched("vcclPagePlan");
+  if (state != vcclSuccess) return state;
   model::planRowsKernel<<<tokens > 0 ? (tokens + 255) / 256 : 1, 256, (batch + 1) * sizeof(int), st>>>(p);
   return model::launched("vcclPagePlan");
 }
