@@ -789,16 +789,25 @@ __global__ void __launch_bounds__(128) joinKernel(const __grid_constant__ AttnAr
   __shared__ float sums[WIDE ? 4 : 1][WIDE ? D : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long id = WIDE ? blockIdx.x : blockIdx.x * 4LL + warp;
-  if (id >= static_cast<long long>(p.tokens) * p.qHeads) return;
-  const int t = static_cast<int>(id / p.qHeads), h = static_cast<int>(id - static_cast<long long>(t) * p.qHeads);
-  const int b = requestOfRow(p, t, lane);
-  const Request r = b < p.batch ? requestOf(p, b) : Request{0, 0, 0};
-  const bool inside = t >= r.start && t < r.start + r.rows;
-  if (inside ? isLong(p, r) : !p.zeroTail) return;
+  int t = 0, h = 0, b = p.batch;
+  Request r{0, 0, 0};
+  bool inside = false, mine = false;
+  if (id < static_cast<long long>(p.tokens) * p.qHeads) {
+    t = static_cast<int>(id / p.qHeads);
+    h = static_cast<int>(id - static_cast<long long>(t) * p.qHeads);
+    b = requestOfRow(p, t, lane);
+    if (b < p.batch) r = requestOf(p, b);
+    inside = t >= r.start && t < r.start + r.rows;
+    mine = inside ? !isLong(p, r) : p.zeroTail != 0;
+  }
   const int nt = inside ? tilesOf(r) : 0;
   float y[2 * G] = {};
   float m = kNone, l = 0.0f;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial sums are there
+  // The partial sums are there.  Every thread waits, those without a row too:
+  // this grid may end only behind the one before it, whose scratch the next
+  // kernel on the stream may take.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!mine) return;
   if (nt > 0) {
     const int row = (t - r.start) * p.group + h % p.group, units = unitsOf(p, r, R);
     const long long total = p.prefix[p.batch];

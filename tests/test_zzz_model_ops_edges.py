@@ -45,3 +45,62 @@ def test_plan_first_of_a_process_takes_every_batch(batch):
     whichever batch it has."""
     done = subprocess.run([sys.executable, "-c", PLAN_FIRST, str(batch)], capture_output=True, text=True, timeout=200, cwd=ROOT)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# ---- attention: scratch ----------------------------------------------------------
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def raw_attention(q, cache, table, kv_lens, q_starts, out, workspace, zero_tail=0):
+    """The library's entry with scratch of the caller's."""
+    from vkccl_b200._lib import lib
+    from vkccl_b200.ops import _args
+
+    dev, (t, n, dim), (batch, width) = q.get_device(), q.shape, table.shape
+    c, _, _, _ = _args.cache4(cache, dim, dev)
+    _args.call(lib().vcclKv4Attention, "vcclKv4Attention", dev, _args.heads(q, "q", q.dtype, dev, t, dim), c, table.data_ptr(), width,
+               kv_lens.data_ptr(), q_starts.data_ptr(), batch, t, dim ** -0.5, _args.heads(out, "out", q.dtype, dev, t, dim, n, True),
+               None, zero_tail, workspace.data_ptr(), _args.DTYPES[q.dtype])
+
+
+def workspace_bytes(batch, tokens, heads, kv_heads, dim):
+    from vkccl_b200._lib import lib
+
+    return lib().vcclKv4AttentionWorkspace(batch, tokens, heads, kv_heads, dim)
+
+
+def random_cache(g, pages, page, kv_heads, dim):
+    from vkccl_b200.ops.kv4 import kv4_alloc, kv4_append
+
+    cache = kv4_alloc(pages, page, kv_heads, dim)
+    kv = torch.randn(pages * page, 2 * kv_heads, dim, device="cuda", generator=g).bfloat16()
+    kv4_append(cache, kv[:, :kv_heads], kv[:, kv_heads:], torch.arange(pages * page, dtype=torch.int32, device="cuda"))
+    return cache
+
+
+@pytest.mark.parametrize("tokens,starts", [(4096, [0, 1024, 2048, 3072, 4096]), (640, [0, 0, 0, 0, 0])])
+def test_scratch_is_free_when_the_call_is_over(tokens, starts):
+    """Requests that are all long, or no rows at all: the next kernel on the stream may take the scratch, whichever of the
+    call's kernels had anything to do."""
+    g = gen(1)
+    cache, table = random_cache(g, 16, 64, 8, 128), torch.arange(16, dtype=torch.int32, device="cuda").view(4, 4)
+    q = torch.randn(tokens, 64, 128, device="cuda", generator=g).bfloat16()
+    kv, qs = ints([256] * 4), ints(starts)
+    out = torch.zeros_like(q)
+    size = workspace_bytes(4, tokens, 64, 8, 128)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    raw_attention(q, cache, table, kv, qs, out, ws)
+    want = out.clone()
+    touched = torch.zeros((), dtype=torch.bool, device="cuda")
+    for _ in range(100):
+        raw_attention(q, cache, table, kv, qs, out, ws)
+        ws.fill_(0xA5)
+        touched |= (ws != 0xA5).any()
+    assert not touched.item() and torch.equal(out, want)
