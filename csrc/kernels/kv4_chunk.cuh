@@ -543,19 +543,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
     sm100::tmemAlloc(&ctl.tmem, 512);
     sm100::tmemRelinquish();
   }
-  // Units before each request: one warp, 32 requests a step.
+  // Units before each request: one warp, 32 requests a step.  Starts that fall
+  // back give the same rows to several requests; units past those that the
+  // scratch was made for are left out.
   if (warp == 0) {
     int before = 0;
     for (int base = 0; base < p.batch; base += 32) {
       const int b = base + lane;
-      int v = b < p.batch ? chunkUnitsOf(p, requestOf(p, b)) : 0;
+      long long v = b < p.batch ? chunkUnitsOf(p, requestOf(p, b)) : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(~0u, v, o);
+        const long long x = __shfl_up_sync(~0u, v, o);
         if (lane >= o) v += x;
       }
-      if (b < p.batch) starts[b + 1] = before + v;
-      before += __shfl_sync(~0u, v, 31);
+      const int upto = static_cast<int>(min(before + v, static_cast<long long>(p.unitsMost)));
+      if (b < p.batch) starts[b + 1] = upto;
+      before = __shfl_sync(~0u, upto, 31);
     }
     if (lane == 0) starts[0] = 0;
   }
@@ -862,7 +865,7 @@ __global__ void __launch_bounds__(128) chunkJoinKernel(const __grid_constant__ A
     const int last = min((row / kChunkRows + 1) * kChunkRows, r.rows * p.group) - 1;
     const int seen = min(max(r.kv - r.rows + last / p.group + 1, 0), r.kv);
     const int all = (seen + kChunkKeys - 1) / kChunkKeys, each = (all + p.splits - 1) / p.splits;
-    if (s * each >= all) break;
+    if (s * each >= all || first + s >= p.chunkStarts[b + 1]) break;
     const long long slot = static_cast<long long>(first + s) * kChunkRows + row % kChunkRows;
     const float2 st = p.chunkStats[slot];
     const float top = fmaxf(m, st.x), old = exp2Fast(m - top), add = exp2Fast(st.x - top);

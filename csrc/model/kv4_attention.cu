@@ -70,6 +70,7 @@ struct AttnArgs {
   float scaleLog2;
   // Requests of at least longRows query rows a key head go to chunkKernel (0: none do).
   int longRows, splits;
+  int unitsMost;        // that the scratch has room for; requests that do not overlap have no more
   int* chunkStarts;     // [batch + 1] units before each request
   float2* chunkStats;   // [units][256] maximum (log2), sum, with splits > 1
   float* chunkPartial;  // [units][256][D]
@@ -887,7 +888,7 @@ constexpr int kLongRows = 64, kLongMean = 24;
 struct ChunkPlan {
   bool use;
   int splits;
-  long long units;  // at most, shares included
+  long long units;  // at most, shares included: below 2^31 as the rows of all heads are
 };
 
 ChunkPlan chunkPlan(int batch, int tokens, int qHeads, int kvHeads) {
@@ -1053,6 +1054,7 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   if (cp.use) {
     p.longRows = kLongRows;
     p.splits = cp.splits;
+    p.unitsMost = static_cast<int>(cp.units);
     p.chunkStarts = reinterpret_cast<int*>(ws);
     ws += align256((batch + 1) * sizeof(int));
     const size_t chunkSlots = cp.splits > 1 ? static_cast<size_t>(cp.units) * kChunkRows : 0;

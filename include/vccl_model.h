@@ -113,7 +113,9 @@ vcclResult_t vcclKv4Read(const vcclKv4_t* cache, const int* slots, const vcclHea
  * [tokens, q heads], may be NULL) = the logarithm of the sum of exponentials.
  * A row that sees nothing is 0 with lse = -inf.  Rows behind the last
  * request: 0 and -inf with zeroTail, else left as they are.  Tokens on a page
- * outside of the cache are not seen.  q heads a multiple of kvHeads,
+ * outside of the cache are not seen.  qStarts must not fall: the rows of
+ * requests that overlap are undefined (nothing outside of out, lse and the
+ * workspace is touched).  q heads a multiple of kvHeads,
  * batch <= 4096, width * pageSize <= 2^30.  workspace: vcclKv4AttentionWorkspace bytes. */
 size_t vcclKv4AttentionWorkspace(int batch, int tokens, int qHeads, int kvHeads, int D);
 vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, const int* table, int width,

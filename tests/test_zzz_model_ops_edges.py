@@ -104,3 +104,19 @@ def test_scratch_is_free_when_the_call_is_over(tokens, starts):
         ws.fill_(0xA5)
         touched |= (ws != 0xA5).any()
     assert not touched.item() and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("tokens,heads,kv_heads,starts", [(100, 8, 1, [0, 100, 0, 100, 0]), (100, 8, 1, [100, 0, 100, 0, 100] * 8),
+                                                          (3000, 64, 8, [0, 3000, 0, 3000, -5, 3000, 7]), (100, 8, 1, [0, 30, 100])])
+def test_attention_starts_that_fall_stay_in_bounds(tokens, heads, kv_heads, starts):
+    """Rows that several requests claim make more work than the scratch was sized for: what has no room is left out."""
+    g = gen(2)
+    batch = len(starts) - 1
+    cache = random_cache(g, 20, 16, kv_heads, 128)
+    table = torch.arange(20, dtype=torch.int32, device="cuda").repeat(batch, 1)
+    q = torch.randn(tokens, heads, 128, device="cuda", generator=g).bfloat16()
+    size = workspace_bytes(batch, tokens, heads, kv_heads, 128)
+    ws = torch.full((size + (4 << 20),), 0xA5, dtype=torch.uint8, device="cuda")
+    rows = torch.full((tokens + 64, heads, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    raw_attention(q, cache, table, ints([320 - i for i in range(batch)]), ints(starts), rows[:tokens], ws)
+    assert (ws[size:] == 0xA5).all() and (rows[tokens:] == 7.0).all()

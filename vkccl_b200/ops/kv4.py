@@ -105,7 +105,7 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     Request b has rows q_starts[b] to q_starts[b + 1] of q and the kv_lens[b]
     tokens of the pages in block_table[b]; its last row sees all of them, the
     row before one less, and so on (the new tokens' keys and values are in the
-    cache already).  q heads is a multiple of kv heads, head h reads key head
+    cache already).  q_starts must not fall.  q heads is a multiple of kv heads, head h reads key head
     h // (q heads / kv heads).  scale defaults to D ** -0.5.
 
     A row that sees nothing is 0 (lse -inf).  Rows behind the last request's
