@@ -11,10 +11,12 @@
 // 16 c * 2^-24), exact in the tensor cores' products; one AND makes a pair
 // of operands.  Query rows are scaled by a power of two and held in f16,
 // which is exact for bf16 and f16 inputs but for channels below 2^-26 of the
-// row's largest.  The weights p_t scale_tg are rounded to f16 (11 bits)
-// relative to a power of two above the scales seen so far; the sum of the
-// rounded ones, which the 7.5 multiplies, is a product with ones on the
-// tensor cores.  Everything else is f32.
+// row's largest.  The weights p_t scale_tg are rounded to f16 (11 bits) in
+// units of the largest one that the row has met, so a large value that a row
+// does not see, or gives no weight, costs the others nothing (with a unit for
+// all rows from the scales alone, one value 2^20 above the rest left a tenth
+// of error); the sum of the rounded ones, which the 7.5 multiplies, is a
+// product with ones on the tensor cores.  Everything else is f32.
 //
 // Shape.  S^T = K Q^T: rows of the m16n8k16 products are 16 tokens, columns 8
 // query rows (a query row is one head of one token; the heads that share a key
@@ -28,7 +30,7 @@
 // write partial sums (unnormalised output, maximum, sum) that a second kernel
 // joins in order.
 //
-// Measured: 135 us, 4.5 TB/s of cache, for 64 requests of 500 to 16000 tokens,
+// Measured: 137 us, 4.4 TB/s of cache, for 64 requests of 500 to 16000 tokens,
 // 64 heads on 8; the widening of codes bounds it (300 instructions a block of
 // 16 tokens, half of them on the ALU pipe).  One request of 900 tokens takes
 // 12 us, which is the latency of two launches and eight dependent loads.
@@ -50,6 +52,10 @@ constexpr int kBlocks = kTile / kv4::kBlockTokens;  // blocks in a tile
 constexpr int kMaxBatch = 4096;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kNone = -1e30f;    // a maximum over nothing
+// Weights in f16: the largest p * scale that a look finds becomes 4; until the
+// next look p grows by 2^8 at most, and scales by what keeps p * scale below
+// 2^15.  The factor that makes it so stays where f32 holds all products.
+constexpr float kWeightTop = 4.0f, kScaleRoom = 128.0f, kFactorMost = 0x1p118f, kFactorLeast = 0x1p-120f;
 
 struct AttnArgs {
   const void* q;
@@ -275,10 +281,11 @@ struct Unit {
   int limit[NT][2];          // tokens that the row sees
   int most, least;           // of all rows of the unit
   float m[NT][2], l[NT][2];
-  float o[NT][G][4][4];      // 2^-24 * 2^-r * sum p' c; odd j: of c + 16 c', c that of j - 1
-  float ones[NT][G][4];      // 2^-r * sum p'
+  float o[NT][G][4][4];      // 2^-24 * by * sum p' c; odd j: of c + 16 c', c that of j - 1
+  float ones[NT][G][4];      // by * sum p'
   float mid[NT][G][2];       // sum p mid
-  float inv[G], lim[G];      // 2^-r, and the scale above which r grows
+  float by[NT][G][2];        // p' = p scale is held as by * p' in f16
+  float lim[G];              // the scale above which by is looked at
 };
 
 template <int G, int NT>
@@ -352,7 +359,10 @@ __device__ __forceinline__ void loadQuery(Unit<G, NT>& u, const AttnArgs& p, con
       most = max(most, u.limit[n][c]);
       least = min(least, u.limit[n][c]);
 #pragma unroll
-      for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] = 0.0f;
+      for (int gr = 0; gr < G; gr++) {
+        u.mid[n][gr][c] = 0.0f;
+        u.by[n][gr][c] = kFactorMost;
+      }
     }
 #pragma unroll
     for (int gr = 0; gr < G; gr++) {
@@ -365,10 +375,7 @@ __device__ __forceinline__ void loadQuery(Unit<G, NT>& u, const AttnArgs& p, con
     }
   }
 #pragma unroll
-  for (int gr = 0; gr < G; gr++) {
-    u.inv[gr] = 1.0f;
-    u.lim[gr] = 0.0f;
-  }
+  for (int gr = 0; gr < G; gr++) u.lim[gr] = kScaleRoom / kFactorMost;
   most = max(most, __shfl_xor_sync(~0u, most, 1));
   u.most = max(most, __shfl_xor_sync(~0u, most, 2));
   least = min(least, __shfl_xor_sync(~0u, least, 1));
@@ -407,11 +414,14 @@ __device__ __forceinline__ void weighValues(Unit<G, NT>& u, float (&x)[kBlocks][
     readValues<G>(v, tile + b * 18 * D, at);
 #pragma unroll
     for (int gr = 0; gr < G; gr++) {
-      const float f0 = s[b][0][gr] * u.inv[gr], f1 = s[b][1][gr] * u.inv[gr];
       uint32_t b0[NT], b1[NT];
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        float w[4] = {x[b][n][0] * f0, x[b][n][1] * f0, x[b][n][2] * f1, x[b][n][3] * f1};
+        // p * by first: it is finite, and nothing where p is, whatever the scale
+        const uint64_t by = pair(u.by[n][gr][0], u.by[n][gr][1]);
+        const float2 w01 = unpair(mul2(mul2(pair(x[b][n][0], x[b][n][1]), by), pair(s[b][0][gr])));
+        const float2 w23 = unpair(mul2(mul2(pair(x[b][n][2], x[b][n][3]), by), pair(s[b][1][gr])));
+        float w[4] = {w01.x, w01.y, w23.x, w23.y};
         if (EDGE) {
 #pragma unroll
           for (int k = 0; k < 4; k++) w[k] = x[b][n][k] == 0.0f ? 0.0f : w[k];
@@ -432,6 +442,14 @@ __device__ __forceinline__ void weighValues(Unit<G, NT>& u, float (&x)[kBlocks][
       }
     }
   }
+}
+
+// Of two pairs of bf16, a without signs: the larger sizes.  Two instructions a
+// word, where scales already in f32 took three microseconds of 140 more.
+__device__ __forceinline__ uint32_t maxSizes(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("{ .reg .b32 s; abs.bf16x2 s, %2; max.bf16x2 %0, %1, s; }" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 // A tile of 32 tokens that starts at token t0 of the request.  Two blocks at a
@@ -486,6 +504,7 @@ __device__ __forceinline__ void tileStep(Unit<G, NT>& u, uint32_t tile, const La
       for (int e = 0; e < 4; e++) x[b][n][e] = fmaf(z[b][n][e], u.qs[n][e & 1], -u.m[n][e & 1]);
   }
   float s[B][2][G], mid[B][2][G];
+  uint32_t widest[G] = {};  // the largest |scale| (low half); of tokens that no row sees, too
 #pragma unroll
   for (int b = 0; b < B; b++) {
     uint32_t vp[2][G];
@@ -496,6 +515,7 @@ __device__ __forceinline__ void tileStep(Unit<G, NT>& u, uint32_t tile, const La
       for (int gr = 0; gr < G; gr++) {
         s[b][i][gr] = kv4::bf16Lo(vp[i][gr]);
         mid[b][i][gr] = kv4::bf16Hi(vp[i][gr]);
+        widest[gr] = maxSizes(widest[gr], vp[i][gr]);
       }
   }
   // Tokens behind some row's last one, or on no page: their scores are none,
@@ -519,8 +539,8 @@ __device__ __forceinline__ void tileStep(Unit<G, NT>& u, uint32_t tile, const La
       }
   }
   // The maximum is followed loosely: it moves when a score passes it by 8
-  // (weights reach 2^8), and the power of two of the scales when one passes
-  // it by 4, so most tiles take neither a reduction nor a rescaling.
+  // (weights reach 2^8), and the factor of the weights when a scale might take
+  // them out of f16, so most tiles take neither a reduction nor a rescaling.
   float high = x[0][0][0], wide[G];
 #pragma unroll
   for (int b = 0; b < B; b++)
@@ -531,31 +551,16 @@ __device__ __forceinline__ void tileStep(Unit<G, NT>& u, uint32_t tile, const La
   bool grow = high > 8.0f;
 #pragma unroll
   for (int gr = 0; gr < G; gr++) {
-    wide[gr] = s[0][0][gr];
-#pragma unroll
-    for (int b = 0; b < B; b++) wide[gr] = fmaxf(wide[gr], fmaxf(s[b][0][gr], s[b][1][gr]));
+    wide[gr] = kv4::bf16Lo(widest[gr]);
     grow = grow || wide[gr] > u.lim[gr];
   }
   if (__any_sync(~0u, grow)) {
-    float beta[G];
+    float most[G];  // of the factors
 #pragma unroll
-    for (int gr = 0; gr < G; gr++) {
-      float top = wide[gr];
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-      beta[gr] = 1.0f;
-      if (top > u.lim[gr]) {
-        // 2^r with top in [2^r, 2^(r+1)); subnormal scales share the smallest r.
-        const int e = max(static_cast<int>(__float_as_uint(top) >> 23), 1);
-        const float inv = __uint_as_float(static_cast<uint32_t>(min(254 - e, 253)) << 23);
-        beta[gr] = u.lim[gr] > 0.0f ? inv / u.inv[gr] : 1.0f;  // a quotient of powers of two
-        u.inv[gr] = inv;
-        u.lim[gr] = e <= 252 ? __uint_as_float(static_cast<uint32_t>(e + 2) << 23) : INFINITY;
-      }
-    }
+    for (int gr = 0; gr < G; gr++) most[gr] = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-      float alpha[2];
+      float f[G][2];
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         float top = kNone;
@@ -566,29 +571,44 @@ __device__ __forceinline__ void tileStep(Unit<G, NT>& u, uint32_t tile, const La
             if (x[b][n][2 * i + c] != -INFINITY) top = fmaxf(top, z[b][n][2 * i + c] * u.qs[n][c]);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        const float m = fmaxf(u.m[n][c], top);
-        alpha[c] = exp2Fast(u.m[n][c] - m);
+        const float m = fmaxf(u.m[n][c], top), alpha = exp2Fast(u.m[n][c] - m);
         u.m[n][c] = m;
-        u.l[n][c] *= alpha[c];
-#pragma unroll
-        for (int gr = 0; gr < G; gr++) u.mid[n][gr][c] *= alpha[c];
+        u.l[n][c] *= alpha;
+        float largest[G] = {};  // p |scale| of the tokens that the row sees
 #pragma unroll
         for (int b = 0; b < B; b++)
 #pragma unroll
           for (int i = 0; i < 2; i++)
-            if (x[b][n][2 * i + c] != -INFINITY) x[b][n][2 * i + c] = fmaf(z[b][n][2 * i + c], u.qs[n][c], -m);
-      }
+            if (x[b][n][2 * i + c] != -INFINITY) {
+              x[b][n][2 * i + c] = fmaf(z[b][n][2 * i + c], u.qs[n][c], -m);
+              const float w = exp2Fast(x[b][n][2 * i + c]);
 #pragma unroll
-      for (int gr = 0; gr < G; gr++) {
-        const float f[2] = {alpha[0] * beta[gr], alpha[1] * beta[gr]};
+              for (int gr = 0; gr < G; gr++) largest[gr] = fmaxf(largest[gr], w * fabsf(s[b][i][gr]));
+            }
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          u.ones[n][gr][k] *= f[k & 1];
+        for (int gr = 0; gr < G; gr++) {
+          u.mid[n][gr][c] *= alpha;
 #pragma unroll
-          for (int j = 0; j < 4; j++) u.o[n][gr][j][k] *= f[k & 1];
+          for (int o = 4; o < 32; o <<= 1) largest[gr] = fmaxf(largest[gr], __shfl_xor_sync(~0u, largest[gr], o));
+          // What was the largest so far has shrunk with the other weights.
+          const float old = u.by[n][gr][c], want = fminf(__fdividef(old, alpha), __fdividef(kWeightTop, largest[gr]));
+          const float by = fmaxf(fminf(want, kFactorMost), kFactorLeast), moved = alpha * by;
+          f[gr][c] = moved == old ? 1.0f : __fdividef(moved, old);
+          u.by[n][gr][c] = by;
+          most[gr] = fmaxf(most[gr], by);
         }
       }
+#pragma unroll
+      for (int gr = 0; gr < G; gr++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          u.ones[n][gr][k] *= f[gr][k & 1];
+#pragma unroll
+          for (int j = 0; j < 4; j++) u.o[n][gr][j][k] *= f[gr][k & 1];
+        }
     }
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) u.lim[gr] = __fdividef(kScaleRoom, most[gr]);
   }
   if (edge) weighValues<G, NT, true>(u, x, s, mid, tile, at);
   else weighValues<G, NT, false>(u, x, s, mid, tile, at);
@@ -626,7 +646,7 @@ __device__ __forceinline__ void finish(Unit<G, NT>& u, const AttnArgs& p, const 
       const float norm = slot < 0 ? (none ? 0.0f : 1.0f / l) : 1.0f;
 #pragma unroll
       for (int gr = 0; gr < G; gr++) {
-        const float back = 1.0f / u.inv[gr];
+        const float back = 1.0f / u.by[n][gr][c];
         const float base = fmaf(-7.5f * u.ones[n][gr][c], back, mid[gr]);
         float y[8];
 #pragma unroll

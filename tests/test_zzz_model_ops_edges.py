@@ -85,7 +85,7 @@ def random_cache(g, pages, page, kv_heads, dim):
     return cache
 
 
-@pytest.mark.parametrize("tokens,starts", [(4096, [0, 1024, 2048, 3072, 4096]), (640, [0, 0, 0, 0, 0])])
+@pytest.mark.parametrize("tokens,starts", [(4096, [0, 1000, 2000, 3000, 4096]), (640, [0, 0, 0, 0, 0])])
 def test_scratch_is_free_when_the_call_is_over(tokens, starts):
     """Requests that are all long, or no rows at all: the next kernel on the stream may take the scratch, whichever of the
     call's kernels had anything to do."""
@@ -120,3 +120,87 @@ def test_attention_starts_that_fall_stay_in_bounds(tokens, heads, kv_heads, star
     rows = torch.full((tokens + 64, heads, 128), 7.0, dtype=torch.bfloat16, device="cuda")
     raw_attention(q, cache, table, ints([320 - i for i in range(batch)]), ints(starts), rows[:tokens], ws)
     assert (ws[size:] == 0xA5).all() and (rows[tokens:] == 7.0).all()
+
+
+# ---- attention: values and keys far apart ----------------------------------------
+
+
+def spread_case(g, kind, n, kv_heads, ratio):
+    """Keys and values [n, kv heads, 128] for queries around 0.5: a key of a * ones has the score 5.7 a."""
+    def noise(x):
+        return x * torch.randn(n, kv_heads, 128, device="cuda", generator=g)
+
+    t = torch.arange(n, device="cuda", dtype=torch.float64)[:, None, None] / n
+    k, v = noise(0.2), noise(1.0)
+    if kind in ("first", "middle", "last"):  # one value is large, and its weight is nothing
+        i = {"first": 0, "middle": n // 2 + 5, "last": n - 1}[kind]
+        v[i] *= 2.0**ratio
+        k[i] = k[i] - 40.0
+    elif kind == "unseen":  # the last token's value is large: its own row sees it alone
+        v[n - 1] *= 2.0**ratio
+    elif kind == "sink":  # the first token has most of the weight and small values
+        v[0] *= 2.0**-ratio
+        k[0] = k[0] + 1.0
+    elif kind == "rising":  # what comes later counts more and is smaller
+        v, k = v * 2.0**(-ratio * t), k + 12.0 * t
+    elif kind == "falling":  # what comes later counts less and is larger: by less than it counts less ...
+        v, k = v * 2.0**(ratio * t), k - 12.0 * t
+    elif kind == "growing":  # ... and by more
+        v, k = v * 2.0**(ratio * t), k - 2.0 * t
+    elif kind == "key unseen":
+        k[n - 1] *= 2.0**ratio
+    elif kind == "key below":  # one key is large, and its weight is nothing
+        k[n // 2 + 5] = k[n // 2 + 5] - 2.0**ratio
+    elif kind == "mixed":  # neighbours far apart
+        v = v * 2.0**torch.randint(-ratio, ratio + 1, (n, kv_heads, 1), device="cuda", generator=g)
+    return k, v
+
+
+def check_rows(got, lse, q, ks, vs, kv_lens, q_starts, long):
+    """Each row against 64 bits, within a slack from the values that it sees itself.
+
+    With a the largest |value| of a token's 64 channels and A = sum p a over the row: the weights are rounded to f16, 2^-11
+    of 7.5 scales <= 1.01 a; in the kernel of long runs the value too, twice (2.1 * 2^-11 a).  What falls under f16's
+    smallest numbers is 2^-27 A a token for single tokens (weights in units of the largest p * scale seen, times 4), and 2^-20 A
+    in long runs (where 32 tokens within 2^6 share their unit).  f32 sums of n terms and exponentials: 2^-15.  Scores are
+    off by 2^-19 of the sizes that they add up."""
+    import model_reference as ref
+
+    scale = q.shape[-1] ** -0.5
+    want, wlse, _ = ref.attention(q, ks, vs, kv_lens, q_starts, scale)
+    tops = [v.abs().unflatten(-1, (-1, 64)).amax(-1, keepdim=True).expand(*v.shape[:-1], -1, 64).flatten(-2) for v in vs]
+    _, _, size = ref.attention(q, ks, tops, kv_lens, q_starts, scale)
+    # sum |q| |k| of a row against the keys of weight: those are near the row's largest score
+    _, _, near = ref.attention(q, ks, [k.abs().amax(-1, keepdim=True).expand_as(k) * 2 for k in ks], kv_lens, q_starts, scale)
+    score = q.double().abs().sum(-1) * near[..., 0] * scale * 2.0**-19
+    n = max(kv_lens)
+    part = (3.2 * 2.0**-11 + n * 2.0**-20 if long else 1.1 * 2.0**-11 + n * 2.0**-27) + 2.0**-15
+    slack = want.abs() * torch.finfo(q.dtype).eps / 2 * 1.02 + size * (part + 4 * score[..., None]) + 2.0**-25
+    d = (got.double() - want).abs() - slack
+    assert torch.isfinite(got).all() and d.max().item() <= 0, (d.max().item(), (d / slack).max().item())
+    assert ((lse.double() - wlse).abs() <= score + wlse.abs() * 2.0**-20 + 2.0**-18).all()
+
+
+KINDS = ["first", "middle", "last", "unseen", "sink", "rising", "falling", "growing", "mixed", "key unseen", "key below"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("ratio", [14, 26])
+@pytest.mark.parametrize("rows,heads,kv_heads,n", [(1, 8, 1, 2000), (3, 2, 1, 700), (40, 2, 2, 700)])
+def test_attention_of_values_far_apart(kind, ratio, rows, heads, kv_heads, n):
+    """Values (and keys) of one request 2^14 and 2^26 apart: a row's result goes by the tokens that it sees and by their weights,
+    not by the largest value around."""
+    from vkccl_b200.ops.kv4 import kv4_alloc, kv4_append, kv4_attention, kv4_read
+
+    g = gen(KINDS.index(kind) * 100 + ratio + rows)
+    pages = -(-n // 16)
+    cache = kv4_alloc(pages, 16, kv_heads, 128)
+    table = torch.randperm(pages, device="cuda", generator=g).int().view(1, -1)
+    t = torch.arange(n, device="cuda")
+    slots = (table[0, t // 16] * 16 + t % 16).int()
+    k, v = spread_case(g, kind, n, kv_heads, ratio)
+    kv4_append(cache, k.bfloat16(), v.bfloat16(), slots)
+    k, v = (x.double() for x in kv4_read(cache, slots, dtype=torch.float32))
+    q = (0.5 + 0.1 * torch.randn(rows, heads, 128, device="cuda", generator=g)).bfloat16()
+    got, lse = kv4_attention(q, cache, table, ints([n]), ints([0, rows]), return_lse=True)
+    check_rows(got, lse, q, [k], [v], [n], [0, rows], rows * heads // kv_heads >= 64)
