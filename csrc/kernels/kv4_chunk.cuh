@@ -30,10 +30,14 @@
 // a query row is scaled to 2^8, 32 neighbouring tokens (what a warp turns, and
 // what a softmax thread takes at once) share a power of two for keys and one
 // for values, which the softmax puts into its scale and into the weights.
-// Scores, maxima, sums and outputs are f32.  The maximum is followed loosely
-// (by 8 in the base-2 logarithm), so the output is rescaled rarely.
+// Where some of the 32 are more than 2^6 below the largest each has powers of
+// its own, and the softmax takes them token by token.  A row's outputs are in
+// units of the largest weight times value that it met, so what it does not see
+// or gives no weight costs the rest no bits.  Scores, maxima, sums and outputs
+// are f32.  The maximum is followed loosely (by 8 in the base-2 logarithm), so
+// the output is rescaled rarely.
 //
-// Measured: 862 us, 700 TFLOP/s, for 4 requests of 1024 rows against 2000 to
+// Measured: 856 us, 700 TFLOP/s, for 4 requests of 1024 rows against 2000 to
 // 9000 tokens, 64 heads on 8 (the single-token kernel takes 3.4 ms).  The
 // softmax bounds it: 2230 of the 3070 clocks that a tile takes.
 #pragma once
@@ -50,6 +54,10 @@ constexpr int kChunkKeys = 64;
 constexpr int kChunkStages = 4;     // tiles of keys, and of values, in shared memory
 constexpr int kChunkThreads = 16 * 32;
 constexpr int kLeastExponent = -112;  // of 32 tokens that are all zero, or next to it
+constexpr int kSpread = 6;            // binary orders that 32 tokens may lie apart and share a power of two
+// The largest weight times value of a row becomes 2^4 in f16, times up to 2^13
+// of the value, when its unit moves, and may grow to 2^14 until it moves again.
+constexpr float kTopWeight = 4.0f, kMostWeight = 14.0f;
 
 // 32 lanes x 32 bit, 32 consecutive columns per thread.
 __device__ __forceinline__ void tmemLoad32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -166,16 +174,20 @@ struct ChunkSmem {
   static constexpr int kQSums = kV + kChunkStages * G * kBlock;  // [2 row tiles]
   static constexpr int kKSums = kQSums + 2 * 128 * 32;           // [stages]
   static constexpr int kInfo = kKSums + kChunkStages * 64 * 32;
-  static constexpr int kStarts = kInfo + 1024;  // units before each request
+  static constexpr int kStarts = kInfo + 1680;  // units before each request
 };
+
+// kApart: tokens have powers of two of their own, of keys or of values.
+constexpr uint32_t kUneven = 1, kApart = 2;
 
 // What the tokens of a tile bring, by 32.
 struct alignas(16) ChunkInfo {
   uint32_t valid[2];               // the token is there
   float keyUnit[2];                // the power of two that its keys are divided by
   float valueExp[2];               // the logarithm of that of its values
-  uint32_t pad[2];
+  uint32_t kind[2];                // kUneven: some tokens are not there, or not finite; kApart
   uint32_t bad[2][2];              // its values of a group are not finite (and zero in the product)
+  signed char keyExps[64], valueExps[64];  // the logarithms token by token, where 32 lie apart
 };
 
 struct ChunkControl {
@@ -187,7 +199,7 @@ struct ChunkControl {
   uint32_t tmem;
   int abort;
 };
-static_assert(sizeof(ChunkControl) <= 1024, "the control block's place");
+static_assert(sizeof(ChunkControl) <= ChunkSmem<2>::kStarts - ChunkSmem<2>::kInfo, "the control block's place");
 
 struct ChunkUnit {
   Request r;
@@ -320,21 +332,57 @@ struct RowState {
   uint32_t poison; // groups whose values are not finite
 };
 
+// Not zero (a softmax scale of zero, or one next to it): unseen scores are
+// -inf, and scores times the smallest number count nothing.
+__device__ __forceinline__ float notZero(float x) { return x < FLT_MIN ? FLT_MIN : x; }
+
+// Moves the maximum and the unit of the outputs where a row of the warp needs
+// it.  top: the largest score; high: the largest score plus logarithm of the
+// value.  Returns false if a wait ran out.
+template <int D>
+__device__ __forceinline__ bool follow(RowState& r, float top, float high, uint32_t output, bool first, uint64_t* before,
+                                       uint32_t beforeParity, volatile int* abortFlag) {
+  if (!__any_sync(~0u, top > r.m + 8.0f || high > r.m + r.ref + kMostWeight)) return true;
+  // What was the largest weight times value shrinks with the other weights.
+  const float next = fmaxf(r.m, top), old = r.ref + (r.m - next), ref = fmaxf(old, high - next - kTopWeight);
+  if (!first) {
+    // the products with the weights before these have ended
+    if (!warpWait(before, beforeParity, abortFlag)) return false;
+    sm100::tcFenceAfter();
+    const float factor = exp2Fast(old - ref);
+#pragma unroll 1
+    for (int k = 0; k < D / 16; k++) {
+      uint32_t o[16];
+      sm100::tmemLoad16(output + 16 * k, o);
+      sm100::tmemLoadWait();
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+      tmemStore16(output + 16 * k, o);
+    }
+  }
+  r.l *= exp2Fast(r.m - next);
+  r.m = next;
+  r.ref = ref;
+  return true;
+}
+
+// Weights of values in much smaller units than the outputs': 2^40 apart they
+// are nothing in f16, and all of them still count in the sum.
+__device__ __forceinline__ float shiftOf(float valueExp, float ref) { return fmaxf(valueExp - ref, -40.0f); }
+
+__device__ __forceinline__ uint32_t poisoned(const ChunkInfo& info, uint32_t seen0, uint32_t seen1) {
+  const uint4 bad = *reinterpret_cast<const uint4*>(info.bad);
+  return (((bad.x & seen0) | (bad.y & seen1)) ? 1u : 0u) | (((bad.z & seen0) | (bad.w & seen1)) ? 2u : 0u);
+}
+
 // One tile's scores to weights.  Returns false if a wait ran out.
 template <int G, bool EDGE>
-__device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32_t output, const ChunkInfo& info, const uint2& valid,
-                                            float unit, int left, bool first, uint64_t* before, uint32_t beforeParity,
-                                            volatile int* abortFlag) {
-  constexpr int D = 64 * G;
+__device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32_t output, const ChunkInfo& info, float unit,
+                                            int left, bool first, uint64_t* before, uint32_t beforeParity, volatile int* abortFlag) {
   const float2 keyUnit = *reinterpret_cast<const float2*>(info.keyUnit), valueExp = *reinterpret_cast<const float2*>(info.valueExp);
-  const uint4 bad = *reinterpret_cast<const uint4*>(info.bad);
-  // Not zero (a softmax scale of zero, or one next to it): unseen scores are
-  // -inf, and scores times the smallest number count nothing.
-  auto above = [](float x) { return x < FLT_MIN ? FLT_MIN : x; };
-  const float scale0 = above(unit * keyUnit.x), scale1 = above(unit * keyUnit.y);
-  const float ref = fmaxf(r.ref, fmaxf(valueExp.x, valueExp.y));
-  const uint32_t seen0 = EDGE ? seenOf(valid.x, left) : ~0u, seen1 = EDGE ? seenOf(valid.y, left - 32) : ~0u;
-  float top = kNone;
+  const float scale0 = notZero(unit * keyUnit.x), scale1 = notZero(unit * keyUnit.y);
+  const uint32_t seen0 = EDGE ? seenOf(info.valid[0], left) : ~0u, seen1 = EDGE ? seenOf(info.valid[1], left - 32) : ~0u;
+  float top = kNone, high = kNone;
 #pragma unroll 1
   for (int k = 0; k < 2; k++) {
     uint32_t s[32];
@@ -345,31 +393,14 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
 #pragma unroll
     for (int i = 4; i < 32; i += 2) x[(i >> 1) & 3] = max3(x[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
     const float most = max3(x[0], x[1], fmaxf(x[2], x[3]));
-    if (!EDGE || most > -INFINITY) top = fmaxf(top, most * (k ? scale1 : scale0));
-  }
-  if (__any_sync(~0u, top > r.m + 8.0f || ref > r.ref)) {
-    const float next = fmaxf(r.m, top), shrink = exp2Fast(r.m - next);
-    if (!first) {
-      // the products with the weights before these have ended
-      if (!warpWait(before, beforeParity, abortFlag)) return false;
-      sm100::tcFenceAfter();
-      const float factor = shrink * exp2Fast(r.ref - ref);
-#pragma unroll 1
-      for (int k = 0; k < D / 16; k++) {
-        uint32_t o[16];
-        sm100::tmemLoad16(output + 16 * k, o);
-        sm100::tmemLoadWait();
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-        tmemStore16(output + 16 * k, o);
-      }
+    if (!EDGE || most > -INFINITY) {
+      const float score = most * (k ? scale1 : scale0);
+      top = fmaxf(top, score);
+      high = fmaxf(high, score + (k ? valueExp.y : valueExp.x));
     }
-    r.l *= shrink;
-    r.m = next;
-    r.ref = ref;
   }
-  // Weights of values in smaller units are smaller; 2^100 apart they vanish.
-  const float shift0 = fmaxf(valueExp.x - r.ref, -100.0f), shift1 = fmaxf(valueExp.y - r.ref, -100.0f);
+  if (!follow<64 * G>(r, top, high, output, first, before, beforeParity, abortFlag)) return false;
+  const float shift0 = shiftOf(valueExp.x, r.ref), shift1 = shiftOf(valueExp.y, r.ref);
 #pragma unroll 1
   for (int k = 0; k < 2; k++) {
     uint32_t s[32];
@@ -377,22 +408,70 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
     const float shift = k ? shift1 : shift0;
     r.l = fmaf(halfWeights(s, scores + 16 * k, k ? scale1 : scale0, shift - r.m), exp2Fast(-shift), r.l);
   }
-  if ((bad.x | bad.y | bad.z | bad.w) != 0) {
-    if ((bad.x & seen0) | (bad.y & seen1)) r.poison |= 1u;
-    if ((bad.z & seen0) | (bad.w & seen1)) r.poison |= 2u;
-  }
+  if (EDGE) r.poison |= poisoned(info, seen0, seen1);
   return true;
 }
 
-// Logarithm of the power of two of 32 tokens' keys or values: divided by it,
-// the largest is below 2^13.  scale, mid: of the lane's token.
+struct Followed {
+  RowState row;
+  bool ok;
+};
+
+// The same where tokens have powers of two of their own.  Rare, and out of the
+// way of the others' code: in line it cost 7 % of the whole kernel.
 template <int G>
-__device__ __forceinline__ int exponentOf32(const float (&scale)[G], const float (&mid)[G]) {
+__device__ __noinline__ Followed tileSoftmaxApart(RowState r, uint32_t scores, uint32_t output, const ChunkInfo* info, float unit,
+                                                  int left, bool first, uint64_t* before, uint32_t beforeParity,
+                                                  volatile int* abortFlag) {
+  const uint32_t seen0 = seenOf(info->valid[0], left), seen1 = seenOf(info->valid[1], left - 32);
+  float top = kNone, high = kNone;
+  auto keyScale = [&](int k, int i) {
+    return notZero(unit * ((info->kind[k] & kApart) ? powerOfTwo(info->keyExps[32 * k + i]) : info->keyUnit[k]));
+  };
+  auto valueExp = [&](int k, int i) { return (info->kind[k] & kApart) ? static_cast<float>(info->valueExps[32 * k + i]) : info->valueExp[k]; };
+#pragma unroll 1
+  for (int k = 0; k < 2; k++) {
+    uint32_t s[32];
+    loadScores<true>(scores + 32 * k, s, k ? seen1 : seen0);
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+      const float score = __uint_as_float(s[i]) * keyScale(k, i);
+      top = fmaxf(top, score);
+      high = fmaxf(high, score + valueExp(k, i));
+    }
+  }
+  if (!follow<64 * G>(r, top, high, output, first, before, beforeParity, abortFlag)) return {r, false};
+#pragma unroll 1
+  for (int k = 0; k < 2; k++) {
+    uint32_t s[32], w[16];
+    loadScores<true>(scores + 32 * k, s, k ? seen1 : seen0);
+    float sum = 0.0f, y[2];
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+      const float x = fmaf(__uint_as_float(s[i]), keyScale(k, i), -r.m);
+      sum += exp2Fast(x);
+      y[i & 1] = exp2Fast(x + shiftOf(valueExp(k, i), r.ref));
+      if (i & 1) w[i >> 1] = packHalf(y[0], y[1]);
+    }
+    tmemStore16(scores + 16 * k, w);
+    r.l += sum;
+  }
+  r.poison |= poisoned(*info, seen0, seen1);
+  return {r, true};
+}
+
+// Logarithm of the power of two of a token's keys or values: divided by it,
+// the largest is below 2^13.  That of the largest of 32, or where they lie
+// apart the token's own.  scale, mid: of the lane's token.
+template <int G>
+__device__ __forceinline__ int exponentOf32(const float (&scale)[G], const float (&mid)[G], bool* apart) {
   float top = 0.0f;
 #pragma unroll
   for (int g = 0; g < G; g++) top = fmaxf(top, fmaf(8.5f, fabsf(scale[g]), fabsf(mid[g])));
   // positive floats are ordered like their bits
-  return max(exponentOf(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top)))) - 12, kLeastExponent);
+  const int most = exponentOf(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top)))), mine = exponentOf(top);
+  *apart = __any_sync(~0u, top > 0.0f && mine < most - kSpread);
+  return max((*apart ? mine : most) - 12, kLeastExponent);
 }
 
 // A token's row of codes with its parameters; a key thread has those of the
@@ -645,14 +724,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
           if (!ok) break;
           sm100::tcFenceAfter();
           const ChunkInfo& info = ctl.info[seq & 7];
-          const uint2 valid = *reinterpret_cast<const uint2*>(info.valid);
           const int left = mineLimit - j * kChunkKeys;  // keys of the tile in the row's range
           uint64_t* before = &ctl.pvDone[t][(count - 1) & 1];
           const uint32_t parity = ((count - 1) >> 1) & 1u;
-          if (__any_sync(~0u, left < kChunkKeys || (valid.x & valid.y) != ~0u))
-            ok = tileSoftmax<G, true>(state, scores, output, info, valid, mineUnit, left, j == c.from, before, parity, abortFlag);
-          else
-            ok = tileSoftmax<G, false>(state, scores, output, info, valid, mineUnit, left, j == c.from, before, parity, abortFlag);
+          const uint32_t kind = info.kind[0] | info.kind[1];
+          if (!__any_sync(~0u, left < kChunkKeys || kind != 0)) {
+            ok = tileSoftmax<G, false>(state, scores, output, info, mineUnit, left, j == c.from, before, parity, abortFlag);
+          } else if ((kind & kApart) == 0) {
+            ok = tileSoftmax<G, true>(state, scores, output, info, mineUnit, left, j == c.from, before, parity, abortFlag);
+          } else {
+            const Followed f = tileSoftmaxApart<G>(state, scores, output, &info, mineUnit, left, j == c.from, before, parity, abortFlag);
+            state = f.row;
+            ok = f.ok;
+          }
           if (!ok) break;
           tmemStoreWait();
           sm100::tcFenceBefore();
@@ -676,7 +760,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
       const int token = live ? mine / p.group : 0, h = c.head * p.group + (live ? mine - token * p.group : 0);
       const float m = state.m, l = state.l;
       const bool whole = p.splits == 1, none = l == 0.0f;
-      const float factor = (whole ? (none ? 0.0f : 1.0f / l) : 1.0f) * powerOfTwo(static_cast<int>(state.ref));
+      const float factor = (whole ? (none ? 0.0f : 1.0f / l) : 1.0f) * exp2Fast(state.ref);
       const long long slot = static_cast<long long>(u) * kChunkRows + t * 128 + row;
 #pragma unroll 1
       for (int k = 0; k < D / 32; k++) {
@@ -783,14 +867,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         if (odd) s[g] = m[g] = 0.0f;
         bad[g] = __ballot_sync(~0u, odd);
       }
-      const int ve = exponentOf32<G>(s, m);
+      bool valuesApart;
+      const int ve = exponentOf32<G>(s, m, &valuesApart);
       if (keys) {
 #pragma unroll
         for (int g = 0; g < G; g++) {
           s[g] = kv4::bf16Lo(raw.keyParams[g]);
           m[g] = kv4::bf16Hi(raw.keyParams[g]);
         }
-        const int ke = exponentOf32<G>(s, m);
+        bool keysApart;
+        const int ke = exponentOf32<G>(s, m, &keysApart);
         const float f = powerOfTwo(-ke);
 #pragma unroll
         for (int g = 0; g < G; g++) {
@@ -799,11 +885,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         }
         const uint32_t present = __ballot_sync(~0u, raw.there);
         if (!warpWait(&ctl.kEmpty[st], parity, abortFlag)) break;
+        ChunkInfo& info = ctl.info[seq & 7];
+        const bool apart = keysApart || valuesApart;
+        if (apart) {
+          info.keyExps[tid] = static_cast<signed char>(ke);
+          info.valueExps[tid] = static_cast<signed char>(ve);
+        }
         if (lane == 0) {
-          ChunkInfo& info = ctl.info[seq & 7];
           info.valid[w] = present;
           info.keyUnit[w] = powerOfTwo(ke);
           info.valueExp[w] = static_cast<float>(ve);
+          info.kind[w] = (present != ~0u || bad[0] != 0 || bad[G - 1] != 0 ? kUneven : 0) | (apart ? kApart : 0);
 #pragma unroll
           for (int g = 0; g < 2; g++) info.bad[g][w] = g < G ? bad[g < G ? g : 0] : 0;
         }

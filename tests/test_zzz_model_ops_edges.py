@@ -125,10 +125,10 @@ def test_attention_starts_that_fall_stay_in_bounds(tokens, heads, kv_heads, star
 # ---- attention: values and keys far apart ----------------------------------------
 
 
-def spread_case(g, kind, n, kv_heads, ratio):
-    """Keys and values [n, kv heads, 128] for queries around 0.5: a key of a * ones has the score 5.7 a."""
+def spread_case(g, kind, n, kv_heads, ratio, dim=128):
+    """Keys and values [n, kv heads, 128] for queries around 0.5: a key of a * ones has a score of 5.7 a (4 a with 64 channels)."""
     def noise(x):
-        return x * torch.randn(n, kv_heads, 128, device="cuda", generator=g)
+        return x * torch.randn(n, kv_heads, dim, device="cuda", generator=g)
 
     t = torch.arange(n, device="cuda", dtype=torch.float64)[:, None, None] / n
     k, v = noise(0.2), noise(1.0)
@@ -186,21 +186,43 @@ KINDS = ["first", "middle", "last", "unseen", "sink", "rising", "falling", "grow
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("ratio", [14, 26])
-@pytest.mark.parametrize("rows,heads,kv_heads,n", [(1, 8, 1, 2000), (3, 2, 1, 700), (40, 2, 2, 700)])
-def test_attention_of_values_far_apart(kind, ratio, rows, heads, kv_heads, n):
+@pytest.mark.parametrize("rows,heads,kv_heads,n,dim", [(1, 8, 1, 2000, 128), (3, 2, 1, 700, 128), (40, 2, 2, 700, 64), (100, 8, 1, 700, 128),
+                                                       (100, 4, 2, 690, 64), (1100, 64, 8, 1100, 128)])
+def test_attention_of_values_far_apart(kind, ratio, rows, heads, kv_heads, n, dim):
     """Values (and keys) of one request 2^14 and 2^26 apart: a row's result goes by the tokens that it sees and by their weights,
-    not by the largest value around."""
+    not by the largest value around.  One row, a few, and runs of rows with and without shares of the keys."""
     from vkccl_b200.ops.kv4 import kv4_alloc, kv4_append, kv4_attention, kv4_read
 
     g = gen(KINDS.index(kind) * 100 + ratio + rows)
     pages = -(-n // 16)
-    cache = kv4_alloc(pages, 16, kv_heads, 128)
+    cache = kv4_alloc(pages, 16, kv_heads, dim)
     table = torch.randperm(pages, device="cuda", generator=g).int().view(1, -1)
     t = torch.arange(n, device="cuda")
     slots = (table[0, t // 16] * 16 + t % 16).int()
-    k, v = spread_case(g, kind, n, kv_heads, ratio)
+    k, v = spread_case(g, kind, n, kv_heads, ratio, dim)
     kv4_append(cache, k.bfloat16(), v.bfloat16(), slots)
     k, v = (x.double() for x in kv4_read(cache, slots, dtype=torch.float32))
-    q = (0.5 + 0.1 * torch.randn(rows, heads, 128, device="cuda", generator=g)).bfloat16()
+    q = (0.5 + 0.1 * torch.randn(rows, heads, dim, device="cuda", generator=g)).bfloat16()
     got, lse = kv4_attention(q, cache, table, ints([n]), ints([0, rows]), return_lse=True)
     check_rows(got, lse, q, [k], [v], [n], [0, rows], rows * heads // kv_heads >= 64)
+
+
+def test_attention_of_a_long_run_among_the_largest_batch():
+    """4096 requests, one of them with 300 rows: the starts of all of them stand in shared memory beside the tiles."""
+    from vkccl_b200.ops.kv4 import kv4_attention
+
+    g = gen(5)
+    q_lens, kv_lens = [1] * 4096, [1 + i % 16 for i in range(4096)]
+    q_lens[1234], kv_lens[1234] = 300, 320
+    cache = random_cache(g, 60, 16, 1, 128)
+    table = torch.randint(0, 60, (4096, 20), device="cuda", generator=g).int()
+    qs = [0] + torch.tensor(q_lens).cumsum(0).tolist()
+    q = torch.randn(qs[-1], 32, 128, device="cuda", generator=g).bfloat16()  # 32 query heads on one: 24 rows a request and more
+    got, lse = kv4_attention(q, cache, table, ints(kv_lens), ints(qs), return_lse=True)
+    some = [0, 1, 1233, 1234, 1235, 4095]
+    rows = torch.cat([torch.arange(qs[i], qs[i + 1], device="cuda") for i in some])
+    one, lse1 = kv4_attention(q[rows], cache, table[some], ints([kv_lens[i] for i in some]),
+                              ints([0] + torch.tensor([q_lens[i] for i in some]).cumsum(0).tolist()), return_lse=True)
+    # the same rows among few requests: shares of the keys differ, and with them f32 sums and one rounding of each weight
+    assert (got[rows].float() - one.float()).abs().max() <= 2.0**-6 and (lse[rows] - lse1).abs().max() <= 2.0**-16
+    assert torch.isfinite(got).all()
