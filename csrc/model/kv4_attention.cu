@@ -40,6 +40,7 @@
 
 #include "kernels/kv4.cuh"
 #include "model/common.cuh"
+#include "vccl_x.h"
 
 namespace vccl {
 namespace model {
@@ -923,7 +924,8 @@ ChunkPlan chunkPlan(int batch, int tokens, int qHeads, int kvHeads) {
 }
 
 // One abort word per device in mapped host memory: a launch that gave up a
-// wait sets it, and the next call on that device reads it.  Made at the first
+// wait sets it, and the next call on that device, or the next look by
+// vcclKv4AttentionStatus, reads it.  Made at the first
 // launch, which may be a captured one: an allocation of host memory puts
 // nothing on a stream, so captures (this thread's and others') allow it in
 // relaxed mode.
@@ -1018,6 +1020,21 @@ size_t vcclKv4AttentionWorkspace(int batch, int tokens, int qHeads, int kvHeads,
          align256((batch + 1) * sizeof(int)) + align256(chunkSlots * sizeof(float2)) + chunkSlots * D * sizeof(float);
 }
 
+vcclResult_t vcclKv4AttentionStatus(void) {
+  if (!takeChunkError()) return vcclSuccess;
+  VERR("vcclKv4Attention: an earlier call on this device gave up (a pipeline wait ran out); its output is invalid");
+  return vcclInternalError;
+}
+
+vcclResult_t vcclxKv4AttentionInjectAbort(void) {
+  if (chunkErrorFlag() == nullptr) return vcclSystemError;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(gFlagMu);
+  *gHostFlags[dev & 63] = 1;
+  return vcclSuccess;
+}
+
 vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, const int* table, int width,
                               const int* kvLens, const int* qStarts, int batch, int tokens, float scale,
                               const vcclHeads_t* out, float* lse, int zeroTail, void* workspace,
@@ -1030,10 +1047,8 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
   if (!headsOk(q, 2) || !headsOk(out, 2) || q->heads != out->heads || q->heads % cache->kvHeads != 0 || !table ||
       !kvLens || !qStarts || !workspace || static_cast<long long>(tokens) * q->heads > INT_MAX)
     return vcclInvalidArgument;
-  if (takeChunkError()) {
-    VERR("vcclKv4Attention: an earlier call on this device gave up (a pipeline wait ran out); its output is invalid");
-    return vcclInternalError;
-  }
+  const vcclResult_t before = vcclKv4AttentionStatus();
+  if (before != vcclSuccess) return before;
   TraceRange trace("vccl Kv4Attention");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int group = q->heads / cache->kvHeads, nt = rowTiles(batch, tokens, group), R = 8 * nt;

@@ -123,6 +123,14 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
                               const vcclHeads_t* out, float* lse, int zeroTail, void* workspace,
                               vcclDataType_t datatype, vcclStream_t stream);
 
+/* The waits inside of vcclKv4Attention are bounded.  A launch that gave one up
+ * leaves its output incomplete and sets a word in host memory; the next
+ * vcclKv4Attention on that device returns vcclInternalError and clears it.  A
+ * program that replays a captured call makes no next call: this looks at the
+ * word of the current device, with the same result (vcclSuccess where nothing
+ * gave up).  It launches nothing and waits for nothing, so synchronise first. */
+vcclResult_t vcclKv4AttentionStatus(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,6 +35,11 @@ vcclResult_t vcclxCheckGuards(vcclComm_t comm, unsigned long long* badBytes);
  * vcclInternalError and clears it.  For tests of that error path. */
 vcclResult_t vcclxNoAllocInjectAbort(int device);
 
+/* The same for vcclKv4Attention on the current device: sets the word that a
+ * launch whose wait ran out leaves behind, which the next vcclKv4Attention or
+ * vcclKv4AttentionStatus reports and clears. */
+vcclResult_t vcclxKv4AttentionInjectAbort(void);
+
 /* The call profile of a communicator created with VCCL_PROF=1: one line per
  * (operation, algorithm or path) this rank ran, collectives and the fused
  * calls of vccl_tp.h alike, "op\talgorithm\tcalls\tbytes\n", bytes being

@@ -226,3 +226,35 @@ def test_attention_of_a_long_run_among_the_largest_batch():
     # the same rows among few requests: shares of the keys differ, and with them f32 sums and one rounding of each weight
     assert (got[rows].float() - one.float()).abs().max() <= 2.0**-6 and (lse[rows] - lse1).abs().max() <= 2.0**-16
     assert torch.isfinite(got).all()
+
+
+# ---- a launch that gave up ---------------------------------------------------------
+
+
+def test_attention_that_gave_up_is_reported():
+    """The word that a launch whose wait ran out leaves behind (set from the host): the next call raises and the one after
+    works; replays of a captured call raise nothing, and the look after them does, once."""
+    import vkccl_b200 as v
+    from vkccl_b200._lib import lib
+    from vkccl_b200.ops.kv4 import kv4_attention, kv4_attention_status
+
+    g = gen(6)
+    cache, table = random_cache(g, 16, 16, 1, 128), torch.arange(16, dtype=torch.int32, device="cuda").view(1, 16)
+    q = torch.randn(100, 8, 128, device="cuda", generator=g).bfloat16()
+    args = (cache, table, ints([256]), ints([0, 100]))
+    want = kv4_attention(q, *args)
+    kv4_attention_status()
+    assert lib().vcclxKv4AttentionInjectAbort() == 0
+    with pytest.raises(v.VcclError):
+        kv4_attention(q, *args)
+    assert torch.equal(kv4_attention(q, *args), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = kv4_attention(q, *args)
+    assert lib().vcclxKv4AttentionInjectAbort() == 0
+    graph.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(v.VcclError):
+        kv4_attention_status("cuda:0")
+    kv4_attention_status()
+    assert torch.equal(got, want) and torch.equal(kv4_attention(q, *args), want)

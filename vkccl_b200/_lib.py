@@ -146,6 +146,7 @@ def _declare_extensions(h: ctypes.CDLL) -> None:
         "vcclxCheckGuards": [P, c.POINTER(c.c_ulonglong)],
         "vcclxBarrierBench": [P, I, I, I, c.POINTER(F)],
         "vcclxNoAllocInjectAbort": [I],
+        "vcclxKv4AttentionInjectAbort": [],
         "vcclxProfSummary": [P, c.c_char_p, Z],
         "vcclGemmSiluMul": [P, P, P, I, I, I, P],
         "vcclGemmReduceScatter": [P, P, P, I, I, I, P, P],
@@ -158,6 +159,7 @@ def _declare_extensions(h: ctypes.CDLL) -> None:
         "vcclQkNormRopeBackward": [P, P, P, P, P, P, P, P, P, P, I, I, I, P],
         "vcclKv4Append": [P, P, P, P, P, P, P, I, I, P],
         "vcclKv4Read": [P, P, P, P, I, I, P],
+        "vcclKv4AttentionStatus": [],
         "vcclKv4Attention": [P, P, P, I, P, P, I, I, F, P, P, I, P, I, P],
     }
     for name, args in ext.items():

@@ -7,6 +7,7 @@ kv4_append_rope(cache, q, k, v, slots, ...)       the same after norm and rotati
 kv4_read(cache, slots)                            the values that it holds
 kv4_attention(q, cache, block_table, kv_lens, q_starts)
                                                   causal attention of ragged query rows
+kv4_attention_status()                            whether an attention launch gave up
 
 64 channels of a token share a bf16 scale and midpoint: value = midpoint +
 scale * (code - 7.5), 4.5 bits a value.  Slots, tables and lengths are those
@@ -22,6 +23,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from vkccl_b200._lib import lib
+from vkccl_b200.comm import _check
 from vkccl_b200.ops._args import DTYPES, cache4, call, current_device, float16s, fresh, heads, on_device, rope_of, vector
 
 MAX_BATCH = 4096
@@ -146,3 +148,17 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
          dim ** -0.5 if scale is None else scale, ho, None if lse is None else lse.data_ptr(), 1 if new else 0,
          ws.data_ptr(), DTYPES[dtype])
     return (out, lse) if return_lse else out
+
+
+def kv4_attention_status(device=None) -> None:
+    """Raises VcclError if an attention launch on the device (default: the current one) gave up a wait, and forgets it.
+
+    The kernels' waits are bounded; a launch that gave one up leaves its output
+    incomplete.  The next ``kv4_attention`` raises this by itself.  A loop that
+    replays a captured step makes no such call: synchronise, then ask here.
+    """
+    index = current_device() if device is None else torch.device(device).index
+    with on_device(current_device() if index is None else index):
+        result = lib().vcclKv4AttentionStatus()
+    if result:
+        _check(result, "vcclKv4Attention")
