@@ -258,3 +258,27 @@ def test_attention_that_gave_up_is_reported():
         kv4_attention_status("cuda:0")
     kv4_attention_status()
     assert torch.equal(got, want) and torch.equal(kv4_attention(q, *args), want)
+
+
+# ---- the decode step ---------------------------------------------------------------
+
+
+def test_decode_step_tells_which_requests_were_refused():
+    """Three requests and pages for two prompts: the third's rows come back, and the plan says that they saw nothing."""
+    import vkccl_b200 as v
+    from vkccl_b200.models.llama_decode import DecodeConfig, TPLlamaDecode
+
+    cfg = DecodeConfig(hidden=1024, intermediate=2048, heads=8, kv_heads=2, head_dim=128, layers=1, page_size=16)
+    comm = v.Communicator(1, v.get_unique_id(), 0, cuda_device=0)
+    try:
+        model, g = TPLlamaDecode(comm, cfg, seed=3), gen(7)
+        x = torch.randn(60, 1024, device="cuda", generator=g).bfloat16()
+        plain = model.step_cached(x.clone(), x, model.new_cache(3, 4, 64), ints([20, 20, 20]))
+        cache = model.new_cache(3, 4, 64)
+        got, plan = model.step_cached(x.clone(), x, cache, ints([20, 20, 20]), return_plan=True)
+        assert torch.equal(got, plain)
+        assert plan.kv_lens.tolist() == [20, 20, 0] and cache.lens.tolist() == [20, 20, 0]
+        assert (plan.slots[40:] == -1).all() and (plan.slots[:40] >= 0).all()
+        assert cache.free_count.tolist() == plan.free_count.tolist() == [0]
+    finally:
+        comm.destroy()

@@ -25,13 +25,13 @@ step is one page plan, then per layer the projection, norm (with
 ``qk_norm``) and rotation of the new rows with their write to the cache in one
 launch, and attention over the cache.  Prompts and single tokens go through it
 alike, and it may be captured into a CUDA graph: lengths, pages and block
-tables stay on the GPU.
+tables stay on the GPU.  ``return_plan`` tells which requests were refused.
 """
 
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, Optional, Tuple, Union
 
 import torch
 
@@ -128,13 +128,19 @@ class TPLlamaDecode:
             torch.full((1,), pages, dtype=torch.int32, device=dev), c.page_size)
 
     def step_cached(self, x: torch.Tensor, x_norm: torch.Tensor, cache: DecodeCache, new_lens: torch.Tensor,
-                    finished: Optional[torch.Tensor] = None, n_layers: int | None = None) -> torch.Tensor:
+                    finished: Optional[torch.Tensor] = None, n_layers: int | None = None, return_plan: bool = False
+                    ) -> Union[torch.Tensor, Tuple[torch.Tensor, PagePlan]]:
         """One step with attention over the cache.
 
         x, x_norm [rows, hidden] hold new_lens[i] (int32 [requests]) new rows of
         each request in order; rows behind them are padding.  finished
         (bool [requests]): requests that end, whose pages are free for this
         step.  x (residual) is updated in place; returns the final normed state.
+
+        A request for which no pages are left, or whose rows or length do not
+        fit, is refused: nothing of it is cached, and its rows come back
+        without attention.  With return_plan also the step's plan, whose
+        ``kv_lens`` is 0 where a request was refused (or holds nothing).
         """
         c, dim = self.cfg, self.cfg.head_dim
         n = self.comm.nranks
@@ -150,7 +156,7 @@ class TPLlamaDecode:
             hid = gemm_silu_mul(x_norm, L["gu"])
             part = gemm_bf16(hid, L["d"])
             x_norm = all_reduce_add_rms_norm(self.comm, part, x, L["ln2"], c.eps)
-        return x_norm
+        return (x_norm, plan) if return_plan else x_norm
 
     def step_nccl(self, x: torch.Tensor, x_norm: torch.Tensor, group=None, n_layers: int | None = None) -> torch.Tensor:
         import torch.distributed as dist
