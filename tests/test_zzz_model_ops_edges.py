@@ -282,3 +282,43 @@ def test_decode_step_tells_which_requests_were_refused():
         assert cache.free_count.tolist() == plan.free_count.tolist() == [0]
     finally:
         comm.destroy()
+
+
+# ---- gradients ---------------------------------------------------------------------
+
+
+def test_norm_rope_inside_an_autograd_function():
+    """The way to train with it: the forward call runs without grad mode, the backward call is explicit."""
+    import model_reference as ref
+    from vkccl_b200.ops.rope import qk_norm_rope, qk_norm_rope_backward
+
+    class NormRope(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, pos, freq, w):
+            ctx.save_for_backward(q, k, pos, freq, w)
+            return qk_norm_rope(q, k, pos, freq, q_weight=w, k_weight=w)
+
+        @staticmethod
+        def backward(ctx, dq, dk):
+            q, k, pos, freq, w = ctx.saved_tensors
+            dq, dk, a, b = qk_norm_rope_backward(dq.contiguous(), dk.contiguous(), q, k, pos, freq, q_weight=w, k_weight=w)
+            return dq, dk, None, None, a + b
+
+    g = gen(8)
+    q, k = (torch.randn(37, n, 64, device="cuda", generator=g).bfloat16().requires_grad_() for n in (4, 2))
+    w = (1 + 0.1 * torch.randn(64, device="cuda", generator=g)).bfloat16().requires_grad_()
+    pos, freq = torch.arange(37, dtype=torch.int32, device="cuda"), (100.0 ** (-torch.arange(32, device="cuda") / 32)).float()
+    dq, dk = (torch.randn(37, n, 64, device="cuda", generator=g).bfloat16() for n in (4, 2))
+    with pytest.raises(ValueError):
+        qk_norm_rope(q, k, pos, freq, q_weight=w, k_weight=w)
+    yq, yk = NormRope.apply(q, k, pos, freq, w)
+    torch.autograd.backward([yq, yk], [dq, dk])
+    q64, k64, w64 = (x.detach().double().requires_grad_() for x in (q, k, w))
+    ((ref.norm_rope(q64, w64, 1e-6, pos, freq, False) * dq.double()).sum()
+     + (ref.norm_rope(k64, w64, 1e-6, pos, freq, False) * dk.double()).sum()).backward()
+    for x, y in ((q, q64), (k, k64)):
+        # half a step of bf16 and f32 arithmetic on terms up to a few times the largest gradient of the row
+        slack = y.grad.abs() * 2.0**-8 * 1.02 + 2.0**-16 * y.grad.abs().amax(-1, keepdim=True)
+        assert ((x.grad.double() - y.grad).abs() <= slack).all()
+    # two sums rounded to bf16, added and rounded: each half a step of its size (at most the sum of the terms' sizes)
+    assert ((w.grad.double() - w64.grad).abs() <= 3 * 2.0**-8 * (w64.grad.abs() + 30)).all()

@@ -13,7 +13,8 @@ kv4_attention_status()                            whether an attention launch ga
 scale * (code - 7.5), 4.5 bits a value.  Slots, tables and lengths are those
 of ``vkccl_b200.ops.paging.plan_pages``.  All calls are stream-ordered on
 torch's current stream, allocate through torch and may be captured into CUDA
-graphs.
+graphs.  They are for serving: there are no gradients, and outputs have no
+autograd history.
 """
 
 from __future__ import annotations
