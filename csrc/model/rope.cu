@@ -4,12 +4,13 @@
 // pass, or alone).
 //
 // A row (one head of one token) is held by LANES neighbouring lanes with 8
-// channels each.  Where the row goes on as it is, a lane has 4 channels of the
-// row's first half and the same 4 of its second (two 8-byte loads): the two
-// channels of a pair then meet in a lane, and a row of 128 takes 4 shuffles
-// instead of 13, which shared the shared-memory pipe with the cosines (88 us
-// before, 8192 tokens of 72 heads).  Where it goes to the cache a lane has 8
-// neighbouring channels, as a word of codes does.  The cosines and sines of a block's tokens are taken
+// channels each.  In norm and rotation by themselves, and their gradients, a
+// lane has 4 channels of the row's first half and the same 4 of its second (two
+// 8-byte loads): the two channels of a pair then meet in a lane, and a row of
+// 128 takes 4 shuffles instead of 13, which shared the shared-memory pipe with
+// the cosines (8192 tokens of 72 heads: 88 us before, 73 now).  In the kernel
+// that writes the cache a lane has 8 neighbouring channels of every row, as a
+// word of codes does.  The cosines and sines of a block's tokens are taken
 // once, into shared memory: the angle position * invFreq is a product in 64
 // bits, reduced to [-pi, pi] there, since positions reach millions.
 //
@@ -169,12 +170,12 @@ __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
   x[7] = b.w;
 }
 
-// Rotates the channels of a row in place; BACK: by the negative angle.
-// angles: of the row's token.  Every operation rounds by itself.
-template <int LANES, bool BACK>
+// Rotates the channels of a row in place.  angles: of the row's token.  Every
+// operation rounds by itself.
+template <int LANES>
 __device__ __forceinline__ void rotate(float (&x)[8], int lane, const Rope& r, const float* angles) {
-  const float* up = angles + (BACK ? 2 : 1) * r.half;    // what the second channel of a pair takes
-  const float* down = angles + (BACK ? 1 : 2) * r.half;  // what the first one takes
+  const float* up = angles + r.half;        // what the second channel of a pair takes
+  const float* down = angles + 2 * r.half;  // what the first one takes
   if (r.interleaved) {
     if (8 * lane < 2 * r.half) {
       const float4 c = *reinterpret_cast<const float4*>(angles + 4 * lane);
@@ -212,7 +213,7 @@ __device__ __forceinline__ void rotate(float (&x)[8], int lane, const Rope& r, c
 // fours in order (rows of 128; one by one for 64), then the sums of the upper
 // half of the row onto those of the lower half, and so on.  Lanes trade what
 // they do not keep, so a row of 128 takes 5 shuffles, one of 64 takes 10.
-// Other rows: fours in order, then a tree over the lanes.
+// Rows of the cache are of these two sizes.
 __device__ __forceinline__ float four(const float* x) {
   float s = __fmul_rn(x[0], x[0]);
 #pragma unroll
@@ -221,8 +222,9 @@ __device__ __forceinline__ float four(const float* x) {
 }
 
 template <int LANES>
-__device__ __forceinline__ float squaresOfRow(const float (&x)[8], int lane, int D) {
-  if (LANES == 16 && D == 128) {
+__device__ __forceinline__ float squaresOfRow(const float (&x)[8], int lane) {
+  static_assert(LANES == 8 || LANES == 16, "rows of 64 or 128");
+  if constexpr (LANES == 16) {
     const float a = four(x), b = four(x + 4);
     const bool up = lane & 8;  // keeps the sums of the second fours
     float v = up ? b : a;
@@ -230,8 +232,7 @@ __device__ __forceinline__ float squaresOfRow(const float (&x)[8], int lane, int
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(~0u, v, o));
     return __fadd_rn(v, __shfl_xor_sync(~0u, v, 8));
-  }
-  if (LANES == 8 && D == 64) {
+  } else {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = __fmul_rn(x[i], x[i]);
@@ -248,10 +249,6 @@ __device__ __forceinline__ float squaresOfRow(const float (&x)[8], int lane, int
     for (int o = 4; o > 0; o >>= 1) v[0] = __fadd_rn(v[0], __shfl_xor_sync(~0u, v[0], o));
     return v[0];
   }
-  float s = __fadd_rn(four(x), four(x + 4));
-#pragma unroll
-  for (int o = 1; o < LANES; o <<= 1) s = __fadd_rn(s, __shfl_xor_sync(~0u, s, o));
-  return s;
 }
 
 // ---- rows in halves: channels 4 lane .. + 3 and D / 2 + 4 lane .. + 3 --------
@@ -278,7 +275,8 @@ __device__ __forceinline__ void loadHalves(const float* row, int lane, int D, fl
   x[7] = b.w;
 }
 
-// The same sums in the same order as squaresOfRow.
+// The same sums in the same order as squaresOfRow; rows of other sizes: fours
+// in order, then a tree over the lanes.
 template <int LANES>
 __device__ __forceinline__ float squaresOfHalves(const float (&x)[8], int lane, int D) {
   if (LANES == 8 && D == 64) {
@@ -444,13 +442,13 @@ __global__ void __launch_bounds__(kThreads, 4) appendKernel(const __grid_constan
     float x[8];
     unpack8<T>(raw, x);
     if (weight != nullptr) {
-      const float r = rsqrtf(__fadd_rn(__fmul_rn(squaresOfRow<LANES>(x, lane, p.D), share), p.rope.eps));
+      const float r = rsqrtf(__fadd_rn(__fmul_rn(squaresOfRow<LANES>(x, lane), share), p.rope.eps));
       float w[8];
       load8(w0 + 8 * lane, w);
 #pragma unroll
       for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
     }
-    rotate<LANES, false>(x, lane, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
+    rotate<LANES>(x, lane, p.rope, angles + min(row.t, n - 1) * 3 * p.rope.half);
     raw = pack8<T>(x);
   };
   uint4 ahead;
@@ -571,7 +569,8 @@ constexpr int kBackwardBlocks = 148 * 4;
 // dx = r (w g - x^ mean(w g x^)), dw = sum g x^ with g = R^-1 dy, x^ = x r,
 // r = 1 / sqrt(mean x^2 + eps).  Sums and products of neighbouring channels go
 // in pairs of f32, one instruction for both: 72 us for 8192 tokens of 40 heads
-// of 128 (3.5 TB/s), 76 without.  The forward pass gains nothing from pairs (73
+// of 128 (3.5 TB/s), 76 without; with rows of neighbouring channels and no
+// pairs it was 72 too.  The forward pass gains nothing from pairs (73
 // us for 72 heads, 4.1 TB/s): its products may not merge with its sums, which
 // the compiler does with pairs.
 template <typename T, int LANES>
