@@ -30,16 +30,19 @@
 // a query row is scaled to 2^8, 32 neighbouring tokens (what a warp turns, and
 // what a softmax thread takes at once) share a power of two for keys and one
 // for values, which the softmax puts into its scale and into the weights.
-// Where some of the 32 are more than 2^6 below the largest each has powers of
-// its own, and the softmax takes them token by token.  A row's outputs are in
+// Where some of the 32 are far below the largest (2^8 for values, 2^14 for
+// keys) each is divided by a power of its own, and the softmax puts that back
+// token by token.  A row's outputs are in
 // units of the largest weight times value that it met, so what it does not see
-// or gives no weight costs the rest no bits.  Scores, maxima, sums and outputs
-// are f32.  The maximum is followed loosely (by 8 in the base-2 logarithm), so
+// or gives no weight costs the rest no bits.  Both groups of 64 channels share
+// a row's weights, so where one's values are more than 2^16 above the other's
+// the other loses bits.  Scores, maxima, sums and outputs are f32.  The maximum is followed loosely (by 8 in the base-2 logarithm), so
 // the output is rescaled rarely.
 //
-// Measured: 856 us, 700 TFLOP/s, for 4 requests of 1024 rows against 2000 to
-// 9000 tokens, 64 heads on 8 (the single-token kernel takes 3.4 ms).  The
-// softmax bounds it: 2230 of the 3070 clocks that a tile takes.
+// Measured: 840 us, 715 TFLOP/s, for 4 requests of 1024 rows against 2000 to
+// 9000 tokens, 64 heads on 8 (the single-token kernel takes 3.4 ms); 1.8 ms where
+// every 32 tokens hold values 2^10 apart.  The softmax bounds it: 2230 of the
+// 3070 clocks that a tile takes.
 #pragma once
 
 #include "kernels/kv4.cuh"
@@ -54,10 +57,13 @@ constexpr int kChunkKeys = 64;
 constexpr int kChunkStages = 4;     // tiles of keys, and of values, in shared memory
 constexpr int kChunkThreads = 16 * 32;
 constexpr int kLeastExponent = -112;  // of 32 tokens that are all zero, or next to it
-constexpr int kSpread = 6;            // binary orders that 32 tokens may lie apart and share a power of two
-// The largest weight times value of a row becomes 2^4 in f16, times up to 2^13
-// of the value, when its unit moves, and may grow to 2^14 until it moves again.
-constexpr float kTopWeight = 4.0f, kMostWeight = 14.0f;
+// Binary orders that 32 tokens may lie apart and share a power of two: keys and
+// their sums then keep all bits; a row whose weight is on the smallest value
+// loses 2^-21 of it for each other token.
+constexpr int kKeysApart = 14, kValuesApart = 8;
+// The largest weight times value of a row becomes 2^6 in f16, times up to 2^13
+// of the value, when its unit moves, and may grow to 2^15 until it moves again.
+constexpr float kTopWeight = 6.0f, kMostWeight = 15.0f;
 
 // 32 lanes x 32 bit, 32 consecutive columns per thread.
 __device__ __forceinline__ void tmemLoad32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -76,16 +82,6 @@ __device__ __forceinline__ void tmemStore16(uint32_t taddr, const uint32_t (&r)[
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmemStore32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
 __device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -177,17 +173,20 @@ struct ChunkSmem {
   static constexpr int kStarts = kInfo + 1680;  // units before each request
 };
 
-// kApart: tokens have powers of two of their own, of keys or of values.
-constexpr uint32_t kUneven = 1, kApart = 2;
+// Of a tile, by 32 tokens: some are not there or not finite; keys, values with
+// powers of two of their own.
+constexpr uint32_t kUneven = 1, kOwnKeys = 2, kOwnValues = 4;
 
 // What the tokens of a tile bring, by 32.
 struct alignas(16) ChunkInfo {
   uint32_t valid[2];               // the token is there
   float keyUnit[2];                // the power of two that its keys are divided by
   float valueExp[2];               // the logarithm of that of its values
-  uint32_t kind[2];                // kUneven: some tokens are not there, or not finite; kApart
+  uint32_t kind[2];
   uint32_t bad[2][2];              // its values of a group are not finite (and zero in the product)
-  signed char keyExps[64], valueExps[64];  // the logarithms token by token, where 32 lie apart
+  // Where they have powers of their own: 127 + the orders that the token's is
+  // below the largest, which the two above are then of.
+  uint8_t keyOrder[64], valueOrder[64];
 };
 
 struct ChunkControl {
@@ -308,16 +307,38 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// The weights of 32 scores, to TMEM in their place; returns their sum.
-__device__ __forceinline__ float halfWeights(const uint32_t (&s)[32], uint32_t at, float scale, float off) {
+// 2^-n and -n from the byte 127 - n that i is of four.
+__device__ __forceinline__ float powerOfOrder(uint32_t four, int i) {
+  return __uint_as_float(__byte_perm(four, 0u, 0x0444 | (i << 12)) >> 1);
+}
+__device__ __forceinline__ float logOfOrder(uint32_t four, int i) {
+  return __uint_as_float(__byte_perm(four, 0x4B000000u, 0x7650 | i)) - 8388735.0f;  // 2^23 + 127
+}
+
+// Scores of keys with powers of their own, in units of the largest one's.
+__device__ __forceinline__ void levelScores(uint32_t (&s)[32], const uint8_t* orders) {
+  const uint32_t* four = reinterpret_cast<const uint32_t*>(orders);
+#pragma unroll
+  for (int i = 0; i < 32; i++) s[i] = __float_as_uint(__uint_as_float(s[i]) * powerOfOrder(four[i >> 2], i & 3));
+}
+
+// The weights of 32 scores, to TMEM in their place; returns their sum.  orders:
+// of the values, where they have powers of their own.
+template <bool OWN>
+__device__ __forceinline__ float halfWeights(const uint32_t (&s)[32], uint32_t at, float scale, float off, const uint8_t* orders) {
+  const uint32_t* four = reinterpret_cast<const uint32_t*>(orders);
   uint64_t part[2] = {0, 0};
   const uint64_t by = pair(scale), plus = pair(off);
   uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 16; i++) {
     const float2 x = unpair(fma2(pair(s[2 * i], s[2 * i + 1]), by, plus));
-    const float a = exp2Fast(x.x), b = exp2Fast(x.y);
+    float a = exp2Fast(x.x), b = exp2Fast(x.y);
     part[i & 1] = add2(part[i & 1], pair(__float_as_uint(a), __float_as_uint(b)));
+    if (OWN) {
+      a *= powerOfOrder(four[i >> 1], (2 * i) & 3);
+      b *= powerOfOrder(four[i >> 1], (2 * i + 1) & 3);
+    }
     w[i] = packHalf(a, b);
   }
   tmemStore16(at, w);
@@ -375,7 +396,8 @@ __device__ __forceinline__ uint32_t poisoned(const ChunkInfo& info, uint32_t see
   return (((bad.x & seen0) | (bad.y & seen1)) ? 1u : 0u) | (((bad.z & seen0) | (bad.w & seen1)) ? 2u : 0u);
 }
 
-// One tile's scores to weights.  Returns false if a wait ran out.
+// One tile's scores to weights.  EDGE: the tile is uneven, or some row of the
+// warp does not see some token.  Returns false if a wait ran out.
 template <int G, bool EDGE>
 __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32_t output, const ChunkInfo& info, float unit,
                                             int left, bool first, uint64_t* before, uint32_t beforeParity, volatile int* abortFlag) {
@@ -387,16 +409,23 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
   for (int k = 0; k < 2; k++) {
     uint32_t s[32];
     loadScores<EDGE>(scores + 32 * k, s, k ? seen1 : seen0);
+    if (EDGE && (info.kind[k] & kOwnKeys)) levelScores(s, info.keyOrder + 32 * k);
     float x[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = __uint_as_float(s[i]);
 #pragma unroll
     for (int i = 4; i < 32; i += 2) x[(i >> 1) & 3] = max3(x[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-    const float most = max3(x[0], x[1], fmaxf(x[2], x[3]));
+    const float most = max3(x[0], x[1], fmaxf(x[2], x[3])), scale = k ? scale1 : scale0;
     if (!EDGE || most > -INFINITY) {
-      const float score = most * (k ? scale1 : scale0);
-      top = fmaxf(top, score);
-      high = fmaxf(high, score + (k ? valueExp.y : valueExp.x));
+      top = fmaxf(top, most * scale);
+      float weighed = most * scale;  // with the values' orders
+      if (EDGE && (info.kind[k] & kOwnValues)) {
+        const uint32_t* four = reinterpret_cast<const uint32_t*>(info.valueOrder + 32 * k);
+        weighed = kNone;
+#pragma unroll
+        for (int i = 0; i < 32; i++) weighed = fmaxf(weighed, fmaf(__uint_as_float(s[i]), scale, logOfOrder(four[i >> 2], i & 3)));
+      }
+      high = fmaxf(high, weighed + (k ? valueExp.y : valueExp.x));
     }
   }
   if (!follow<64 * G>(r, top, high, output, first, before, beforeParity, abortFlag)) return false;
@@ -405,73 +434,49 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
   for (int k = 0; k < 2; k++) {
     uint32_t s[32];
     loadScores<EDGE>(scores + 32 * k, s, k ? seen1 : seen0);
-    const float shift = k ? shift1 : shift0;
-    r.l = fmaf(halfWeights(s, scores + 16 * k, k ? scale1 : scale0, shift - r.m), exp2Fast(-shift), r.l);
+    const float shift = k ? shift1 : shift0, scale = k ? scale1 : scale0;
+    float sum;
+    if (EDGE && (info.kind[k] & kOwnKeys)) levelScores(s, info.keyOrder + 32 * k);
+    if (EDGE && (info.kind[k] & kOwnValues)) sum = halfWeights<true>(s, scores + 16 * k, scale, shift - r.m, info.valueOrder + 32 * k);
+    else sum = halfWeights<false>(s, scores + 16 * k, scale, shift - r.m, nullptr);
+    r.l = fmaf(sum, exp2Fast(-shift), r.l);
   }
   if (EDGE) r.poison |= poisoned(info, seen0, seen1);
   return true;
 }
 
+// The uneven tiles' code stands out of the way of the others': in line it cost
+// 2 % of the whole kernel.
 struct Followed {
   RowState row;
   bool ok;
 };
-
-// The same where tokens have powers of two of their own.  Rare, and out of the
-// way of the others' code: in line it cost 7 % of the whole kernel.
 template <int G>
-__device__ __noinline__ Followed tileSoftmaxApart(RowState r, uint32_t scores, uint32_t output, const ChunkInfo* info, float unit,
-                                                  int left, bool first, uint64_t* before, uint32_t beforeParity,
-                                                  volatile int* abortFlag) {
-  const uint32_t seen0 = seenOf(info->valid[0], left), seen1 = seenOf(info->valid[1], left - 32);
-  float top = kNone, high = kNone;
-  auto keyScale = [&](int k, int i) {
-    return notZero(unit * ((info->kind[k] & kApart) ? powerOfTwo(info->keyExps[32 * k + i]) : info->keyUnit[k]));
-  };
-  auto valueExp = [&](int k, int i) { return (info->kind[k] & kApart) ? static_cast<float>(info->valueExps[32 * k + i]) : info->valueExp[k]; };
-#pragma unroll 1
-  for (int k = 0; k < 2; k++) {
-    uint32_t s[32];
-    loadScores<true>(scores + 32 * k, s, k ? seen1 : seen0);
-#pragma unroll
-    for (int i = 0; i < 32; i++) {
-      const float score = __uint_as_float(s[i]) * keyScale(k, i);
-      top = fmaxf(top, score);
-      high = fmaxf(high, score + valueExp(k, i));
-    }
-  }
-  if (!follow<64 * G>(r, top, high, output, first, before, beforeParity, abortFlag)) return {r, false};
-#pragma unroll 1
-  for (int k = 0; k < 2; k++) {
-    uint32_t s[32], w[16];
-    loadScores<true>(scores + 32 * k, s, k ? seen1 : seen0);
-    float sum = 0.0f, y[2];
-#pragma unroll
-    for (int i = 0; i < 32; i++) {
-      const float x = fmaf(__uint_as_float(s[i]), keyScale(k, i), -r.m);
-      sum += exp2Fast(x);
-      y[i & 1] = exp2Fast(x + shiftOf(valueExp(k, i), r.ref));
-      if (i & 1) w[i >> 1] = packHalf(y[0], y[1]);
-    }
-    tmemStore16(scores + 16 * k, w);
-    r.l += sum;
-  }
-  r.poison |= poisoned(*info, seen0, seen1);
-  return {r, true};
+__device__ __noinline__ Followed edgeSoftmax(RowState r, uint32_t scores, uint32_t output, const ChunkInfo* info, float unit, int left,
+                                             bool first, uint64_t* before, uint32_t beforeParity, volatile int* abortFlag) {
+  const bool ok = tileSoftmax<G, true>(r, scores, output, *info, unit, left, first, before, beforeParity, abortFlag);
+  return {r, ok};
 }
 
 // Logarithm of the power of two of a token's keys or values: divided by it,
-// the largest is below 2^13.  That of the largest of 32, or where they lie
-// apart the token's own.  scale, mid: of the lane's token.
+// the largest is below 2^13.  That of the largest of 32, most, or the token's
+// own where some lie more than `apart` orders below (at most kMostOrders then:
+// a weight times 2^kMostOrders is an f32).  scale, mid: of the lane's token.
+constexpr int kMostOrders = 100;
+struct Exponent {
+  int most, mine;
+  bool own;
+};
 template <int G>
-__device__ __forceinline__ int exponentOf32(const float (&scale)[G], const float (&mid)[G], bool* apart) {
+__device__ __forceinline__ Exponent exponentOf32(const float (&scale)[G], const float (&mid)[G], int apart) {
   float top = 0.0f;
 #pragma unroll
   for (int g = 0; g < G; g++) top = fmaxf(top, fmaf(8.5f, fabsf(scale[g]), fabsf(mid[g])));
   // positive floats are ordered like their bits
   const int most = exponentOf(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top)))), mine = exponentOf(top);
-  *apart = __any_sync(~0u, top > 0.0f && mine < most - kSpread);
-  return max((*apart ? mine : most) - 12, kLeastExponent);
+  const bool own = __any_sync(~0u, top > 0.0f && mine < most - apart);
+  const int e = max(most - 12, kLeastExponent);
+  return {e, own ? max(max(mine - 12, kLeastExponent), e - kMostOrders) : e, own};
 }
 
 // A token's row of codes with its parameters; a key thread has those of the
@@ -727,13 +732,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
           const int left = mineLimit - j * kChunkKeys;  // keys of the tile in the row's range
           uint64_t* before = &ctl.pvDone[t][(count - 1) & 1];
           const uint32_t parity = ((count - 1) >> 1) & 1u;
-          const uint32_t kind = info.kind[0] | info.kind[1];
-          if (!__any_sync(~0u, left < kChunkKeys || kind != 0)) {
+          if (!__any_sync(~0u, left < kChunkKeys || (info.kind[0] | info.kind[1]) != 0)) {
             ok = tileSoftmax<G, false>(state, scores, output, info, mineUnit, left, j == c.from, before, parity, abortFlag);
-          } else if ((kind & kApart) == 0) {
-            ok = tileSoftmax<G, true>(state, scores, output, info, mineUnit, left, j == c.from, before, parity, abortFlag);
           } else {
-            const Followed f = tileSoftmaxApart<G>(state, scores, output, &info, mineUnit, left, j == c.from, before, parity, abortFlag);
+            const Followed f = edgeSoftmax<G>(state, scores, output, &info, mineUnit, left, j == c.from, before, parity, abortFlag);
             state = f.row;
             ok = f.ok;
           }
@@ -867,17 +869,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         if (odd) s[g] = m[g] = 0.0f;
         bad[g] = __ballot_sync(~0u, odd);
       }
-      bool valuesApart;
-      const int ve = exponentOf32<G>(s, m, &valuesApart);
+      const Exponent ve = exponentOf32<G>(s, m, kValuesApart);
       if (keys) {
 #pragma unroll
         for (int g = 0; g < G; g++) {
           s[g] = kv4::bf16Lo(raw.keyParams[g]);
           m[g] = kv4::bf16Hi(raw.keyParams[g]);
         }
-        bool keysApart;
-        const int ke = exponentOf32<G>(s, m, &keysApart);
-        const float f = powerOfTwo(-ke);
+        const Exponent ke = exponentOf32<G>(s, m, kKeysApart);
+        const float f = powerOfTwo(-ke.mine);
 #pragma unroll
         for (int g = 0; g < G; g++) {
           s[g] *= f;
@@ -886,16 +886,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         const uint32_t present = __ballot_sync(~0u, raw.there);
         if (!warpWait(&ctl.kEmpty[st], parity, abortFlag)) break;
         ChunkInfo& info = ctl.info[seq & 7];
-        const bool apart = keysApart || valuesApart;
-        if (apart) {
-          info.keyExps[tid] = static_cast<signed char>(ke);
-          info.valueExps[tid] = static_cast<signed char>(ve);
-        }
+        if (ke.own) info.keyOrder[tid] = static_cast<uint8_t>(127 + ke.mine - ke.most);
+        if (ve.own) info.valueOrder[tid] = static_cast<uint8_t>(127 + ve.mine - ve.most);
         if (lane == 0) {
           info.valid[w] = present;
-          info.keyUnit[w] = powerOfTwo(ke);
-          info.valueExp[w] = static_cast<float>(ve);
-          info.kind[w] = (present != ~0u || bad[0] != 0 || bad[G - 1] != 0 ? kUneven : 0) | (apart ? kApart : 0);
+          info.keyUnit[w] = powerOfTwo(ke.most);
+          info.valueExp[w] = static_cast<float>(ve.most);
+          info.kind[w] = (present != ~0u || bad[0] != 0 || bad[G - 1] != 0 ? kUneven : 0) | (ke.own ? kOwnKeys : 0) | (ve.own ? kOwnValues : 0);
 #pragma unroll
           for (int g = 0; g < 2; g++) info.bad[g][w] = g < G ? bad[g < G ? g : 0] : 0;
         }
@@ -904,7 +901,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         sm100::fenceProxyAsyncShared();
         sm100::mbarArrive(&ctl.kFull[st]);
       } else {
-        const float f = powerOfTwo(-ve);
+        const float f = powerOfTwo(-ve.mine);
 #pragma unroll
         for (int g = 0; g < G; g++) {
           s[g] *= f;
