@@ -322,3 +322,85 @@ def test_norm_rope_inside_an_autograd_function():
         assert ((x.grad.double() - y.grad).abs() <= slack).all()
     # two sums rounded to bf16, added and rounded: each half a step of its size (at most the sum of the terms' sizes)
     assert ((w.grad.double() - w64.grad).abs() <= 3 * 2.0**-8 * (w64.grad.abs() + 30)).all()
+
+
+# ---- long runs of rows: what the short ones are tested for -------------------------
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([300, 7, 100], [0, 3, 40]), ([90] * 40, [0, 1, 89, 90, 91, 63, 64, 65, 127, 200] * 4)])
+@pytest.mark.parametrize("page", [16, 48])
+def test_long_runs_without_keys_and_with_fewer_keys_than_rows(q_lens, kv_lens, page):
+    """Requests of many rows that hold nothing, or fewer tokens than rows, with and without shares of the keys; pages of 48."""
+    from test_zzz_kv4 import check_attention, filled, starts
+    from vkccl_b200.ops.kv4 import kv4_attention
+
+    g = gen(11)
+    cache, table, ks, vs = filled(g, kv_lens, page, 8, 128)
+    qs = starts(q_lens)
+    q = torch.randn(qs[-1] + 5, 16, 128, device="cuda", generator=g).bfloat16()
+    out, lse = kv4_attention(q, cache, table, ints(kv_lens), ints(qs), return_lse=True)
+    check_attention(out, lse, q, ks, vs, kv_lens, qs)
+    assert out[qs[-1]:].abs().max() == 0 and torch.isinf(lse[qs[-1]:]).all()
+    again = kv4_attention(q, cache, table, ints(kv_lens), ints(qs))
+    assert torch.equal(out, again)
+
+
+def test_long_runs_do_not_see_bad_pages():
+    from vkccl_b200.ops.kv4 import kv4_attention
+
+    g = gen(12)
+    n, rows = 300, 40
+    cache = random_cache(g, 40, 16, 1, 128)
+    table = torch.randperm(40, device="cuda", generator=g).int()[:19].view(1, 19)
+    bad = table.clone()
+    bad[0, 3], bad[0, 7], bad[0, 8] = -1, cache.shape[0], 2**31 - 1
+    q = torch.randn(rows, 8, 128, device="cuda", generator=g).bfloat16()
+    out, lse = kv4_attention(q, cache, bad, ints([n]), ints([0, rows]), return_lse=True)
+    keep = [i for i in range(19) if i not in (3, 7, 8)]
+    # the pages that are left, in order: the last rows see the same tokens, 48 fewer
+    want, wlse = kv4_attention(q, cache, table[:, keep].contiguous(), ints([n - 48]), ints([0, rows]), return_lse=True)
+    # sums of the same terms in other tiles: f32, and weights rounded to f16 in other units
+    assert (out.float() - want.float()).abs().max() <= 2.0**-7 and (lse - wlse).abs().max() <= 2.0**-16
+
+
+@pytest.mark.parametrize("dtype,f", [(torch.bfloat16, 2.0**-60), (torch.bfloat16, 2.0**60), (torch.bfloat16, 0.0), (torch.float16, 2.0**-13),
+                                     (torch.float16, 2.0**12)])
+@pytest.mark.parametrize("rows", [2, 30])
+def test_queries_of_every_size(dtype, f, rows):
+    """Queries next to the ends of their type, the scale making up for it: few rows and long runs."""
+    from test_zzz_kv4 import check_attention, filled
+    from vkccl_b200.ops.kv4 import kv4_attention
+
+    g = gen(13)
+    cache, table, ks, vs = filled(g, [500], 16, 2, 128)
+    q = (torch.randn(rows, 16, 128, device="cuda", generator=g) * f).to(dtype)
+    scale = 0.1 / f if f else 0.1
+    out, lse = kv4_attention(q, cache, table, ints([500]), ints([0, rows]), return_lse=True, scale=scale)
+    check_attention(out, lse, q, ks, vs, [500], [0, rows], scale=scale)
+
+
+@pytest.mark.parametrize("dim,rot", [(24, 16), (40, 32), (72, 64), (104, 48), (136, 128), (200, 112), (248, 240)])
+@pytest.mark.parametrize("inter", [False, True])
+def test_norm_rope_of_odd_head_dimensions(dim, rot, inter):
+    """Head dimensions that are multiples of 8 and not of 16: a row's halves end inside of 8 channels."""
+    import model_reference as ref
+    from test_zzz_kv4 import close, inv_freq, rope_slack
+    from vkccl_b200.ops.rope import qk_norm_rope, qk_norm_rope_backward
+
+    g = gen(dim)
+    tokens, w = 53, (1 + 0.2 * torch.randn(dim, device="cuda", generator=g)).bfloat16()
+    q, k, dq, dk = (torch.randn(tokens, n, dim, device="cuda", generator=g).bfloat16() for n in (3, 1, 3, 1))
+    pos, freq = ints([i * 1001 for i in range(tokens)]), inv_freq(rot)
+    out = torch.full((tokens, 5, dim), 7.0, device="cuda").bfloat16()
+    yq, yk = qk_norm_rope(q, k, pos, freq, q_weight=w, k_weight=w, interleaved=inter, q_out=out[:, :3], k_out=out[:, 3:4])
+    assert (out[:, 4] == 7.0).all()
+    gq, gk, dwq, dwk = qk_norm_rope_backward(dq, dk, q, k, pos, freq, q_weight=w, k_weight=w, interleaved=inter)
+    for x, y, d, dx, dw in ((q, yq, dq, gq, dwq), (k, yk, dk, gk, dwk)):
+        leaf, wl = x.double().requires_grad_(), w.double().requires_grad_()
+        want = ref.norm_rope(leaf, wl, 1e-6, pos, freq, inter)
+        close(y, want.detach(), rope_slack(want.detach(), torch.bfloat16, want.detach().abs().amax(-1, keepdim=True)), "forward")
+        (want * d.double()).sum().backward()
+        size = leaf.grad.abs().amax(-1, keepdim=True) + d.double().abs().amax(-1, keepdim=True) * 6 / x.double().square().mean(-1, keepdim=True).sqrt()
+        close(dx, leaf.grad, rope_slack(leaf.grad, torch.bfloat16, size), "dx")
+        # terms |g x^| of at most 6 * 6, f32 sums of a lane's rows
+        close(dw, wl.grad, wl.grad.abs() * 2.0**-8 + tokens * 3 * 36 * 2.0**-20, "dw")
