@@ -682,13 +682,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         if (p.half16) unpack8<__half>(raw[i], x);
         else unpack8<__nv_bfloat16>(raw[i], x);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          amax = fmaxf(amax, fabsf(x[e]));
-          sums[i / 8] += x[e];
-        }
+        for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[e]));
       }
       const int e = exponentOf(amax);
-      const bool plain = amax == 0.0f || e > 120 || e < -100;
+      const bool plain = e > 127 || e < -118;  // not finite; counts as zero
       const float f = (plain ? 1.0f : powerOfTwo(8 - e)) * (p.scaleLog2 < 0.0f ? -1.0f : 1.0f);
       unit = (plain ? 1.0f : powerOfTwo(e - 8)) * fabsf(p.scaleLog2);
 #pragma unroll
@@ -697,11 +694,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
         if (p.half16) unpack8<__half>(raw[i], x);
         else unpack8<__nv_bfloat16>(raw[i], x);
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[k] *= f;
+        for (int k = 0; k < 8; k++) {
+          x[k] *= f;
+          sums[i / 8] += x[k];
+        }
         *reinterpret_cast<uint4*>(smem + L::kQ + (t * G + i / 8) * L::kQBlock + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = pack8<__half>(x);
       }
-#pragma unroll
-      for (int g = 0; g < G; g++) sums[g] *= f;
       storeSums<G, true>(smem + L::kQSums + t * (128 * 32), row, sums);
       sm100::fenceProxyAsyncShared();
       sm100::mbarArrive(&ctl.qFull[t]);

@@ -323,9 +323,10 @@ __device__ __forceinline__ void loadQuery(Unit<G, NT>& u, const AttnArgs& p, con
     }
     amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-    // f = 2^(12 - exponent of the largest); kept in f32's range.
+    // f = 2^(12 - exponent of the largest), 1 / f beside it; a row below 2^-114
+    // counts as zero, one that is not finite stays so.
     const int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-    const bool plain = amax == 0.0f || e > 120 || e < -100;
+    const bool plain = e > 127 || e < -114;
     const float f = plain ? 1.0f : __uint_as_float(static_cast<uint32_t>(127 + 12 - e) << 23);
     const float back = plain ? 1.0f : __uint_as_float(static_cast<uint32_t>(127 - 12 + e) << 23);
     float qs = back * p.scaleLog2 * 16777216.0f;
@@ -334,10 +335,10 @@ __device__ __forceinline__ void loadQuery(Unit<G, NT>& u, const AttnArgs& p, con
     for (int gr = 0; gr < G; gr++) {
       float s = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 16; j++) s += x[gr][j];
+      for (int j = 0; j < 16; j++) s = fmaf(x[gr][j], f, s);
       s += __shfl_xor_sync(~0u, s, 1);
       s += __shfl_xor_sync(~0u, s, 2);
-      sq[gr] = s * f * 5.9604644775390625e-8f;
+      sq[gr] = s * 5.9604644775390625e-8f;
 #pragma unroll
       for (int w = 0; w < 4; w++) {  // word half w / 2, code pair w % 2: channels 4w .. 4w + 3 of the lane's 16
         const float* y = &x[gr][4 * w];

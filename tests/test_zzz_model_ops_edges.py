@@ -363,7 +363,8 @@ def test_long_runs_do_not_see_bad_pages():
     assert (out.float() - want.float()).abs().max() <= 2.0**-7 and (lse - wlse).abs().max() <= 2.0**-16
 
 
-@pytest.mark.parametrize("dtype,f", [(torch.bfloat16, 2.0**-60), (torch.bfloat16, 2.0**60), (torch.bfloat16, 0.0), (torch.float16, 2.0**-13),
+@pytest.mark.parametrize("dtype,f", [(torch.bfloat16, 2.0**-60), (torch.bfloat16, 2.0**60), (torch.bfloat16, 2.0**-112),
+                                     (torch.bfloat16, 2.0**124), (torch.bfloat16, 0.0), (torch.float16, 2.0**-13),
                                      (torch.float16, 2.0**12)])
 @pytest.mark.parametrize("rows", [2, 30])
 def test_queries_of_every_size(dtype, f, rows):
