@@ -39,7 +39,7 @@
 // the other loses bits.  Scores, maxima, sums and outputs are f32.  The maximum is followed loosely (by 8 in the base-2 logarithm), so
 // the output is rescaled rarely.
 //
-// Measured: 840 us, 715 TFLOP/s, for 4 requests of 1024 rows against 2000 to
+// Measured: 842 us, 715 TFLOP/s, for 4 requests of 1024 rows against 2000 to
 // 9000 tokens, 64 heads on 8 (the single-token kernel takes 3.4 ms); 1.8 ms where
 // every 32 tokens hold values 2^10 apart.  The softmax bounds it: 2230 of the
 // 3070 clocks that a tile takes.
@@ -396,9 +396,10 @@ __device__ __forceinline__ uint32_t poisoned(const ChunkInfo& info, uint32_t see
   return (((bad.x & seen0) | (bad.y & seen1)) ? 1u : 0u) | (((bad.z & seen0) | (bad.w & seen1)) ? 2u : 0u);
 }
 
-// One tile's scores to weights.  EDGE: the tile is uneven, or some row of the
-// warp does not see some token.  Returns false if a wait ran out.
-template <int G, bool EDGE>
+// One tile's scores to weights.  EDGE: tokens are missing or not finite, or some
+// row of the warp does not see some; OWN: some have powers of two of their own.
+// Returns false if a wait ran out.
+template <int G, bool EDGE, bool OWN>
 __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32_t output, const ChunkInfo& info, float unit,
                                             int left, bool first, uint64_t* before, uint32_t beforeParity, volatile int* abortFlag) {
   const float2 keyUnit = *reinterpret_cast<const float2*>(info.keyUnit), valueExp = *reinterpret_cast<const float2*>(info.valueExp);
@@ -409,7 +410,7 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
   for (int k = 0; k < 2; k++) {
     uint32_t s[32];
     loadScores<EDGE>(scores + 32 * k, s, k ? seen1 : seen0);
-    if (EDGE && (info.kind[k] & kOwnKeys)) levelScores(s, info.keyOrder + 32 * k);
+    if (OWN && (info.kind[k] & kOwnKeys)) levelScores(s, info.keyOrder + 32 * k);
     float x[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = __uint_as_float(s[i]);
@@ -419,7 +420,7 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
     if (!EDGE || most > -INFINITY) {
       top = fmaxf(top, most * scale);
       float weighed = most * scale;  // with the values' orders
-      if (EDGE && (info.kind[k] & kOwnValues)) {
+      if (OWN && (info.kind[k] & kOwnValues)) {
         const uint32_t* four = reinterpret_cast<const uint32_t*>(info.valueOrder + 32 * k);
         weighed = kNone;
 #pragma unroll
@@ -436,8 +437,8 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
     loadScores<EDGE>(scores + 32 * k, s, k ? seen1 : seen0);
     const float shift = k ? shift1 : shift0, scale = k ? scale1 : scale0;
     float sum;
-    if (EDGE && (info.kind[k] & kOwnKeys)) levelScores(s, info.keyOrder + 32 * k);
-    if (EDGE && (info.kind[k] & kOwnValues)) sum = halfWeights<true>(s, scores + 16 * k, scale, shift - r.m, info.valueOrder + 32 * k);
+    if (OWN && (info.kind[k] & kOwnKeys)) levelScores(s, info.keyOrder + 32 * k);
+    if (OWN && (info.kind[k] & kOwnValues)) sum = halfWeights<true>(s, scores + 16 * k, scale, shift - r.m, info.valueOrder + 32 * k);
     else sum = halfWeights<false>(s, scores + 16 * k, scale, shift - r.m, nullptr);
     r.l = fmaf(sum, exp2Fast(-shift), r.l);
   }
@@ -445,16 +446,16 @@ __device__ __forceinline__ bool tileSoftmax(RowState& r, uint32_t scores, uint32
   return true;
 }
 
-// The uneven tiles' code stands out of the way of the others': in line it cost
-// 2 % of the whole kernel.
+// Rare code stands out of the way of the other: in line it cost the whole
+// kernel 2 %, and short requests, whose tiles all are at an edge, 8 %.
 struct Followed {
   RowState row;
   bool ok;
 };
 template <int G>
-__device__ __noinline__ Followed edgeSoftmax(RowState r, uint32_t scores, uint32_t output, const ChunkInfo* info, float unit, int left,
-                                             bool first, uint64_t* before, uint32_t beforeParity, volatile int* abortFlag) {
-  const bool ok = tileSoftmax<G, true>(r, scores, output, *info, unit, left, first, before, beforeParity, abortFlag);
+__device__ __noinline__ Followed ownSoftmax(RowState r, uint32_t scores, uint32_t output, const ChunkInfo* info, float unit, int left,
+                                            bool first, uint64_t* before, uint32_t beforeParity, volatile int* abortFlag) {
+  const bool ok = tileSoftmax<G, true, true>(r, scores, output, *info, unit, left, first, before, beforeParity, abortFlag);
   return {r, ok};
 }
 
@@ -730,10 +731,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunkKernel(const __grid_con
           const int left = mineLimit - j * kChunkKeys;  // keys of the tile in the row's range
           uint64_t* before = &ctl.pvDone[t][(count - 1) & 1];
           const uint32_t parity = ((count - 1) >> 1) & 1u;
-          if (!__any_sync(~0u, left < kChunkKeys || (info.kind[0] | info.kind[1]) != 0)) {
-            ok = tileSoftmax<G, false>(state, scores, output, info, mineUnit, left, j == c.from, before, parity, abortFlag);
+          const uint32_t kind = info.kind[0] | info.kind[1];
+          if (!__any_sync(~0u, left < kChunkKeys || kind != 0)) {
+            ok = tileSoftmax<G, false, false>(state, scores, output, info, mineUnit, left, j == c.from, before, parity, abortFlag);
+          } else if (kind <= kUneven) {
+            ok = tileSoftmax<G, true, false>(state, scores, output, info, mineUnit, left, j == c.from, before, parity, abortFlag);
           } else {
-            const Followed f = edgeSoftmax<G>(state, scores, output, &info, mineUnit, left, j == c.from, before, parity, abortFlag);
+            const Followed f = ownSoftmax<G>(state, scores, output, &info, mineUnit, left, j == c.from, before, parity, abortFlag);
             state = f.row;
             ok = f.ok;
           }

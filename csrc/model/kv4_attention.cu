@@ -648,7 +648,7 @@ __device__ __forceinline__ void finish(Unit<G, NT>& u, const AttnArgs& p, const 
       const float norm = slot < 0 ? (none ? 0.0f : 1.0f / l) : 1.0f;
 #pragma unroll
       for (int gr = 0; gr < G; gr++) {
-        const float back = 1.0f / u.by[n][gr][c];
+        const float back = __fdividef(1.0f, u.by[n][gr][c]);
         const float base = fmaf(-7.5f * u.ones[n][gr][c], back, mid[gr]);
         float y[8];
 #pragma unroll
