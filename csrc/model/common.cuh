@@ -17,6 +17,10 @@
 namespace vccl {
 namespace model {
 
+// Rows of a call: row numbers rounded up to whole blocks stay in an int.
+constexpr int kMaxTokens = 1 << 30;
+inline bool tokensOk(int tokens) { return tokens >= 0 && tokens <= kMaxTokens; }
+
 // 16-byte vectors: base and strides in whole vectors, and strides and head
 // counts that the kernels' index arithmetic holds (products are 64 bits).
 inline bool headsOk(const vcclHeads_t* h, int elemBytes) {

@@ -1040,7 +1040,7 @@ vcclResult_t vcclKv4Attention(const vcclHeads_t* q, const vcclKv4_t* cache, cons
                               const int* kvLens, const int* qStarts, int batch, int tokens, float scale,
                               const vcclHeads_t* out, float* lse, int zeroTail, void* workspace,
                               vcclDataType_t datatype, vcclStream_t stream) {
-  if (!cacheOk(cache) || tokens < 0 || batch <= 0 || batch > kMaxBatch || width <= 0 ||
+  if (!cacheOk(cache) || !tokensOk(tokens) || batch <= 0 || batch > kMaxBatch || width <= 0 ||
       static_cast<long long>(width) * cache->pageSize > (1 << 30) ||  // token numbers and a tile more fit an int
       (datatype != vcclBfloat16 && datatype != vcclFloat16))
     return vcclInvalidArgument;

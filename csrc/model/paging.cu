@@ -208,7 +208,7 @@ extern "C" vcclResult_t vcclPagePlan(const int* lens, const int* newLens, const 
                                      int pageSize, int tokens, int* positions, int* slots, int* requests,
                                      int* qStarts, int* kvLens, int* lensOut, int* countOut, int* scratch, vcclStream_t stream) {
   if (!lens || !newLens || !table || !freePages || !freeCount || !qStarts || !kvLens || !lensOut || !countOut || !scratch ||
-      batch <= 0 || batch > model::kPlanMaxBatch || width <= 0 || poolSize <= 0 || pageSize <= 0 || tokens < 0 ||
+      batch <= 0 || batch > model::kPlanMaxBatch || width <= 0 || poolSize <= 0 || pageSize <= 0 || !model::tokensOk(tokens) ||
       static_cast<long long>(poolSize) * pageSize > INT_MAX || static_cast<long long>(width) * pageSize > INT_MAX ||
       (tokens > 0 && (!positions || !slots || !requests)))
     return vcclInvalidArgument;

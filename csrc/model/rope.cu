@@ -784,7 +784,7 @@ extern "C" {
 vcclResult_t vcclQkNormRope(const vcclHeads_t* q, const vcclHeads_t* k, const vcclRope_t* rope,
                             const vcclHeads_t* qOut, const vcclHeads_t* kOut, int tokens, int D,
                             vcclDataType_t datatype, vcclStream_t stream) {
-  if (tokens < 0 || D <= 0 || D % 8 != 0 || D > 256 || !sixteenBit(datatype) || !ropeOk(rope, D, tokens))
+  if (!tokensOk(tokens) || D <= 0 || D % 8 != 0 || D > 256 || !sixteenBit(datatype) || !ropeOk(rope, D, tokens))
     return vcclInvalidArgument;
   if (tokens == 0) return vcclSuccess;
   if (!headsOk(q, 2) || !headsOk(k, 2) || !headsOk(qOut, 2) || !headsOk(kOut, 2) || q->heads != qOut->heads ||
@@ -812,7 +812,7 @@ vcclResult_t vcclQkNormRopeBackward(const vcclHeads_t* dq, const vcclHeads_t* dk
                                     const vcclHeads_t* k, const vcclRope_t* rope, const vcclHeads_t* dqIn,
                                     const vcclHeads_t* dkIn, void* dqWeight, void* dkWeight, void* workspace,
                                     int tokens, int D, vcclDataType_t datatype, vcclStream_t stream) {
-  if (tokens < 0 || D <= 0 || D % 8 != 0 || D > 256 || !sixteenBit(datatype) || !ropeOk(rope, D, tokens))
+  if (!tokensOk(tokens) || D <= 0 || D % 8 != 0 || D > 256 || !sixteenBit(datatype) || !ropeOk(rope, D, tokens))
     return vcclInvalidArgument;
   const bool weights = rope->qWeight != nullptr || rope->kWeight != nullptr;
   if ((rope->qWeight != nullptr) != (dqWeight != nullptr) || (rope->kWeight != nullptr) != (dkWeight != nullptr) ||
@@ -856,7 +856,7 @@ vcclResult_t vcclQkNormRopeBackward(const vcclHeads_t* dq, const vcclHeads_t* dk
 vcclResult_t vcclKv4Append(const vcclKv4_t* cache, const vcclHeads_t* k, const vcclHeads_t* v, const int* slots,
                            const vcclRope_t* rope, const vcclHeads_t* q, const vcclHeads_t* qOut, int tokens,
                            vcclDataType_t datatype, vcclStream_t stream) {
-  if (tokens < 0 || !cacheOk(cache) || !sixteenBit(datatype)) return vcclInvalidArgument;
+  if (!tokensOk(tokens) || !cacheOk(cache) || !sixteenBit(datatype)) return vcclInvalidArgument;
   if (rope != nullptr && !ropeOk(rope, cache->D, tokens)) return vcclInvalidArgument;
   if ((rope == nullptr) != (q == nullptr) || (q == nullptr) != (qOut == nullptr)) return vcclInvalidArgument;
   if (tokens == 0) return vcclSuccess;
@@ -882,7 +882,7 @@ vcclResult_t vcclKv4Append(const vcclKv4_t* cache, const vcclHeads_t* k, const v
 
 vcclResult_t vcclKv4Read(const vcclKv4_t* cache, const int* slots, const vcclHeads_t* k, const vcclHeads_t* v,
                          int tokens, vcclDataType_t datatype, vcclStream_t stream) {
-  if (tokens < 0 || !cacheOk(cache) || !(sixteenBit(datatype) || datatype == vcclFloat32)) return vcclInvalidArgument;
+  if (!tokensOk(tokens) || !cacheOk(cache) || !(sixteenBit(datatype) || datatype == vcclFloat32)) return vcclInvalidArgument;
   if (tokens == 0) return vcclSuccess;
   const int elem = datatype == vcclFloat32 ? 4 : 2;
   if (slots == nullptr || !headsOk(k, elem) || !headsOk(v, elem) || k->heads != cache->kvHeads ||

@@ -8,7 +8,8 @@
  * *Workspace calls), so a call may be captured into a CUDA graph.  Activation
  * tensors are vcclBfloat16 or vcclFloat16; [T, heads, D] tensors have
  * contiguous channels, and token and head strides (in elements, below 2^31)
- * that are multiples of 8 on a 16-byte aligned base; at most 32768 heads.
+ * that are multiples of 8 on a 16-byte aligned base; at most 32768 heads and
+ * 2^30 tokens.
  *
  * The cache of one layer: uint8 [pages, kvHeads, pageSize / 16, 18 * D] with
  * pageSize a multiple of 16 and D 64 or 128.  A block of 16 tokens holds the

@@ -89,9 +89,9 @@ def heads(t, name: str, dtype: torch.dtype, index: int, tokens: int, dim: int, n
     if count <= 1:
         s1 = 0
     vec, at = _VECTOR[dtype], t.data_ptr()
-    if s2 != 1 or s0 % vec or s1 % vec or at % 16 or s0 >= 2**31 or s1 >= 2**31 or count > 32768:
+    if s2 != 1 or s0 % vec or s1 % vec or at % 16 or s0 >= 2**31 or s1 >= 2**31 or count > 32768 or rows > 2**30:
         raise ValueError(f"{name} must have contiguous channels, token and head strides that are multiples of {vec} "
-                         "elements below 2^31, a 16-byte aligned base and at most 32768 heads")
+                         "elements below 2^31, a 16-byte aligned base, at most 32768 heads and 2^30 tokens")
     if written:
         (near, a), (far, b) = sorted(((s, c) for s, c in ((s0, rows), (s1, count))), key=lambda x: (x[1] > 1, x[0]))
         if (a > 1 and near < dim) or (b > 1 and far < (near * (a - 1) if a > 1 else 0) + dim):

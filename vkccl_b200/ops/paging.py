@@ -62,8 +62,8 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     if not isinstance(free_pages, torch.Tensor) or free_pages.dim() != 1 or free_pages.shape[0] < 1:
         raise ValueError("free_pages must be a one-dimensional int32 tensor with room for every page")
     pool, page_size, tokens = free_pages.shape[0], int(page_size), int(tokens)
-    if page_size < 1 or tokens < 0 or pool * page_size > 2**31 - 1 or width * page_size > 2**31 - 1:
-        raise ValueError("page_size must be positive, tokens not negative, and slots and lengths fit in 31 bits")
+    if page_size < 1 or not 0 <= tokens <= 2**30 or pool * page_size > 2**31 - 1 or width * page_size > 2**31 - 1:
+        raise ValueError("page_size must be positive, tokens 0 to 2^30, and slots and lengths fit in 31 bits")
     i32 = torch.int32
     a_lens, a_new = vector(lens, "lens", i32, batch, dev), vector(new_lens, "new_lens", i32, batch, dev)
     a_free, a_count = vector(free_pages, "free_pages", i32, pool, dev), vector(free_count, "free_count", i32, 1, dev)
