@@ -97,7 +97,8 @@ typedef struct {
 /* Writes k, v [tokens, kvHeads, D] to slots (distinct where not skipped).
  * With rope (and q, qOut) the queries and keys go through vcclQkNormRope
  * first: qOut is written, and the keys are rounded to the type and stored.
- * A group of 64 channels with a NaN or an infinity is stored as NaN. */
+ * A group of 64 channels with a NaN or an infinity, or whose extremes' sum or
+ * difference is not an f32, is stored as NaN. */
 vcclResult_t vcclKv4Append(const vcclKv4_t* cache, const vcclHeads_t* k, const vcclHeads_t* v, const int* slots,
                            const vcclRope_t* rope, const vcclHeads_t* q, const vcclHeads_t* qOut, int tokens,
                            vcclDataType_t datatype, vcclStream_t stream);
@@ -112,7 +113,8 @@ vcclResult_t vcclKv4Read(const vcclKv4_t* cache, const int* slots, const vcclHea
  * table[b, :] (width columns); its last row sees all of them, the row before
  * one less, and so on.  out = softmax(scale * q k^T) v; lse (f32
  * [tokens, q heads], may be NULL) = the logarithm of the sum of exponentials.
- * A row that sees nothing is 0 with lse = -inf.  Rows behind the last
+ * A row that sees nothing is 0 with lse = -inf; one whose channels are all
+ * below 2^-114 counts as zero.  Rows behind the last
  * request: 0 and -inf with zeroTail, else left as they are.  Tokens on a page
  * outside of the cache are not seen.  qStarts must not fall: the rows of
  * requests that overlap are undefined (nothing outside of out, lse and the

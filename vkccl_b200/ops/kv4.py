@@ -45,8 +45,8 @@ def kv4_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: tor
     """Writes k, v [T, kv heads, D] (bf16 or fp16) to slots [T] (int32).
 
     A negative slot, or one behind the cache, is skipped; the others must be
-    distinct.  A group of 64 channels with a NaN or an infinity reads back as
-    NaN.
+    distinct.  A group of 64 channels with a NaN or an infinity (or whose
+    extremes' sum or difference is not an f32) reads back as NaN.
     """
     dev, dtype = float16s(k, "k"), k.dtype
     t, _, dim = k.shape
