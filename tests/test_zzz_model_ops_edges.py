@@ -405,3 +405,41 @@ def test_norm_rope_of_odd_head_dimensions(dim, rot, inter):
         close(dx, leaf.grad, rope_slack(leaf.grad, torch.bfloat16, size), "dx")
         # terms |g x^| of at most 6 * 6, f32 sums of a lane's rows
         close(dw, wl.grad, wl.grad.abs() * 2.0**-8 + tokens * 3 * 36 * 2.0**-20, "dw")
+
+
+# ---- attention: long sums ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,heads", [(1, 64), (2, 8), (16, 64)])
+def test_attention_of_many_long_contexts(rows, heads):
+    """250 requests of 60000 tokens (of the same pages): a warp adds up whole requests, and the error must not grow with them.
+
+    In the norm of a row: the output is rounded to f16 (2^-11 of it at most), and every weight (2^-11 of p * 7.5 scales <= 1.01 p a, a
+    the largest |value| of the token's 64 channels, which add up as sqrt(sum p^2 a^2): the roundings of different tokens have
+    nothing to do with one another).  The tensor cores add 16 tokens a step to an f32 and drop what is below its last bit, 2^-23 of
+    it at most: n / 16 steps of the row itself, and for single tokens 8 steps of what 128 tokens add up to before the middle of
+    their codes is taken out, codes up to 255 / 16 of a scale where values go to 7.5 of it (2.2 a, half of it on average).  Runs of
+    rows round every value twice (2.1 * 2^-11 a)."""
+    from vkccl_b200.ops.kv4 import kv4_attention, kv4_read
+
+    g = gen(14)
+    n, batch, page, kv_heads = 60000, 250, 64, 8
+    pages = -(-n // page)
+    cache = random_cache(g, pages, page, kv_heads, 128)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(batch, 1)
+    q = (torch.randn(batch * rows, heads, 128, device="cuda", generator=g) * 0.5).half()
+    out = kv4_attention(q, cache, table, ints([n] * batch), ints([i * rows for i in range(batch + 1)]))
+    k, v = (x.double() for x in kv4_read(cache, torch.arange(n, dtype=torch.int32, device="cuda"), dtype=torch.float32))
+    tops = v.abs().unflatten(-1, (-1, 64)).amax(-1)  # [n, kv heads, 2]
+    for t in (0, 7 * rows, 249 * rows):
+        for h in (0, heads - 1):
+            j = h // (heads // kv_heads)
+            see = n - (rows - 1 - t % rows)
+            p = torch.softmax(k[:see, j] @ q[t, h].double() * 128 ** -0.5, 0)
+            want = p @ v[:see, j]
+            a = tops[:see, j].repeat_interleave(64, -1)
+            roundings = 3.1 if rows * heads // kv_heads >= 64 else 1.01
+            slack = ((want.norm() + (p.square() @ a.square()).sqrt().norm() * roundings) * 2.0**-11 + want.norm() * n / 16 * 2.0**-23
+                     + (p @ a).norm() * 8 * 1.1 * 2.0**-23)
+            d = (out[t, h].double() - want).norm()
+            assert d <= slack, (t, h, d.item(), slack.item(), want.norm().item())
