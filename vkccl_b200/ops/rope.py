@@ -47,9 +47,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     gradient are refused.  Train with the call in torch.no_grad() (or in an
     autograd.Function's forward) and ``qk_norm_rope_backward``.
     """
-    if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, q_weight, k_weight)):
-        raise ValueError("qk_norm_rope has no autograd history, and an input requires a gradient: call it in torch.no_grad(), and "
-                         "qk_norm_rope_backward for the gradients")
+    if torch.is_grad_enabled():
+        for x in (q, k, q_weight, k_weight):
+            if getattr(x, "requires_grad", False):
+                raise ValueError("qk_norm_rope has no autograd history, and an input requires a gradient: call it in "
+                                 "torch.no_grad(), and qk_norm_rope_backward for the gradients")
     dev, dtype, t, nq, nk, dim = _sizes(q, k)
     hq, hk = heads(q, "q", dtype, dev, t, dim), heads(k, "k", dtype, dev, t, dim)
     rope = rope_of(positions, inv_freq, q_weight, k_weight, eps, interleaved, dtype, dev, t, dim)
