@@ -41,8 +41,8 @@
 //
 // Measured: 842 us, 715 TFLOP/s, for 4 requests of 1024 rows against 2000 to
 // 9000 tokens, 64 heads on 8 (the single-token kernel takes 3.4 ms); 1.8 ms where
-// every 32 tokens hold values 2^10 apart.  The softmax bounds it: 2230 of the
-// 3070 clocks that a tile takes.
+// every 32 tokens hold values 2^10 apart.  The softmax bounds it: 2230 of
+// 3070 clocks when a tile took as many.
 #pragma once
 
 #include "kernels/kv4.cuh"

@@ -30,9 +30,9 @@
 // write partial sums (unnormalised output, maximum, sum) that a second kernel
 // joins in order.
 //
-// Measured: 137 us, 4.4 TB/s of cache, for 64 requests of 500 to 16000 tokens,
-// 64 heads on 8; the widening of codes bounds it (300 instructions a block of
-// 16 tokens, half of them on the ALU pipe).  One request of 900 tokens takes
+// Measured: 140 us, 4.3 TB/s of cache, for 64 requests of 500 to 16000 tokens,
+// 64 heads on 8; the widening of codes bounds it (280 instructions a block of
+// 16 tokens, almost half of them on the ALU pipe).  One request of 900 tokens takes
 // 12 us, which is the latency of two launches and eight dependent loads.
 #include <cfloat>
 #include <climits>
