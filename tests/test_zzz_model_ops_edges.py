@@ -147,6 +147,8 @@ def spread_case(g, kind, n, kv_heads, ratio, dim=128):
         v, k = v * 2.0**(ratio * t), k - 12.0 * t
     elif kind == "growing":  # ... and by more
         v, k = v * 2.0**(ratio * t), k - 2.0 * t
+    elif kind == "groups":  # some tokens' first 64 channels far above their others, which are like the rest
+        v[..., :64] *= torch.where(torch.rand(n, kv_heads, 1, device="cuda", generator=g) < 0.05, 2.0**ratio, 1.0)
     elif kind == "key unseen":
         k[n - 1] *= 2.0**ratio
     elif kind == "key below":  # one key is large, and its weight is nothing
@@ -181,7 +183,7 @@ def check_rows(got, lse, q, ks, vs, kv_lens, q_starts, long):
     assert ((lse.double() - wlse).abs() <= score + wlse.abs() * 2.0**-20 + 2.0**-18).all()
 
 
-KINDS = ["first", "middle", "last", "unseen", "sink", "rising", "falling", "growing", "mixed", "key unseen", "key below"]
+KINDS = ["first", "middle", "last", "unseen", "sink", "rising", "falling", "growing", "mixed", "key unseen", "key below", "groups"]
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -193,6 +195,9 @@ def test_attention_of_values_far_apart(kind, ratio, rows, heads, kv_heads, n, di
     not by the largest value around.  One row, a few, and runs of rows with and without shares of the keys."""
     from vkccl_b200.ops.kv4 import kv4_alloc, kv4_append, kv4_attention, kv4_read
 
+    long = rows * heads // kv_heads >= 64
+    if kind == "groups" and long and ratio > 14:
+        ratio = 14  # the groups of a row share its weights there: bits of the smaller one's go from 2^16 on
     g = gen(KINDS.index(kind) * 100 + ratio + rows)
     pages = -(-n // 16)
     cache = kv4_alloc(pages, 16, kv_heads, dim)
@@ -204,7 +209,7 @@ def test_attention_of_values_far_apart(kind, ratio, rows, heads, kv_heads, n, di
     k, v = (x.double() for x in kv4_read(cache, slots, dtype=torch.float32))
     q = (0.5 + 0.1 * torch.randn(rows, heads, dim, device="cuda", generator=g)).bfloat16()
     got, lse = kv4_attention(q, cache, table, ints([n]), ints([0, rows]), return_lse=True)
-    check_rows(got, lse, q, [k], [v], [n], [0, rows], rows * heads // kv_heads >= 64)
+    check_rows(got, lse, q, [k], [v], [n], [0, rows], long)
 
 
 def test_attention_of_a_long_run_among_the_largest_batch():
