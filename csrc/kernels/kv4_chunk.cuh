@@ -32,12 +32,12 @@
 // for values, which the softmax puts into its scale and into the weights.
 // Where some of the 32 are far below the largest (2^8 for values, 2^14 for
 // keys) each is divided by a power of its own, and the softmax puts that back
-// token by token.  A row's outputs are in
-// units of the largest weight times value that it met, so what it does not see
-// or gives no weight costs the rest no bits.  Both groups of 64 channels share
-// a row's weights, so where one's values are more than 2^16 above the other's
-// the other loses bits.  Scores, maxima, sums and outputs are f32.  The maximum is followed loosely (by 8 in the base-2 logarithm), so
-// the output is rescaled rarely.
+// token by token.  A row's outputs are in units of the largest weight times
+// value that it met, so what it does not see or gives no weight costs the rest
+// no bits.  Both groups of 64 channels share a row's weights, so where one's
+// values are more than 2^16 above the other's the other loses bits.  Scores,
+// maxima, sums and outputs are f32.  The maximum is followed loosely (by 8 in
+// the base-2 logarithm), so the output is rescaled rarely.
 //
 // Measured: 842 us, 715 TFLOP/s, for 4 requests of 1024 rows against 2000 to
 // 9000 tokens, 64 heads on 8 (the single-token kernel takes 3.4 ms); 1.8 ms where
