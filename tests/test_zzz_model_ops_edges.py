@@ -448,3 +448,48 @@ def test_attention_of_many_long_contexts(rows, heads):
                      + (p @ a).norm() * 8 * 1.1 * 2.0**-23)
             d = (out[t, h].double() - want).norm()
             assert d <= slack, (t, h, d.item(), slack.item(), want.norm().item())
+
+
+# ---- calls at once -------------------------------------------------------------------
+
+
+def test_long_runs_on_two_streams_beside_a_gemm():
+    """Kernels that take all of an SM's tensor memory, beside one that takes a part of it: the same bits as one after another."""
+    from vkccl_b200.ops.gemm import gemm_bf16
+    from vkccl_b200.ops.kv4 import kv4_attention
+
+    g = gen(15)
+    cache, table = random_cache(g, 64, 16, 2, 128), torch.arange(64, dtype=torch.int32, device="cuda").view(2, 32)
+    args = (cache, table, ints([500, 512]), ints([0, 200, 300]))
+    qa, qb = (torch.randn(300, 16, 128, device="cuda", generator=g).bfloat16() for _ in range(2))
+    x, w = (torch.randn(n, 1024, device="cuda", generator=g).bfloat16() for n in (512, 2048))
+    want = kv4_attention(qa, *args), kv4_attention(qb, *args), gemm_bf16(x, w)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for s, f in zip(streams, (lambda: kv4_attention(qa, *args), lambda: kv4_attention(qb, *args), lambda: gemm_bf16(x, w))):
+            with torch.cuda.stream(s):
+                got.append(f())
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 3]) for i, y in enumerate(got))
+
+
+def test_constant_values_and_a_late_scale():
+    """Groups of equal channels have a scale of zero, and no weight of f16 goes by it; behind them come ordinary ones."""
+    from test_zzz_kv4 import check_attention
+    from vkccl_b200.ops.kv4 import kv4_alloc, kv4_append, kv4_attention, kv4_read
+
+    g = gen(16)
+    n = 400
+    cache, table = kv4_alloc(25, 16, 1, 128), torch.arange(25, dtype=torch.int32, device="cuda").view(1, 25)
+    kv = torch.randn(n, 2, 128, device="cuda", generator=g).bfloat16()
+    kv[:300, 1] = kv[:300, 1, :1]  # all channels of a token's value alike
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    kv4_append(cache, kv[:, :1], kv[:, 1:], slots)
+    k, v = (x.double() for x in kv4_read(cache, slots, dtype=torch.float32))
+    for rows in (1, 3, 120):
+        for length in (299, 301, n):
+            q = torch.randn(rows, 8, 128, device="cuda", generator=g).bfloat16()
+            out, lse = kv4_attention(q, cache, table, ints([length]), ints([0, rows]), return_lse=True)
+            check_attention(out, lse, q, [k[:length]], [v[:length]], [length], [0, rows])
